@@ -18,8 +18,9 @@ H4B_ETOOBIG = -3
 STATUS_WAIT_TIMEOUT = 1
 STATUS_BAD_TOKEN = 2
 STATUS_BAD_POSITION = 4
+STATUS_BAD_PAGE = 8
 
-_vp, _i32, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_vp, _i32, _f32, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
 
 class ModelDesc(ctypes.Structure):
@@ -73,6 +74,14 @@ class TpGroupDesc(ctypes.Structure):
     _fields_ = [("world", _i32), ("rank", _i32), ("capacity", _i32), ("buffers", _vp * 8), ("generation", _vp)]
 
 
+class PagedKvDesc(ctypes.Structure):
+    """Mirror of ``h4b_paged_kv``."""
+
+    _fields_ = [(n, _vp) for n in ("k_pages", "v_pages", "page_table", "q_offsets", "kv_lens")] + [
+        (n, _i32) for n in ("dtype", "pages", "page_size", "kv_heads", "head_dim", "sequences", "table_stride",
+                            "tokens")]
+
+
 _SIGNATURES = {
     "h4b_prepare": [],
     "h4b_get_status": [_vp],
@@ -123,12 +132,19 @@ _SIGNATURES = {
                     _vp],
     "h4b_prefill_tp_stage": [ctypes.POINTER(ModelDesc), ctypes.POINTER(StateDesc), ctypes.POINTER(PrefillScratchDesc),
                              _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp],
+    "h4b_paged_append": [ctypes.POINTER(PagedKvDesc), _vp, _i32, _i64, _i32, _vp, _vp, _f32, _vp, _vp, _i32, _vp, _i64,
+                         _vp],
+    "h4b_paged_attention": [ctypes.POINTER(PagedKvDesc), _vp, _i64, _i32, _f32, _i32, _i32, _i32, _vp, _i64, _vp, _vp,
+                            _i64, _vp],
+    "h4b_paged_attention_workspace_bytes": [_i32],
+    "h4b_pages_copy": [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i32, _vp],
     "h4b_lattice_scratch_bytes": [_i32],
     "h4b_lattice_to_int4": [ctypes.POINTER(LatticeProjectionDesc), _vp, _vp, _vp, ctypes.POINTER(_i32), _vp],
     "h4b_rows_to_int4": [_vp, _i32, _i32, _i32, _vp, _vp, _vp],
 }
 _RESTYPES = {"h4b_persistent_exchange_words": ctypes.c_longlong, "h4b_sample_scratch_bytes": ctypes.c_longlong,
-             "h4b_tp_buffer_bytes": ctypes.c_longlong, "h4b_lattice_scratch_bytes": ctypes.c_longlong}
+             "h4b_tp_buffer_bytes": ctypes.c_longlong, "h4b_lattice_scratch_bytes": ctypes.c_longlong,
+             "h4b_paged_attention_workspace_bytes": ctypes.c_longlong}
 
 
 def exported_symbols() -> list[str]:

@@ -1,0 +1,984 @@
+// Paged K/V cache: the append of new tokens, page copies, and the attention
+// of few query rows a sequence (decode, short chunks). paged_tc.cu holds the
+// attention of long chunks.
+//
+// A layer's pages are [pages][kv_heads][page_size][head_dim] of fp16 or bf16,
+// one buffer for K and one for V. Sequence b's token j lives in page
+// page_table[b][j / page_size], slot j % page_size. Its new tokens are rows
+// q_offsets[b] .. q_offsets[b + 1] - 1 of the batch, at positions
+// kv_lens[b] - n_b + i (n_b new tokens): a token sees the keys j <= its own
+// position p, with a window w only j > p - w or j < sinks.
+//
+// Every table is read on the device, so a captured graph follows its contents.
+// Nothing a table says makes a kernel read or write out of bounds: a page id,
+// an offset or a length out of range sets status bit 8 (kStatusBadPage), a
+// page that is needed and out of range reads as zeros and is not written, a
+// sequence with such an offset or length counts as empty.
+#include <cuda_bf16.h>
+
+namespace h4b {
+
+constexpr int kStatusBadPage = 8;  // page id, row offset or length out of range
+
+template <typename T>
+struct Pair;  // two 16-bit values of a 32-bit word
+template <>
+struct Pair<__half> {
+    __device__ static uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ static float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+    __device__ static uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ static float2 unpack(uint32_t w) {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    }
+};
+
+// The batch as the kernels see it (h4b_paged_kv without its pointers' types).
+struct PagedView {
+    int pages, page_shift, kv_heads, sequences, table_stride, tokens;
+    const int32_t* table;
+    const int32_t* q_offsets;
+    const int32_t* kv_lens;
+};
+
+// Rows and lengths of one sequence, made safe: first row, new tokens and
+// position of the first one.
+struct SequenceSpan {
+    int first, count, base;
+};
+__device__ __forceinline__ SequenceSpan sequence_span(const PagedView& p, int b) {
+    SequenceSpan s{p.q_offsets[b], 0, 0};
+    const int end = p.q_offsets[b + 1], len = p.kv_lens[b];
+    const bool good = s.first >= 0 && end >= s.first && end <= p.tokens && len >= 0 &&
+                      len <= static_cast<long long>(p.table_stride) << p.page_shift;
+    if (!good) {
+        report(kStatusBadPage);
+        // its rows, as far as they exist, still get an (empty) answer
+        const long long lo = min(max(s.first, 0), p.tokens), hi = min(max(end, 0), p.tokens);
+        return SequenceSpan{static_cast<int>(lo), static_cast<int>(max(hi - lo, 0ll)), -(1 << 30)};
+    }
+    s.count = end - s.first;
+    s.base = len - s.count;
+    return s;
+}
+
+// ---- append ---------------------------------------------------------------
+// One warp per (token, head) in steps: q and k heads are divided by their
+// root mean square and scaled (norm weights), then rotated (cos/sin rows of
+// the token's position, halves d and d + D/2 paired); v passes through. One
+// rounding to 16 bits at the end, everything before in fp32. A head takes D/4
+// lanes: lane i holds dims 2i, 2i + 1 and their partners D/2 further, so the
+// rotation needs no exchange.
+// Bound by HBM: (heads + 2 kv_heads) D (source + 2) bytes a token.
+struct AppendArgs {
+    PagedView p;
+    const void* qkv;
+    long long qkv_stride;   // values from token to token
+    const float *norm_q, *norm_k, *cos, *sin;
+    int max_pos, heads;
+    float eps;
+    void *q_out, *k_pages, *v_pages;
+    long long q_stride;
+};
+
+constexpr int kAppendWarps = 8;
+
+template <typename S>
+__device__ __forceinline__ float2 load_pair(const S* p) {
+    return Pair<S>::unpack(__ldg(reinterpret_cast<const uint32_t*>(p)));
+}
+template <>
+__device__ __forceinline__ float2 load_pair<float>(const float* p) {
+    return __ldg(reinterpret_cast<const float2*>(p));
+}
+
+template <typename S, typename T, int D>
+__global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const AppendArgs a) {
+    constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;  // heads a warp holds at once
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int token = blockIdx.x, page_size = 1 << a.p.page_shift;
+
+    // the token's sequence: the last b whose offset is not past the token
+    int b = -1;
+    for (int j = 0; j < a.p.sequences; j += 32) {
+        const bool before = j + lane < a.p.sequences && a.p.q_offsets[j + lane] <= token;
+        b += __popc(__ballot_sync(0xffffffffu, before));
+    }
+    long long slot = -1;  // of the token in its page's buffers, in rows of kv head 0
+    int position = -1;
+    if (b >= 0) {
+        const SequenceSpan s = sequence_span(a.p, b);
+        position = token < s.first + s.count ? s.base + token - s.first : -1;
+        if (position >= 0) {
+            const int page = a.p.table[static_cast<long long>(b) * a.p.table_stride + (position >> a.p.page_shift)];
+            if (page >= 0 && page < a.p.pages)
+                slot = (static_cast<long long>(page) * a.p.kv_heads << a.p.page_shift) + (position & (page_size - 1));
+            else if (lane == 0)
+                report(kStatusBadPage);
+        }
+    }
+
+    const int i = lane % kLanes, sub = lane / kLanes;
+    float2 cos = make_float2(1.f, 1.f), sin = make_float2(0.f, 0.f);
+    if (a.cos != nullptr && position >= 0) {
+        if (position < a.max_pos) {
+            cos = load_pair(a.cos + static_cast<long long>(position) * (D / 2) + 2 * i);
+            sin = load_pair(a.sin + static_cast<long long>(position) * (D / 2) + 2 * i);
+        } else if (lane == 0) {
+            report(kStatusBadPosition);
+        }
+    }
+    const int total = a.heads + 2 * a.p.kv_heads;
+    const S* row = static_cast<const S*>(a.qkv) + token * a.qkv_stride;
+    T* q_row = static_cast<T*>(a.q_out) + token * a.q_stride;
+    for (int h0 = (blockIdx.y * kAppendWarps + warp) * kPerWarp; h0 < total;
+         h0 += gridDim.y * kAppendWarps * kPerWarp) {
+        const int h = h0 + sub;
+        const bool valid = h < total, is_v = h >= a.heads + a.p.kv_heads, is_q = h < a.heads;
+        float2 x = make_float2(0.f, 0.f), y = x;
+        if (valid) {
+            x = load_pair(row + h * D + 2 * i);
+            y = load_pair(row + h * D + D / 2 + 2 * i);
+        }
+        const float* weight = is_q ? a.norm_q : a.norm_k;
+        if (weight != nullptr) {
+            float sum = x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y;
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (!is_v) {
+                const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
+                const float2 w0 = load_pair(weight + 2 * i), w1 = load_pair(weight + D / 2 + 2 * i);
+                x = make_float2(x.x * inv * w0.x, x.y * inv * w0.y);
+                y = make_float2(y.x * inv * w1.x, y.y * inv * w1.y);
+            }
+        }
+        if (!valid) continue;
+        if (!is_v) {
+            const float2 u = x;
+            x = make_float2(u.x * cos.x - y.x * sin.x, u.y * cos.y - y.y * sin.y);
+            y = make_float2(y.x * cos.x + u.x * sin.x, y.y * cos.y + u.y * sin.y);
+        }
+        T* dst = nullptr;
+        if (is_q) {
+            dst = q_row + h * D;
+        } else if (slot >= 0) {
+            const int kv = is_v ? h - a.heads - a.p.kv_heads : h - a.heads;
+            dst = static_cast<T*>(is_v ? a.v_pages : a.k_pages) +
+                  (slot + (static_cast<long long>(kv) << a.p.page_shift)) * D;
+        }
+        if (dst != nullptr) {
+            *reinterpret_cast<uint32_t*>(dst + 2 * i) = Pair<T>::pack(x.x, x.y);
+            *reinterpret_cast<uint32_t*>(dst + D / 2 + 2 * i) = Pair<T>::pack(y.x, y.y);
+        }
+    }
+}
+
+// ---- page copies ------------------------------------------------------------
+// Page dst[i] <- page src[i] in every layer, K and V: one CTA moves up to
+// kCopyBytes of one (layer, K or V, move), every thread with all its 16-byte
+// loads in flight before its first store. Bound by HBM: twice the page bytes.
+constexpr int kCopyThreads = 256, kCopyUnroll = 8, kCopyBytes = kCopyThreads * kCopyUnroll * 16;
+
+__global__ void __launch_bounds__(kCopyThreads)
+    pages_copy_kernel(uint8_t* k_pages, uint8_t* v_pages, int pages, long long page_bytes, int parts,
+                      const int32_t* src, const int32_t* dst) {
+    const int move = blockIdx.x / parts, part = blockIdx.x % parts;
+    const int from = src[move], to = dst[move];
+    if (from < 0 || from >= pages || to < 0 || to >= pages) {
+        if (threadIdx.x == 0) report(kStatusBadPage);
+        return;
+    }
+    uint8_t* base = (blockIdx.z ? v_pages : k_pages) + static_cast<long long>(blockIdx.y) * pages * page_bytes;
+    const uint4* s = reinterpret_cast<const uint4*>(base + from * page_bytes);
+    uint4* d = reinterpret_cast<uint4*>(base + to * page_bytes);
+    const long long words = page_bytes / 16, first = static_cast<long long>(part) * (kCopyBytes / 16) + threadIdx.x;
+    uint4 v[kCopyUnroll];
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u)
+        if (first + u * kCopyThreads < words) v[u] = __ldcs(s + first + u * kCopyThreads);
+#pragma unroll
+    for (int u = 0; u < kCopyUnroll; ++u)
+        if (first + u * kCopyThreads < words) __stcs(d + first + u * kCopyThreads, v[u]);
+}
+
+// ---- attention: the split of the work ------------------------------------------
+// An item is (sequence, tile of ROWS / group new tokens, kv head): its query
+// rows r = (token i, q head j of the group), r = i * group + j, share the
+// item's keys. A unit is one block of KEYS keys of an item, from the blocks
+// that some row of it sees: the sink blocks [0, sink_blocks) and then
+// [low, high); an item has one unit at least, so that every row is answered.
+// The units of all items in order (sequence, tile, kv head, block) are cut
+// into one equal contiguous range per CTA, whatever the lengths. An item that
+// lies across CTAs leaves one partial result (o, m, l) in each; the CTA that
+// finishes last joins them in the order of the CTAs, so the result does not
+// depend on which one that is.
+struct AttendArgs {
+    PagedView p;
+    const void *q, *k_pages, *v_pages;
+    void* out;
+    float* lse;               // may be null
+    long long q_stride, out_stride;
+    int heads, group, window, sinks;
+    float scale;              // of a score in base-2 units: scale * log2(e)
+    float* partials;          // [2 * CTAs][ROWS * (D + 2)]: a CTA's first and last item
+    unsigned int* counters;   // [CTAs], zero between calls
+};
+
+struct Tile {  // one tile of new tokens of a sequence
+    int first, tokens;        // first row (token index in the batch), tokens
+    int p0, p1;               // positions of its first and last token
+    int low, high, sink_blocks;
+    __device__ __forceinline__ int units() const { return high - low + sink_blocks; }
+    __device__ __forceinline__ int block(int unit) const {
+        return unit < sink_blocks ? unit : low + unit - sink_blocks;
+    }
+};
+
+template <int KEYS>
+__device__ __forceinline__ Tile make_tile(const SequenceSpan& s, int t, int tile_tokens, int window, int sinks) {
+    Tile x;
+    x.first = s.first + t * tile_tokens;
+    x.tokens = min(tile_tokens, s.count - t * tile_tokens);
+    x.p0 = s.base + t * tile_tokens;
+    x.p1 = x.p0 + x.tokens - 1;
+    const int end = max(x.p1 + 1, 0);
+    const int from = window > 0 ? max(x.p0 - window + 1, 0) : 0;
+    x.high = max((end + KEYS - 1) / KEYS, 1);
+    x.low = min(from / KEYS, x.high - 1);
+    x.sink_blocks = window > 0 ? min((min(sinks, end) + KEYS - 1) / KEYS, x.low) : 0;
+    return x;
+}
+
+// Units of all tiles of a sequence, one kv head.
+template <int KEYS>
+__device__ __forceinline__ long long sequence_units(const SequenceSpan& s, int tile_tokens, int window, int sinks) {
+    long long n = 0;
+    for (int t = 0; t * tile_tokens < s.count; ++t) n += make_tile<KEYS>(s, t, tile_tokens, window, sinks).units();
+    return n;
+}
+
+// The CTA's range of units and where it starts.
+struct Range {
+    long long begin, end, total;  // [begin, end) of total
+    long long skip;               // units of its sequence before `begin`
+    int sequence;                 // of unit `begin`
+    int ctas;                     // that have a range: every one of them has a unit at least
+};
+__device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
+// The CTA that holds a unit: the largest c with range_begin(c) <= unit.
+__device__ __forceinline__ int range_owner(long long total, long long unit, int ctas) {
+    return static_cast<int>(((unit + 1) * ctas - 1) / total);
+}
+
+// Every thread of the CTA takes part; `shared` holds THREADS / 32 + 1 long
+// longs and a Range. Each thread sums its share of the sequences, a prefix
+// sum over the threads follows, and the thread whose sequences hold unit
+// `begin` finds it.
+template <int THREADS, int KEYS>
+__device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens, void* shared) {
+    long long* warp_sums = static_cast<long long*>(shared);
+    Range* found = reinterpret_cast<Range*>(warp_sums + THREADS / 32 + 1);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int each = (a.p.sequences + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
+    const int b1 = min(b0 + each, a.p.sequences);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b)
+        mine += a.p.kv_heads * sequence_units<KEYS>(sequence_span(a.p, b), tile_tokens, a.window, a.sinks);
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += up;
+    }
+    if (lane == 31) warp_sums[warp] = before;
+    __syncthreads();
+    long long total = 0;
+    before -= mine;
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
+    }
+    Range r;
+    r.total = total;
+    r.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    r.begin = r.end = 0;
+    if (static_cast<int>(blockIdx.x) < r.ctas) {
+        r.begin = range_begin(total, blockIdx.x, r.ctas);
+        r.end = range_begin(total, blockIdx.x + 1, r.ctas);
+    }
+    if (r.begin < r.end && r.begin >= before && r.begin < before + mine) {
+        long long at = before;
+        for (int b = b0;; ++b) {
+            const long long n =
+                a.p.kv_heads * sequence_units<KEYS>(sequence_span(a.p, b), tile_tokens, a.window, a.sinks);
+            if (r.begin < at + n) {
+                r.sequence = b;
+                r.skip = r.begin - at;
+                break;
+            }
+            at += n;
+        }
+        *found = r;
+    }
+    __syncthreads();
+    if (r.begin < r.end) {
+        r.sequence = found->sequence;
+        r.skip = found->skip;
+    }
+    return r;
+}
+
+// A walk over the CTA's units, item by item.
+template <int KEYS>
+struct Walk {
+    SequenceSpan span;
+    Tile tile;
+    int b, t, h, unit;        // unit within the item
+    long long left;           // units of the range from here on
+
+    __device__ __forceinline__ void start(const AttendArgs& a, const Range& r, int tile_tokens) {
+        b = r.sequence;
+        left = r.end - r.begin;
+        span = sequence_span(a.p, b);
+        long long skip = r.skip;
+        for (t = 0;; ++t) {
+            tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
+            const long long n = static_cast<long long>(tile.units()) * a.p.kv_heads;
+            if (skip < n) break;
+            skip -= n;
+        }
+        h = static_cast<int>(skip / tile.units());
+        unit = static_cast<int>(skip % tile.units());
+    }
+    // Past the item's last unit: to the next item that has any.
+    __device__ __forceinline__ void next_item(const AttendArgs& a, int tile_tokens) {
+        unit = 0;
+        if (++h < a.p.kv_heads) return;
+        h = 0;
+        ++t;
+        while (t * tile_tokens >= span.count) {
+            t = 0;
+            span = sequence_span(a.p, ++b);
+        }
+        tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
+    }
+    // To the next unit; false past the range's end.
+    __device__ __forceinline__ bool next(const AttendArgs& a, int tile_tokens) {
+        if (--left <= 0) return false;
+        if (++unit >= tile.units()) next_item(a, tile_tokens);
+        return true;
+    }
+};
+
+// Whether some row of the tile sees key j.
+__device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, int j) {
+    return j <= t.p1 && (window <= 0 || j > t.p0 - window || j < sinks);
+}
+
+// ---- attention of few rows -----------------------------------------------------
+// For decode and short chunks the keys are read once and each takes part in
+// few products, so HBM is the bound: 4 D kv_heads bytes a key. The products
+// run on mma.sync (m16n8k16): its 16 rows hold the item's rows, and its
+// operands come from shared memory without the tensor-memory allocation, the
+// MMA-issuing thread and the 128-row tiles that tcgen05 asks for.
+//
+// A CTA has four warps, a unit is 64 keys: each warp takes 16 of them, a
+// 16-key piece of one page (page sizes are multiples of 16), with a ring of
+// its own in shared memory fed by its own 16-byte asynchronous copies. So no
+// barrier is needed between the loads and the products: a warp waits for its
+// own copies only, and the ring runs on over the item boundaries. Each warp
+// keeps its own (o, m, l); at an item's end (or the range's) the warps join
+// theirs through shared memory.
+// Softmax in base 2: p = 2^(s - m + 8), m moves only when a score passes
+// m + 7 (p < 2^15 fits fp16; the 8 keeps small p clear of fp16's subnormals);
+// l is summed from the fp32 p, which is rounded to 16 bits for the p v
+// products only. Rows that no row sees are zero-filled by the copy, so what
+// such a slot holds cannot reach a sum.
+constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 64;
+constexpr float kFewOffset = 8.f, kFewSlack = 7.f;
+
+template <int D, int ROWS>
+struct FewCfg {
+    static constexpr int kTiles = ROWS <= 16 ? 1 : ROWS / 16;  // m16 tiles
+    static constexpr int kHalves = ROWS == 8 ? 1 : 2;          // 8-row halves of an m16 tile in use
+    static constexpr int kPiece = 16 * D * 2;                  // bytes of 16 keys, K or V
+    static constexpr int kStages = (ROWS <= 16 ? 3 : 2) * (128 / D);
+    static constexpr int kRing = kFewWarps * kStages * 2 * kPiece;
+    static constexpr int kJoin = (ROWS < 16 ? 16 : ROWS) * D * 4;  // one warp's o
+    static constexpr int kJoinOff = kRing;
+    static constexpr int kStatOff = kJoinOff + 2 * kJoin;
+    static constexpr int kSmem = kStatOff + 2 * (ROWS < 16 ? 16 : ROWS) * 2 * 4 + 256;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                 "{%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes global -> shared; with `fill` zeros instead and no read.
+__device__ __forceinline__ void async_copy16_or_zero(uint32_t dst, const void* src, bool fill) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fill ? 0 : 16)
+                 : "memory");
+}
+
+// Byte of 16-byte chunk c of row r in a 16-row piece: the chunks of eight
+// consecutive rows lie in distinct banks.
+template <int D>
+__device__ __forceinline__ uint32_t piece_at(int r, int c) {
+    return static_cast<uint32_t>(r * (D * 2) + ((c ^ (r & 7)) * 16));
+}
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(const AttendArgs a) {
+    using C = FewCfg<D, ROWS>;
+    constexpr int kSteps = D / 16, kCols = D / 8;
+    extern __shared__ __align__(128) uint8_t few_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tile_tokens = ROWS / a.group;
+    const Range range = find_range<kFewThreads, kFewKeys>(a, tile_tokens, few_smem + C::kStatOff);
+    if (range.begin >= range.end) return;
+    __syncthreads();  // the range's scratch is reused below
+
+    const uint32_t ring = smem_addr(few_smem) + warp * C::kStages * 2 * C::kPiece;
+    const long long head_rows = 1ll << a.p.page_shift;  // rows of one head of a page
+    const int page_mask = (1 << a.p.page_shift) - 1;
+
+    // Page of the walk's piece: -1 when no row sees any key of it.
+    auto page_of = [&](const Walk<kFewKeys>& w) -> int {
+        const int key = w.tile.block(w.unit) * kFewKeys + warp * 16;
+        const Tile& t = w.tile;
+        const bool seen = key <= t.p1 && (a.window <= 0 || key + 15 > t.p0 - a.window || key < a.sinks);
+        if (!seen) return -1;
+        const int page = a.p.table[static_cast<long long>(w.b) * a.p.table_stride + (key >> a.p.page_shift)];
+        if (page < 0 || page >= a.p.pages) {
+            if (lane == 0) report(kStatusBadPage);
+            return -2;  // needed, but nowhere: reads as zeros
+        }
+        return page;
+    };
+    auto load = [&](const Walk<kFewKeys>& w, int page, int stage) {
+        if (page == -1) return;
+        const int key = w.tile.block(w.unit) * kFewKeys + warp * 16;
+        const long long row = (static_cast<long long>(max(page, 0)) * a.p.kv_heads + w.h) * head_rows + (key & page_mask);
+        const uint32_t dst = ring + stage * 2 * C::kPiece;
+        constexpr int kChunks = D / 8, kRowsStep = 32 / kChunks;  // 16-byte chunks a row, rows a pass
+        const int c = lane % kChunks, r0 = lane / kChunks;
+        const T* k = static_cast<const T*>(a.k_pages) + row * D + c * 8;
+        const T* v = static_cast<const T*>(a.v_pages) + row * D + c * 8;
+#pragma unroll
+        for (int r = 0; r < 16; r += kRowsStep) {
+            const bool fill = page < 0 || !tile_sees(w.tile, a.window, a.sinks, key + r + r0);
+            async_copy16_or_zero(dst + piece_at<D>(r + r0, c), k + (r + r0) * D, fill);
+            async_copy16_or_zero(dst + C::kPiece + piece_at<D>(r + r0, c), v + (r + r0) * D, fill);
+        }
+    };
+
+    Walk<kFewKeys> now, ahead;
+    now.start(a, range, tile_tokens);
+    ahead = now;
+    // the ring's first stages; `page` belongs to the piece `ahead` stands at
+    int page = page_of(ahead);
+    bool more = true;
+    int pages_now[C::kStages];  // page of the piece in each stage (stage 0: `now`)
+#pragma unroll
+    for (int s = 0; s < C::kStages - 1; ++s) {
+        pages_now[s] = -1;
+        if (more) {
+            load(ahead, page, s);
+            pages_now[s] = page;
+            more = ahead.next(a, tile_tokens);
+            if (more) page = page_of(ahead);
+        }
+        async_copy_commit();
+    }
+    pages_now[C::kStages - 1] = -1;
+
+    uint32_t qf[C::kTiles][kSteps][4];
+    float o[C::kTiles][kCols][4];
+    float m[C::kTiles][2], l[C::kTiles][2];
+    int pos[C::kTiles][2];
+    int stage = 0;
+    bool begun = now.unit == 0;  // the item's first unit is in this range
+    bool fresh = true;
+    while (true) {
+        if (fresh) {  // a new item: its q fragments and empty sums
+            fresh = false;
+#pragma unroll
+            for (int mt = 0; mt < C::kTiles; ++mt) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int r = mt * 16 + half * 8 + lane / 4;
+                    const int i = r / a.group;
+                    const bool valid = (half < C::kHalves) && i < now.tile.tokens;
+                    pos[mt][half] = valid ? now.tile.p0 + i : -1;
+                    m[mt][half] = -INFINITY;
+                    l[mt][half] = 0.f;
+                    const T* q = static_cast<const T*>(a.q) + (now.tile.first + (valid ? i : 0)) * a.q_stride +
+                                 (now.h * a.group + (valid ? r - i * a.group : 0)) * D + (lane & 3) * 2;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        qf[mt][k][half] = valid ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
+                        qf[mt][k][2 + half] = valid ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+            }
+        }
+        async_copy_wait_prior<C::kStages - 2>();
+        __syncwarp();
+        if (pages_now[0] != -1) {
+            const uint32_t kbase = ring + stage * 2 * C::kPiece, vbase = kbase + C::kPiece;
+            float s[C::kTiles][2][4];
+#pragma unroll
+            for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t b[4];  // keys 0-7 and 8-15, dims 16k..16k+15
+                ldmatrix4(b, kbase + piece_at<D>((lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int mt = 0; mt < C::kTiles; ++mt) {
+                    mma_16816<T>(s[mt][0], qf[mt][k], b[0], b[1]);
+                    mma_16816<T>(s[mt][1], qf[mt][k], b[2], b[3]);
+                }
+            }
+            const int key = now.tile.block(now.unit) * kFewKeys + warp * 16;
+            const Tile& t = now.tile;
+            const bool all = key + 15 <= t.p0 && (a.window <= 0 || key > t.p1 - a.window || key + 15 < a.sinks);
+            bool grow = false;
+#pragma unroll
+            for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                for (int half = 0; half < C::kHalves; ++half)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& x = s[mt][n][half * 2 + e];
+                            x *= a.scale;
+                            const int j = key + n * 8 + (lane & 3) * 2 + e, p = pos[mt][half];
+                            if (!all && !(j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks))) x = -INFINITY;
+                            grow |= x > m[mt][half] + kFewSlack;
+                        }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                    for (int half = 0; half < C::kHalves; ++half) {
+                        float top = fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
+                                          fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1]));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        if (top > m[mt][half]) {
+                            const float f = ex2_approx(m[mt][half] - top);  // 0 for the first keys
+                            m[mt][half] = top;
+                            l[mt][half] *= f;
+#pragma unroll
+                            for (int n = 0; n < kCols; ++n) {
+                                o[mt][n][half * 2] *= f;
+                                o[mt][n][half * 2 + 1] *= f;
+                            }
+                        }
+                    }
+            }
+            uint32_t pf[C::kTiles][4];
+#pragma unroll
+            for (int mt = 0; mt < C::kTiles; ++mt) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (half >= C::kHalves) {
+                        pf[mt][half] = pf[mt][2 + half] = 0u;
+                        continue;
+                    }
+                    const float base = m[mt][half] == -INFINITY ? 0.f : kFewOffset - m[mt][half];
+                    float p[4];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) p[n * 2 + e] = ex2_approx(s[mt][n][half * 2 + e] + base);
+                    l[mt][half] += (p[0] + p[1]) + (p[2] + p[3]);
+                    pf[mt][half] = Pair<T>::pack(p[0], p[1]);
+                    pf[mt][2 + half] = Pair<T>::pack(p[2], p[3]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < kCols; n += 2) {
+                uint32_t b[4];  // dims 8n..8n+7 (keys 0-7, 8-15), then the next eight
+                ldmatrix4_trans(b, vbase + piece_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), n + (lane >> 4)));
+#pragma unroll
+                for (int mt = 0; mt < C::kTiles; ++mt) {
+                    mma_16816<T>(o[mt][n], pf[mt], b[0], b[1]);
+                    mma_16816<T>(o[mt][n + 1], pf[mt], b[2], b[3]);
+                }
+            }
+        }
+        // refill the stage freed one step ago
+        __syncwarp();
+        int page_new = -1;
+        if (more) {
+            load(ahead, page, (stage + C::kStages - 1) % C::kStages);
+            page_new = page;
+            more = ahead.next(a, tile_tokens);
+            if (more) page = page_of(ahead);
+        }
+        async_copy_commit();
+#pragma unroll
+        for (int s = 0; s + 1 < C::kStages - 1; ++s) pages_now[s] = pages_now[s + 1];
+        pages_now[C::kStages - 2] = page_new;
+        stage = (stage + 1) % C::kStages;
+
+        const bool item_done = now.unit + 1 >= now.tile.units();
+        if (!item_done && now.left > 1) {
+            now.next(a, tile_tokens);
+            continue;
+        }
+
+        // ---- the warps join their sums: 2, 3 into 0, 1, then 1 into 0 --------
+        float* stat = reinterpret_cast<float*>(few_smem + C::kStatOff);
+        constexpr int kAll = 16 * C::kTiles;
+#pragma unroll
+        for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+            for (int half = 0; half < C::kHalves; ++half) {
+                l[mt][half] += __shfl_xor_sync(0xffffffffu, l[mt][half], 1);
+                l[mt][half] += __shfl_xor_sync(0xffffffffu, l[mt][half], 2);
+            }
+#pragma unroll
+        for (int round = 2; round >= 1; round >>= 1) {
+            if (warp >= round && warp < 2 * round) {
+                float* dst = reinterpret_cast<float*>(few_smem + C::kJoinOff + (warp - round) * C::kJoin);
+                float* st = stat + (warp - round) * 2 * kAll;
+#pragma unroll
+                for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                    for (int half = 0; half < C::kHalves; ++half) {
+                        const int r = mt * 16 + half * 8 + lane / 4;
+                        if ((lane & 3) == 0) {
+                            st[r] = m[mt][half];
+                            st[kAll + r] = l[mt][half];
+                        }
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n)
+                            *reinterpret_cast<float2*>(dst + r * D + ((n ^ (r & 7)) * 8) + (lane & 3) * 2) =
+                                make_float2(o[mt][n][half * 2], o[mt][n][half * 2 + 1]);
+                    }
+            }
+            __syncthreads();
+            if (warp < round) {
+                const float* src = reinterpret_cast<const float*>(few_smem + C::kJoinOff + warp * C::kJoin);
+                const float* st = stat + warp * 2 * kAll;
+#pragma unroll
+                for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                    for (int half = 0; half < C::kHalves; ++half) {
+                        const int r = mt * 16 + half * 8 + lane / 4;
+                        const float mo = st[r], top = fmaxf(m[mt][half], mo);
+                        const float f = m[mt][half] == -INFINITY ? 0.f : ex2_approx(m[mt][half] - top);
+                        const float g = mo == -INFINITY ? 0.f : ex2_approx(mo - top);
+                        m[mt][half] = top;
+                        l[mt][half] = l[mt][half] * f + st[kAll + r] * g;
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n) {
+                            const float2 x = *reinterpret_cast<const float2*>(src + r * D + ((n ^ (r & 7)) * 8) +
+                                                                              (lane & 3) * 2);
+                            o[mt][n][half * 2] = o[mt][n][half * 2] * f + x.x * g;
+                            o[mt][n][half * 2 + 1] = o[mt][n][half * 2 + 1] * f + x.y * g;
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+
+        // ---- the item's result, or this CTA's part of it --------------------
+        const bool whole = begun && item_done;
+        float* part = a.partials + static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * ROWS * (D + 2);
+        if (warp == 0) {
+#pragma unroll
+            for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                for (int half = 0; half < C::kHalves; ++half) {
+                    const int r = mt * 16 + half * 8 + lane / 4, i = r / a.group;
+                    if (i >= now.tile.tokens) continue;
+                    if (whole) {
+                        const float inv = l[mt][half] > 0.f || isnan(l[mt][half]) ? 1.0f / l[mt][half] : 0.f;
+                        const int head = now.h * a.group + r - i * a.group;
+                        T* out = static_cast<T*>(a.out) + (now.tile.first + i) * a.out_stride + head * D + (lane & 3) * 2;
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n)
+                            *reinterpret_cast<uint32_t*>(out + n * 8) =
+                                Pair<T>::pack(o[mt][n][half * 2] * inv, o[mt][n][half * 2 + 1] * inv);
+                        if (a.lse != nullptr && (lane & 3) == 0)
+                            a.lse[static_cast<long long>(now.tile.first + i) * a.heads + head] =
+                                l[mt][half] == 0.f
+                                    ? -INFINITY
+                                    : (m[mt][half] - kFewOffset) * 0.6931471805599453f + logf(l[mt][half]);
+                    } else {
+                        if ((lane & 3) == 0) {
+                            __stcg(part + ROWS * D + 2 * r, m[mt][half]);
+                            __stcg(part + ROWS * D + 2 * r + 1, l[mt][half]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n)
+                            __stcg(reinterpret_cast<float2*>(part + r * D + n * 8 + (lane & 3) * 2),
+                                   make_float2(o[mt][n][half * 2], o[mt][n][half * 2 + 1]));
+                    }
+                }
+        }
+        if (!whole) {
+            // the CTAs that hold this item: from its first unit's to its last's
+            const long long at = range.end - now.left;  // this unit
+            const long long first = at - now.unit, last = first + now.tile.units() - 1;
+            const int c0 = range_owner(range.total, first, range.ctas), c1 = range_owner(range.total, last, range.ctas);
+            int* flag = reinterpret_cast<int*>(few_smem + C::kStatOff);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const unsigned seen = atom_acq_rel_add(a.counters + c0, 1u);
+                *flag = seen == static_cast<unsigned>(c1 - c0);
+                if (*flag) a.counters[c0] = 0u;  // zero for the next call
+            }
+            __syncthreads();
+            if (*flag) {
+                __threadfence();
+                const int rows = now.tile.tokens * a.group;
+                for (int x = threadIdx.x; x < rows * (D / 4); x += kFewThreads) {
+                    const int r = x / (D / 4), c = x % (D / 4), i = r / a.group;
+                    float top = -INFINITY;
+                    for (int cta = c0; cta <= c1; ++cta)
+                        top = fmaxf(top, __ldcg(a.partials + static_cast<long long>(2 * cta + (cta == c0)) * ROWS * (D + 2) +
+                                                ROWS * D + 2 * r));
+                    float sum = 0.f;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int cta = c0; cta <= c1; ++cta) {
+                        const float* q = a.partials + static_cast<long long>(2 * cta + (cta == c0)) * ROWS * (D + 2);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + ROWS * D + 2 * r));
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(q + r * D) + c);
+                        const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+                        sum += ml.y * f;
+                        v.x += y.x * f, v.y += y.y * f, v.z += y.z * f, v.w += y.w * f;
+                    }
+                    const float inv = sum > 0.f || isnan(sum) ? 1.0f / sum : 0.f;
+                    const int head = now.h * a.group + r - i * a.group;
+                    T* out = static_cast<T*>(a.out) + (now.tile.first + i) * a.out_stride + head * D;
+                    *(reinterpret_cast<uint2*>(out) + c) =
+                        make_uint2(Pair<T>::pack(v.x * inv, v.y * inv), Pair<T>::pack(v.z * inv, v.w * inv));
+                    if (a.lse != nullptr && c == 0)
+                        a.lse[static_cast<long long>(now.tile.first + i) * a.heads + head] =
+                            sum == 0.f ? -INFINITY : (top - kFewOffset) * 0.6931471805599453f + logf(sum);
+                }
+            }
+            __syncthreads();
+        }
+        if (!now.next(a, tile_tokens)) break;
+        begun = true;
+        fresh = true;
+    }
+    async_copy_wait_all();
+}
+
+// ---- host side -----------------------------------------------------------------
+
+static bool paged_view(const h4b_paged_kv* kv, PagedView* out) {
+    if (kv == nullptr || kv->pages < 1 || kv->kv_heads < 1 || kv->sequences < 0 || kv->table_stride < 0 || kv->tokens < 0)
+        return false;
+    if (kv->page_size < 16 || kv->page_size > 1024 || (kv->page_size & (kv->page_size - 1))) return false;
+    if (kv->k_pages == nullptr || kv->v_pages == nullptr ||
+        ((reinterpret_cast<uintptr_t>(kv->k_pages) | reinterpret_cast<uintptr_t>(kv->v_pages)) & 15))
+        return false;
+    if (kv->sequences > 0 && (kv->q_offsets == nullptr || kv->kv_lens == nullptr ||
+                              (kv->page_table == nullptr && kv->table_stride > 0)))
+        return false;
+    int shift = 0;
+    while ((1 << shift) < kv->page_size) ++shift;
+    *out = PagedView{kv->pages, shift, kv->kv_heads, kv->sequences, kv->table_stride, kv->tokens, kv->page_table,
+                     kv->q_offsets, kv->kv_lens};
+    return true;
+}
+
+static bool paged_shape_supported(const h4b_paged_kv* kv) {
+    return (kv->dtype == H4B_FP16 || kv->dtype == H4B_BF16) && (kv->head_dim == 64 || kv->head_dim == 128);
+}
+
+static int paged_sm_count(int* sms) {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0;
+    H4B_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= kMaxDevices) return H4B_EUNSUPPORTED;
+    int n = known[dev].load(std::memory_order_acquire);
+    if (n == 0) {
+        H4B_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        known[dev].store(n, std::memory_order_release);
+    }
+    *sms = n;
+    return 0;
+}
+
+// Largest row tile (rows an item holds) of any attention kernel, and CTAs of
+// the few-row kernel an SM: they size the workspace.
+constexpr int kFewCtasPerSm = 2, kFewMaxRows = 32;
+constexpr long long kCounterBytes = 4096;
+
+template <typename S, typename T, int D>
+static int launch_append(const AppendArgs& a, cudaStream_t stream) {
+    // Few tokens: the heads of a token are spread over several CTAs, so that
+    // the chip is full; many: one CTA walks all heads of its token.
+    const int per_cta = kAppendWarps * (128 / D), total = a.heads + 2 * a.p.kv_heads;
+    const int most = (total + per_cta - 1) / per_cta;
+    const int y = a.p.tokens >= 1024 ? 1 : most;
+    paged_append_kernel<S, T, D><<<dim3(a.p.tokens, y), 32 * kAppendWarps, 0, stream>>>(a);
+    H4B_CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
+template <typename T, int D, int ROWS>
+static int launch_few(const AttendArgs& a, int sms, cudaStream_t stream) {
+    using C = FewCfg<D, ROWS>;
+    static std::atomic<bool> opted_in[kMaxDevices];
+    int dev = 0;
+    H4B_CUDA_TRY(cudaGetDevice(&dev));
+    if (!opted_in[dev].load(std::memory_order_acquire)) {
+        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_few_kernel<T, D, ROWS>,
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        opted_in[dev].store(true, std::memory_order_release);
+    }
+    paged_attention_few_kernel<T, D, ROWS><<<kFewCtasPerSm * sms, kFewThreads, C::kSmem, stream>>>(a);
+    H4B_CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
+template <typename T, int D>
+static int launch_attention(const AttendArgs& a, int max_query, int sms, cudaStream_t stream) {
+    const long long rows = static_cast<long long>(max_query) * a.group;
+    if (rows <= 8) return launch_few<T, D, 8>(a, sms, stream);
+    if (rows <= 16) return launch_few<T, D, 16>(a, sms, stream);
+    return launch_few<T, D, 32>(a, sms, stream);
+}
+
+}  // namespace h4b
+
+extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv_dtype, long long qkv_stride, int heads,
+                                const float* norm_q, const float* norm_k, float eps, const float* rope_cos,
+                                const float* rope_sin, int max_pos, void* q_out, long long q_stride, void* stream) {
+    using namespace h4b;
+    AppendArgs a{};
+    if (!paged_view(kv, &a.p) || heads < 0 || qkv == nullptr || (heads > 0 && q_out == nullptr)) return H4B_EINVAL;
+    if (!paged_shape_supported(kv) || (qkv_dtype != H4B_FP32 && qkv_dtype != kv->dtype)) return H4B_EUNSUPPORTED;
+    if ((norm_q == nullptr) != (norm_k == nullptr) || (rope_cos == nullptr) != (rope_sin == nullptr) ||
+        (rope_cos != nullptr && max_pos < 1))
+        return H4B_EINVAL;
+    if (qkv_stride < static_cast<long long>(heads + 2 * kv->kv_heads) * kv->head_dim || (qkv_stride & 1) ||
+        (heads > 0 && (q_stride < static_cast<long long>(heads) * kv->head_dim || (q_stride & 1))))
+        return H4B_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin) |
+         reinterpret_cast<uintptr_t>(norm_q) | reinterpret_cast<uintptr_t>(norm_k)) & 7 ||
+        (reinterpret_cast<uintptr_t>(q_out) & 3))
+        return H4B_EINVAL;
+    if (kv->tokens == 0 || kv->sequences == 0) return 0;
+    a.qkv = qkv, a.qkv_stride = qkv_stride, a.norm_q = norm_q, a.norm_k = norm_k, a.cos = rope_cos, a.sin = rope_sin;
+    a.max_pos = max_pos, a.heads = heads, a.eps = eps, a.q_out = q_out, a.q_stride = q_stride;
+    a.k_pages = kv->k_pages, a.v_pages = kv->v_pages;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool wide = kv->head_dim == 128, from32 = qkv_dtype == H4B_FP32;
+    if (kv->dtype == H4B_FP16) {
+        if (from32) return wide ? launch_append<float, __half, 128>(a, s) : launch_append<float, __half, 64>(a, s);
+        return wide ? launch_append<__half, __half, 128>(a, s) : launch_append<__half, __half, 64>(a, s);
+    }
+    if (from32)
+        return wide ? launch_append<float, __nv_bfloat16, 128>(a, s) : launch_append<float, __nv_bfloat16, 64>(a, s);
+    return wide ? launch_append<__nv_bfloat16, __nv_bfloat16, 128>(a, s)
+                : launch_append<__nv_bfloat16, __nv_bfloat16, 64>(a, s);
+}
+
+extern "C" int h4b_pages_copy(void* k_pages, void* v_pages, int layers, int pages, long long page_bytes,
+                              const int32_t* src, const int32_t* dst, int count, void* stream) {
+    using namespace h4b;
+    if (k_pages == nullptr || v_pages == nullptr || layers < 1 || layers > 65535 || pages < 1 || page_bytes < 16 ||
+        (page_bytes & 15) || count < 0 || (count > 0 && (src == nullptr || dst == nullptr)) ||
+        ((reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages)) & 15))
+        return H4B_EINVAL;
+    if (count == 0) return 0;
+    const long long parts = (page_bytes + kCopyBytes - 1) / kCopyBytes;
+    if (parts * count > 0x7fffffffll) return H4B_EUNSUPPORTED;
+    pages_copy_kernel<<<dim3(static_cast<unsigned>(parts * count), layers, 2), kCopyThreads, 0,
+                        static_cast<cudaStream_t>(stream)>>>(static_cast<uint8_t*>(k_pages),
+                                                             static_cast<uint8_t*>(v_pages), pages, page_bytes,
+                                                             static_cast<int>(parts), src, dst);
+    H4B_CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
+extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
+    using namespace h4b;
+    int sms = 0;
+    if (head_dim != 64 && head_dim != 128) return H4B_EUNSUPPORTED;
+    if (const int rc = paged_sm_count(&sms)) return rc > 0 ? -1000 - rc : rc;
+    const long long few = 2ll * kFewCtasPerSm * sms * kFewMaxRows * (head_dim + 2) * 4;
+    return kCounterBytes + few;
+}
+
+extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long long q_stride, int heads, float scale,
+                                   int window, int sinks, int max_query, void* out, long long out_stride, float* lse,
+                                   void* workspace, long long workspace_bytes, void* stream) {
+    using namespace h4b;
+    AttendArgs a{};
+    if (!paged_view(kv, &a.p) || heads < 1 || heads % kv->kv_heads || q == nullptr || out == nullptr || window < 0 ||
+        sinks < 0 || (sinks > 0 && window == 0) || max_query < 1 || workspace == nullptr)
+        return H4B_EINVAL;
+    if (!paged_shape_supported(kv) || heads / kv->kv_heads > kFewMaxRows) return H4B_EUNSUPPORTED;
+    const long long width = static_cast<long long>(heads) * kv->head_dim;
+    if (q_stride < width || out_stride < width || ((q_stride | out_stride) & 7) ||
+        ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) &
+         15))
+        return H4B_EINVAL;
+    if (kv->tokens == 0 || kv->sequences == 0) return 0;
+    const long long need = h4b_paged_attention_workspace_bytes(kv->head_dim);
+    if (need < 0 || workspace_bytes < need) return H4B_EINVAL;
+    int sms = 0;
+    if (const int rc = paged_sm_count(&sms)) return rc;
+    a.q = q, a.k_pages = kv->k_pages, a.v_pages = kv->v_pages, a.out = out, a.lse = lse;
+    a.q_stride = q_stride, a.out_stride = out_stride, a.heads = heads, a.group = heads / kv->kv_heads;
+    a.window = window < (1 << 30) ? window : 1 << 30, a.sinks = sinks, a.scale = scale * 1.4426950408889634f;
+    a.counters = static_cast<unsigned int*>(workspace);
+    a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+    const int longest = max_query < kv->tokens ? max_query : kv->tokens;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool wide = kv->head_dim == 128;
+    if (kv->dtype == H4B_FP16)
+        return wide ? launch_attention<__half, 128>(a, longest, sms, s) : launch_attention<__half, 64>(a, longest, sms, s);
+    return wide ? launch_attention<__nv_bfloat16, 128>(a, longest, sms, s)
+                : launch_attention<__nv_bfloat16, 64>(a, longest, sms, s);
+}

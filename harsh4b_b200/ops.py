@@ -6,9 +6,12 @@ must already be CUDA tensors; nothing here copies to or from the host.
 """
 from __future__ import annotations
 
+import ctypes
+from functools import lru_cache
+
 import torch
 
-from ._lib import check, lib, stream_handle
+from ._lib import PagedKvDesc, check, lib, stream_handle
 
 
 def _dev(tensor: torch.Tensor, dtype: torch.dtype, name: str) -> int:
@@ -225,3 +228,148 @@ def residual_acc(x: torch.Tensor, acc: torch.Tensor, absmax: torch.Tensor, scale
                                  _dev(absmax, torch.float32, "absmax"), _dev(scales, torch.float32, "scales"),
                                  x.numel(), stream_handle()), "h4b_residual_acc")
     return x
+
+
+# ---- paged K/V cache -------------------------------------------------------------
+_PAGED_DTYPES = {torch.float16: 1, torch.bfloat16: 2}  # H4B_FP16, H4B_BF16
+
+
+def _rows(tensor: torch.Tensor, dtype: torch.dtype, name: str) -> int:
+    """Data pointer of a CUDA tensor whose rows (dim 0) may be strided."""
+    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if tensor.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {tensor.dtype}")
+    if not tensor.is_contiguous() and tensor.numel() and not tensor[0].is_contiguous():
+        raise ValueError(f"{name} must be contiguous within each row")
+    return tensor.data_ptr()
+
+
+def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> PagedKvDesc:
+    """The h4b_paged_kv of one layer's pages and a batch's tables."""
+    code = _PAGED_DTYPES.get(k_pages.dtype)
+    if code is None:
+        raise ValueError(f"k_pages must be float16 or bfloat16, got {k_pages.dtype}")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be [pages][kv_heads][page_size][head_dim]")
+    pages, kv_heads, page_size, head_dim = k_pages.shape
+    if page_table.dim() != 2 or page_table.shape[0] != kv_lens.numel() or q_offsets.numel() != kv_lens.numel() + 1:
+        raise ValueError("page_table must be [sequences][pages each], q_offsets [sequences + 1], kv_lens [sequences]")
+    return PagedKvDesc(_dev(k_pages, k_pages.dtype, "k_pages"), _dev(v_pages, k_pages.dtype, "v_pages"),
+                       _dev(page_table, torch.int32, "page_table"), _dev(q_offsets, torch.int32, "q_offsets"),
+                       _dev(kv_lens, torch.int32, "kv_lens"), code, pages, page_size, kv_heads, head_dim,
+                       page_table.shape[0], page_table.shape[1], tokens)
+
+
+def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 q_offsets: torch.Tensor, kv_lens: torch.Tensor, *, heads: int, norm_q: torch.Tensor | None = None,
+                 norm_k: torch.Tensor | None = None, eps: float = 1e-6, rope_cos: torch.Tensor | None = None,
+                 rope_sin: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """h4b_paged_append: the new tokens' k and v into one layer's pages, their
+    q heads back. `qkv` holds `heads` q heads, the k heads and the v heads of
+    every new token ([tokens][(heads + 2 kv_heads) * head_dim], fp32 or the
+    cache's type, rows may be strided); q and k are RMS-normalised with
+    `norm_q` / `norm_k` and rotated with `rope_cos` / `rope_sin` where given.
+    Returns q [tokens][heads][head_dim] in the cache's type."""
+    tokens = qkv.shape[0]
+    kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
+    if qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv.kv_heads) * kv.head_dim:
+        raise ValueError("qkv must be [tokens][(heads + 2 kv_heads) * head_dim]")
+    if qkv.dtype not in (torch.float32, k_pages.dtype):
+        raise ValueError(f"qkv must be float32 or {k_pages.dtype}, got {qkv.dtype}")
+    if out is None:
+        out = torch.empty(tokens, heads, kv.head_dim, dtype=k_pages.dtype, device=qkv.device)
+    elif tuple(out.shape) != (tokens, heads, kv.head_dim):
+        raise ValueError("out must be [tokens][heads][head_dim]")
+    for name, norm in (("norm_q", norm_q), ("norm_k", norm_k)):
+        if norm is not None and norm.numel() != kv.head_dim:
+            raise ValueError(f"{name} must hold head_dim values")
+    if rope_cos is not None and (rope_sin is None or rope_cos.shape != rope_sin.shape
+                                 or rope_cos.shape[-1] != kv.head_dim // 2):
+        raise ValueError("rope_cos and rope_sin must be [positions][head_dim / 2]")
+
+    def vector(tensor, name):
+        return None if tensor is None else _dev(tensor, torch.float32, name)
+
+    check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, qkv.dtype, "qkv"),
+                                 0 if qkv.dtype == torch.float32 else kv.dtype, qkv.stride(0) if tokens > 1 else qkv.shape[1],
+                                 heads, vector(norm_q, "norm_q"), vector(norm_k, "norm_k"), float(eps),
+                                 vector(rope_cos, "rope_cos"), vector(rope_sin, "rope_sin"),
+                                 0 if rope_cos is None else rope_cos.shape[0], _rows(out, k_pages.dtype, "out"),
+                                 out.stride(0) if tokens > 1 else heads * kv.head_dim, stream_handle()),
+          "h4b_paged_append")
+    return out
+
+
+@lru_cache(None)
+def _paged_workspace_bytes(head_dim: int, device: int) -> int:
+    with torch.cuda.device(device):
+        nbytes = int(lib().h4b_paged_attention_workspace_bytes(head_dim))
+    if nbytes < 0:
+        check(nbytes, "h4b_paged_attention_workspace_bytes")
+    return nbytes
+
+
+def paged_workspace(head_dim: int = 128, device=None) -> torch.Tensor:
+    """A workspace for paged_attention calls that follow each other (one
+    stream): zeroed once, every call leaves it ready for the next."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch.zeros(_paged_workspace_bytes(head_dim, index), dtype=torch.uint8, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    q_offsets: torch.Tensor, kv_lens: torch.Tensor, *, max_query: int | None = None, window: int = 0,
+                    sinks: int = 0, scale: float | None = None, out: torch.Tensor | None = None,
+                    lse: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """h4b_paged_attention: causal attention of a ragged batch's new tokens
+    (q [tokens][heads][head_dim], rows may be strided; sequence b's are rows
+    q_offsets[b] .. q_offsets[b + 1] - 1) over their sequences' pages, which
+    hold the new tokens already (paged_append). `window` > 0: a token sees the
+    last `window` keys (itself among them) and the first `sinks`. `max_query`
+    is the longest chunk to expect (it picks the kernel; by default 1 when
+    there are no more rows than sequences, else all rows). `lse`, if given,
+    receives the float32 [tokens][heads] log-sum-exp. `workspace`: from
+    paged_workspace, kept between calls (one is made per call otherwise)."""
+    if q.dim() != 3:
+        raise ValueError("q must be [tokens][heads][head_dim]")
+    tokens, heads, head_dim = q.shape
+    kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
+    if head_dim != kv.head_dim or heads % kv.kv_heads:
+        raise ValueError("q must have the cache's head_dim and a multiple of its kv heads")
+    if out is None:
+        out = torch.empty(tokens, heads, head_dim, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    if lse is not None and tuple(lse.shape) != (tokens, heads):
+        raise ValueError("lse must be [tokens][heads]")
+    if max_query is None:
+        max_query = 1 if tokens <= kv.sequences else tokens
+    if workspace is None:
+        workspace = paged_workspace(head_dim, q.device)
+    width = heads * head_dim
+    check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, k_pages.dtype, "q"), q.stride(0) if tokens > 1 else width,
+                                    heads, head_dim ** -0.5 if scale is None else float(scale), int(window),
+                                    int(sinks), int(max_query), _rows(out, k_pages.dtype, "out"),
+                                    out.stride(0) if tokens > 1 else width,
+                                    None if lse is None else _dev(lse, torch.float32, "lse"),
+                                    _dev(workspace, torch.uint8, "workspace"), workspace.numel(), stream_handle()),
+          "h4b_paged_attention")
+    return out
+
+
+def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """h4b_pages_copy: page src[i] to page dst[i] in every layer of
+    [layers][pages][kv_heads][page_size][head_dim] (or one layer's [pages]...)
+    caches of any type; int32 ids on the device. No page may be the
+    destination of two moves, nor a source and a destination."""
+    if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
+        raise ValueError("k_pages and v_pages must be [layers][pages][kv_heads][page_size][head_dim]")
+    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
+    pages, kv_heads, page_size, head_dim = k_pages.shape[-4:]
+    if src.numel() != dst.numel():
+        raise ValueError("src and dst must hold as many page ids")
+    check(lib().h4b_pages_copy(_dev(k_pages, k_pages.dtype, "k_pages"), _dev(v_pages, k_pages.dtype, "v_pages"), layers,
+                               pages, kv_heads * page_size * head_dim * k_pages.element_size(),
+                               _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst"), src.numel(),
+                               stream_handle()), "h4b_pages_copy")

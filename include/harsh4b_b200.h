@@ -30,7 +30,8 @@ extern "C" {
 #define H4B_ETOOBIG (-3)      /* request exceeds the library's static scratch */
 
 /* Device-side status word (bit 1: a bounded wait gave up; bit 2: token id
- * out of range; bit 4: position beyond capacity). Reads and clears it; the
+ * out of range; bit 4: position beyond capacity; bit 8: page id, row offset
+ * or length of a paged batch out of range). Reads and clears it; the
  * read synchronises with the device. */
 int h4b_get_status(int *host_status);
 
@@ -441,6 +442,75 @@ int h4b_prefill_attention(const h4b_model *model, const h4b_state *state, const 
 int h4b_prefill_tp_stage(const h4b_model *model, const h4b_state *state, const h4b_prefill_scratch *scratch,
                          int count, int layer, int stage, const uint8_t *table, const float *table_scales,
                          int table_vocab, float *absmax, int32_t *acc, void *stream);
+
+/* ---- paged K/V cache ---------------------------------------------------------
+ * No counterpart in the reference, whose sessions hold one contiguous cache
+ * each (cpu_lightspark.py:275-309). One layer's cache is two buffers
+ * [pages][kv_heads][page_size][head_dim] in fp16 or bf16; sequence b's token
+ * j lives in page page_table[b * table_stride + j / page_size], slot
+ * j % page_size. A batch feeds sequence b the rows q_offsets[b] ..
+ * q_offsets[b + 1] - 1 (none, one, or a chunk of any length) of `tokens`
+ * rows; kv_lens[b] counts the sequence's tokens with them, so its new token i
+ * stands at position kv_lens[b] - (its new tokens) + i. The tables are device
+ * memory and read on the device: a captured graph follows their contents.
+ *
+ * page_size is a power of two in 16..1024, head_dim 64 or 128, buffers
+ * 16-byte aligned. Page ids of places that no call reads may be anything
+ * (-1 for freed pages). A page id that is needed and out of range reads as
+ * zeros and is not written, a sequence with an offset or a length out of
+ * range counts as empty, and both set status bit 8. */
+#define H4B_FP32 0
+#define H4B_FP16 1
+#define H4B_BF16 2
+typedef struct h4b_paged_kv {
+    void *k_pages, *v_pages;      /* this layer's */
+    const int32_t *page_table;    /* [sequences][table_stride] */
+    const int32_t *q_offsets;     /* [sequences + 1], ascending from 0 to tokens */
+    const int32_t *kv_lens;       /* [sequences] */
+    int dtype;                    /* of the cache: H4B_FP16 or H4B_BF16 */
+    int pages, page_size, kv_heads, head_dim;
+    int sequences, table_stride, tokens;
+} h4b_paged_kv;
+
+/* Writes the new tokens into the pages: row t of qkv (qkv_stride values
+ * apart, H4B_FP32 or the cache's type) holds `heads` q heads, then kv_heads
+ * k heads, then kv_heads v heads. q and k heads are RMS-normalised with
+ * norm_q / norm_k (float[head_dim]; both null: not normalised) and rotated by
+ * the rows of rope_cos / rope_sin ([max_pos][head_dim / 2] as in h4b_model;
+ * both null: not rotated) at the token's position; q goes to q_out (rows
+ * q_stride values apart, in the cache's type), k and v into the pages. A
+ * position past max_pos sets status bit 4 and is not rotated. heads may be 0
+ * (then q_out is not used). */
+int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, long long qkv_stride, int heads,
+                     const float *norm_q, const float *norm_k, float eps, const float *rope_cos,
+                     const float *rope_sin, int max_pos, void *q_out, long long q_stride, void *stream);
+
+/* Causal attention of the batch's new tokens over their sequences' pages
+ * (the new tokens' own k and v are in the pages already). q and out: rows of
+ * heads * head_dim values of the cache's type, q_stride / out_stride values
+ * apart (multiples of 8); q head h reads kv head h / (heads / kv_heads), at
+ * most 32 heads to a kv head. A token at position p sees the keys j <= p; with
+ * window > 0 only j > p - window or j < sinks. lse (may be null): float
+ * [tokens][heads], the natural logarithm of each row's sum of exp(scale q.k).
+ * A row that sees no key gets zeros and lse -inf. max_query is the longest
+ * chunk that the caller expects: it picks the kernel, and a longer chunk is
+ * computed as well, only slower. workspace: zeroed when it is created, left
+ * ready for the next call; h4b_paged_attention_workspace_bytes bytes. Calls
+ * that may overlap on the GPU need workspaces of their own. */
+int h4b_paged_attention(const h4b_paged_kv *kv, const void *q, long long q_stride, int heads, float scale, int window,
+                        int sinks, int max_query, void *out, long long out_stride, float *lse, void *workspace,
+                        long long workspace_bytes, void *stream);
+/* Workspace bytes of h4b_paged_attention on the current device, for any batch
+ * of that head_dim. */
+long long h4b_paged_attention_workspace_bytes(int head_dim);
+
+/* Copies page src[i] to page dst[i], i < count, in every layer's K and V
+ * (k_pages and v_pages: [layers][pages][page_bytes]; src and dst device
+ * memory). No page may be the destination of two moves, nor a source and a
+ * destination. A move with an id out of range is skipped and sets status bit
+ * 8. */
+int h4b_pages_copy(void *k_pages, void *v_pages, int layers, int pages, long long page_bytes, const int32_t *src,
+                   const int32_t *dst, int count, void *stream);
 
 /* ---- format producer: LATTICE checkpoint -> packed int4 cache ------------- */
 
