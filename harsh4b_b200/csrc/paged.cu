@@ -24,6 +24,7 @@ template <typename T>
 struct Pair;  // two 16-bit values of a 32-bit word
 template <>
 struct Pair<__half> {
+    static constexpr bool kBf16 = false;
     __device__ static uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -32,6 +33,7 @@ struct Pair<__half> {
 };
 template <>
 struct Pair<__nv_bfloat16> {
+    static constexpr bool kBf16 = true;
     __device__ static uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -49,25 +51,31 @@ struct PagedView {
     const int32_t* kv_lens;
 };
 
-// Rows and lengths of one sequence, made safe: first row, new tokens and
-// position of the first one.
-struct SequenceSpan {
-    int first, count, base;
+// Rows and lengths of one sequence: as the tables have them (a load whose
+// values nothing waits for yet), and made safe.
+struct RawSpan {
+    int first, end, len;
 };
-__device__ __forceinline__ SequenceSpan sequence_span(const PagedView& p, int b) {
-    SequenceSpan s{p.q_offsets[b], 0, 0};
-    const int end = p.q_offsets[b + 1], len = p.kv_lens[b];
-    const bool good = s.first >= 0 && end >= s.first && end <= p.tokens && len >= 0 &&
-                      len <= static_cast<long long>(p.table_stride) << p.page_shift;
+__device__ __forceinline__ RawSpan raw_span(const PagedView& p, int b) {
+    return RawSpan{p.q_offsets[b], p.q_offsets[b + 1], p.kv_lens[b]};
+}
+constexpr int kMaxLength = 1 << 30;  // keeps position - window in 32 bits
+struct SequenceSpan {
+    int first, count, base;  // first row, new tokens, position of the first one
+};
+__device__ __forceinline__ SequenceSpan checked_span(const PagedView& p, const RawSpan& r) {
+    const bool good = r.first >= 0 && r.end >= r.first && r.end <= p.tokens && r.len >= 0 &&
+                      r.len <= kMaxLength && r.len <= static_cast<long long>(p.table_stride) << p.page_shift;
     if (!good) {
         report(kStatusBadPage);
         // its rows, as far as they exist, still get an (empty) answer
-        const long long lo = min(max(s.first, 0), p.tokens), hi = min(max(end, 0), p.tokens);
-        return SequenceSpan{static_cast<int>(lo), static_cast<int>(max(hi - lo, 0ll)), -(1 << 30)};
+        const int lo = min(max(r.first, 0), p.tokens), hi = min(max(r.end, 0), p.tokens);
+        return SequenceSpan{lo, max(hi - lo, 0), -kMaxLength};
     }
-    s.count = end - s.first;
-    s.base = len - s.count;
-    return s;
+    return SequenceSpan{r.first, r.end - r.first, r.len - (r.end - r.first)};
+}
+__device__ __forceinline__ SequenceSpan sequence_span(const PagedView& p, int b) {
+    return checked_span(p, raw_span(p, b));
 }
 
 // ---- append ---------------------------------------------------------------
@@ -257,11 +265,26 @@ __device__ __forceinline__ Tile make_tile(const SequenceSpan& s, int t, int tile
     return x;
 }
 
-// Units of all tiles of a sequence, one kv head.
+// Units of one kv head of every lane's sequence. The whole warp takes part: a
+// lane sums a few tiles by itself, a long chunk's are summed by all lanes.
 template <int KEYS>
-__device__ __forceinline__ long long sequence_units(const SequenceSpan& s, int tile_tokens, int window, int sinks) {
+__device__ __forceinline__ long long warp_units(const SequenceSpan& s, int tile_tokens, int window, int sinks) {
+    const int lane = threadIdx.x & 31;
     long long n = 0;
-    for (int t = 0; t * tile_tokens < s.count; ++t) n += make_tile<KEYS>(s, t, tile_tokens, window, sinks).units();
+    const bool is_long = s.count > 4 * tile_tokens;
+    if (!is_long)
+        for (int t = 0; t * tile_tokens < s.count; ++t) n += make_tile<KEYS>(s, t, tile_tokens, window, sinks).units();
+    for (unsigned todo = __ballot_sync(0xffffffffu, is_long); todo; todo &= todo - 1) {
+        const int who = __ffs(todo) - 1;
+        const SequenceSpan x{__shfl_sync(0xffffffffu, s.first, who), __shfl_sync(0xffffffffu, s.count, who),
+                             __shfl_sync(0xffffffffu, s.base, who)};
+        long long sum = 0;
+        for (int t = lane; static_cast<long long>(t) * tile_tokens < x.count; t += 32)
+            sum += make_tile<KEYS>(x, t, tile_tokens, window, sinks).units();
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == who) n = sum;
+    }
     return n;
 }
 
@@ -278,20 +301,23 @@ __device__ __forceinline__ int range_owner(long long total, long long unit, int 
     return static_cast<int>(((unit + 1) * ctas - 1) / total);
 }
 
-// Every thread of the CTA takes part; `shared` holds THREADS / 32 + 1 long
-// longs and a Range. Each thread sums its share of the sequences, a prefix
-// sum over the threads follows, and the thread whose sequences hold unit
-// `begin` finds it.
+// Every thread of the CTA takes part; `shared` holds THREADS / 32 long longs
+// and a Range. Each thread has a share of the sequences, a prefix sum over
+// the threads follows, and the thread whose sequences hold unit `begin`
+// finds it.
 template <int THREADS, int KEYS>
 __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens, void* shared) {
     long long* warp_sums = static_cast<long long*>(shared);
-    Range* found = reinterpret_cast<Range*>(warp_sums + THREADS / 32 + 1);
+    Range* found = reinterpret_cast<Range*>(warp_sums + THREADS / 32);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int each = (a.p.sequences + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
-    const int b1 = min(b0 + each, a.p.sequences);
+    auto units_of = [&](int e) {  // of the thread's e-th sequence, all kv heads
+        SequenceSpan s{0, 0, 0};
+        if (b0 + e < a.p.sequences) s = sequence_span(a.p, b0 + e);
+        return a.p.kv_heads * warp_units<KEYS>(s, tile_tokens, a.window, a.sinks);
+    };
     long long mine = 0;
-    for (int b = b0; b < b1; ++b)
-        mine += a.p.kv_heads * sequence_units<KEYS>(sequence_span(a.p, b), tile_tokens, a.window, a.sinks);
+    for (int e = 0; e < each; ++e) mine += units_of(e);
     long long before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -314,19 +340,19 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
         r.begin = range_begin(total, blockIdx.x, r.ctas);
         r.end = range_begin(total, blockIdx.x + 1, r.ctas);
     }
-    if (r.begin < r.end && r.begin >= before && r.begin < before + mine) {
+    const bool here = r.begin < r.end && r.begin >= before && r.begin < before + mine;
+    if (__any_sync(0xffffffffu, here)) {
         long long at = before;
-        for (int b = b0;; ++b) {
-            const long long n =
-                a.p.kv_heads * sequence_units<KEYS>(sequence_span(a.p, b), tile_tokens, a.window, a.sinks);
-            if (r.begin < at + n) {
-                r.sequence = b;
-                r.skip = r.begin - at;
-                break;
+        bool open = here;
+        for (int e = 0; e < each; ++e) {
+            const long long n = each == 1 ? mine : units_of(e);
+            if (open && r.begin < at + n) {
+                found->sequence = b0 + e;
+                found->skip = r.begin - at;
+                open = false;
             }
             at += n;
         }
-        *found = r;
     }
     __syncthreads();
     if (r.begin < r.end) {
@@ -340,21 +366,43 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
 template <int KEYS>
 struct Walk {
     SequenceSpan span;
+    RawSpan following;        // of sequence b + 1, requested when b was entered
     Tile tile;
     int b, t, h, unit;        // unit within the item
     long long left;           // units of the range from here on
 
+    __device__ __forceinline__ void request(const AttendArgs& a) {
+        if (b + 1 < a.p.sequences) following = raw_span(a.p, b + 1);
+    }
+    // By whole warps: the lanes look for the tile together, 32 at a time.
     __device__ __forceinline__ void start(const AttendArgs& a, const Range& r, int tile_tokens) {
+        const int lane = threadIdx.x & 31;
         b = r.sequence;
         left = r.end - r.begin;
         span = sequence_span(a.p, b);
+        request(a);
         long long skip = r.skip;
-        for (t = 0;; ++t) {
-            tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
-            const long long n = static_cast<long long>(tile.units()) * a.p.kv_heads;
-            if (skip < n) break;
-            skip -= n;
+        for (int t0 = 0;; t0 += 32) {
+            long long n = 0;
+            if (static_cast<long long>(t0 + lane) * tile_tokens < span.count)
+                n = make_tile<KEYS>(span, t0 + lane, tile_tokens, a.window, a.sinks).units() *
+                    static_cast<long long>(a.p.kv_heads);
+            long long upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += up;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, skip < upto);
+            if (past) {
+                const int who = __ffs(past) - 1;
+                t = t0 + who;
+                skip -= __shfl_sync(0xffffffffu, upto - n, who);
+                break;
+            }
+            skip -= __shfl_sync(0xffffffffu, upto, 31);
         }
+        tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
         h = static_cast<int>(skip / tile.units());
         unit = static_cast<int>(skip % tile.units());
     }
@@ -366,7 +414,9 @@ struct Walk {
         ++t;
         while (t * tile_tokens >= span.count) {
             t = 0;
-            span = sequence_span(a.p, ++b);
+            ++b;
+            span = checked_span(a.p, following);
+            request(a);
         }
         tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
     }
@@ -810,6 +860,12 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     async_copy_wait_all();
 }
 
+}  // namespace h4b
+
+#include "paged_tc.cu"
+
+namespace h4b {
+
 // ---- host side -----------------------------------------------------------------
 
 static bool paged_view(const h4b_paged_kv* kv, PagedView* out) {
@@ -881,8 +937,9 @@ static int launch_few(const AttendArgs& a, int sms, cudaStream_t stream) {
 }
 
 template <typename T, int D>
-static int launch_attention(const AttendArgs& a, int max_query, int sms, cudaStream_t stream) {
+static int launch_attention(const AttendArgs& a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     const long long rows = static_cast<long long>(max_query) * a.group;
+    if (rows > kFewMaxRows) return launch_chunk<T, D>(a, kv, sms, stream);
     if (rows <= 8) return launch_few<T, D, 8>(a, sms, stream);
     if (rows <= 16) return launch_few<T, D, 16>(a, sms, stream);
     return launch_few<T, D, 32>(a, sms, stream);
@@ -946,8 +1003,11 @@ extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
     int sms = 0;
     if (head_dim != 64 && head_dim != 128) return H4B_EUNSUPPORTED;
     if (const int rc = paged_sm_count(&sms)) return rc > 0 ? -1000 - rc : rc;
-    const long long few = 2ll * kFewCtasPerSm * sms * kFewMaxRows * (head_dim + 2) * 4;
-    return kCounterBytes + few;
+    // two parts a CTA: an SM's rows of the few-row kernel are fewer than
+    // the 256 of the chunk kernel's CTA
+    static_assert(kFewCtasPerSm * kFewMaxRows <= 2 * kChunkRows, "the chunk kernel's parts are the larger");
+    if (sms * 2 * 4 > kCounterBytes) return H4B_EUNSUPPORTED;
+    return kCounterBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
 }
 
 extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long long q_stride, int heads, float scale,
@@ -958,7 +1018,9 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     if (!paged_view(kv, &a.p) || heads < 1 || heads % kv->kv_heads || q == nullptr || out == nullptr || window < 0 ||
         sinks < 0 || (sinks > 0 && window == 0) || max_query < 1 || workspace == nullptr)
         return H4B_EINVAL;
-    if (!paged_shape_supported(kv) || heads / kv->kv_heads > kFewMaxRows) return H4B_EUNSUPPORTED;
+    if (!paged_shape_supported(kv) || heads / kv->kv_heads > kFewMaxRows ||
+        static_cast<long long>(kv->pages) * kv->kv_heads > 0x7fffffffll)
+        return H4B_EUNSUPPORTED;
     const long long width = static_cast<long long>(heads) * kv->head_dim;
     if (q_stride < width || out_stride < width || ((q_stride | out_stride) & 7) ||
         ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) &
@@ -971,14 +1033,14 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     if (const int rc = paged_sm_count(&sms)) return rc;
     a.q = q, a.k_pages = kv->k_pages, a.v_pages = kv->v_pages, a.out = out, a.lse = lse;
     a.q_stride = q_stride, a.out_stride = out_stride, a.heads = heads, a.group = heads / kv->kv_heads;
-    a.window = window < (1 << 30) ? window : 1 << 30, a.sinks = sinks, a.scale = scale * 1.4426950408889634f;
+    a.window = window < kMaxLength ? window : kMaxLength, a.sinks = sinks, a.scale = scale * 1.4426950408889634f;
     a.counters = static_cast<unsigned int*>(workspace);
     a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
     const int longest = max_query < kv->tokens ? max_query : kv->tokens;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = kv->head_dim == 128;
     if (kv->dtype == H4B_FP16)
-        return wide ? launch_attention<__half, 128>(a, longest, sms, s) : launch_attention<__half, 64>(a, longest, sms, s);
-    return wide ? launch_attention<__nv_bfloat16, 128>(a, longest, sms, s)
-                : launch_attention<__nv_bfloat16, 64>(a, longest, sms, s);
+        return wide ? launch_attention<__half, 128>(a, kv, longest, sms, s) : launch_attention<__half, 64>(a, kv, longest, sms, s);
+    return wide ? launch_attention<__nv_bfloat16, 128>(a, kv, longest, sms, s)
+                : launch_attention<__nv_bfloat16, 64>(a, kv, longest, sms, s);
 }

@@ -1,0 +1,556 @@
+// Paged attention of long chunks on the 5th-generation tensor cores:
+// tcgen05.mma kind::f16, fp32 accumulators in tensor memory, pages fetched by
+// TMA. The split of the work over the CTAs, the visibility rules and the join
+// of partial results are those of paged.cu.
+//
+// An item is (sequence, 256 query rows, kv head): two tiles A and B of 128
+// rows (128 / group tokens each, row = token * group + q head) that share
+// every K/V tile of 128 keys. While the tensor cores work for one tile the
+// softmax of the other runs. B is left out where A holds all tokens.
+//
+// Warps: 0-3 and 4-7 are the softmax of A and B (thread = query row, TMEM lane
+// = thread), 8 issues the loads, 9 the MMAs (10 and 11 only fill its
+// warpgroup, whose registers go to the softmax). Per key block n and tile x:
+//   MMA:     S_x = Q_x K_n^T                              -> s_full[x]
+//   softmax: S_x to registers, maximum, p; P_x over S_x    -> p_full[x]
+//   MMA:     O_x += P_x V_n, then S_x of block n + 1 (the tensor cores run a
+//            CTA's MMAs in issue order, so P_x is read before it is
+//            overwritten)
+// s_full of block n + 1 also stands for the completion of P V of block n: a
+// commit tracks every earlier MMA. So a row may rescale its O after s_full,
+// and o_full is needed only where an item (or the CTA's range) ends; o_free
+// says that the softmax has read O and a new item may overwrite it.
+//
+// Operands: Q and the K/V ring in shared memory in the 128-byte swizzle
+// layout, 64 values (128 bytes) of head_dim a row, one slab per 64; P in
+// tensor memory. A tile's 128 keys are 128 / page_size boxes of one page each
+// (or one box inside a page), issued by the lanes of the load warp at the same
+// time; a page that is not there is a box outside the tensor, which reads as
+// zeros. Q is one box per slab: group heads x 128 / group tokens.
+//
+// Softmax in base 2 with a lazily moved reference, as in the kernel of few
+// rows: p = 2^(s - m + 8), m moves when a score passes m + 7.
+//
+// Keys that no row of the item sees (past its last token, before its window)
+// may lie in slots that hold anything: their scores are selected away, and
+// their V rows are zeroed in shared memory before the product, since 0 * NaN
+// would reach the sum.
+//
+// Every wait is bounded (mbar_wait). A role whose wait runs out marks the CTA
+// as failed and stops; the load warp waits for the copies it issued, the MMA
+// thread commits a last barrier, and the tensor memory is freed on every path.
+
+namespace h4b {
+
+constexpr int kChunkRows = 128, kChunkKeys = 128;
+constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 9, kChunkThreads = 384;
+// Registers a thread: three warpgroups at the launch's 168 are shared out
+// anew, 2 x 208 for the softmax (a row's 128 scores) and 88 for the others.
+constexpr int kChunkSoftmaxRegs = 208, kChunkOtherRegs = 88;
+static_assert(2 * kChunkSoftmaxRegs + kChunkOtherRegs <= 3 * 168, "registers of the CTA");
+
+template <int D>
+struct ChunkCfg {
+    static constexpr int kSlabs = D / 64;                        // 64 values of head_dim each
+    static constexpr int kSlab = 128 * 128;                      // 128 rows x 128 bytes
+    static constexpr int kTile = kSlabs * kSlab;                 // 128 keys (or query rows)
+    static constexpr int kStages = D == 128 ? 5 : 10;
+    static constexpr int kQOff = 0, kRingOff = 2 * kTile;
+    static constexpr int kBarOff = kRingOff + kStages * kTile;
+    static constexpr int kBars = 2 * kStages + 2 + 8 + 1;
+    static constexpr int kSmem = kBarOff + kBars * 8 + 16 + 64 + 1024;  // flags, alignment slack
+    static constexpr uint32_t kSCol = 0, kOCol = 256;            // S_x at 128 x, O_x at 256 + 128 x
+    static_assert(kSmem <= 232448, "shared memory per CTA");
+};
+
+// Instruction descriptors: D f32, A and B f16 (0) or bf16 (1), M 128.
+template <typename T>
+__host__ __device__ constexpr uint32_t chunk_idesc(int n, bool b_mn_major) {
+    constexpr uint32_t format = Pair<T>::kBf16 ? 1u : 0u;
+    return (1u << 4) | (format << 7) | (format << 10) | (b_mn_major ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kChunkRows >> 4) << 24);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                                 const __grid_constant__ CUtensorMap vmap, const AttendArgs a) {
+    using C = ChunkCfg<D>;
+    extern __shared__ uint8_t chunk_smem_raw[];
+    uint8_t* smem = chunk_smem_raw + ((1024u - (smem_addr(chunk_smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* q_full = empty + C::kStages;
+    uint64_t* q_empty = q_full + 1;
+    uint64_t* s_full = q_empty + 1;  // [2]
+    uint64_t* p_full = s_full + 2;   // [2]
+    uint64_t* o_full = p_full + 2;   // [2]
+    uint64_t* o_free = o_full + 2;   // [2]
+    uint64_t* mma_done = o_free + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+    volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* last_part = reinterpret_cast<int*>(tmem_slot + 2);  // [2]: this CTA joins the tile's parts
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int half_tokens = kChunkRows / a.group, tile_tokens = 2 * half_tokens;
+    const Range range = find_range<kChunkThreads, kChunkKeys>(a, tile_tokens, smem);
+    if (range.begin >= range.end) return;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&s_full[x], 1);
+            mbar_init(&p_full[x], 4);
+            mbar_init(&o_full[x], 1);
+            mbar_init(&o_free[x], 4);
+        }
+        mbar_init(mma_done, 1);
+        *failed = wait_failed_before() ? 1 : 0;
+        fence_mbar_init();
+    }
+    if (warp == kChunkMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_addr(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto ring = [&](uint32_t i) { return smem + C::kRingOff + (i % C::kStages) * C::kTile; };
+    auto phase = [&](uint32_t i) { return (i / C::kStages) & 1u; };
+
+    Walk<kChunkKeys> w;
+    w.start(a, range, tile_tokens);
+
+    // K of the CTA's step n is tile 2 n of the ring, V tile 2 n + 1.
+    if (warp >= kChunkLoadWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChunkOtherRegs));
+        if (warp == kChunkLoadWarp) {
+            // Each lane one box: page `lane / kSlabs` of the tile, slab `lane % kSlabs`.
+            const int page_size = 1 << a.p.page_shift, box = min(page_size, kChunkKeys);
+            const int boxes = kChunkKeys / box, my_page = lane / C::kSlabs, my_slab = lane % C::kSlabs;
+            const bool mine = my_page < boxes;
+            auto page_of = [&](const Walk<kChunkKeys>& u) -> int {  // -1: read as zeros
+                const int key = u.tile.block(u.unit) * kChunkKeys + my_page * box;
+                const Tile& t = u.tile;
+                if (!mine || key > t.p1 || !(a.window <= 0 || key + box - 1 > t.p0 - a.window || key < a.sinks)) return -1;
+                const int page = a.p.table[static_cast<long long>(u.b) * a.p.table_stride + (key >> a.p.page_shift)];
+                if (page >= 0 && page < a.p.pages) return page;
+                report(kStatusBadPage);
+                return -1;
+            };
+            uint32_t issued = 0;
+            bool ok = !*failed;
+            if (lane == 0) {
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
+            }
+            int page = page_of(w), items = 0;
+            bool new_item = true, more = true;
+            while (ok && more) {
+                if (new_item) {  // both tiles' q rows, once the previous item's are no longer read
+                    if (items > 0) ok = __all_sync(0xffffffffu, !*failed && mbar_wait(q_empty, (items - 1) & 1));
+                    if (!ok) break;
+                    const int tiles = w.tile.tokens > half_tokens ? 2 : 1;
+                    if (lane == 0)
+                        mbar_arrive_expect_tx(q_full, tiles * C::kSlabs * half_tokens * a.group * 128);
+                    __syncwarp();
+                    if (lane < tiles * C::kSlabs) {
+                        const int x = lane / C::kSlabs;
+                        tma_load_3d(smem + C::kQOff + x * C::kTile + my_slab * C::kSlab, &qmap, my_slab * 64,
+                                    w.h * a.group, w.tile.first + x * half_tokens, q_full);
+                    }
+                    ++items;
+                }
+                const int key = w.tile.block(w.unit) * kChunkKeys;
+                const int y = boxes > 1 ? 0 : key & (page_size - 1);
+                const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
+                // the next step's page ids are on their way while this step's copies are issued
+                const int h0 = w.h, t0 = w.t, b0 = w.b;
+                more = w.next(a, tile_tokens);
+                new_item = w.h != h0 || w.t != t0 || w.b != b0;
+                if (more) page = page_of(w);
+    #pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    if (issued >= C::kStages)
+                        ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&empty[issued % C::kStages],
+                                                                           phase(issued - C::kStages)));
+                    if (!ok) break;
+                    uint64_t* bar = &full[issued % C::kStages];
+                    if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+                    __syncwarp();
+                    if (mine)
+                        tma_load_3d(ring(issued) + my_slab * C::kSlab + my_page * box * 128, v ? &vmap : &kmap, my_slab * 64,
+                                    y, z, bar);
+                    ++issued;
+                }
+            }
+            if (!ok) *failed = 1;
+            // the copies issued must land before the CTA may exit
+            if (items > 0) mbar_wait(q_full, (items - 1) & 1);
+            for (uint32_t i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+                mbar_wait(&full[i % C::kStages], phase(i));
+            __syncwarp();
+        } else if (warp == kChunkMmaWarp) {
+            if (lane == 0) {
+                struct Step {
+                    int tiles;
+                    bool first, last;  // of the item, in this range
+                };
+                auto step_of = [&](bool first) {
+                    return Step{w.tile.tokens > half_tokens ? 2 : 1, first,
+                                w.unit + 1 >= w.tile.units() || w.left <= 1};
+                };
+                // descriptors of byte 0 of shared memory; addresses are added in units of 16 bytes
+                const uint32_t base = smem_addr(smem) >> 4;
+                constexpr uint64_t kmajor = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+                constexpr uint64_t mnmajor = (static_cast<uint64_t>(C::kSlab >> 4) << 16) | (64ull << 32) | (1ull << 46) |
+                                             (2ull << 61);
+                auto tile_of = [&](uint32_t i) { return base + ((C::kRingOff + (i % C::kStages) * C::kTile) >> 4); };
+                uint32_t n = 0;  // the step whose S comes next; `now` is the one before
+                Step now{0, false, false}, after = step_of(true);
+                uint32_t q_items = 0, p_phase = 0, o_phase = 3, o_used = 0;  // the last three: a bit per tile
+                bool ok = true, more = true;
+                while (ok) {
+    #pragma unroll 1
+                    for (int x = 0; x < 2; ++x) {
+                        const uint32_t s_tmem = tmem + C::kSCol + 128 * x, bit = 1u << x;
+                        if (x < now.tiles) {
+                            ok = !*failed && mbar_wait(&p_full[x], (p_phase >> x) & 1u);
+                            if (ok && x == 0) ok = mbar_wait(&full[(2 * n - 1) % C::kStages], phase(2 * n - 1));
+                            if (ok && now.first) {
+                                if (o_used & bit) ok = mbar_wait(&o_free[x], (o_phase >> x) & 1u);
+                                o_used |= bit;
+                                o_phase ^= bit;
+                            }
+                            if (!ok) break;
+                            p_phase ^= bit;
+                            tc_fence_after();
+                            const uint64_t bd = mnmajor | tile_of(2 * n - 1);
+                            const uint32_t o_tmem = tmem + C::kOCol + 128 * x;
+    #pragma unroll
+                            for (int kk = 0; kk < kChunkKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                                tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true),
+                                              !now.first || kk != 0);
+                            if (now.last) tc_commit(&o_full[x]);
+                            if (x == now.tiles - 1) tc_commit(&empty[(2 * n - 1) % C::kStages]);
+                        }
+                        if (more && x < after.tiles) {
+                            if (x == 0) {
+                                if (after.first) ok = !*failed && mbar_wait(q_full, q_items++ & 1);
+                                ok = ok && !*failed && mbar_wait(&full[(2 * n) % C::kStages], phase(2 * n));
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
+                            const uint64_t ad = kmajor | (base + ((C::kQOff + x * C::kTile) >> 4));
+                            const uint64_t bd = kmajor | tile_of(2 * n);
+    #pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t step = (kk >> 2) * (C::kSlab >> 4) + 2 * (kk & 3);
+                                tc_mma_f16(s_tmem, ad + step, bd + step, chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                            }
+                            tc_commit(&s_full[x]);
+                            if (x == after.tiles - 1) {
+                                tc_commit(&empty[(2 * n) % C::kStages]);
+                                if (after.last) tc_commit(q_empty);
+                            }
+                        }
+                    }
+                    if (!ok || !more) break;
+                    now = after;
+                    ++n;
+                    const int h0 = w.h, t0 = w.t, b0 = w.b;
+                    more = w.next(a, tile_tokens);
+                    if (more) after = step_of(w.h != h0 || w.t != t0 || w.b != b0);
+                }
+                if (!ok) *failed = 1;
+                tc_commit(mma_done);  // arrives once every MMA issued above has completed
+            }
+            __syncwarp();
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kChunkSoftmaxRegs));
+        const int x = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+        const uint32_t s_col = lane_base + C::kSCol + 128 * x, o_col = lane_base + C::kOCol + 128 * x;
+        const int token = row / a.group, head = row - token * a.group;
+        bool ok = !*failed, more = true;
+        bool begun = w.unit == 0;  // the item's first unit is in this range
+        uint32_t n = 0;            // the CTA's step
+        uint32_t s_count = 0, o_items = 0;
+        while (ok && more) {
+            const int my_tokens = min(half_tokens, w.tile.tokens - x * half_tokens);
+            if (my_tokens <= 0) {  // B has nothing to do for this item
+                const int h0 = w.h, t0 = w.t, b0 = w.b;
+                while ((more = w.next(a, tile_tokens)) && w.h == h0 && w.t == t0 && w.b == b0) ++n;
+                ++n;
+                begun = true;
+                continue;
+            }
+            const bool valid = token < my_tokens;
+            const int pos = valid ? w.tile.p0 + x * half_tokens + token : -1;
+            float m = -INFINITY, l = 0.f;
+            bool done = false;
+            while (true) {
+                ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&s_full[x], s_count & 1));
+                if (!ok) break;
+                ++s_count;
+                tc_fence_after();
+                float sv[kChunkKeys];
+#pragma unroll
+                for (int c = 0; c < kChunkKeys; c += 16) tmem_ld16_nowait(s_col + c, sv, c);
+                tmem_wait_regs(sv);
+                const int key = w.tile.block(w.unit) * kChunkKeys;
+                const bool all = !valid || (key + kChunkKeys - 1 <= pos &&
+                                            (a.window <= 0 || key > pos - a.window || key + kChunkKeys - 1 < a.sinks));
+                if (!__all_sync(0xffffffffu, all)) {
+                    const int upto = pos - key, from = a.window > 0 ? pos - a.window - key : -1;
+                    const int sinks = a.window > 0 ? a.sinks - key : 0;
+#pragma unroll
+                    for (int c = 0; c < kChunkKeys; ++c)
+                        sv[c] = c <= upto && (c > from || c < sinks) ? sv[c] : -INFINITY;
+                }
+                float top[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) top[c] = fmaxf(sv[c], sv[c + 8]);
+#pragma unroll
+                for (int c = 16; c < kChunkKeys; c += 16)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) top[k] = fmaxf(fmaxf(top[k], sv[c + k]), sv[c + k + 8]);
+                const float mx = a.scale * fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
+                                                 fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+                const bool move = valid && mx > m + kFewSlack;
+                if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
+                    // P V of every earlier block has completed (see above)
+                    const float f = move ? ex2_approx(m - mx) : 1.f;  // 0 for m = -inf, whose l and O are 0
+                    l *= f;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {  // rare: few registers beside the scores
+                        float v[16];
+                        tmem_ld16_nowait(o_col + c, v, 0);
+                        tmem_wait_regs(v);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] *= f;
+                        tmem_st16(o_col + c, v, 0);
+                    }
+                }
+                if (move) m = mx;
+                const float base = m == -INFINITY ? 0.f : kFewOffset - m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < kChunkKeys; c += 32) {
+                    uint32_t p16[16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float p0 = ex2_approx(__fmaf_rn(sv[c + k], a.scale, base));
+                        const float p1 = ex2_approx(__fmaf_rn(sv[c + k + 1], a.scale, base));
+                        sum[(k >> 1) & 3] += p0 + p1;
+                        p16[k / 2] = Pair<T>::pack(p0, p1);
+                    }
+                    tmem_st16u(s_col + c / 2, p16, 0);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (x == 0 && !(key + kChunkKeys - 1 <= w.tile.p1 &&
+                                (a.window <= 0 || key > w.tile.p0 - a.window || key + kChunkKeys - 1 < a.sinks))) {
+                    // V rows of keys that no row of the item sees (A is part of every item)
+                    ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&full[(2 * n + 1) % C::kStages], phase(2 * n + 1)));
+                    if (!ok) break;
+                    if (!tile_sees(w.tile, a.window, a.sinks, key + row)) {
+#pragma unroll
+                        for (int c = 0; c < C::kTile / 128; c += 16)
+                            *reinterpret_cast<uint4*>(ring(2 * n + 1) + (c >> 7) * C::kSlab + row * 128 + (c & 127)) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
+                done = w.unit + 1 >= w.tile.units();
+                if (done || w.left <= 1) break;
+                w.next(a, tile_tokens);
+                ++n;
+            }
+            if (!ok) break;
+            ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&o_full[x], o_items & 1));
+            if (!ok) break;
+            ++o_items;
+            tc_fence_after();
+
+            // ---- the tile's result, or this CTA's part of it -----------------
+            const bool whole = begun && done;
+            const long long out_row = w.tile.first + x * half_tokens + (valid ? token : 0);
+            const int out_head = w.h * a.group + head;
+            T* out = static_cast<T*>(a.out) + out_row * a.out_stride + out_head * D;
+            constexpr int kPart = kChunkRows * (D + 2);
+            auto part_of = [&](int cta, int which) {
+                return a.partials + (static_cast<long long>(2 * cta + which) * 2 + x) * kPart;
+            };
+            // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
+            float4* part = reinterpret_cast<float4*>(part_of(blockIdx.x, begun ? 1 : 0));
+            const float inv = whole && l != 0.f ? 1.0f / l : (whole ? 0.f : 1.f);
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float v[32];
+                tmem_ld16_nowait(o_col + c, v, 0);
+                tmem_ld16_nowait(o_col + c + 16, v, 16);
+                tmem_wait_regs(v);
+                if (whole) {
+                    if (valid && l == 0.f)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = 0.f;
+                    if (valid)
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8)
+                            *reinterpret_cast<uint4*>(out + c + k) = make_uint4(
+                                Pair<T>::pack(v[k] * inv, v[k + 1] * inv), Pair<T>::pack(v[k + 2] * inv, v[k + 3] * inv),
+                                Pair<T>::pack(v[k + 4] * inv, v[k + 5] * inv), Pair<T>::pack(v[k + 6] * inv, v[k + 7] * inv));
+                } else if (valid) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        __stcg(part + ((c + k) / 4) * kChunkRows + row, make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&o_free[x]);
+            if (whole) {
+                if (valid && a.lse != nullptr)
+                    a.lse[out_row * a.heads + out_head] =
+                        l == 0.f ? -INFINITY : (m - kFewOffset) * 0.6931471805599453f + logf(l);
+            } else {
+                if (valid)
+                    __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
+                const long long at = range.end - w.left;  // this unit
+                const long long first = at - w.unit, final = first + w.tile.units() - 1;
+                const int c0 = range_owner(range.total, first, range.ctas);
+                const int c1 = range_owner(range.total, final, range.ctas);
+                __threadfence();
+                named_sync(1 + x, 128);
+                if (row == 0) {
+                    unsigned* counter = reinterpret_cast<unsigned*>(a.counters) + 2 * c0 + x;
+                    const unsigned seen = atom_acq_rel_add(counter, 1u);
+                    last_part[x] = seen == static_cast<unsigned>(c1 - c0);
+                    if (last_part[x]) *counter = 0u;  // zero for the next call
+                }
+                named_sync(1 + x, 128);
+                if (last_part[x]) {
+                    __threadfence();
+                    if (valid) {
+                        auto stat = [&](int cta) {
+                            return __ldcg(reinterpret_cast<const float2*>(part_of(cta, cta == c0) + D * kChunkRows) + row);
+                        };
+                        float most = -INFINITY, total = 0.f;
+                        for (int cta = c0; cta <= c1; ++cta) most = fmaxf(most, stat(cta).x);
+                        for (int cta = c0; cta <= c1; ++cta) {
+                            const float2 ml = stat(cta);
+                            if (ml.y != 0.f) total += ml.y * ex2_approx(ml.x - most);
+                        }
+                        const float scale = total != 0.f ? 1.0f / total : 0.f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 4; c += 8) {
+                            float4 v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            for (int cta = c0; cta <= c1; ++cta) {
+                                const float2 ml = stat(cta);
+                                if (ml.y == 0.f) continue;  // saw no key: its o was never formed
+                                const float f = scale * ex2_approx(ml.x - most);
+                                const float4* o = reinterpret_cast<const float4*>(part_of(cta, cta == c0));
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const float4 y = __ldcg(o + (c + k) * kChunkRows + row);
+                                    v[k].x += y.x * f, v[k].y += y.y * f, v[k].z += y.z * f, v[k].w += y.w * f;
+                                }
+                            }
+#pragma unroll
+                            for (int k = 0; k < 8; k += 2)
+                                *reinterpret_cast<uint4*>(out + 4 * (c + k)) =
+                                    make_uint4(Pair<T>::pack(v[k].x, v[k].y), Pair<T>::pack(v[k].z, v[k].w),
+                                               Pair<T>::pack(v[k + 1].x, v[k + 1].y), Pair<T>::pack(v[k + 1].z, v[k + 1].w));
+                        }
+                        if (a.lse != nullptr)
+                            a.lse[out_row * a.heads + out_head] =
+                                total == 0.f ? -INFINITY : (most - kFewOffset) * 0.6931471805599453f + logf(total);
+                    }
+                }
+                named_sync(1 + x, 128);  // last_part is free again
+            }
+            more = w.next(a, tile_tokens);
+            ++n;
+            begun = true;
+        }
+        if (!ok) *failed = 1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kChunkMmaWarp) {
+        // the MMAs must be complete before their tensor memory is released
+        mbar_wait(mma_done, 0);
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// A layer's pages as a 3-D tensor map [pages * kv_heads][page_size][D] with
+// boxes of 64 values x min(page_size, 128) rows.
+static bool paged_kv_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv) {
+    auto encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kv->head_dim), static_cast<cuuint64_t>(kv->page_size),
+                                static_cast<cuuint64_t>(kv->pages) * kv->kv_heads};
+    const cuuint64_t strides[2] = {kv->head_dim * 2ull, static_cast<cuuint64_t>(kv->page_size) * kv->head_dim * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(kv->page_size < kChunkKeys ? kv->page_size : kChunkKeys), 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return encode(out, kv->dtype == H4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The q rows [tokens][heads][D] with boxes of 64 values x group heads x
+// 128 / group tokens: a tile's rows in their order.
+static bool paged_q_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv, int heads, int group,
+                        long long q_stride) {
+    auto encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kv->head_dim), static_cast<cuuint64_t>(heads),
+                                static_cast<cuuint64_t>(kv->tokens)};
+    const cuuint64_t strides[2] = {kv->head_dim * 2ull, static_cast<cuuint64_t>(q_stride) * 2};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(kChunkRows / group)};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    return encode(out, kv->dtype == H4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+static int launch_chunk(const AttendArgs& a, const h4b_paged_kv* kv, int sms, cudaStream_t stream) {
+    using C = ChunkCfg<D>;
+    static std::atomic<bool> opted_in[kMaxDevices];
+    int dev = 0;
+    H4B_CUDA_TRY(cudaGetDevice(&dev));
+    if (!opted_in[dev].load(std::memory_order_acquire)) {
+        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_chunk_kernel<T, D>,
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        opted_in[dev].store(true, std::memory_order_release);
+    }
+    CUtensorMap qmap, kmap, vmap;
+    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.q_stride) || !paged_kv_map(&kmap, a.k_pages, kv) ||
+        !paged_kv_map(&vmap, a.v_pages, kv))
+        return H4B_EUNSUPPORTED;
+    paged_attention_chunk_kernel<T, D><<<sms, kChunkThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
+    H4B_CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
+}  // namespace h4b
