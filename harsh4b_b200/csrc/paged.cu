@@ -223,13 +223,16 @@ __global__ void __launch_bounds__(kCopyThreads)
 // item's keys. A unit is one block of KEYS keys of an item, from the blocks
 // that some row of it sees: the sink blocks [0, sink_blocks) and then
 // [low, high); an item has one unit at least, so that every row is answered.
-// The units of all items in order (sequence, tile, kv head, block) are cut
-// into one equal contiguous range per CTA, whatever the lengths. An item that
-// lies across CTAs leaves one partial result (o, m, l) in each; the CTA that
+// All items in order (sequence, tile, kv head) are laid out on a line, `extra`
+// places for what an item costs beside its units and then one place a unit,
+// and the line is cut into one equal contiguous range per CTA, whatever the
+// lengths. A cut among an item's first places counts as one before its first
+// unit. An item that lies across CTAs leaves one partial result (o, m, l) in each; the CTA that
 // finishes last joins them in the order of the CTAs, so the result does not
 // depend on which one that is.
 struct AttendArgs {
     PagedView p;
+    int extra;                // places of an item beside its units
     const void *q, *k_pages, *v_pages;
     void* out;
     float* lse;               // may be null
@@ -265,22 +268,27 @@ __device__ __forceinline__ Tile make_tile(const SequenceSpan& s, int t, int tile
     return x;
 }
 
-// Units of one kv head of every lane's sequence. The whole warp takes part: a
+template <int KEYS>
+__device__ __forceinline__ int item_places(const AttendArgs& a, const SequenceSpan& s, int t, int tile_tokens) {
+    return a.extra + make_tile<KEYS>(s, t, tile_tokens, a.window, a.sinks).units();
+}
+
+// Places of one kv head of every lane's sequence. The whole warp takes part: a
 // lane sums a few tiles by itself, a long chunk's are summed by all lanes.
 template <int KEYS>
-__device__ __forceinline__ long long warp_units(const SequenceSpan& s, int tile_tokens, int window, int sinks) {
+__device__ __forceinline__ long long warp_places(const AttendArgs& a, const SequenceSpan& s, int tile_tokens) {
     const int lane = threadIdx.x & 31;
     long long n = 0;
     const bool is_long = s.count > 4 * tile_tokens;
     if (!is_long)
-        for (int t = 0; t * tile_tokens < s.count; ++t) n += make_tile<KEYS>(s, t, tile_tokens, window, sinks).units();
+        for (int t = 0; t * tile_tokens < s.count; ++t) n += item_places<KEYS>(a, s, t, tile_tokens);
     for (unsigned todo = __ballot_sync(0xffffffffu, is_long); todo; todo &= todo - 1) {
         const int who = __ffs(todo) - 1;
         const SequenceSpan x{__shfl_sync(0xffffffffu, s.first, who), __shfl_sync(0xffffffffu, s.count, who),
                              __shfl_sync(0xffffffffu, s.base, who)};
         long long sum = 0;
         for (int t = lane; static_cast<long long>(t) * tile_tokens < x.count; t += 32)
-            sum += make_tile<KEYS>(x, t, tile_tokens, window, sinks).units();
+            sum += item_places<KEYS>(a, x, t, tile_tokens);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == who) n = sum;
@@ -288,22 +296,22 @@ __device__ __forceinline__ long long warp_units(const SequenceSpan& s, int tile_
     return n;
 }
 
-// The CTA's range of units and where it starts.
+// The CTA's range of places and where it starts.
 struct Range {
     long long begin, end, total;  // [begin, end) of total
-    long long skip;               // units of its sequence before `begin`
-    int sequence;                 // of unit `begin`
-    int ctas;                     // that have a range: every one of them has a unit at least
+    long long skip;               // places of its sequence before `begin`
+    int sequence;                 // of place `begin`
+    int ctas;                     // that have a range: every one of them has a place at least
 };
 __device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
-// The CTA that holds a unit: the largest c with range_begin(c) <= unit.
-__device__ __forceinline__ int range_owner(long long total, long long unit, int ctas) {
-    return static_cast<int>(((unit + 1) * ctas - 1) / total);
+// The CTA that holds a place: the largest c with range_begin(c) <= place.
+__device__ __forceinline__ int range_owner(long long total, long long place, int ctas) {
+    return static_cast<int>(((place + 1) * ctas - 1) / total);
 }
 
 // Every thread of the CTA takes part; `shared` holds THREADS / 32 long longs
 // and a Range. Each thread has a share of the sequences, a prefix sum over
-// the threads follows, and the thread whose sequences hold unit `begin`
+// the threads follows, and the thread whose sequences hold place `begin`
 // finds it.
 template <int THREADS, int KEYS>
 __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens, void* shared) {
@@ -311,13 +319,13 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     Range* found = reinterpret_cast<Range*>(warp_sums + THREADS / 32);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int each = (a.p.sequences + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
-    auto units_of = [&](int e) {  // of the thread's e-th sequence, all kv heads
+    auto places_of = [&](int e) {  // of the thread's e-th sequence, all kv heads
         SequenceSpan s{0, 0, 0};
         if (b0 + e < a.p.sequences) s = sequence_span(a.p, b0 + e);
-        return a.p.kv_heads * warp_units<KEYS>(s, tile_tokens, a.window, a.sinks);
+        return a.p.kv_heads * warp_places<KEYS>(a, s, tile_tokens);
     };
     long long mine = 0;
-    for (int e = 0; e < each; ++e) mine += units_of(e);
+    for (int e = 0; e < each; ++e) mine += places_of(e);
     long long before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -345,7 +353,7 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
         long long at = before;
         bool open = here;
         for (int e = 0; e < each; ++e) {
-            const long long n = each == 1 ? mine : units_of(e);
+            const long long n = each == 1 ? mine : places_of(e);
             if (open && r.begin < at + n) {
                 found->sequence = b0 + e;
                 found->skip = r.begin - at;
@@ -369,13 +377,14 @@ struct Walk {
     RawSpan following;        // of sequence b + 1, requested when b was entered
     Tile tile;
     int b, t, h, unit;        // unit within the item
-    long long left;           // units of the range from here on
+    long long left;           // places of the range from this unit on
 
     __device__ __forceinline__ void request(const AttendArgs& a) {
         if (b + 1 < a.p.sequences) following = raw_span(a.p, b + 1);
     }
     // By whole warps: the lanes look for the tile together, 32 at a time.
-    __device__ __forceinline__ void start(const AttendArgs& a, const Range& r, int tile_tokens) {
+    // False when the range holds no unit.
+    __device__ __forceinline__ bool start(const AttendArgs& a, const Range& r, int tile_tokens) {
         const int lane = threadIdx.x & 31;
         b = r.sequence;
         left = r.end - r.begin;
@@ -385,8 +394,7 @@ struct Walk {
         for (int t0 = 0;; t0 += 32) {
             long long n = 0;
             if (static_cast<long long>(t0 + lane) * tile_tokens < span.count)
-                n = make_tile<KEYS>(span, t0 + lane, tile_tokens, a.window, a.sinks).units() *
-                    static_cast<long long>(a.p.kv_heads);
+                n = item_places<KEYS>(a, span, t0 + lane, tile_tokens) * static_cast<long long>(a.p.kv_heads);
             long long upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -403,8 +411,14 @@ struct Walk {
             skip -= __shfl_sync(0xffffffffu, upto, 31);
         }
         tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
-        h = static_cast<int>(skip / tile.units());
-        unit = static_cast<int>(skip % tile.units());
+        const int places = a.extra + tile.units();
+        h = static_cast<int>(skip / places);
+        unit = static_cast<int>(skip % places) - a.extra;
+        if (unit < 0) {
+            left += unit;
+            unit = 0;
+        }
+        return left > 0;
     }
     // Past the item's last unit: to the next item that has any.
     __device__ __forceinline__ void next_item(const AttendArgs& a, int tile_tokens) {
@@ -420,13 +434,30 @@ struct Walk {
         }
         tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
     }
+    __device__ __forceinline__ bool item_ends() const { return unit + 1 >= tile.units(); }
+    // Whether this unit is the last of the item in this range, or of all.
+    __device__ __forceinline__ bool part_ends() const { return item_ends() || left <= 1; }
     // To the next unit; false past the range's end.
     __device__ __forceinline__ bool next(const AttendArgs& a, int tile_tokens) {
-        if (--left <= 0) return false;
-        if (++unit >= tile.units()) next_item(a, tile_tokens);
+        const bool over = item_ends();
+        left -= over ? 1 + a.extra : 1;
+        if (left <= 0) return false;
+        if (over)
+            next_item(a, tile_tokens);
+        else
+            ++unit;
         return true;
     }
 };
+
+// The CTAs that hold units of an item, given one of its units (walk state of
+// the CTA of `range`): from its first unit's to its last's.
+template <int KEYS>
+__device__ __forceinline__ int2 item_owners(const Range& range, const Walk<KEYS>& w) {
+    const long long first = range.end - w.left - w.unit;
+    return make_int2(range_owner(range.total, first, range.ctas),
+                     range_owner(range.total, first + w.tile.units() - 1, range.ctas));
+}
 
 // Whether some row of the tile sees key j.
 __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, int j) {
@@ -453,6 +484,7 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // products only. Rows that no row sees are zero-filled by the copy, so what
 // such a slot holds cannot reach a sum.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 64;
+constexpr int kFewExtra = 2;  // an item's start and join, in units
 constexpr float kFewOffset = 8.f, kFewSlack = 7.f;
 
 template <int D, int ROWS>
@@ -552,7 +584,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     };
 
     Walk<kFewKeys> now, ahead;
-    now.start(a, range, tile_tokens);
+    if (!now.start(a, range, tile_tokens)) return;
     ahead = now;
     // the ring's first stages; `page` belongs to the piece `ahead` stands at
     int page = page_of(ahead);
@@ -711,8 +743,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         pages_now[C::kStages - 2] = page_new;
         stage = (stage + 1) % C::kStages;
 
-        const bool item_done = now.unit + 1 >= now.tile.units();
-        if (!item_done && now.left > 1) {
+        const bool item_done = now.item_ends();
+        if (!now.part_ends()) {
             now.next(a, tile_tokens);
             continue;
         }
@@ -809,10 +841,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                 }
         }
         if (!whole) {
-            // the CTAs that hold this item: from its first unit's to its last's
-            const long long at = range.end - now.left;  // this unit
-            const long long first = at - now.unit, last = first + now.tile.units() - 1;
-            const int c0 = range_owner(range.total, first, range.ctas), c1 = range_owner(range.total, last, range.ctas);
+            const int2 owners = item_owners(range, now);
+            const int c0 = owners.x, c1 = owners.y;
             int* flag = reinterpret_cast<int*>(few_smem + C::kStatOff);
             __threadfence();
             __syncthreads();
@@ -921,8 +951,9 @@ static int launch_append(const AppendArgs& a, cudaStream_t stream) {
 }
 
 template <typename T, int D, int ROWS>
-static int launch_few(const AttendArgs& a, int sms, cudaStream_t stream) {
+static int launch_few(AttendArgs a, int sms, cudaStream_t stream) {
     using C = FewCfg<D, ROWS>;
+    a.extra = kFewExtra;
     static std::atomic<bool> opted_in[kMaxDevices];
     int dev = 0;
     H4B_CUDA_TRY(cudaGetDevice(&dev));

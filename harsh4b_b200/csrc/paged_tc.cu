@@ -9,8 +9,8 @@
 // softmax of the other runs. B is left out where A holds all tokens.
 //
 // Warps: 0-3 and 4-7 are the softmax of A and B (thread = query row, TMEM lane
-// = thread), 8 issues the loads, 9 the MMAs (10 and 11 only fill its
-// warpgroup, whose registers go to the softmax). Per key block n and tile x:
+// = thread), 8 issues the loads, 9 and 10 the MMAs of A and B, 11 cleans V
+// tiles (below). Per key block n and tile x:
 //   MMA:     S_x = Q_x K_n^T                              -> s_full[x]
 //   softmax: S_x to registers, maximum, p; P_x over S_x    -> p_full[x]
 //   MMA:     O_x += P_x V_n, then S_x of block n + 1 (the tensor cores run a
@@ -34,7 +34,8 @@
 // Keys that no row of the item sees (past its last token, before its window)
 // may lie in slots that hold anything: their scores are selected away, and
 // their V rows are zeroed in shared memory before the product, since 0 * NaN
-// would reach the sum.
+// would reach the sum: such a V tile lands on a barrier of its own, warp 11
+// zeroes the rows and then completes the tile's barrier in the loads' place.
 //
 // Every wait is bounded (mbar_wait). A role whose wait runs out marks the CTA
 // as failed and stops; the load warp waits for the copies it issued, the MMA
@@ -43,7 +44,11 @@
 namespace h4b {
 
 constexpr int kChunkRows = 128, kChunkKeys = 128;
-constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 9, kChunkThreads = 384;
+constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 9, kChunkCleanWarp = 11, kChunkThreads = 384;
+constexpr int kChunkExtra = 2;  // an item's start, end and pipeline fill, in units
+// A step's flags: it has both tiles; first, last of its item in this range; last of all.
+constexpr uint32_t kStepTwo = 1, kStepFirst = 2, kStepLast = 4, kStepFinal = 8;
+constexpr uint32_t kStepNone = 16;  // the range held no unit
 // Registers a thread: three warpgroups at the launch's 168 are shared out
 // anew, 2 x 208 for the softmax (a row's 128 scores) and 88 for the others.
 constexpr int kChunkSoftmaxRegs = 208, kChunkOtherRegs = 88;
@@ -57,8 +62,10 @@ struct ChunkCfg {
     static constexpr int kStages = D == 128 ? 5 : 10;
     static constexpr int kQOff = 0, kRingOff = 2 * kTile;
     static constexpr int kBarOff = kRingOff + kStages * kTile;
-    static constexpr int kBars = 2 * kStages + 2 + 8 + 1;
-    static constexpr int kSmem = kBarOff + kBars * 8 + 16 + 64 + 1024;  // flags, alignment slack
+    static constexpr int kBars = 3 * kStages + 2 + 8 + 1;
+    // barriers, words of the CTA, steps' flags, range, alignment slack
+    static constexpr int kFlagOff = kBarOff + kBars * 8 + 16, kRangeOff = kFlagOff + kStages * 4 + 4 * (kStages & 1);
+    static constexpr int kSmem = kRangeOff + sizeof(Range) + 1024;
     static constexpr uint32_t kSCol = 0, kOCol = 256;            // S_x at 128 x, O_x at 256 + 128 x
     static_assert(kSmem <= 232448, "shared memory per CTA");
 };
@@ -71,6 +78,39 @@ __host__ __device__ constexpr uint32_t chunk_idesc(int n, bool b_mn_major) {
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kChunkRows >> 4) << 24);
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Whether the block of keys from `key` on has one that no row of the tile sees.
+__device__ __forceinline__ bool has_unseen_keys(const Tile& t, int window, int sinks, int key) {
+    const int end = key + kChunkKeys - 1;
+    return !(end <= t.p1 && (window <= 0 || key > t.p0 - window || end < sinks));
+}
+
+// Bits 0 .. n - 1, of 32.
+__device__ __forceinline__ uint32_t bits_below(int n) {
+    return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -80,7 +120,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint8_t* smem = chunk_smem_raw + ((1024u - (smem_addr(chunk_smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
     uint64_t* empty = full + C::kStages;
-    uint64_t* q_full = empty + C::kStages;
+    uint64_t* raw = empty + C::kStages;  // a V tile on its way to the cleaning warp
+    uint64_t* q_full = raw + C::kStages;
     uint64_t* q_empty = q_full + 1;
     uint64_t* s_full = q_empty + 1;  // [2]
     uint64_t* p_full = s_full + 2;   // [2]
@@ -89,27 +130,33 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint64_t* mma_done = o_free + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile uint32_t* flags = reinterpret_cast<volatile uint32_t*>(smem + C::kFlagOff);
     int* last_part = reinterpret_cast<int*>(tmem_slot + 2);  // [2]: this CTA joins the tile's parts
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half_tokens = kChunkRows / a.group, tile_tokens = 2 * half_tokens;
-    const Range range = find_range<kChunkThreads, kChunkKeys>(a, tile_tokens, smem);
-    if (range.begin >= range.end) return;
+    Range* shared_range = reinterpret_cast<Range*>(smem + C::kRangeOff);
+    {
+        const Range r = find_range<kChunkThreads, kChunkKeys>(a, tile_tokens, smem);
+        if (r.begin >= r.end) return;
+        if (threadIdx.x == 0) *shared_range = r;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], 2);  // both tiles' MMA warps
+            mbar_init(&raw[s], 1);
         }
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
+        mbar_init(q_empty, 2);
         for (int x = 0; x < 2; ++x) {
             mbar_init(&s_full[x], 1);
             mbar_init(&p_full[x], 4);
             mbar_init(&o_full[x], 1);
             mbar_init(&o_free[x], 4);
         }
-        mbar_init(mma_done, 1);
+        mbar_init(mma_done, 2);
         *failed = wait_failed_before() ? 1 : 0;
         fence_mbar_init();
     }
@@ -125,13 +172,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     auto ring = [&](uint32_t i) { return smem + C::kRingOff + (i % C::kStages) * C::kTile; };
     auto phase = [&](uint32_t i) { return (i / C::kStages) & 1u; };
 
-    Walk<kChunkKeys> w;
-    w.start(a, range, tile_tokens);
-
-    // K of the CTA's step n is tile 2 n of the ring, V tile 2 n + 1.
+    // K of the CTA's step n is tile 2 n of the ring, V tile 2 n + 1. A step is a
+    // unit; its flags lie beside K's barrier, written before K's copies start.
+    // (Each role starts its walk after its registers are set: what is live
+    // across setmaxnreg would be kept on the stack.)
     if (warp >= kChunkLoadWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChunkOtherRegs));
         if (warp == kChunkLoadWarp) {
+            Walk<kChunkKeys> w;
             // Each lane one box: page `lane / kSlabs` of the tile, slab `lane % kSlabs`.
             const int page_size = 1 << a.p.page_shift, box = min(page_size, kChunkKeys);
             const int boxes = kChunkKeys / box, my_page = lane / C::kSlabs, my_slab = lane % C::kSlabs;
@@ -145,20 +193,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 report(kStatusBadPage);
                 return -1;
             };
-            uint32_t issued = 0;
-            bool ok = !*failed;
+            uint32_t issued = 0, raw_open = 0, raw_phase = 0;  // a bit per stage
+            bool ok = !*failed, more = w.start(a, *shared_range, tile_tokens);
             if (lane == 0) {
                 asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
                 asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
                 asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
             }
-            int page = page_of(w), items = 0;
-            bool new_item = true, more = true;
+            if (!more && lane == 0) {
+                flags[0] = kStepNone;
+                mbar_arrive(&full[0]);
+            }
+            int page = more ? page_of(w) : -1, items = 0;
+            bool new_item = true;
             while (ok && more) {
+                const int tiles = w.tile.tokens > half_tokens ? 2 : 1;
                 if (new_item) {  // both tiles' q rows, once the previous item's are no longer read
                     if (items > 0) ok = __all_sync(0xffffffffu, !*failed && mbar_wait(q_empty, (items - 1) & 1));
                     if (!ok) break;
-                    const int tiles = w.tile.tokens > half_tokens ? 2 : 1;
                     if (lane == 0)
                         mbar_arrive_expect_tx(q_full, tiles * C::kSlabs * half_tokens * a.group * 128);
                     __syncwarp();
@@ -172,125 +224,155 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 const int key = w.tile.block(w.unit) * kChunkKeys;
                 const int y = boxes > 1 ? 0 : key & (page_size - 1);
                 const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
+                const bool unclean = has_unseen_keys(w.tile, a.window, a.sinks, key);
+                uint32_t flag = (tiles == 2 ? kStepTwo : 0u) | (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u);
                 // the next step's page ids are on their way while this step's copies are issued
-                const int h0 = w.h, t0 = w.t, b0 = w.b;
+                new_item = w.part_ends();
                 more = w.next(a, tile_tokens);
-                new_item = w.h != h0 || w.t != t0 || w.b != b0;
                 if (more) page = page_of(w);
-    #pragma unroll
+                if (!more) flag |= kStepFinal;
+#pragma unroll
                 for (int v = 0; v < 2; ++v) {
+                    const uint32_t stage = issued % C::kStages;
                     if (issued >= C::kStages)
-                        ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&empty[issued % C::kStages],
-                                                                           phase(issued - C::kStages)));
+                        ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&empty[stage], phase(issued - C::kStages)));
                     if (!ok) break;
-                    uint64_t* bar = &full[issued % C::kStages];
-                    if (lane == 0) mbar_arrive_expect_tx(bar, C::kTile);
+                    // a V tile with unseen keys goes through the cleaning warp
+                    uint64_t* bar = v == 1 && unclean ? &raw[stage] : &full[stage];
+                    if (lane == 0) {
+                        if (v == 0) flags[stage] = flag;
+                        mbar_arrive_expect_tx(bar, C::kTile);
+                    }
                     __syncwarp();
                     if (mine)
-                        tma_load_3d(ring(issued) + my_slab * C::kSlab + my_page * box * 128, v ? &vmap : &kmap, my_slab * 64,
-                                    y, z, bar);
+                        tma_load_3d(ring(issued) + my_slab * C::kSlab + my_page * box * 128, v ? &vmap : &kmap,
+                                    my_slab * 64, y, z, bar);
+                    if (v == 1 && unclean) raw_phase ^= 1u << stage, raw_open |= 1u << stage;
+                    else raw_open &= ~(1u << stage);
                     ++issued;
                 }
             }
             if (!ok) *failed = 1;
             // the copies issued must land before the CTA may exit
             if (items > 0) mbar_wait(q_full, (items - 1) & 1);
-            for (uint32_t i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
-                mbar_wait(&full[i % C::kStages], phase(i));
-            __syncwarp();
-        } else if (warp == kChunkMmaWarp) {
-            if (lane == 0) {
-                struct Step {
-                    int tiles;
-                    bool first, last;  // of the item, in this range
-                };
-                auto step_of = [&](bool first) {
-                    return Step{w.tile.tokens > half_tokens ? 2 : 1, first,
-                                w.unit + 1 >= w.tile.units() || w.left <= 1};
-                };
-                // descriptors of byte 0 of shared memory; addresses are added in units of 16 bytes
-                const uint32_t base = smem_addr(smem) >> 4;
-                constexpr uint64_t kmajor = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-                constexpr uint64_t mnmajor = (static_cast<uint64_t>(C::kSlab >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-                                             (2ull << 61);
-                auto tile_of = [&](uint32_t i) { return base + ((C::kRingOff + (i % C::kStages) * C::kTile) >> 4); };
-                uint32_t n = 0;  // the step whose S comes next; `now` is the one before
-                Step now{0, false, false}, after = step_of(true);
-                uint32_t q_items = 0, p_phase = 0, o_phase = 3, o_used = 0;  // the last three: a bit per tile
-                bool ok = true, more = true;
-                while (ok) {
-    #pragma unroll 1
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t s_tmem = tmem + C::kSCol + 128 * x, bit = 1u << x;
-                        if (x < now.tiles) {
-                            ok = !*failed && mbar_wait(&p_full[x], (p_phase >> x) & 1u);
-                            if (ok && x == 0) ok = mbar_wait(&full[(2 * n - 1) % C::kStages], phase(2 * n - 1));
-                            if (ok && now.first) {
-                                if (o_used & bit) ok = mbar_wait(&o_free[x], (o_phase >> x) & 1u);
-                                o_used |= bit;
-                                o_phase ^= bit;
-                            }
-                            if (!ok) break;
-                            p_phase ^= bit;
-                            tc_fence_after();
-                            const uint64_t bd = mnmajor | tile_of(2 * n - 1);
-                            const uint32_t o_tmem = tmem + C::kOCol + 128 * x;
-    #pragma unroll
-                            for (int kk = 0; kk < kChunkKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
-                                tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true),
-                                              !now.first || kk != 0);
-                            if (now.last) tc_commit(&o_full[x]);
-                            if (x == now.tiles - 1) tc_commit(&empty[(2 * n - 1) % C::kStages]);
-                        }
-                        if (more && x < after.tiles) {
-                            if (x == 0) {
-                                if (after.first) ok = !*failed && mbar_wait(q_full, q_items++ & 1);
-                                ok = ok && !*failed && mbar_wait(&full[(2 * n) % C::kStages], phase(2 * n));
-                                if (!ok) break;
-                                tc_fence_after();
-                            }
-                            const uint64_t ad = kmajor | (base + ((C::kQOff + x * C::kTile) >> 4));
-                            const uint64_t bd = kmajor | tile_of(2 * n);
-    #pragma unroll
-                            for (int kk = 0; kk < D / 16; ++kk) {
-                                const uint32_t step = (kk >> 2) * (C::kSlab >> 4) + 2 * (kk & 3);
-                                tc_mma_f16(s_tmem, ad + step, bd + step, chunk_idesc<T>(kChunkKeys, false), kk != 0);
-                            }
-                            tc_commit(&s_full[x]);
-                            if (x == after.tiles - 1) {
-                                tc_commit(&empty[(2 * n) % C::kStages]);
-                                if (after.last) tc_commit(q_empty);
-                            }
-                        }
-                    }
-                    if (!ok || !more) break;
-                    now = after;
-                    ++n;
-                    const int h0 = w.h, t0 = w.t, b0 = w.b;
-                    more = w.next(a, tile_tokens);
-                    if (more) after = step_of(w.h != h0 || w.t != t0 || w.b != b0);
-                }
-                if (!ok) *failed = 1;
-                tc_commit(mma_done);  // arrives once every MMA issued above has completed
+            for (uint32_t i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i) {
+                const uint32_t stage = i % C::kStages;
+                if ((raw_open >> stage) & 1u)
+                    mbar_wait(&raw[stage], ((raw_phase >> stage) & 1u) ^ 1u);
+                else
+                    mbar_wait(&full[stage], phase(i));
             }
             __syncwarp();
+        } else if (warp == kChunkCleanWarp) {
+            // V rows of keys that no row of the item sees: zeros
+            Walk<kChunkKeys> w;
+            uint32_t n = 0, raw_phase = 0;
+            bool more = w.start(a, *shared_range, tile_tokens);
+            for (; more; more = w.next(a, tile_tokens), ++n) {
+                const int key = w.tile.block(w.unit) * kChunkKeys;
+                if (!has_unseen_keys(w.tile, a.window, a.sinks, key)) continue;
+                const uint32_t stage = (2 * n + 1) % C::kStages;
+                if (!__all_sync(0xffffffffu, !*failed && mbar_wait(&raw[stage], (raw_phase >> stage) & 1u))) {
+                    *failed = 1;
+                    break;
+                }
+                raw_phase ^= 1u << stage;
+                uint8_t* tile = ring(2 * n + 1);
+                for (int r = lane; r < kChunkKeys; r += 32)
+                    if (!tile_sees(w.tile, a.window, a.sinks, key + r))
+#pragma unroll
+                        for (int c = 0; c < 2 * D; c += 16)
+                            *reinterpret_cast<uint4*>(tile + (c >> 7) * C::kSlab + r * 128 + (c & 127)) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[stage]);
+            }
+        } else if (lane == 0) {
+            // The MMAs of tile x, one warp each, so that neither waits for the
+            // other's softmax. A step without B is passed on by B's warp at once.
+            const int x = warp - kChunkMmaWarp;
+            // descriptors of byte 0 of shared memory; addresses are added in units of 16 bytes
+            const uint32_t base = smem_addr(smem) >> 4;
+            constexpr uint64_t kmajor = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+            constexpr uint64_t mnmajor = (static_cast<uint64_t>(C::kSlab >> 4) << 16) | (64ull << 32) | (1ull << 46) |
+                                         (2ull << 61);
+            const uint64_t q_desc = kmajor | (base + ((C::kQOff + x * C::kTile) >> 4));
+            const uint32_t s_tmem = tmem + C::kSCol + 128 * x, o_tmem = tmem + C::kOCol + 128 * x;
+            uint32_t stage = 0, turn = 0;  // of the ring: K's, then V's
+            uint32_t q_items = 0, o_items = 0, p_count = 0;
+            bool ok = !*failed, first = false;
+            while (ok) {
+                ok = mbar_wait(&full[stage], turn);
+                if (!ok) break;
+                const uint32_t flag = flags[stage];
+                if (flag & kStepNone) break;
+                const bool active = x == 0 || (flag & kStepTwo);
+                if (flag & kStepFirst) {
+                    ok = mbar_wait(q_full, q_items++ & 1);
+                    if (!ok) break;
+                    first = true;
+                }
+                tc_fence_after();
+                if (active) {
+                    const uint64_t bd = kmajor | (base + ((C::kRingOff + stage * C::kTile) >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t step = (kk >> 2) * (C::kSlab >> 4) + 2 * (kk & 3);
+                        tc_mma_f16(s_tmem, q_desc + step, bd + step, chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                    }
+                    tc_commit(&s_full[x]);
+                    tc_commit(&empty[stage]);
+                    if (flag & kStepLast) tc_commit(q_empty);
+                } else {
+                    mbar_arrive(&empty[stage]);
+                    if (flag & kStepLast) mbar_arrive(q_empty);
+                }
+                if (++stage == C::kStages) stage = 0, turn ^= 1u;
+                if (active) {
+                    const uint64_t bd = mnmajor | (base + ((C::kRingOff + stage * C::kTile) >> 4));
+                    if (first && o_items > 0) ok = mbar_wait(&o_free[x], (o_items - 1) & 1);
+                    ok = ok && mbar_wait(&full[stage], turn) && mbar_wait(&p_full[x], p_count++ & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < kChunkKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                        tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), !first || kk != 0);
+                    if (flag & kStepLast) {
+                        tc_commit(&o_full[x]);
+                        ++o_items;
+                    }
+                    tc_commit(&empty[stage]);
+                    first = false;
+                } else {
+                    // not before the tile has landed: the barrier's last phase is over only then
+                    ok = mbar_wait(&full[stage], turn);
+                    if (!ok) break;
+                    mbar_arrive(&empty[stage]);
+                }
+                if (++stage == C::kStages) stage = 0, turn ^= 1u;
+                if (flag & kStepFinal) break;
+            }
+            if (!ok) *failed = 1;
+            tc_commit(mma_done);  // arrives once every MMA issued above has completed
         }
+        __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kChunkSoftmaxRegs));
+        Walk<kChunkKeys> w;
+        bool more = w.start(a, *shared_range, tile_tokens);
         const int x = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
         const uint32_t s_col = lane_base + C::kSCol + 128 * x, o_col = lane_base + C::kOCol + 128 * x;
         const int token = row / a.group, head = row - token * a.group;
-        bool ok = !*failed, more = true;
+        bool ok = !*failed;
         bool begun = w.unit == 0;  // the item's first unit is in this range
-        uint32_t n = 0;            // the CTA's step
         uint32_t s_count = 0, o_items = 0;
         while (ok && more) {
             const int my_tokens = min(half_tokens, w.tile.tokens - x * half_tokens);
             if (my_tokens <= 0) {  // B has nothing to do for this item
-                const int h0 = w.h, t0 = w.t, b0 = w.b;
-                while ((more = w.next(a, tile_tokens)) && w.h == h0 && w.t == t0 && w.b == b0) ++n;
-                ++n;
+                while (!w.part_ends()) w.next(a, tile_tokens);
+                more = w.next(a, tile_tokens);
                 begun = true;
                 continue;
             }
@@ -311,11 +393,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 const bool all = !valid || (key + kChunkKeys - 1 <= pos &&
                                             (a.window <= 0 || key > pos - a.window || key + kChunkKeys - 1 < a.sinks));
                 if (!__all_sync(0xffffffffu, all)) {
-                    const int upto = pos - key, from = a.window > 0 ? pos - a.window - key : -1;
+                    // visible keys as bits, 32 at a time, and a select each: no branches
+                    const int upto = pos - key + 1, from = a.window > 0 ? pos - a.window - key + 1 : 0;
                     const int sinks = a.window > 0 ? a.sinks - key : 0;
 #pragma unroll
-                    for (int c = 0; c < kChunkKeys; ++c)
-                        sv[c] = c <= upto && (c > from || c < sinks) ? sv[c] : -INFINITY;
+                    for (int c = 0; c < kChunkKeys; c += 32) {
+                        const uint32_t seen = bits_below(upto - c) & (~bits_below(from - c) | bits_below(sinks - c));
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) sv[c + k] = (seen >> k) & 1u ? sv[c + k] : -INFINITY;
+                    }
                 }
                 float top[8];
 #pragma unroll
@@ -343,41 +429,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
                 if (move) m = mx;
                 const float base = m == -INFINITY ? 0.f : kFewOffset - m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t scale2 = pack2(a.scale, a.scale), base2 = pack2(base, base);
+                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int c = 0; c < kChunkKeys; c += 32) {
                     uint32_t p16[16];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        const float p0 = ex2_approx(__fmaf_rn(sv[c + k], a.scale, base));
-                        const float p1 = ex2_approx(__fmaf_rn(sv[c + k + 1], a.scale, base));
-                        sum[(k >> 1) & 3] += p0 + p1;
+                        const float2 y = unpack2(fma2(pack2(sv[c + k], sv[c + k + 1]), scale2, base2));
+                        const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
+                        sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pack2(p0, p1));
                         p16[k / 2] = Pair<T>::pack(p0, p1);
                     }
                     tmem_st16u(s_col + c / 2, p16, 0);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (x == 0 && !(key + kChunkKeys - 1 <= w.tile.p1 &&
-                                (a.window <= 0 || key > w.tile.p0 - a.window || key + kChunkKeys - 1 < a.sinks))) {
-                    // V rows of keys that no row of the item sees (A is part of every item)
-                    ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&full[(2 * n + 1) % C::kStages], phase(2 * n + 1)));
-                    if (!ok) break;
-                    if (!tile_sees(w.tile, a.window, a.sinks, key + row)) {
-#pragma unroll
-                        for (int c = 0; c < C::kTile / 128; c += 16)
-                            *reinterpret_cast<uint4*>(ring(2 * n + 1) + (c >> 7) * C::kSlab + row * 128 + (c & 127)) =
-                                make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
-                }
+                const float2 sums = unpack2(add2(sum[0], sum[1]));
+                l += sums.x + sums.y;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[x]);
-                done = w.unit + 1 >= w.tile.units();
-                if (done || w.left <= 1) break;
+                done = w.item_ends();
+                if (w.part_ends()) break;
                 w.next(a, tile_tokens);
-                ++n;
             }
             if (!ok) break;
             ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&o_full[x], o_items & 1));
@@ -429,10 +503,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             } else {
                 if (valid)
                     __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
-                const long long at = range.end - w.left;  // this unit
-                const long long first = at - w.unit, final = first + w.tile.units() - 1;
-                const int c0 = range_owner(range.total, first, range.ctas);
-                const int c1 = range_owner(range.total, final, range.ctas);
+                const Range range = *shared_range;
+                const int2 owners = item_owners(range, w);
+                const int c0 = owners.x, c1 = owners.y;
                 __threadfence();
                 named_sync(1 + x, 128);
                 if (row == 0) {
@@ -485,7 +558,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 named_sync(1 + x, 128);  // last_part is free again
             }
             more = w.next(a, tile_tokens);
-            ++n;
             begun = true;
         }
         if (!ok) *failed = 1;
@@ -534,8 +606,9 @@ static bool paged_q_map(CUtensorMap* out, const void* base, const h4b_paged_kv* 
 }
 
 template <typename T, int D>
-static int launch_chunk(const AttendArgs& a, const h4b_paged_kv* kv, int sms, cudaStream_t stream) {
+static int launch_chunk(AttendArgs a, const h4b_paged_kv* kv, int sms, cudaStream_t stream) {
     using C = ChunkCfg<D>;
+    a.extra = kChunkExtra;
     static std::atomic<bool> opted_in[kMaxDevices];
     int dev = 0;
     H4B_CUDA_TRY(cudaGetDevice(&dev));
