@@ -12,7 +12,7 @@
 // = thread), 8 issues the loads, 9 and 10 the MMAs of A and B, 11 cleans V
 // tiles (below). Per key block n and tile x:
 //   MMA:     S_x = Q_x K_n^T                              -> s_full[x]
-//   softmax: S_x to registers, maximum, p; P_x over S_x    -> p_full[x]
+//   softmax: S_x to registers, p; P_x over S_x    -> p_half[x] (64 keys), p_full[x]
 //   MMA:     O_x += P_x V_n, then S_x of block n + 1 (the tensor cores run a
 //            CTA's MMAs in issue order, so P_x is read before it is
 //            overwritten)
@@ -62,7 +62,7 @@ struct ChunkCfg {
     static constexpr int kStages = D == 128 ? 5 : 10;
     static constexpr int kQOff = 0, kRingOff = 2 * kTile;
     static constexpr int kBarOff = kRingOff + kStages * kTile;
-    static constexpr int kBars = 3 * kStages + 2 + 8 + 1;
+    static constexpr int kBars = 3 * kStages + 2 + 18 + 1;
     // barriers, words of the CTA, steps' flags, range, alignment slack
     static constexpr int kFlagOff = kBarOff + kBars * 8 + 16, kRangeOff = kFlagOff + kStages * 4 + 4 * (kStages & 1);
     static constexpr int kSmem = kRangeOff + sizeof(Range) + 1024;
@@ -125,7 +125,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint64_t* q_empty = q_full + 1;
     uint64_t* s_full = q_empty + 1;  // [2]
     uint64_t* p_full = s_full + 2;   // [2]
-    uint64_t* o_full = p_full + 2;   // [2]
+    uint64_t* p_half = p_full + 2;   // [2]
+    uint64_t* turn = p_half + 2;     // [2][4]: a warp may form its weights
+    uint64_t* o_full = turn + 8;     // [2]
     uint64_t* o_free = o_full + 2;   // [2]
     uint64_t* mma_done = o_free + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
@@ -153,6 +155,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int x = 0; x < 2; ++x) {
             mbar_init(&s_full[x], 1);
             mbar_init(&p_full[x], 4);
+            mbar_init(&p_half[x], 4);
+            for (int k = 0; k < 4; ++k) mbar_init(&turn[4 * x + k], 1);
             mbar_init(&o_full[x], 1);
             mbar_init(&o_free[x], 4);
         }
@@ -299,11 +303,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                          (2ull << 61);
             const uint64_t q_desc = kmajor | (base + ((C::kQOff + x * C::kTile) >> 4));
             const uint32_t s_tmem = tmem + C::kSCol + 128 * x, o_tmem = tmem + C::kOCol + 128 * x;
-            uint32_t stage = 0, turn = 0;  // of the ring: K's, then V's
+            uint32_t stage = 0, phase = 0;  // of the ring: K's, then V's
             uint32_t q_items = 0, o_items = 0, p_count = 0;
             bool ok = !*failed, first = false;
             while (ok) {
-                ok = mbar_wait(&full[stage], turn);
+                ok = mbar_wait(&full[stage], phase);
                 if (!ok) break;
                 const uint32_t flag = flags[stage];
                 if (flag & kStepNone) break;
@@ -328,16 +332,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     mbar_arrive(&empty[stage]);
                     if (flag & kStepLast) mbar_arrive(q_empty);
                 }
-                if (++stage == C::kStages) stage = 0, turn ^= 1u;
+                if (++stage == C::kStages) stage = 0, phase ^= 1u;
                 if (active) {
                     const uint64_t bd = mnmajor | (base + ((C::kRingOff + stage * C::kTile) >> 4));
                     if (first && o_items > 0) ok = mbar_wait(&o_free[x], (o_items - 1) & 1);
-                    ok = ok && mbar_wait(&full[stage], turn) && mbar_wait(&p_full[x], p_count++ & 1);
+                    ok = ok && mbar_wait(&full[stage], phase) && mbar_wait(&p_half[x], p_count & 1);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int kk = 0; kk < kChunkKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                    for (int kk = 0; kk < kChunkKeys / 32; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
                         tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), !first || kk != 0);
+                    ok = mbar_wait(&p_full[x], p_count++ & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = kChunkKeys / 32; kk < kChunkKeys / 16; ++kk)
+                        tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), 1);
                     if (flag & kStepLast) {
                         tc_commit(&o_full[x]);
                         ++o_items;
@@ -346,11 +356,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     first = false;
                 } else {
                     // not before the tile has landed: the barrier's last phase is over only then
-                    ok = mbar_wait(&full[stage], turn);
+                    ok = mbar_wait(&full[stage], phase);
                     if (!ok) break;
                     mbar_arrive(&empty[stage]);
                 }
-                if (++stage == C::kStages) stage = 0, turn ^= 1u;
+                if (++stage == C::kStages) stage = 0, phase ^= 1u;
                 if (flag & kStepFinal) break;
             }
             if (!ok) *failed = 1;
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int token = row / a.group, head = row - token * a.group;
         bool ok = !*failed;
         bool begun = w.unit == 0;  // the item's first unit is in this range
-        uint32_t s_count = 0, o_items = 0;
+        uint32_t s_count = 0, o_items = 0, turns = 0;
         while (ok && more) {
             const int my_tokens = min(half_tokens, w.tile.tokens - x * half_tokens);
             if (my_tokens <= 0) {  // B has nothing to do for this item
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             float m = -INFINITY, l = 0.f;
             bool done = false;
             while (true) {
-                ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&s_full[x], s_count & 1));
+                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[x], s_count & 1));
                 if (!ok) break;
                 ++s_count;
                 tc_fence_after();
@@ -403,6 +413,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         for (int k = 0; k < 32; ++k) sv[c + k] = (seen >> k) & 1u ? sv[c + k] : -INFINITY;
                     }
                 }
+                // A and B take turns at the exponentials (warp w of each on one
+                // sub-partition), so that one's run while the other's MMAs do.
+                if (w.tile.tokens > half_tokens) {
+                    if (x == 1 || turns > 0)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&turn[4 * x + (warp & 3)], (turns - 1 + x) & 1));
+                    if (!ok) break;
+                    ++turns;
+                }
+                uint64_t sum[2];
+                auto weights = [&](int c0) {  // p of 32 keys, to the P columns
+                    const float base = m == -INFINITY ? 0.f : kFewOffset - m;
+                    const uint64_t scale2 = pack2(a.scale, a.scale), base2 = pack2(base, base);
+                    uint32_t p16[16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float2 y = unpack2(fma2(pack2(sv[c0 + k], sv[c0 + k + 1]), scale2, base2));
+                        const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
+                        sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pack2(p0, p1));
+                        p16[k / 2] = Pair<T>::pack(p0, p1);
+                    }
+                    tmem_st16u(s_col + c0 / 2, p16, 0);
+                };
+                // The first half's p with the m of the blocks before, while the
+                // maximum of all scores is found beside it; where it passes
+                // m + slack (always at first) m moves and they are formed anew.
+                sum[0] = sum[1] = 0ull;
+                weights(0);
+                weights(32);
                 float top[8];
 #pragma unroll
                 for (int c = 0; c < 8; ++c) top[c] = fmaxf(sv[c], sv[c + 8]);
@@ -413,42 +451,41 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 const float mx = a.scale * fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
                                                  fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
                 const bool move = valid && mx > m + kFewSlack;
-                if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
-                    // P V of every earlier block has completed (see above)
-                    const float f = move ? ex2_approx(m - mx) : 1.f;  // 0 for m = -inf, whose l and O are 0
-                    l *= f;
+                if (__any_sync(0xffffffffu, move)) {
+                    if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
+                        // P V of every earlier block has completed (see above)
+                        const float f = move ? ex2_approx(m - mx) : 1.f;  // 0 for m = -inf, whose l and O are 0
+                        l *= f;
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {  // rare: few registers beside the scores
-                        float v[16];
-                        tmem_ld16_nowait(o_col + c, v, 0);
-                        tmem_wait_regs(v);
+                        for (int c = 0; c < D; c += 16) {  // rare: few registers beside the scores
+                            float v[16];
+                            tmem_ld16_nowait(o_col + c, v, 0);
+                            tmem_wait_regs(v);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) v[k] *= f;
-                        tmem_st16(o_col + c, v, 0);
+                            for (int k = 0; k < 16; ++k) v[k] *= f;
+                            tmem_st16(o_col + c, v, 0);
+                        }
                     }
+                    if (move) m = mx;
+                    sum[0] = sum[1] = 0ull;
+                    weights(0);
+                    weights(32);
                 }
-                if (move) m = mx;
-                const float base = m == -INFINITY ? 0.f : kFewOffset - m;
-                const uint64_t scale2 = pack2(a.scale, a.scale), base2 = pack2(base, base);
-                uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                for (int c = 0; c < kChunkKeys; c += 32) {
-                    uint32_t p16[16];
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float2 y = unpack2(fma2(pack2(sv[c + k], sv[c + k + 1]), scale2, base2));
-                        const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
-                        sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pack2(p0, p1));
-                        p16[k / 2] = Pair<T>::pack(p0, p1);
-                    }
-                    tmem_st16u(s_col + c / 2, p16, 0);
-                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_half[x]);
+                weights(64);
+                weights(96);
                 const float2 sums = unpack2(add2(sum[0], sum[1]));
                 l += sums.x + sums.y;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[x]);
+                if (lane == 0) {
+                    mbar_arrive(&p_full[x]);
+                    if (w.tile.tokens > half_tokens) mbar_arrive(&turn[4 * (x ^ 1) + (warp & 3)]);
+                }
                 done = w.item_ends();
                 if (w.part_ends()) break;
                 w.next(a, tile_tokens);
