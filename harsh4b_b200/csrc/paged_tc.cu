@@ -78,6 +78,18 @@ __host__ __device__ constexpr uint32_t chunk_idesc(int n, bool b_mn_major) {
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kChunkRows >> 4) << 24);
 }
 
+// True in one lane of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+// mbar_wait by a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -292,79 +304,97 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[stage]);
             }
-        } else if (lane == 0) {
+        } else {
             // The MMAs of tile x, one warp each, so that neither waits for the
             // other's softmax. A step without B is passed on by B's warp at once.
-            const int x = warp - kChunkMmaWarp;
+            // The whole warp runs the loop on uniform values and one elected
+            // lane issues: the MMAs' operands then stay in uniform registers.
+            const int x = __shfl_sync(0xffffffffu, warp, 0) - kChunkMmaWarp;
             // descriptors of byte 0 of shared memory; addresses are added in units of 16 bytes
-            const uint32_t base = smem_addr(smem) >> 4;
+            const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0) >> 4;
             constexpr uint64_t kmajor = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
             constexpr uint64_t mnmajor = (static_cast<uint64_t>(C::kSlab >> 4) << 16) | (64ull << 32) | (1ull << 46) |
                                          (2ull << 61);
             const uint64_t q_desc = kmajor | (base + ((C::kQOff + x * C::kTile) >> 4));
-            const uint32_t s_tmem = tmem + C::kSCol + 128 * x, o_tmem = tmem + C::kOCol + 128 * x;
+            const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t s_tmem = t0 + C::kSCol + 128 * x, o_tmem = t0 + C::kOCol + 128 * x;
             uint32_t stage = 0, phase = 0;  // of the ring: K's, then V's
             uint32_t q_items = 0, o_items = 0, p_count = 0;
-            bool ok = !*failed, first = false;
-            while (ok) {
-                ok = mbar_wait(&full[stage], phase);
-                if (!ok) break;
-                const uint32_t flag = flags[stage];
-                if (flag & kStepNone) break;
+            bool ok = !*failed && warp_wait(&full[0], 0), first = false;
+            uint32_t flag = ok ? flags[0] : 0u;
+            if (flag & kStepNone) ok = false;
+            bool none = (flag & kStepNone) != 0;
+            while (ok) {  // K of this step has landed
                 const bool active = x == 0 || (flag & kStepTwo);
+                const uint32_t k_stage = stage;
                 if (flag & kStepFirst) {
-                    ok = mbar_wait(q_full, q_items++ & 1);
+                    ok = warp_wait(q_full, q_items++ & 1);
                     if (!ok) break;
                     first = true;
                 }
                 tc_fence_after();
                 if (active) {
-                    const uint64_t bd = kmajor | (base + ((C::kRingOff + stage * C::kTile) >> 4));
+                    if (elect_one()) {
+                        const uint64_t bd = kmajor | (base + ((C::kRingOff + k_stage * C::kTile) >> 4));
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t step = (kk >> 2) * (C::kSlab >> 4) + 2 * (kk & 3);
-                        tc_mma_f16(s_tmem, q_desc + step, bd + step, chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t step = (kk >> 2) * (C::kSlab >> 4) + 2 * (kk & 3);
+                            tc_mma_f16(s_tmem, q_desc + step, bd + step, chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                        }
+                        tc_commit(&s_full[x]);
+                        tc_commit(&empty[k_stage]);
+                        if (flag & kStepLast) tc_commit(q_empty);
                     }
-                    tc_commit(&s_full[x]);
-                    tc_commit(&empty[stage]);
-                    if (flag & kStepLast) tc_commit(q_empty);
-                } else {
-                    mbar_arrive(&empty[stage]);
+                } else if (lane == 0) {
+                    mbar_arrive(&empty[k_stage]);
                     if (flag & kStepLast) mbar_arrive(q_empty);
                 }
+                __syncwarp();
                 if (++stage == C::kStages) stage = 0, phase ^= 1u;
-                if (active) {
-                    const uint64_t bd = mnmajor | (base + ((C::kRingOff + stage * C::kTile) >> 4));
-                    if (first && o_items > 0) ok = mbar_wait(&o_free[x], (o_items - 1) & 1);
-                    ok = ok && mbar_wait(&full[stage], phase) && mbar_wait(&p_half[x], p_count & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int kk = 0; kk < kChunkKeys / 32; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
-                        tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), !first || kk != 0);
-                    ok = mbar_wait(&p_full[x], p_count++ & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int kk = kChunkKeys / 32; kk < kChunkKeys / 16; ++kk)
-                        tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), 1);
-                    if (flag & kStepLast) {
-                        tc_commit(&o_full[x]);
-                        ++o_items;
-                    }
-                    tc_commit(&empty[stage]);
-                    first = false;
-                } else {
-                    // not before the tile has landed: the barrier's last phase is over only then
-                    ok = mbar_wait(&full[stage], phase);
-                    if (!ok) break;
-                    mbar_arrive(&empty[stage]);
+                const uint32_t v_stage = stage, v_phase = phase;
+                if (++stage == C::kStages) stage = 0, phase ^= 1u;
+                ok = warp_wait(&full[v_stage], v_phase);
+                // the next step's K now, so that its S follows this step's P V at once
+                uint32_t next_flag = 0;
+                if (ok && !(flag & kStepFinal)) {
+                    ok = warp_wait(&full[stage], phase);
+                    next_flag = flags[stage];
                 }
-                if (++stage == C::kStages) stage = 0, phase ^= 1u;
+                if (!ok) break;
+                if (active) {
+                    if (first && o_items > 0) ok = warp_wait(&o_free[x], (o_items - 1) & 1);
+                    ok = ok && warp_wait(&p_half[x], p_count & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t bd = mnmajor | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = 0; kk < kChunkKeys / 32; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true),
+                                          !first || kk != 0);
+                    }
+                    __syncwarp();
+                    ok = warp_wait(&p_full[x], p_count++ & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = kChunkKeys / 32; kk < kChunkKeys / 16; ++kk)
+                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), 1);
+                        if (flag & kStepLast) tc_commit(&o_full[x]);
+                        tc_commit(&empty[v_stage]);
+                    }
+                    if (flag & kStepLast) ++o_items;
+                    first = false;
+                } else if (lane == 0) {
+                    mbar_arrive(&empty[v_stage]);
+                }
+                __syncwarp();
                 if (flag & kStepFinal) break;
+                flag = next_flag;
             }
-            if (!ok) *failed = 1;
-            tc_commit(mma_done);  // arrives once every MMA issued above has completed
+            if (!ok && !none) *failed = 1;
+            if (elect_one()) tc_commit(mma_done);  // arrives once every MMA issued above has completed
         }
         __syncwarp();
     } else {
@@ -391,7 +421,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             float m = -INFINITY, l = 0.f;
             bool done = false;
             while (true) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[x], s_count & 1));
+                ok = warp_wait(&s_full[x], s_count & 1);
                 if (!ok) break;
                 ++s_count;
                 tc_fence_after();
@@ -417,7 +447,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 // sub-partition), so that one's run while the other's MMAs do.
                 if (w.tile.tokens > half_tokens) {
                     if (x == 1 || turns > 0)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&turn[4 * x + (warp & 3)], (turns - 1 + x) & 1));
+                        ok = warp_wait(&turn[4 * x + (warp & 3)], (turns - 1 + x) & 1);
                     if (!ok) break;
                     ++turns;
                 }
@@ -491,7 +521,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 w.next(a, tile_tokens);
             }
             if (!ok) break;
-            ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&o_full[x], o_items & 1));
+            ok = warp_wait(&o_full[x], o_items & 1);
             if (!ok) break;
             ++o_items;
             tc_fence_after();
