@@ -23,10 +23,16 @@
 //
 // Operands: Q and the K/V ring in shared memory in the 128-byte swizzle
 // layout, 64 values (128 bytes) of head_dim a row, one slab per 64; P in
-// tensor memory. A tile's 128 keys are 128 / page_size boxes of one page each
-// (or one box inside a page), issued by the lanes of the load warp at the same
-// time; a page that is not there is a box outside the tensor, which reads as
-// zeros. Q is one box per slab: group heads x 128 / group tokens.
+// tensor memory. A K/V tile is 16 groups of 8 keys, each group its slabs of 8
+// rows one after the other, so that a page of any size is one contiguous part
+// of the tile and one 5-D box (64 values x 8 rows x slabs x groups x page): a
+// box costs the copy engine about 50 cycles beside its bytes, and with boxes
+// of one slab 16-token pages came at 24 bytes a cycle and SM, now at 34 (32
+// KB tiles from L2, 148 SMs; 64-token pages 43 and 50). A tile's 128 keys are
+// 128 / page_size boxes (or one box inside a page), issued by the lanes of the
+// load warp at the same time; a page that is not there is a box outside the
+// tensor, which reads as zeros. Q is one box per slab: group heads x 128 /
+// group tokens.
 //
 // Softmax in base 2 with a lazily moved reference, as in the kernel of few
 // rows: p = 2^(s - m + 8), m moves when a score passes m + 7.
@@ -57,7 +63,8 @@ static_assert(2 * kChunkSoftmaxRegs + kChunkOtherRegs <= 3 * 168, "registers of 
 template <int D>
 struct ChunkCfg {
     static constexpr int kSlabs = D / 64;                        // 64 values of head_dim each
-    static constexpr int kSlab = 128 * 128;                      // 128 rows x 128 bytes
+    static constexpr int kSlab = 128 * 128;                      // of Q: 128 rows x 128 bytes
+    static constexpr int kGroup = kSlabs * 1024;                 // of K or V: 8 keys, all slabs
     static constexpr int kTile = kSlabs * kSlab;                 // 128 keys (or query rows)
     static constexpr int kStages = D == 128 ? 5 : 10;
     static constexpr int kQOff = 0, kRingOff = 2 * kTile;
@@ -76,6 +83,15 @@ __host__ __device__ constexpr uint32_t chunk_idesc(int n, bool b_mn_major) {
     constexpr uint32_t format = Pair<T>::kBf16 ? 1u : 0u;
     return (1u << 4) | (format << 7) | (format << 10) | (b_mn_major ? 1u << 16 : 0u) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kChunkRows >> 4) << 24);
+}
+
+// Groups `group`.. of a page's head into a K/V tile.
+__device__ __forceinline__ void tma_load_tile(void* dst, const CUtensorMap* map, int group, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, "
+        "%4}], [%5];"
+        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(group), "r"(page), "r"(smem_addr(bar))
+        : "memory");
 }
 
 // True in one lane of the (converged) warp.
@@ -112,6 +128,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t y) {
+    const float2 v = unpack2(y);
+    return pack2(ex2_approx(v.x), ex2_approx(v.y));
+}
 // Whether the block of keys from `key` on has one that no row of the tile sees.
 __device__ __forceinline__ bool has_unseen_keys(const Tile& t, int window, int sinks, int key) {
     const int end = key + kChunkKeys - 1;
@@ -196,12 +216,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kChunkOtherRegs));
         if (warp == kChunkLoadWarp) {
             Walk<kChunkKeys> w;
-            // Each lane one box: page `lane / kSlabs` of the tile, slab `lane % kSlabs`.
-            const int page_size = 1 << a.p.page_shift, box = min(page_size, kChunkKeys);
-            const int boxes = kChunkKeys / box, my_page = lane / C::kSlabs, my_slab = lane % C::kSlabs;
-            const bool mine = my_page < boxes;
+            const int page_size = 1 << a.p.page_shift, box = min(page_size, kChunkKeys);  // a box: keys of one page
+            const int boxes = kChunkKeys / box;
+            const bool mine = lane < boxes;  // each lane one box
             auto page_of = [&](const Walk<kChunkKeys>& u) -> int {  // -1: read as zeros
-                const int key = u.tile.block(u.unit) * kChunkKeys + my_page * box;
+                const int key = u.tile.block(u.unit) * kChunkKeys + lane * box;
                 const Tile& t = u.tile;
                 if (!mine || key > t.p1 || !(a.window <= 0 || key + box - 1 > t.p0 - a.window || key < a.sinks)) return -1;
                 const int page = a.p.table[static_cast<long long>(u.b) * a.p.table_stride + (key >> a.p.page_shift)];
@@ -231,7 +250,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         mbar_arrive_expect_tx(q_full, tiles * C::kSlabs * half_tokens * a.group * 128);
                     __syncwarp();
                     if (lane < tiles * C::kSlabs) {
-                        const int x = lane / C::kSlabs;
+                        const int x = lane / C::kSlabs, my_slab = lane % C::kSlabs;
                         tma_load_3d(smem + C::kQOff + x * C::kTile + my_slab * C::kSlab, &qmap, my_slab * 64,
                                     w.h * a.group, w.tile.first + x * half_tokens, q_full);
                     }
@@ -261,8 +280,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     }
                     __syncwarp();
                     if (mine)
-                        tma_load_3d(ring(issued) + my_slab * C::kSlab + my_page * box * 128, v ? &vmap : &kmap,
-                                    my_slab * 64, y, z, bar);
+                        tma_load_tile(ring(issued) + lane * box * 2 * D, v ? &vmap : &kmap, y >> 3, z, bar);
                     if (v == 1 && unclean) raw_phase ^= 1u << stage, raw_open |= 1u << stage;
                     else raw_open &= ~(1u << stage);
                     ++issued;
@@ -298,8 +316,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (!tile_sees(w.tile, a.window, a.sinks, key + r))
 #pragma unroll
                         for (int c = 0; c < 2 * D; c += 16)
-                            *reinterpret_cast<uint4*>(tile + (c >> 7) * C::kSlab + r * 128 + (c & 127)) =
-                                make_uint4(0u, 0u, 0u, 0u);
+                            *reinterpret_cast<uint4*>(tile + (r >> 3) * C::kGroup + (c >> 7) * 1024 + (r & 7) * 128 +
+                                                      (c & 127)) = make_uint4(0u, 0u, 0u, 0u);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[stage]);
@@ -312,13 +330,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const int x = __shfl_sync(0xffffffffu, warp, 0) - kChunkMmaWarp;
             // descriptors of byte 0 of shared memory; addresses are added in units of 16 bytes
             const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0) >> 4;
-            constexpr uint64_t kmajor = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-            constexpr uint64_t mnmajor = (static_cast<uint64_t>(C::kSlab >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-                                         (2ull << 61);
-            const uint64_t q_desc = kmajor | (base + ((C::kQOff + x * C::kTile) >> 4));
+            // (swizzle 128 bytes; 8-row groups 1024 bytes apart in Q, kGroup in a K/V
+            // tile; V, read along its rows, has its next 64 values 1024 bytes on)
+            constexpr uint64_t common = (1ull << 46) | (2ull << 61);
+            constexpr uint64_t q_major = common | (1ull << 16) | (64ull << 32);
+            constexpr uint64_t k_major = common | (1ull << 16) | (static_cast<uint64_t>(C::kGroup >> 4) << 32);
+            constexpr uint64_t v_major = common | (64ull << 16) | (static_cast<uint64_t>(C::kGroup >> 4) << 32);
+            const uint64_t q_desc = q_major | (base + ((C::kQOff + x * C::kTile) >> 4));
             const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
             const uint32_t s_tmem = t0 + C::kSCol + 128 * x, o_tmem = t0 + C::kOCol + 128 * x;
             uint32_t stage = 0, phase = 0;  // of the ring: K's, then V's
+            uint32_t v_done = C::kStages;   // V stage whose release is due (none)
             uint32_t q_items = 0, o_items = 0, p_count = 0;
             bool ok = !*failed && warp_wait(&full[0], 0), first = false;
             uint32_t flag = ok ? flags[0] : 0u;
@@ -333,22 +355,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     first = true;
                 }
                 tc_fence_after();
-                if (active) {
-                    if (elect_one()) {
-                        const uint64_t bd = kmajor | (base + ((C::kRingOff + k_stage * C::kTile) >> 4));
+                if (elect_one()) {
+                    if (active) {
+                        const uint64_t bd = k_major | (base + ((C::kRingOff + k_stage * C::kTile) >> 4));
 #pragma unroll
                         for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t step = (kk >> 2) * (C::kSlab >> 4) + 2 * (kk & 3);
-                            tc_mma_f16(s_tmem, q_desc + step, bd + step, chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                            const uint32_t in_slab = 2 * (kk & 3), slab = kk >> 2;  // 16 values: 32 bytes
+                            tc_mma_f16(s_tmem, q_desc + slab * (C::kSlab >> 4) + in_slab, bd + slab * 64 + in_slab,
+                                       chunk_idesc<T>(kChunkKeys, false), kk != 0);
                         }
                         tc_commit(&s_full[x]);
+                    }
+                    if (v_done < C::kStages) tc_commit(&empty[v_done]);
+                    if (active) {
                         tc_commit(&empty[k_stage]);
                         if (flag & kStepLast) tc_commit(q_empty);
+                    } else {
+                        mbar_arrive(&empty[k_stage]);
+                        if (flag & kStepLast) mbar_arrive(q_empty);
                     }
-                } else if (lane == 0) {
-                    mbar_arrive(&empty[k_stage]);
-                    if (flag & kStepLast) mbar_arrive(q_empty);
                 }
+                v_done = C::kStages;
                 __syncwarp();
                 if (++stage == C::kStages) stage = 0, phase ^= 1u;
                 const uint32_t v_stage = stage, v_phase = phase;
@@ -366,11 +393,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     ok = ok && warp_wait(&p_half[x], p_count & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t bd = mnmajor | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
+                    const uint64_t bd = v_major | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = 0; kk < kChunkKeys / 32; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
-                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true),
+                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * (C::kGroup >> 3), chunk_idesc<T>(D, true),
                                           !first || kk != 0);
                     }
                     __syncwarp();
@@ -380,10 +407,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = kChunkKeys / 32; kk < kChunkKeys / 16; ++kk)
-                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * 128, chunk_idesc<T>(D, true), 1);
+                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * (C::kGroup >> 3), chunk_idesc<T>(D, true), 1);
                         if (flag & kStepLast) tc_commit(&o_full[x]);
-                        tc_commit(&empty[v_stage]);
+                        if (flag & kStepFinal) tc_commit(&empty[v_stage]);
                     }
+                    v_done = v_stage;  // released after the next S, which nothing should hold up
                     if (flag & kStepLast) ++o_items;
                     first = false;
                 } else if (lane == 0) {
@@ -425,61 +453,73 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (!ok) break;
                 ++s_count;
                 tc_fence_after();
-                float sv[kChunkKeys];
+                constexpr int kHalf = kChunkKeys / 2;
+                float s1[kHalf], s2[kHalf];  // the scores of the first and the last 64 keys
 #pragma unroll
-                for (int c = 0; c < kChunkKeys; c += 16) tmem_ld16_nowait(s_col + c, sv, c);
-                tmem_wait_regs(sv);
+                for (int c = 0; c < kHalf; c += 16) tmem_ld16_nowait(s_col + c, s1, c);
+                tmem_wait_regs(s1);
+#pragma unroll
+                for (int c = 0; c < kHalf; c += 16) tmem_ld16_nowait(s_col + kHalf + c, s2, c);
                 const int key = w.tile.block(w.unit) * kChunkKeys;
                 const bool all = !valid || (key + kChunkKeys - 1 <= pos &&
                                             (a.window <= 0 || key > pos - a.window || key + kChunkKeys - 1 < a.sinks));
-                if (!__all_sync(0xffffffffu, all)) {
+                const bool masked = !__all_sync(0xffffffffu, all);
+                auto mask = [&](float (&v)[kHalf], int first) {
                     // visible keys as bits, 32 at a time, and a select each: no branches
-                    const int upto = pos - key + 1, from = a.window > 0 ? pos - a.window - key + 1 : 0;
-                    const int sinks = a.window > 0 ? a.sinks - key : 0;
+                    const int upto = pos - first + 1, from = a.window > 0 ? pos - a.window - first + 1 : 0;
+                    const int sinks = a.window > 0 ? a.sinks - first : 0;
 #pragma unroll
-                    for (int c = 0; c < kChunkKeys; c += 32) {
+                    for (int c = 0; c < kHalf; c += 32) {
                         const uint32_t seen = bits_below(upto - c) & (~bits_below(from - c) | bits_below(sinks - c));
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) sv[c + k] = (seen >> k) & 1u ? sv[c + k] : -INFINITY;
+                        for (int k = 0; k < 32; ++k) v[c + k] = (seen >> k) & 1u ? v[c + k] : -INFINITY;
                     }
-                }
+                };
+                if (masked) mask(s1, key);
                 // A and B take turns at the exponentials (warp w of each on one
                 // sub-partition), so that one's run while the other's MMAs do.
                 if (w.tile.tokens > half_tokens) {
-                    if (x == 1 || turns > 0)
-                        ok = warp_wait(&turn[4 * x + (warp & 3)], (turns - 1 + x) & 1);
+                    if (x == 1 || turns > 0) ok = warp_wait(&turn[4 * x + (warp & 3)], (turns - 1 + x) & 1);
                     if (!ok) break;
                     ++turns;
                 }
-                uint64_t sum[2];
-                auto weights = [&](int c0) {  // p of 32 keys, to the P columns
+                uint64_t sum[2] = {0ull, 0ull};
+                auto weights = [&](const float (&v)[kHalf], int column) {  // p of 64 keys, to the P columns
                     const float base = m == -INFINITY ? 0.f : kFewOffset - m;
                     const uint64_t scale2 = pack2(a.scale, a.scale), base2 = pack2(base, base);
-                    uint32_t p16[16];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float2 y = unpack2(fma2(pack2(sv[c0 + k], sv[c0 + k + 1]), scale2, base2));
-                        const float p0 = ex2_approx(y.x), p1 = ex2_approx(y.y);
-                        sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], pack2(p0, p1));
-                        p16[k / 2] = Pair<T>::pack(p0, p1);
+                    for (int c = 0; c < kHalf; c += 32) {
+                        uint32_t p16[16];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            const uint64_t y = fma2(pack2(v[c + k], v[c + k + 1]), scale2, base2);
+                            const uint64_t p2 = exp2_pair(y);
+                            sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], p2);
+                            const float2 p = unpack2(p2);
+                            p16[k / 2] = Pair<T>::pack(p.x, p.y);
+                        }
+                        tmem_st16u(s_col + column + c / 2, p16, 0);
                     }
-                    tmem_st16u(s_col + c0 / 2, p16, 0);
+                };
+                auto largest = [&](const float (&v)[kHalf]) {
+                    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                    for (int c = 4; c < kHalf - 4; c += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(top[k], v[c + k]), v[c + k + 4]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], v[kHalf - 4 + k]);
+                    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 };
                 // The first half's p with the m of the blocks before, while the
-                // maximum of all scores is found beside it; where it passes
-                // m + slack (always at first) m moves and they are formed anew.
-                sum[0] = sum[1] = 0ull;
-                weights(0);
-                weights(32);
-                float top[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) top[c] = fmaxf(sv[c], sv[c + 8]);
-#pragma unroll
-                for (int c = 16; c < kChunkKeys; c += 16)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) top[k] = fmaxf(fmaxf(top[k], sv[c + k]), sv[c + k + 8]);
-                const float mx = a.scale * fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
-                                                 fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+                // second half's scores arrive and the maximum is found beside
+                // it. Where that passes m + slack (always at a row's first
+                // keys) m moves and they are formed anew.
+                weights(s1, 0);
+                const float mx1 = largest(s1);
+                tmem_wait_regs(s2);
+                if (masked) mask(s2, key + kHalf);
+                const float mx = a.scale * fmaxf(mx1, largest(s2));
                 const bool move = valid && mx > m + kFewSlack;
                 if (__any_sync(0xffffffffu, move)) {
                     if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
@@ -498,15 +538,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     }
                     if (move) m = mx;
                     sum[0] = sum[1] = 0ull;
-                    weights(0);
-                    weights(32);
+                    weights(s1, 0);
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_half[x]);
-                weights(64);
-                weights(96);
+                weights(s2, kHalf / 2);
                 const float2 sums = unpack2(add2(sum[0], sum[1]));
                 l += sums.x + sums.y;
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -639,17 +677,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
 }
 
-// A layer's pages as a 3-D tensor map [pages * kv_heads][page_size][D] with
-// boxes of 64 values x min(page_size, 128) rows.
+// A layer's pages [pages * kv_heads][page_size][D] as a 5-D tensor map (value,
+// row of its group of 8, slab of 64 values, group, page and head).
 static bool paged_kv_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv) {
     auto encode = tensor_map_encoder();
     if (!encode) return false;
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kv->head_dim), static_cast<cuuint64_t>(kv->page_size),
+    const cuuint64_t row = kv->head_dim * 2ull;
+    const cuuint32_t slabs = kv->head_dim / 64, box_rows = kv->page_size < kChunkKeys ? kv->page_size : kChunkKeys;
+    const cuuint64_t dims[5] = {64, 8, slabs, static_cast<cuuint64_t>(kv->page_size) / 8,
                                 static_cast<cuuint64_t>(kv->pages) * kv->kv_heads};
-    const cuuint64_t strides[2] = {kv->head_dim * 2ull, static_cast<cuuint64_t>(kv->page_size) * kv->head_dim * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(kv->page_size < kChunkKeys ? kv->page_size : kChunkKeys), 1};
-    const cuuint32_t elem[3] = {1, 1, 1};
-    return encode(out, kv->dtype == H4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+    const cuuint64_t strides[4] = {row, 128, 8 * row, kv->page_size * row};
+    const cuuint32_t box[5] = {64, 8, slabs, box_rows / 8, 1};
+    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    return encode(out, kv->dtype == H4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
                   const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
