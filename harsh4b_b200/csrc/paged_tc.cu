@@ -106,6 +106,27 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
+// 4 x 4 transpose among the lanes of a quad: v[k] of lane i <-> v[i] of lane k.
+// A row's 64 bytes then leave with one store of its quad; with one thread a
+// row every store touched 32 rows and took 32 turns at the memory pipe.
+__device__ __forceinline__ void quad_transpose(uint32_t (&v)[16]) {  // v[4 k + e]: word e of 16-byte unit k
+#pragma unroll
+    for (int step = 1; step <= 2; step <<= 1) {
+        const bool odd = (threadIdx.x & step) != 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k & step) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t low = v[4 * k + e], high = v[4 * (k | step) + e];
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? low : high, step);
+                v[4 * k + e] = odd ? other : low;
+                v[4 * (k | step) + e] = odd ? high : other;
+            }
+        }
+    }
+}
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -568,14 +589,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const bool whole = begun && done;
             const long long out_row = w.tile.first + x * half_tokens + (valid ? token : 0);
             const int out_head = w.h * a.group + head;
-            T* out = static_cast<T*>(a.out) + out_row * a.out_stride + out_head * D;
+            T* out_tile = static_cast<T*>(a.out) + (w.tile.first + x * half_tokens) * a.out_stride + w.h * a.group * D;
+            const long long my_place = valid ? token * a.out_stride + head * D : -1;
+            long long to[4];  // the places of the quad's four rows
+#pragma unroll
+            for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, my_place, (lane & 28) + k);
             constexpr int kPart = kChunkRows * (D + 2);
             auto part_of = [&](int cta, int which) {
                 return a.partials + (static_cast<long long>(2 * cta + which) * 2 + x) * kPart;
             };
             // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
             float4* part = reinterpret_cast<float4*>(part_of(blockIdx.x, begun ? 1 : 0));
-            const float inv = whole && l != 0.f ? 1.0f / l : (whole ? 0.f : 1.f);
+            const float inv = 1.0f / l;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float v[32];
@@ -583,15 +608,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 tmem_ld16_nowait(o_col + c + 16, v, 16);
                 tmem_wait_regs(v);
                 if (whole) {
-                    if (valid && l == 0.f)
+                    uint32_t o16[16];
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = 0.f;
-                    if (valid)
+                    for (int k = 0; k < 16; ++k)  // a row without keys: its O was never formed
+                        o16[k] = l == 0.f ? 0u : Pair<T>::pack(v[2 * k] * inv, v[2 * k + 1] * inv);
+                    quad_transpose(o16);
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8)
-                            *reinterpret_cast<uint4*>(out + c + k) = make_uint4(
-                                Pair<T>::pack(v[k] * inv, v[k + 1] * inv), Pair<T>::pack(v[k + 2] * inv, v[k + 3] * inv),
-                                Pair<T>::pack(v[k + 4] * inv, v[k + 5] * inv), Pair<T>::pack(v[k + 6] * inv, v[k + 7] * inv));
+                    for (int k = 0; k < 4; ++k)
+                        if (to[k] >= 0)
+                            *reinterpret_cast<uint4*>(out_tile + to[k] + c + 8 * (lane & 3)) =
+                                make_uint4(o16[4 * k], o16[4 * k + 1], o16[4 * k + 2], o16[4 * k + 3]);
                 } else if (valid) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
@@ -651,7 +677,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                             }
 #pragma unroll
                             for (int k = 0; k < 8; k += 2)
-                                *reinterpret_cast<uint4*>(out + 4 * (c + k)) =
+                                *reinterpret_cast<uint4*>(out_tile + my_place + 4 * (c + k)) =
                                     make_uint4(Pair<T>::pack(v[k].x, v[k].y), Pair<T>::pack(v[k].z, v[k].w),
                                                Pair<T>::pack(v[k + 1].x, v[k + 1].y), Pair<T>::pack(v[k + 1].z, v[k + 1].w));
                         }
