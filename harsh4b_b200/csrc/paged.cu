@@ -970,10 +970,11 @@ static int launch_few(AttendArgs a, int sms, cudaStream_t stream) {
 template <typename T, int D>
 static int launch_attention(const AttendArgs& a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     const long long rows = static_cast<long long>(max_query) * a.group;
-    if (rows > kFewMaxRows) return launch_chunk<T, D>(a, kv, sms, stream);
     if (rows <= 8) return launch_few<T, D, 8>(a, sms, stream);
     if (rows <= 16) return launch_few<T, D, 16>(a, sms, stream);
-    return launch_few<T, D, 32>(a, sms, stream);
+    if constexpr (D == 64)
+        if (rows <= 32) return launch_few<T, D, 32>(a, sms, stream);
+    return launch_chunk<T, D>(a, kv, sms, stream);
 }
 
 }  // namespace h4b

@@ -231,34 +231,40 @@ def residual_acc(x: torch.Tensor, acc: torch.Tensor, absmax: torch.Tensor, scale
 
 
 # ---- paged K/V cache -------------------------------------------------------------
+# A decode step calls these once a layer, so what they do on the host is kept
+# to a few microseconds: one pass over the tensors' attributes, one C call.
 _PAGED_DTYPES = {torch.float16: 1, torch.bfloat16: 2}  # H4B_FP16, H4B_BF16
 
 
 def _rows(tensor: torch.Tensor, dtype: torch.dtype, name: str) -> int:
     """Data pointer of a CUDA tensor whose rows (dim 0) may be strided."""
-    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if tensor.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {tensor.dtype}")
-    if not tensor.is_contiguous() and tensor.numel() and not tensor[0].is_contiguous():
-        raise ValueError(f"{name} must be contiguous within each row")
-    return tensor.data_ptr()
+    if tensor.is_cuda and tensor.dtype == dtype and (tensor.is_contiguous() or tensor[:1].squeeze(0).is_contiguous()):
+        return tensor.data_ptr()
+    _dev(tensor, dtype, name)
+    raise ValueError(f"{name} must be contiguous within each row")
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream's handle, as stream_handle() but without the stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> PagedKvDesc:
     """The h4b_paged_kv of one layer's pages and a batch's tables."""
-    code = _PAGED_DTYPES.get(k_pages.dtype)
+    dtype = k_pages.dtype
+    code = _PAGED_DTYPES.get(dtype)
     if code is None:
-        raise ValueError(f"k_pages must be float16 or bfloat16, got {k_pages.dtype}")
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"k_pages must be float16 or bfloat16, got {dtype}")
+    shape, table = k_pages.shape, page_table.shape
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must be [pages][kv_heads][page_size][head_dim]")
-    pages, kv_heads, page_size, head_dim = k_pages.shape
-    if page_table.dim() != 2 or page_table.shape[0] != kv_lens.numel() or q_offsets.numel() != kv_lens.numel() + 1:
+    sequences = kv_lens.numel()
+    if len(table) != 2 or table[0] != sequences or q_offsets.numel() != sequences + 1:
         raise ValueError("page_table must be [sequences][pages each], q_offsets [sequences + 1], kv_lens [sequences]")
-    return PagedKvDesc(_dev(k_pages, k_pages.dtype, "k_pages"), _dev(v_pages, k_pages.dtype, "v_pages"),
+    return PagedKvDesc(_dev(k_pages, dtype, "k_pages"), _dev(v_pages, dtype, "v_pages"),
                        _dev(page_table, torch.int32, "page_table"), _dev(q_offsets, torch.int32, "q_offsets"),
-                       _dev(kv_lens, torch.int32, "kv_lens"), code, pages, page_size, kv_heads, head_dim,
-                       page_table.shape[0], page_table.shape[1], tokens)
+                       _dev(kv_lens, torch.int32, "kv_lens"), code, shape[0], shape[2], shape[1], shape[3],
+                       sequences, table[1], tokens)
 
 
 def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -271,33 +277,36 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     cache's type, rows may be strided); q and k are RMS-normalised with
     `norm_q` / `norm_k` and rotated with `rope_cos` / `rope_sin` where given.
     Returns q [tokens][heads][head_dim] in the cache's type."""
-    tokens = qkv.shape[0]
+    tokens, width = qkv.shape if qkv.dim() == 2 else (0, -1)
+    dtype, source = k_pages.dtype, qkv.dtype
     kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
-    if qkv.dim() != 2 or qkv.shape[1] != (heads + 2 * kv.kv_heads) * kv.head_dim:
+    head_dim = kv.head_dim
+    if width != (heads + 2 * kv.kv_heads) * head_dim:
         raise ValueError("qkv must be [tokens][(heads + 2 kv_heads) * head_dim]")
-    if qkv.dtype not in (torch.float32, k_pages.dtype):
-        raise ValueError(f"qkv must be float32 or {k_pages.dtype}, got {qkv.dtype}")
+    if source is not torch.float32 and source is not dtype:
+        raise ValueError(f"qkv must be float32 or {dtype}, got {source}")
     if out is None:
-        out = torch.empty(tokens, heads, kv.head_dim, dtype=k_pages.dtype, device=qkv.device)
-    elif tuple(out.shape) != (tokens, heads, kv.head_dim):
+        out = torch.empty((tokens, heads, head_dim), dtype=dtype, device=qkv.device)
+    elif out.shape != (tokens, heads, head_dim):
         raise ValueError("out must be [tokens][heads][head_dim]")
-    for name, norm in (("norm_q", norm_q), ("norm_k", norm_k)):
-        if norm is not None and norm.numel() != kv.head_dim:
-            raise ValueError(f"{name} must hold head_dim values")
-    if rope_cos is not None and (rope_sin is None or rope_cos.shape != rope_sin.shape
-                                 or rope_cos.shape[-1] != kv.head_dim // 2):
-        raise ValueError("rope_cos and rope_sin must be [positions][head_dim / 2]")
-
-    def vector(tensor, name):
-        return None if tensor is None else _dev(tensor, torch.float32, name)
-
-    check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, qkv.dtype, "qkv"),
-                                 0 if qkv.dtype == torch.float32 else kv.dtype, qkv.stride(0) if tokens > 1 else qkv.shape[1],
-                                 heads, vector(norm_q, "norm_q"), vector(norm_k, "norm_k"), float(eps),
-                                 vector(rope_cos, "rope_cos"), vector(rope_sin, "rope_sin"),
-                                 0 if rope_cos is None else rope_cos.shape[0], _rows(out, k_pages.dtype, "out"),
-                                 out.stride(0) if tokens > 1 else heads * kv.head_dim, stream_handle()),
-          "h4b_paged_append")
+    weights = [None, None]
+    for k, (name, norm) in enumerate((("norm_q", norm_q), ("norm_k", norm_k))):
+        if norm is not None:
+            if norm.numel() != head_dim:
+                raise ValueError(f"{name} must hold head_dim values")
+            weights[k] = _dev(norm, torch.float32, name)
+    cos = sin = None
+    positions = 0
+    if rope_cos is not None or rope_sin is not None:
+        if rope_cos is None or rope_sin is None or rope_cos.shape != rope_sin.shape or rope_cos.dim() != 2 \
+                or rope_cos.shape[1] != head_dim // 2:
+            raise ValueError("rope_cos and rope_sin must be [positions][head_dim / 2]")
+        positions = rope_cos.shape[0]
+        cos, sin = _dev(rope_cos, torch.float32, "rope_cos"), _dev(rope_sin, torch.float32, "rope_sin")
+    check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, source, "qkv"), 0 if source is torch.float32 else kv.dtype,
+                                 qkv.stride(0) if tokens > 1 else width, heads, weights[0], weights[1], eps, cos, sin,
+                                 positions, _rows(out, dtype, "out"), out.stride(0) if tokens > 1 else heads * head_dim,
+                                 _raw_stream(qkv.device.index)), "h4b_paged_append")
     return out
 
 
@@ -333,28 +342,29 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     paged_workspace, kept between calls (one is made per call otherwise)."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens][heads][head_dim]")
-    tokens, heads, head_dim = q.shape
+    tokens, heads, head_dim = shape = q.shape
+    dtype = k_pages.dtype
     kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
     if head_dim != kv.head_dim or heads % kv.kv_heads:
         raise ValueError("q must have the cache's head_dim and a multiple of its kv heads")
     if out is None:
-        out = torch.empty(tokens, heads, head_dim, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.shape != shape:
         raise ValueError("out must have q's shape")
-    if lse is not None and tuple(lse.shape) != (tokens, heads):
+    if lse is not None and lse.shape != (tokens, heads):
         raise ValueError("lse must be [tokens][heads]")
     if max_query is None:
         max_query = 1 if tokens <= kv.sequences else tokens
     if workspace is None:
         workspace = paged_workspace(head_dim, q.device)
     width = heads * head_dim
-    check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, k_pages.dtype, "q"), q.stride(0) if tokens > 1 else width,
-                                    heads, head_dim ** -0.5 if scale is None else float(scale), int(window),
-                                    int(sinks), int(max_query), _rows(out, k_pages.dtype, "out"),
-                                    out.stride(0) if tokens > 1 else width,
+    several = tokens > 1
+    check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, dtype, "q"), q.stride(0) if several else width, heads,
+                                    head_dim ** -0.5 if scale is None else scale, window, sinks, max_query,
+                                    _rows(out, dtype, "out"), out.stride(0) if several else width,
                                     None if lse is None else _dev(lse, torch.float32, "lse"),
-                                    _dev(workspace, torch.uint8, "workspace"), workspace.numel(), stream_handle()),
-          "h4b_paged_attention")
+                                    _dev(workspace, torch.uint8, "workspace"), workspace.numel(),
+                                    _raw_stream(q.device.index)), "h4b_paged_attention")
     return out
 
 
@@ -363,13 +373,14 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     [layers][pages][kv_heads][page_size][head_dim] (or one layer's [pages]...)
     caches of any type; int32 ids on the device. No page may be the
     destination of two moves, nor a source and a destination."""
-    if k_pages.shape != v_pages.shape or k_pages.dim() not in (4, 5):
+    shape, dtype, count = k_pages.shape, k_pages.dtype, src.numel()
+    if shape != v_pages.shape or len(shape) not in (4, 5):
         raise ValueError("k_pages and v_pages must be [layers][pages][kv_heads][page_size][head_dim]")
-    layers = k_pages.shape[0] if k_pages.dim() == 5 else 1
-    pages, kv_heads, page_size, head_dim = k_pages.shape[-4:]
-    if src.numel() != dst.numel():
+    if count != dst.numel():
         raise ValueError("src and dst must hold as many page ids")
-    check(lib().h4b_pages_copy(_dev(k_pages, k_pages.dtype, "k_pages"), _dev(v_pages, k_pages.dtype, "v_pages"), layers,
-                               pages, kv_heads * page_size * head_dim * k_pages.element_size(),
-                               _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst"), src.numel(),
-                               stream_handle()), "h4b_pages_copy")
+    pages, kv_heads, page_size, head_dim = shape[-4:]
+    check(lib().h4b_pages_copy(_dev(k_pages, dtype, "k_pages"), _dev(v_pages, dtype, "v_pages"),
+                               shape[0] if len(shape) == 5 else 1, pages,
+                               kv_heads * page_size * head_dim * k_pages.element_size(),
+                               _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst"), count,
+                               _raw_stream(k_pages.device.index)), "h4b_pages_copy")
