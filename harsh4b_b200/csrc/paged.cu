@@ -16,6 +16,8 @@
 // sequence with such an offset or length counts as empty.
 #include <cuda_bf16.h>
 
+#include <climits>
+
 namespace h4b {
 
 constexpr int kStatusBadPage = 8;  // page id, row offset or length out of range
@@ -82,8 +84,8 @@ __device__ __forceinline__ SequenceSpan sequence_span(const PagedView& p, int b)
 // One warp per (token, head) in steps: q and k heads are divided by their
 // root mean square and scaled (norm weights), then rotated (cos/sin rows of
 // the token's position, halves d and d + D/2 paired); v passes through. One
-// rounding to 16 bits at the end, everything before in fp32. A head takes D/4
-// lanes: lane i holds dims 2i, 2i + 1 and their partners D/2 further, so the
+// rounding to 16 bits at the end, everything before in fp32. A head takes D/8
+// lanes: lane i holds dims 4i .. 4i + 3 and their partners D/2 further, so the
 // rotation needs no exchange.
 // Bound by HBM: (heads + 2 kv_heads) D (source + 2) bytes a token.
 struct AppendArgs {
@@ -92,27 +94,66 @@ struct AppendArgs {
     long long qkv_stride;   // values from token to token
     const float *norm_q, *norm_k, *cos, *sin;
     int max_pos, heads;
+    unsigned parts;         // warps that share a token
     float eps;
     void *q_out, *k_pages, *v_pages;
     long long q_stride;
 };
 
-constexpr int kAppendWarps = 8;
+// Warps that share a token of a long chunk, and turns a warp has in flight
+// (8192 tokens, 48 heads of 128, fp32: 8 and 1 58 us, 4 and 2 53, 2 and 3 52;
+// 10 heads 16, 18 and 15).
+constexpr int kAppendWarps = 8, kAppendShare = 2, kAppendTurns = 3;
 
+// Four consecutive values, of 2 or 4 bytes, as they come.
 template <typename S>
-__device__ __forceinline__ float2 load_pair(const S* p) {
-    return Pair<S>::unpack(__ldg(reinterpret_cast<const uint32_t*>(p)));
-}
+struct RawQuad {
+    using type = uint2;
+    __device__ static float4 value(uint2 w) {
+        const float2 a = Pair<S>::unpack(w.x), b = Pair<S>::unpack(w.y);
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+};
 template <>
-__device__ __forceinline__ float2 load_pair<float>(const float* p) {
-    return __ldg(reinterpret_cast<const float2*>(p));
+struct RawQuad<float> {
+    using type = float4;
+    __device__ static float4 value(float4 w) { return w; }
+};
+__device__ __forceinline__ float4 scaled(const float4& v, float f, const float4& w) {
+    return make_float4(v.x * f * w.x, v.y * f * w.y, v.z * f * w.z, v.w * f * w.w);
+}
+// a c + b s, four at a time.
+__device__ __forceinline__ float4 turned(const float4& a, const float4& c, const float4& b, const float4& s) {
+    return make_float4(a.x * c.x + b.x * s.x, a.y * c.y + b.y * s.y, a.z * c.z + b.z * s.z, a.w * c.w + b.w * s.w);
 }
 
 template <typename S, typename T, int D>
 __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const AppendArgs a) {
-    constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;  // heads a warp holds at once
+    using Raw = typename RawQuad<S>::type;
+    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes;  // heads a warp holds in its lanes
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int token = blockIdx.x, page_size = 1 << a.p.page_shift;
+    const int page_size = 1 << a.p.page_shift;
+    const int i = lane % kLanes, sub = lane / kLanes;
+    // warp `part` of the `parts` that share a token
+    const unsigned place = blockIdx.x * kAppendWarps + warp;
+    const int token = static_cast<int>(place / a.parts), part = static_cast<int>(place % a.parts);
+    if (token >= a.p.tokens) return;
+    const int total = a.heads + 2 * a.p.kv_heads, stride = a.parts * kPerWarp;
+    const S* row = static_cast<const S*>(a.qkv) + token * a.qkv_stride + 4 * i;
+    T* q_row = static_cast<T*>(a.q_out) + token * a.q_stride + 4 * i;
+
+    // the first heads are on their way while the token's place is looked up
+    int h0 = part * kPerWarp + sub;
+    Raw x[kAppendTurns], y[kAppendTurns];
+    auto load = [&]() {
+#pragma unroll
+        for (int k = 0; k < kAppendTurns; ++k) {
+            const int h = min(h0 + k * stride, total - 1);  // (a head too many is read and not used)
+            x[k] = __ldcs(reinterpret_cast<const Raw*>(row + h * D));
+            y[k] = __ldcs(reinterpret_cast<const Raw*>(row + h * D + D / 2));
+        }
+    };
+    load();
 
     // the token's sequence: the last b whose offset is not past the token
     int b = -1;
@@ -120,72 +161,71 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const A
         const bool before = j + lane < a.p.sequences && a.p.q_offsets[j + lane] <= token;
         b += __popc(__ballot_sync(0xffffffffu, before));
     }
-    long long slot = -1;  // of the token in its page's buffers, in rows of kv head 0
+    T *k_row = nullptr, *v_row = nullptr;  // of the token, kv head 0
     int position = -1;
     if (b >= 0) {
         const SequenceSpan s = sequence_span(a.p, b);
         position = token < s.first + s.count ? s.base + token - s.first : -1;
         if (position >= 0) {
             const int page = a.p.table[static_cast<long long>(b) * a.p.table_stride + (position >> a.p.page_shift)];
-            if (page >= 0 && page < a.p.pages)
-                slot = (static_cast<long long>(page) * a.p.kv_heads << a.p.page_shift) + (position & (page_size - 1));
-            else if (lane == 0)
+            if (page >= 0 && page < a.p.pages) {
+                const long long at = ((static_cast<long long>(page) * a.p.kv_heads << a.p.page_shift) +
+                                      (position & (page_size - 1))) * D + 4 * i;
+                k_row = static_cast<T*>(a.k_pages) + at;
+                v_row = static_cast<T*>(a.v_pages) + at;
+            } else if (lane == 0) {
                 report(kStatusBadPage);
+            }
         }
     }
-
-    const int i = lane % kLanes, sub = lane / kLanes;
-    float2 cos = make_float2(1.f, 1.f), sin = make_float2(0.f, 0.f);
+    float4 cos = make_float4(1.f, 1.f, 1.f, 1.f), sin = make_float4(0.f, 0.f, 0.f, 0.f);
     if (a.cos != nullptr && position >= 0) {
         if (position < a.max_pos) {
-            cos = load_pair(a.cos + static_cast<long long>(position) * (D / 2) + 2 * i);
-            sin = load_pair(a.sin + static_cast<long long>(position) * (D / 2) + 2 * i);
+            cos = __ldg(reinterpret_cast<const float4*>(a.cos + static_cast<long long>(position) * (D / 2)) + i);
+            sin = __ldg(reinterpret_cast<const float4*>(a.sin + static_cast<long long>(position) * (D / 2)) + i);
         } else if (lane == 0) {
             report(kStatusBadPosition);
         }
     }
-    const int total = a.heads + 2 * a.p.kv_heads;
-    const S* row = static_cast<const S*>(a.qkv) + token * a.qkv_stride;
-    T* q_row = static_cast<T*>(a.q_out) + token * a.q_stride;
-    for (int h0 = (blockIdx.y * kAppendWarps + warp) * kPerWarp; h0 < total;
-         h0 += gridDim.y * kAppendWarps * kPerWarp) {
-        const int h = h0 + sub;
-        const bool valid = h < total, is_v = h >= a.heads + a.p.kv_heads, is_q = h < a.heads;
-        float2 x = make_float2(0.f, 0.f), y = x;
-        if (valid) {
-            x = load_pair(row + h * D + 2 * i);
-            y = load_pair(row + h * D + D / 2 + 2 * i);
-        }
-        const float* weight = is_q ? a.norm_q : a.norm_k;
-        if (weight != nullptr) {
-            float sum = x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y;
+    const float4 minus = make_float4(-sin.x, -sin.y, -sin.z, -sin.w);
+    const bool normed = a.norm_q != nullptr;
+    while (true) {  // (the same number of turns in every lane)
 #pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int k = 0; k < kAppendTurns; ++k) {
+            const int h = h0 + k * stride;
+            const bool is_v = h >= a.heads + a.p.kv_heads, is_q = h < a.heads;
+            float4 u = RawQuad<S>::value(x[k]), w = RawQuad<S>::value(y[k]);
+            if (normed) {
+                float sum = (u.x * u.x + u.y * u.y) + (u.z * u.z + u.w * u.w) + (w.x * w.x + w.y * w.y) +
+                            (w.z * w.z + w.w * w.w);
+#pragma unroll
+                for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (!is_v) {
+                    const float inv = rsqrtf(sum * (1.0f / D) + a.eps);  // to 2 ulp; the result has 16 bits
+                    const float4* weight = reinterpret_cast<const float4*>(is_q ? a.norm_q : a.norm_k) + i;
+                    u = scaled(u, inv, __ldg(weight));
+                    w = scaled(w, inv, __ldg(weight + kLanes));
+                }
+            }
             if (!is_v) {
-                const float inv = 1.0f / sqrtf(sum * (1.0f / D) + a.eps);
-                const float2 w0 = load_pair(weight + 2 * i), w1 = load_pair(weight + D / 2 + 2 * i);
-                x = make_float2(x.x * inv * w0.x, x.y * inv * w0.y);
-                y = make_float2(y.x * inv * w1.x, y.y * inv * w1.y);
+                const float4 t = u;
+                u = turned(t, cos, w, minus);
+                w = turned(w, cos, t, sin);
+            }
+            T* dst = nullptr;
+            if (is_q)
+                dst = q_row + h * D;
+            else if (k_row != nullptr && h < total)
+                dst = is_v ? v_row + ((h - a.heads - a.p.kv_heads) << a.p.page_shift) * D
+                           : k_row + ((h - a.heads) << a.p.page_shift) * D;
+            if (dst != nullptr) {
+                *reinterpret_cast<uint2*>(dst) = make_uint2(Pair<T>::pack(u.x, u.y), Pair<T>::pack(u.z, u.w));
+                *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(Pair<T>::pack(w.x, w.y), Pair<T>::pack(w.z, w.w));
             }
         }
-        if (!valid) continue;
-        if (!is_v) {
-            const float2 u = x;
-            x = make_float2(u.x * cos.x - y.x * sin.x, u.y * cos.y - y.y * sin.y);
-            y = make_float2(y.x * cos.x + u.x * sin.x, y.y * cos.y + u.y * sin.y);
-        }
-        T* dst = nullptr;
-        if (is_q) {
-            dst = q_row + h * D;
-        } else if (slot >= 0) {
-            const int kv = is_v ? h - a.heads - a.p.kv_heads : h - a.heads;
-            dst = static_cast<T*>(is_v ? a.v_pages : a.k_pages) +
-                  (slot + (static_cast<long long>(kv) << a.p.page_shift)) * D;
-        }
-        if (dst != nullptr) {
-            *reinterpret_cast<uint32_t*>(dst + 2 * i) = Pair<T>::pack(x.x, x.y);
-            *reinterpret_cast<uint32_t*>(dst + D / 2 + 2 * i) = Pair<T>::pack(y.x, y.y);
-        }
+        h0 += kAppendTurns * stride;
+        if (h0 - sub >= total) break;
+        load();
     }
 }
 
@@ -232,6 +272,7 @@ __global__ void __launch_bounds__(kCopyThreads)
 // depend on which one that is.
 struct AttendArgs {
     PagedView p;
+    int fewest, most;         // sequences with so many new tokens are this kernel's
     int extra;                // places of an item beside its units
     const void *q, *k_pages, *v_pages;
     void* out;
@@ -242,6 +283,14 @@ struct AttendArgs {
     float* partials;          // [2 * CTAs][ROWS * (D + 2)]: a CTA's first and last item
     unsigned int* counters;   // [CTAs], zero between calls
 };
+
+// A sequence as this kernel's share of the batch has it: without new tokens if
+// it is another kernel's.
+__device__ __forceinline__ SequenceSpan own_span(const AttendArgs& a, const RawSpan& r) {
+    SequenceSpan s = checked_span(a.p, r);
+    if (s.count < a.fewest || s.count > a.most) s.count = 0;
+    return s;
+}
 
 struct Tile {  // one tile of new tokens of a sequence
     int first, tokens;        // first row (token index in the batch), tokens
@@ -321,7 +370,7 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     const int each = (a.p.sequences + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
     auto places_of = [&](int e) {  // of the thread's e-th sequence, all kv heads
         SequenceSpan s{0, 0, 0};
-        if (b0 + e < a.p.sequences) s = sequence_span(a.p, b0 + e);
+        if (b0 + e < a.p.sequences) s = own_span(a, raw_span(a.p, b0 + e));
         return a.p.kv_heads * warp_places<KEYS>(a, s, tile_tokens);
     };
     long long mine = 0;
@@ -388,7 +437,7 @@ struct Walk {
         const int lane = threadIdx.x & 31;
         b = r.sequence;
         left = r.end - r.begin;
-        span = sequence_span(a.p, b);
+        span = own_span(a, raw_span(a.p, b));
         request(a);
         long long skip = r.skip;
         for (int t0 = 0;; t0 += 32) {
@@ -429,7 +478,7 @@ struct Walk {
         while (t * tile_tokens >= span.count) {
             t = 0;
             ++b;
-            span = checked_span(a.p, following);
+            span = own_span(a, following);
             request(a);
         }
         tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
@@ -939,13 +988,15 @@ constexpr int kFewCtasPerSm = 2, kFewMaxRows = 32;
 constexpr long long kCounterBytes = 4096;
 
 template <typename S, typename T, int D>
-static int launch_append(const AppendArgs& a, cudaStream_t stream) {
-    // Few tokens: the heads of a token are spread over several CTAs, so that
-    // the chip is full; many: one CTA walks all heads of its token.
-    const int per_cta = kAppendWarps * (128 / D), total = a.heads + 2 * a.p.kv_heads;
-    const int most = (total + per_cta - 1) / per_cta;
-    const int y = a.p.tokens >= 1024 ? 1 : most;
-    paged_append_kernel<S, T, D><<<dim3(a.p.tokens, y), 32 * kAppendWarps, 0, stream>>>(a);
+static int launch_append(AppendArgs a, cudaStream_t stream) {
+    // Few tokens: a token's heads are spread over as many warps as it takes;
+    // many: kAppendShare warps walk them, which look up the token's place once
+    // each.
+    const int total = a.heads + 2 * a.p.kv_heads, most = (total * D + 255) / 256;
+    a.parts = a.p.tokens >= 1024 && most > kAppendShare ? kAppendShare : most;
+    const long long ctas = (static_cast<long long>(a.p.tokens) * a.parts + kAppendWarps - 1) / kAppendWarps;
+    if (ctas > INT_MAX / kAppendWarps) return H4B_EUNSUPPORTED;
+    paged_append_kernel<S, T, D><<<static_cast<unsigned>(ctas), 32 * kAppendWarps, 0, stream>>>(a);
     H4B_CUDA_TRY(cudaGetLastError());
     return 0;
 }
@@ -968,13 +1019,39 @@ static int launch_few(AttendArgs a, int sms, cudaStream_t stream) {
 }
 
 template <typename T, int D>
-static int launch_attention(const AttendArgs& a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
-    const long long rows = static_cast<long long>(max_query) * a.group;
+static int launch_few_rows(const AttendArgs& a, int rows, int sms, cudaStream_t stream) {
     if (rows <= 8) return launch_few<T, D, 8>(a, sms, stream);
-    if (rows <= 16) return launch_few<T, D, 16>(a, sms, stream);
     if constexpr (D == 64)
-        if (rows <= 32) return launch_few<T, D, 32>(a, sms, stream);
-    return launch_chunk<T, D>(a, kv, sms, stream);
+        if (rows > 16) return launch_few<T, D, 32>(a, sms, stream);
+    return launch_few<T, D, 16>(a, sms, stream);
+}
+
+template <typename T, int D>
+static int launch_attention(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
+    // Few rows: up to 16 (32 at head_dim 64, where the registers last): 32 x
+    // 32768 tokens of 8 kv heads in 644 us with 4 to 8 rows, 697 with 16, 1883
+    // with 32 (spilled), the chunk kernel 804 to 863. At head_dim 64 64 ragged
+    // sequences with 32 rows: 78 us, the chunk kernel 99.
+    constexpr int kMost = D == 64 ? 32 : 16;
+    const long long rows = static_cast<long long>(max_query) * a.group;
+    a.fewest = 1;
+    a.most = INT_MAX;
+    if (rows > kMost) {
+        // A step of few long chunks among many short ones (the mean is under
+        // half of the longest): the short ones go to the kernel of few rows, in
+        // a launch of its own. Three 255-token chunks and 5, 21 or 61 decoding
+        // sequences, 24 / 8 heads of 64: one launch 42, 66 and 139 us, two
+        // launches 47, 61 and 98.
+        const int few_rows = a.group <= 8 ? 8 : (a.group <= 16 ? 16 : 32);
+        if (few_rows <= kMost && a.p.sequences >= 20 && 2ll * a.p.tokens < static_cast<long long>(a.p.sequences) * max_query) {
+            a.most = few_rows / a.group;
+            if (const int rc = launch_few_rows<T, D>(a, few_rows, sms, stream)) return rc;
+            a.fewest = a.most + 1;
+            a.most = INT_MAX;
+        }
+        return launch_chunk<T, D>(a, kv, sms, stream);
+    }
+    return launch_few_rows<T, D>(a, static_cast<int>(rows), sms, stream);
 }
 
 }  // namespace h4b
@@ -989,12 +1066,12 @@ extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv
     if ((norm_q == nullptr) != (norm_k == nullptr) || (rope_cos == nullptr) != (rope_sin == nullptr) ||
         (rope_cos != nullptr && max_pos < 1))
         return H4B_EINVAL;
-    if (qkv_stride < static_cast<long long>(heads + 2 * kv->kv_heads) * kv->head_dim || (qkv_stride & 1) ||
-        (heads > 0 && (q_stride < static_cast<long long>(heads) * kv->head_dim || (q_stride & 1))))
+    const auto misaligned = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
+    if (qkv_stride < static_cast<long long>(heads + 2 * kv->kv_heads) * kv->head_dim || (qkv_stride & 3) ||
+        (heads > 0 && (q_stride < static_cast<long long>(heads) * kv->head_dim || (q_stride & 3))))
         return H4B_EINVAL;
-    if ((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin) |
-         reinterpret_cast<uintptr_t>(norm_q) | reinterpret_cast<uintptr_t>(norm_k)) & 7 ||
-        (reinterpret_cast<uintptr_t>(q_out) & 3))
+    if (misaligned(qkv, qkv_dtype == H4B_FP32 ? 16 : 8) || misaligned(rope_cos, 16) || misaligned(rope_sin, 16) ||
+        misaligned(norm_q, 16) || misaligned(norm_k, 16) || misaligned(q_out, 8))
         return H4B_EINVAL;
     if (kv->tokens == 0 || kv->sequences == 0) return 0;
     a.qkv = qkv, a.qkv_stride = qkv_stride, a.norm_q = norm_q, a.norm_k = norm_k, a.cos = rope_cos, a.sin = rope_sin;

@@ -480,7 +480,8 @@ typedef struct h4b_paged_kv {
  * both null: not rotated) at the token's position; q goes to q_out (rows
  * q_stride values apart, in the cache's type), k and v into the pages. A
  * position past max_pos sets status bit 4 and is not rotated. heads may be 0
- * (then q_out is not used). */
+ * (then q_out is not used). Strides are multiples of 4, fp32 pointers 16-byte
+ * aligned and 16-bit ones 8-byte. */
 int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, long long qkv_stride, int heads,
                      const float *norm_q, const float *norm_k, float eps, const float *rope_cos,
                      const float *rope_sin, int max_pos, void *q_out, long long q_stride, void *stream);
