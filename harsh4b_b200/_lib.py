@@ -82,6 +82,14 @@ class PagedKvDesc(ctypes.Structure):
                             "tokens")]
 
 
+class PagedStepDesc(ctypes.Structure):
+    """Mirror of ``h4b_paged_step``."""
+
+    _fields_ = [("kv", PagedKvDesc), ("layer_bytes", _i64), ("window", _i32), ("sinks", _i32), ("max_query", _i32)] + [
+        (n, _vp) for n in ("tokens", "x", "x8", "act_scale", "act_sum", "qkv", "q", "attended16", "attended", "gate_up",
+                           "act", "last", "logits", "next_tokens", "workspace")] + [("workspace_bytes", _i64)]
+
+
 _SIGNATURES = {
     "h4b_prepare": [],
     "h4b_get_status": [_vp],
@@ -137,6 +145,7 @@ _SIGNATURES = {
     "h4b_paged_attention": [ctypes.POINTER(PagedKvDesc), _vp, _i64, _i32, _f32, _i32, _i32, _i32, _vp, _i64, _vp, _vp,
                             _i64, _vp],
     "h4b_paged_attention_workspace_bytes": [_i32],
+    "h4b_forward_paged": [ctypes.POINTER(ModelDesc), ctypes.POINTER(PagedStepDesc), _vp],
     "h4b_pages_copy": [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i32, _vp],
     "h4b_lattice_scratch_bytes": [_i32],
     "h4b_lattice_to_int4": [ctypes.POINTER(LatticeProjectionDesc), _vp, _vp, _vp, ctypes.POINTER(_i32), _vp],

@@ -513,6 +513,36 @@ long long h4b_paged_attention_workspace_bytes(int head_dim);
 int h4b_pages_copy(void *k_pages, void *v_pages, int layers, int pages, long long page_bytes, const int32_t *src,
                    const int32_t *dst, int count, void *stream);
 
+/* One step of the model over a paged cache: sequence b of kv feeds its rows
+ * of `tokens` (a prompt's chunk, one decoded token, none), which are appended
+ * and attended in every layer; the reference runs one token of one sequence
+ * at a time (LiteSparkQwen.forward_token, cpu_lightspark.py:424-468).
+ * kv.k_pages / v_pages are layer 0's, layer l's lie l * layer_bytes further.
+ * All buffers are the caller's, on the device, 16-byte aligned; T = kv.tokens
+ * and B = kv.sequences rows. logits [B][vocab] and next_tokens [B] (greedy)
+ * belong to each sequence's last new row (of a sequence without one they mean
+ * nothing). window, sinks, max_query, workspace: as for h4b_paged_attention.
+ * Capturable in a CUDA graph after a first call. */
+typedef struct h4b_paged_step {
+    h4b_paged_kv kv;
+    long long layer_bytes;
+    int window, sinks, max_query;
+    const int32_t *tokens;            /* [T] token ids */
+    float *x;                         /* [T][hidden] */
+    int8_t *x8;                       /* [max(T, B)][max(hidden, heads*head_dim, intermediate)] */
+    float *act_scale;                 /* [max(T, B)] */
+    int32_t *act_sum;                 /* [max(T, B)] */
+    float *qkv;                       /* [T][(heads + 2 kv_heads) * head_dim] */
+    void *q, *attended16;             /* [T][heads * head_dim] of the cache's type */
+    float *attended;                  /* [T][heads * head_dim] */
+    float *gate_up, *act;             /* [T][2 intermediate], [T][intermediate] */
+    float *last, *logits;             /* [B][hidden], [B][vocab] */
+    int32_t *next_tokens;             /* [B] */
+    void *workspace;                  /* of h4b_paged_attention */
+    long long workspace_bytes;
+} h4b_paged_step;
+int h4b_forward_paged(const h4b_model *model, const h4b_paged_step *step, void *stream);
+
 /* ---- format producer: LATTICE checkpoint -> packed int4 cache ------------- */
 
 /* One LATTICE projection as stored in the checkpoint (all pointers are
