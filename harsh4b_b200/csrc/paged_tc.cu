@@ -56,8 +56,8 @@ constexpr int kChunkExtra = 2;  // an item's start, end and pipeline fill, in un
 constexpr uint32_t kStepTwo = 1, kStepFirst = 2, kStepLast = 4, kStepFinal = 8;
 constexpr uint32_t kStepNone = 16;  // the range held no unit
 // Registers a thread: three warpgroups at the launch's 168 are shared out
-// anew, 2 x 208 for the softmax (a row's 128 scores) and 88 for the others.
-constexpr int kChunkSoftmaxRegs = 208, kChunkOtherRegs = 88;
+// anew, 2 x 200 for the softmax (a row's 128 scores) and 104 for the others.
+constexpr int kChunkSoftmaxRegs = 200, kChunkOtherRegs = 104;
 static_assert(2 * kChunkSoftmaxRegs + kChunkOtherRegs <= 3 * 168, "registers of the CTA");
 
 template <int D>
