@@ -635,22 +635,21 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     Walk<kFewKeys> now, ahead;
     if (!now.start(a, range, tile_tokens)) return;
     ahead = now;
-    // the ring's first stages; `page` belongs to the piece `ahead` stands at
+    // the ring's first stages; `page` belongs to the piece `ahead` stands at, and
+    // `live` says which of the ring's pieces, from the current one on, some row sees
     int page = page_of(ahead);
     bool more = true;
-    int pages_now[C::kStages];  // page of the piece in each stage (stage 0: `now`)
-#pragma unroll
+    uint32_t live = 0;
+#pragma unroll 1
     for (int s = 0; s < C::kStages - 1; ++s) {
-        pages_now[s] = -1;
         if (more) {
             load(ahead, page, s);
-            pages_now[s] = page;
+            live |= (page != -1 ? 1u : 0u) << s;
             more = ahead.next(a, tile_tokens);
             if (more) page = page_of(ahead);
         }
         async_copy_commit();
     }
-    pages_now[C::kStages - 1] = -1;
 
     uint32_t qf[C::kTiles][kSteps][4];
     float o[C::kTiles][kCols][4];
@@ -688,7 +687,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         }
         async_copy_wait_prior<C::kStages - 2>();
         __syncwarp();
-        if (pages_now[0] != -1) {
+        if (live & 1u) {
             const uint32_t kbase = ring + stage * 2 * C::kPiece, vbase = kbase + C::kPiece;
             float s[C::kTiles][2][4];
 #pragma unroll
@@ -779,17 +778,14 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         }
         // refill the stage freed one step ago
         __syncwarp();
-        int page_new = -1;
+        live >>= 1;
         if (more) {
             load(ahead, page, (stage + C::kStages - 1) % C::kStages);
-            page_new = page;
+            live |= (page != -1 ? 1u : 0u) << (C::kStages - 2);
             more = ahead.next(a, tile_tokens);
             if (more) page = page_of(ahead);
         }
         async_copy_commit();
-#pragma unroll
-        for (int s = 0; s + 1 < C::kStages - 1; ++s) pages_now[s] = pages_now[s + 1];
-        pages_now[C::kStages - 2] = page_new;
         stage = (stage + 1) % C::kStages;
 
         const bool item_done = now.item_ends();
@@ -907,11 +903,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                 for (int x = threadIdx.x; x < rows * (D / 4); x += kFewThreads) {
                     const int r = x / (D / 4), c = x % (D / 4), i = r / a.group;
                     float top = -INFINITY;
+#pragma unroll 8
                     for (int cta = c0; cta <= c1; ++cta)
                         top = fmaxf(top, __ldcg(a.partials + static_cast<long long>(2 * cta + (cta == c0)) * ROWS * (D + 2) +
                                                 ROWS * D + 2 * r));
                     float sum = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
                     for (int cta = c0; cta <= c1; ++cta) {
                         const float* q = a.partials + static_cast<long long>(2 * cta + (cta == c0)) * ROWS * (D + 2);
                         const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + ROWS * D + 2 * r));
