@@ -426,7 +426,7 @@ struct Walk {
     RawSpan following;        // of sequence b + 1, requested when b was entered
     Tile tile;
     int b, t, h, unit;        // unit within the item
-    long long left;           // places of the range from this unit on
+    int left;                 // places of the range from this unit on
 
     __device__ __forceinline__ void request(const AttendArgs& a) {
         if (b + 1 < a.p.sequences) following = raw_span(a.p, b + 1);
@@ -436,7 +436,7 @@ struct Walk {
     __device__ __forceinline__ bool start(const AttendArgs& a, const Range& r, int tile_tokens) {
         const int lane = threadIdx.x & 31;
         b = r.sequence;
-        left = r.end - r.begin;
+        left = static_cast<int>(min(r.end - r.begin, static_cast<long long>(INT_MAX)));
         span = own_span(a, raw_span(a.p, b));
         request(a);
         long long skip = r.skip;
@@ -580,6 +580,10 @@ __device__ __forceinline__ void async_copy16_or_zero(uint32_t dst, const void* s
                  : "memory");
 }
 
+__device__ __forceinline__ void async_copy16_l2(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // Byte of 16-byte chunk c of row r in a 16-row piece: the chunks of eight
 // consecutive rows lie in distinct banks.
 template <int D>
@@ -615,22 +619,40 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         }
         return page;
     };
+    // A lane copies chunk c of rows r0, r0 + kRowsStep, ..: byte `to` of row r0,
+    // the others by constants (piece_at's exclusive or is linear in the row).
+    constexpr int kChunks = D / 8, kRowsStep = 32 / kChunks;  // 16-byte chunks a row, rows a pass
+    const int r0 = lane / kChunks;
+    const uint32_t from = r0 * D + (lane % kChunks) * 8, to = piece_at<D>(r0, lane % kChunks);
     auto load = [&](const Walk<kFewKeys>& w, int page, int stage) {
         if (page == -1) return;
         const int key = w.tile.block(w.unit) * kFewKeys + warp * 16;
         const long long row = (static_cast<long long>(max(page, 0)) * a.p.kv_heads + w.h) * head_rows + (key & page_mask);
         const uint32_t dst = ring + stage * 2 * C::kPiece;
-        constexpr int kChunks = D / 8, kRowsStep = 32 / kChunks;  // 16-byte chunks a row, rows a pass
-        const int c = lane % kChunks, r0 = lane / kChunks;
-        const T* k = static_cast<const T*>(a.k_pages) + row * D + c * 8;
-        const T* v = static_cast<const T*>(a.v_pages) + row * D + c * 8;
+        const T* k = static_cast<const T*>(a.k_pages) + row * D + from;
+        const T* v = static_cast<const T*>(a.v_pages) + row * D + from;
+        if (page >= 0 && key + 15 <= w.tile.p1 &&
+            (a.window <= 0 || key > w.tile.p0 - a.window || key + 15 < a.sinks)) {  // the usual: every key is seen
 #pragma unroll
-        for (int r = 0; r < 16; r += kRowsStep) {
-            const bool fill = page < 0 || !tile_sees(w.tile, a.window, a.sinks, key + r + r0);
-            async_copy16_or_zero(dst + piece_at<D>(r + r0, c), k + (r + r0) * D, fill);
-            async_copy16_or_zero(dst + C::kPiece + piece_at<D>(r + r0, c), v + (r + r0) * D, fill);
+            for (int r = 0; r < 16; r += kRowsStep) {
+                const uint32_t at = dst + (to ^ ((r & 7) << 4)) + r * (D * 2);
+                async_copy16_l2(at, k + r * D);
+                async_copy16_l2(at + C::kPiece, v + r * D);
+            }
+        } else {
+#pragma unroll 1
+            for (int r = 0; r < 16; r += kRowsStep) {
+                const bool fill = page < 0 || !tile_sees(w.tile, a.window, a.sinks, key + r + r0);
+                const uint32_t at = dst + (to ^ ((r & 7) << 4)) + r * (D * 2);
+                async_copy16_or_zero(at, k + r * D, fill);
+                async_copy16_or_zero(at + C::kPiece, v + r * D, fill);
+            }
         }
     };
+    // ldmatrix addresses within a piece, for the first 16 dims (K), 16 dims (V):
+    // K keys 0-7 and 8-15 of two chunks; V the same keys, transposed
+    const uint32_t k_at = piece_at<D>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
+    const uint32_t v_at = piece_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
 
     Walk<kFewKeys> now, ahead;
     if (!now.start(a, range, tile_tokens)) return;
@@ -699,7 +721,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 uint32_t b[4];  // keys 0-7 and 8-15, dims 16k..16k+15
-                ldmatrix4(b, kbase + piece_at<D>((lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)));
+                ldmatrix4(b, kbase + (k_at ^ (k << 5)));
 #pragma unroll
                 for (int mt = 0; mt < C::kTiles; ++mt) {
                     mma_16816<T>(s[mt][0], qf[mt][k], b[0], b[1]);
@@ -709,28 +731,35 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
             const int key = now.tile.block(now.unit) * kFewKeys + warp * 16;
             const Tile& t = now.tile;
             const bool all = key + 15 <= t.p0 && (a.window <= 0 || key > t.p1 - a.window || key + 15 < a.sinks);
+            if (!all) {
+#pragma unroll
+                for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                    for (int half = 0; half < C::kHalves; ++half)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int j = key + n * 8 + (lane & 3) * 2 + e, p = pos[mt][half];
+                                if (j > p || (a.window > 0 && j <= p - a.window && j >= a.sinks))
+                                    s[mt][n][half * 2 + e] = -INFINITY;
+                            }
+            }
+            // (the scale is positive: maxima can be taken before it)
             bool grow = false;
 #pragma unroll
             for (int mt = 0; mt < C::kTiles; ++mt)
 #pragma unroll
                 for (int half = 0; half < C::kHalves; ++half)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float& x = s[mt][n][half * 2 + e];
-                            x *= a.scale;
-                            const int j = key + n * 8 + (lane & 3) * 2 + e, p = pos[mt][half];
-                            if (!all && !(j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks))) x = -INFINITY;
-                            grow |= x > m[mt][half] + kFewSlack;
-                        }
+                    grow |= a.scale * fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
+                                            fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1])) > m[mt][half] + kFewSlack;
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int mt = 0; mt < C::kTiles; ++mt)
 #pragma unroll
                     for (int half = 0; half < C::kHalves; ++half) {
-                        float top = fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
-                                          fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1]));
+                        float top = a.scale * fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
+                                                    fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1]));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                         if (top > m[mt][half]) {
@@ -759,7 +788,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) p[n * 2 + e] = ex2_approx(s[mt][n][half * 2 + e] + base);
+                        for (int e = 0; e < 2; ++e) p[n * 2 + e] = ex2_approx(__fmaf_rn(s[mt][n][half * 2 + e], a.scale, base));
                     l[mt][half] += (p[0] + p[1]) + (p[2] + p[3]);
                     pf[mt][half] = Pair<T>::pack(p[0], p[1]);
                     pf[mt][2 + half] = Pair<T>::pack(p[2], p[3]);
@@ -768,7 +797,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
 #pragma unroll
             for (int n = 0; n < kCols; n += 2) {
                 uint32_t b[4];  // dims 8n..8n+7 (keys 0-7, 8-15), then the next eight
-                ldmatrix4_trans(b, vbase + piece_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), n + (lane >> 4)));
+                ldmatrix4_trans(b, vbase + (v_at ^ (n << 4)));
 #pragma unroll
                 for (int mt = 0; mt < C::kTiles; ++mt) {
                     mma_16816<T>(o[mt][n], pf[mt], b[0], b[1]);
