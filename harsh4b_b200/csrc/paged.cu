@@ -1088,11 +1088,13 @@ extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv
                                 const float* rope_sin, int max_pos, void* q_out, long long q_stride, void* stream) {
     using namespace h4b;
     AppendArgs a{};
-    if (!paged_view(kv, &a.p) || heads < 0 || qkv == nullptr || (heads > 0 && q_out == nullptr)) return H4B_EINVAL;
+    if (!paged_view(kv, &a.p) || heads < 0) return H4B_EINVAL;
     if (!paged_shape_supported(kv) || (qkv_dtype != H4B_FP32 && qkv_dtype != kv->dtype)) return H4B_EUNSUPPORTED;
     if ((norm_q == nullptr) != (norm_k == nullptr) || (rope_cos == nullptr) != (rope_sin == nullptr) ||
         (rope_cos != nullptr && max_pos < 1))
         return H4B_EINVAL;
+    if (kv->tokens == 0 || kv->sequences == 0) return 0;
+    if (qkv == nullptr || (heads > 0 && q_out == nullptr)) return H4B_EINVAL;
     const auto misaligned = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
     if (qkv_stride < static_cast<long long>(heads + 2 * kv->kv_heads) * kv->head_dim || (qkv_stride & 3) ||
         (heads > 0 && (q_stride < static_cast<long long>(heads) * kv->head_dim || (q_stride & 3))))
@@ -1100,7 +1102,6 @@ extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv
     if (misaligned(qkv, qkv_dtype == H4B_FP32 ? 16 : 8) || misaligned(rope_cos, 16) || misaligned(rope_sin, 16) ||
         misaligned(norm_q, 16) || misaligned(norm_k, 16) || misaligned(q_out, 8))
         return H4B_EINVAL;
-    if (kv->tokens == 0 || kv->sequences == 0) return 0;
     a.qkv = qkv, a.qkv_stride = qkv_stride, a.norm_q = norm_q, a.norm_k = norm_k, a.cos = rope_cos, a.sin = rope_sin;
     a.max_pos = max_pos, a.heads = heads, a.eps = eps, a.q_out = q_out, a.q_stride = q_stride;
     a.k_pages = kv->k_pages, a.v_pages = kv->v_pages;
@@ -1151,18 +1152,19 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
                                    void* workspace, long long workspace_bytes, void* stream) {
     using namespace h4b;
     AttendArgs a{};
-    if (!paged_view(kv, &a.p) || heads < 1 || heads % kv->kv_heads || q == nullptr || out == nullptr || window < 0 ||
-        sinks < 0 || (sinks > 0 && window == 0) || max_query < 1 || workspace == nullptr)
+    if (!paged_view(kv, &a.p) || heads < 1 || heads % kv->kv_heads || window < 0 || sinks < 0 ||
+        (sinks > 0 && window == 0) || max_query < 1)
         return H4B_EINVAL;
     if (!paged_shape_supported(kv) || heads / kv->kv_heads > kFewMaxRows ||
         static_cast<long long>(kv->pages) * kv->kv_heads > 0x7fffffffll)
         return H4B_EUNSUPPORTED;
+    if (kv->tokens == 0 || kv->sequences == 0) return 0;
+    if (q == nullptr || out == nullptr || workspace == nullptr) return H4B_EINVAL;
     const long long width = static_cast<long long>(heads) * kv->head_dim;
     if (q_stride < width || out_stride < width || ((q_stride | out_stride) & 7) ||
         ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) &
          15))
         return H4B_EINVAL;
-    if (kv->tokens == 0 || kv->sequences == 0) return 0;
     const long long need = h4b_paged_attention_workspace_bytes(kv->head_dim);
     if (need < 0 || workspace_bytes < need) return H4B_EINVAL;
     int sms = 0;

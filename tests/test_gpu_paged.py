@@ -311,6 +311,28 @@ def test_refusals():
         ops.paged_append(qkv, *args, heads=8, norm_q=torch.ones(128, device="cuda"))
 
 
+def test_empty_batches():
+    batch = Batch([0, 0], [40, 3], heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16)
+    batch.check()
+    nobody = Batch([], [], heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16)
+    nobody.check()
+    for b in (batch, nobody):
+        q = ops.paged_append(torch.zeros(0, 12 * 128, device="cuda"), b.k_pages, b.v_pages, b.table, b.offsets, b.lens, heads=8)
+        assert q.shape == (0, 8, 128)
+
+
+def test_another_keys_infinity_stays_out_of_the_scores():
+    """An infinite k of a later token of the chunk is selected away in the rows that do not see it."""
+    batch = Batch([40], [100], heads=4, kv_heads=1, dim=128, page=16, dtype=torch.float16, seed=8)
+    want, _, bound = batch.expected()
+    for hint in (1, 40):
+        batch.k_pages[int(batch.table[0, 5]), :, 10:] = float("inf")  # tokens 90..95; row i stands at 60 + i
+        batch.k_pages[int(batch.table[0, 6]), :, :4] = float("nan")   # 96..99
+        out, lse = batch.call(max_query=hint)
+        assert ((out.double() - want).abs() <= bound)[:30].all()
+        assert torch.isfinite(lse[:30]).all()
+
+
 # ---- append -----------------------------------------------------------------------
 @pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", SHAPES[:6])
 @pytest.mark.parametrize("source", ["fp32", "same"])
