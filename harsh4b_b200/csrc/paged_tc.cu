@@ -7,6 +7,10 @@
 // rows (128 / group tokens each, row = token * group + q head) that share
 // every K/V tile of 128 keys. While the tensor cores work for one tile the
 // softmax of the other runs. B is left out where A holds all tokens.
+// Measured: an 8192-token prompt, 32 / 8 heads of 128, 500 us (1100 TFLOP/s), 577
+// once the power cap holds the clock at 1.65 GHz; over 8K of history 1195
+// TFLOP/s, and 1604 with the softmax taken out: what bounds it is how well one
+// tile's softmax hides under the other's MMAs.
 //
 // Warps: 0-3 and 4-7 are the softmax of A and B (thread = query row, TMEM lane
 // = thread), 8 issues the loads, 9 and 10 the MMAs of A and B, 11 cleans V
