@@ -277,6 +277,7 @@ struct AttendArgs {
     PagedView p;
     int fewest, most;         // sequences with so many new tokens are this kernel's
     int extra;                // places of an item beside its units
+    int least;                // places of a CTA's range, where there are few
     const void *q, *k_pages, *v_pages;
     void* out;
     float* lse;               // may be null
@@ -394,7 +395,7 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     }
     Range r;
     r.total = total;
-    r.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    r.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + a.least - 1) / a.least));
     r.begin = r.end = 0;
     if (static_cast<int>(blockIdx.x) < r.ctas) {
         r.begin = range_begin(total, blockIdx.x, r.ctas);
@@ -539,6 +540,7 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // such a slot holds cannot reach a sum.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 64;
 constexpr int kFewExtra = 2;  // an item's start and join, in units
+constexpr int kFewLeast = 1;  // a part is 4 KB beside 32 KB of keys
 constexpr float kFewOffset = 8.f, kFewSlack = 7.f;
 
 template <int D, int ROWS>
@@ -1037,6 +1039,7 @@ template <typename T, int D, int ROWS>
 static int launch_few(AttendArgs a, int sms, cudaStream_t stream) {
     using C = FewCfg<D, ROWS>;
     a.extra = kFewExtra;
+    a.least = kFewLeast;
     static std::atomic<bool> opted_in[kMaxDevices];
     int dev = 0;
     H4B_CUDA_TRY(cudaGetDevice(&dev));
