@@ -270,9 +270,10 @@ __global__ void __launch_bounds__(kCopyThreads)
 // places for what an item costs beside its units and then one place a unit,
 // and the line is cut into one equal contiguous range per CTA, whatever the
 // lengths. A cut among an item's first places counts as one before its first
-// unit. An item that lies across CTAs leaves one partial result (o, m, l) in each; the CTA that
-// finishes last joins them in the order of the CTAs, so the result does not
-// depend on which one that is.
+// unit. An item that lies across CTAs leaves one partial result (o, m, l) in
+// each; they are joined in the order of the CTAs, by the CTA that finishes last
+// (few rows) or by a kernel of its own (long chunks), so the same bits come out
+// every time.
 struct AttendArgs {
     PagedView p;
     int fewest, most;         // sequences with so many new tokens are this kernel's
@@ -285,7 +286,9 @@ struct AttendArgs {
     int heads, group, window, sinks;
     float scale;              // of a score in base-2 units: scale * log2(e)
     float* partials;          // [2 * CTAs][ROWS * (D + 2)]: a CTA's first and last item
-    unsigned int* counters;   // [CTAs], zero between calls
+    unsigned int* counters;   // [CTAs], zero between calls (few-row kernel)
+    int4* entries;            // [CTAs] the item that begins last in each (chunk kernel)
+    int half_tokens;          // new tokens of each of an item's two tiles (chunk kernel)
 };
 
 // A sequence as this kernel's share of the batch has it: without new tokens if
@@ -1019,7 +1022,7 @@ static int paged_sm_count(int* sms) {
 // The few-row kernel's CTAs an SM and largest tile; as many q heads may share a
 // kv head (a token's group stays in one tile of either kernel).
 constexpr int kFewCtasPerSm = 2, kFewMaxRows = 32;
-constexpr long long kCounterBytes = 4096;
+constexpr long long kCounterBytes = 4096, kEntryBytes = 4096;
 
 template <typename S, typename T, int D>
 static int launch_append(AppendArgs a, cudaStream_t stream) {
@@ -1152,8 +1155,8 @@ extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
     // two parts a CTA: an SM's rows of the few-row kernel are fewer than
     // the 256 of the chunk kernel's CTA
     static_assert(kFewCtasPerSm * kFewMaxRows <= 2 * kChunkRows, "the chunk kernel's parts are the larger");
-    if (sms * 2 * 4 > kCounterBytes) return H4B_EUNSUPPORTED;
-    return kCounterBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
+    if (kFewCtasPerSm * sms * 4 > kCounterBytes || sms * 16 > kEntryBytes) return H4B_EUNSUPPORTED;
+    return kCounterBytes + kEntryBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
 }
 
 extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long long q_stride, int heads, float scale,
@@ -1182,7 +1185,8 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     a.q_stride = q_stride, a.out_stride = out_stride, a.heads = heads, a.group = heads / kv->kv_heads;
     a.window = window < kMaxLength ? window : kMaxLength, a.sinks = sinks, a.scale = scale * 1.4426950408889634f;
     a.counters = static_cast<unsigned int*>(workspace);
-    a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+    a.entries = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+    a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes + kEntryBytes);
     const int longest = max_query < kv->tokens ? max_query : kv->tokens;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = kv->head_dim == 128;

@@ -1,7 +1,7 @@
 // Paged attention of long chunks on the 5th-generation tensor cores:
 // tcgen05.mma kind::f16, fp32 accumulators in tensor memory, pages fetched by
-// TMA. The split of the work over the CTAs, the visibility rules and the join
-// of partial results are those of paged.cu.
+// TMA. The split of the work over the CTAs and the visibility rules are those
+// of paged.cu; partial results are joined by paged_join_kernel.
 //
 // An item is (sequence, 256 query rows, kv head): two tiles A and B of 128
 // rows (128 / group tokens each, row = token * group + q head) that share
@@ -56,9 +56,9 @@ namespace h4b {
 constexpr int kChunkRows = 128, kChunkKeys = 128;
 constexpr int kChunkLoadWarp = 8, kChunkMmaWarp = 9, kChunkCleanWarp = 11, kChunkThreads = 384;
 // Places of a CTA's range, where there are few: a part of an item is written
-// and read again, twice the bytes of a block's keys (303 tokens over 4400, one
-// kv head: 60 us with 1, 44 with 3, 56 with 12).
-constexpr int kChunkLeast = 3;
+// and read again, twice the bytes of a block's keys (303 tokens over 4400 of one
+// kv head: 43 us with 1, 34 with 2 to 4; a 512-token prompt of 8: 21, 21, 22, 24).
+constexpr int kChunkLeast = 2;
 constexpr int kChunkExtra = 2;  // an item's start, end and pipeline fill, in units
 // A step's flags: it has both tiles; first, last of its item in this range; last of all.
 constexpr uint32_t kStepTwo = 1, kStepFirst = 2, kStepLast = 4, kStepFinal = 8;
@@ -194,15 +194,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile uint32_t* flags = reinterpret_cast<volatile uint32_t*>(smem + C::kFlagOff);
-    int* last_part = reinterpret_cast<int*>(tmem_slot + 2);  // [2]: this CTA joins the tile's parts
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half_tokens = kChunkRows / a.group, tile_tokens = 2 * half_tokens;
     Range* shared_range = reinterpret_cast<Range*>(smem + C::kRangeOff);
     {
         const Range r = find_range<kChunkThreads, kChunkKeys>(a, tile_tokens, smem);
+        if (threadIdx.x == 0) {
+            *shared_range = r;
+            a.entries[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        }
         if (r.begin >= r.end) return;
-        if (threadIdx.x == 0) *shared_range = r;
     }
 
     if (threadIdx.x == 0) {
@@ -603,11 +605,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
             for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, my_place, (lane & 28) + k);
             constexpr int kPart = kChunkRows * (D + 2);
-            auto part_of = [&](int cta, int which) {
-                return a.partials + (static_cast<long long>(2 * cta + which) * 2 + x) * kPart;
-            };
             // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
-            float4* part = reinterpret_cast<float4*>(part_of(blockIdx.x, begun ? 1 : 0));
+            float4* part = reinterpret_cast<float4*>(
+                a.partials + (static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * 2 + x) * kPart);
             const float inv = 1.0f / l;
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -642,61 +642,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             } else {
                 if (valid)
                     __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
-                const Range range = *shared_range;
-                const int2 owners = item_owners(range, w);
-                const int c0 = owners.x, c1 = owners.y;
-                __threadfence();
-                named_sync(1 + x, 128);
-                if (row == 0) {
-                    unsigned* counter = reinterpret_cast<unsigned*>(a.counters) + 2 * c0 + x;
-                    const unsigned seen = atom_acq_rel_add(counter, 1u);
-                    last_part[x] = seen == static_cast<unsigned>(c1 - c0);
-                    if (last_part[x]) *counter = 0u;  // zero for the next call
-                }
-                named_sync(1 + x, 128);
-                if (last_part[x]) {
-                    __threadfence();
-                    if (valid) {
-                        auto stat = [&](int cta) {
-                            return __ldcg(reinterpret_cast<const float2*>(part_of(cta, cta == c0) + D * kChunkRows) + row);
-                        };
-                        float most = -INFINITY, total = 0.f;
-#pragma unroll 4
-                        for (int cta = c0; cta <= c1; ++cta) most = fmaxf(most, stat(cta).x);
-#pragma unroll 4
-                        for (int cta = c0; cta <= c1; ++cta) {
-                            const float2 ml = stat(cta);
-                            if (ml.y != 0.f) total += ml.y * ex2_approx(ml.x - most);
-                        }
-                        const float scale = total != 0.f ? 1.0f / total : 0.f;
-#pragma unroll 1
-                        for (int c = 0; c < D / 4; c += 8) {
-                            float4 v[8];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                            for (int cta = c0; cta <= c1; ++cta) {
-                                const float2 ml = stat(cta);  // l = 0: saw no key
-                                const float f = ml.y == 0.f ? 0.f : scale * ex2_approx(ml.x - most);
-                                const float4* o = reinterpret_cast<const float4*>(part_of(cta, cta == c0));
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    const float4 y = __ldcg(o + (c + k) * kChunkRows + row);
-                                    v[k].x += y.x * f, v[k].y += y.y * f, v[k].z += y.z * f, v[k].w += y.w * f;
-                                }
-                            }
-#pragma unroll
-                            for (int k = 0; k < 8; k += 2)
-                                *reinterpret_cast<uint4*>(out_tile + my_place + 4 * (c + k)) =
-                                    make_uint4(Pair<T>::pack(v[k].x, v[k].y), Pair<T>::pack(v[k].z, v[k].w),
-                                               Pair<T>::pack(v[k + 1].x, v[k + 1].y), Pair<T>::pack(v[k + 1].z, v[k + 1].w));
-                        }
-                        if (a.lse != nullptr)
-                            a.lse[out_row * a.heads + out_head] =
-                                total == 0.f ? -INFINITY : (most - kFewOffset) * 0.6931471805599453f + logf(total);
-                    }
-                }
-                named_sync(1 + x, 128);  // last_part is free again
+                if (threadIdx.x == 0 && begun)  // the item's first part: what the join needs to know
+                    a.entries[blockIdx.x] = make_int4(item_owners(*shared_range, w).y, w.tile.first, w.tile.tokens, w.h);
             }
             more = w.next(a, tile_tokens);
             begun = true;
@@ -711,6 +658,63 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
+}
+
+// Joins the parts of the items that lie across CTAs: block (c, tile * slices +
+// slice) the item that begins last in CTA c, if it goes on in others, in the
+// order of the CTAs. A launch of its own, on all SMs: one SM that reads an
+// item's parts (64 KB a tile at head_dim 128) took as long as the products (64
+// tokens over 16000: 60 us with the join in the CTA that ends last, 47 so; an
+// 8192-token prompt 506 and 501).
+constexpr int kJoinRows = 16, kJoinThreads = 128;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendArgs a) {
+    constexpr int kPart = kChunkRows * (D + 2), kCols = D / 8 / 4;  // float4s a thread
+    pdl_wait();
+    const int4 entry = a.entries[blockIdx.x];
+    const int c0 = blockIdx.x, c1 = entry.x, x = blockIdx.y / (kChunkRows / kJoinRows);
+    if (c1 < 0) return;
+    const int row = (blockIdx.y % (kChunkRows / kJoinRows)) * kJoinRows + (threadIdx.x % kJoinRows);
+    const int token = row / a.group, head = row - token * a.group;
+    const int tokens = min(a.half_tokens, entry.z - x * a.half_tokens);
+    if (token >= tokens) return;
+    const int c = (threadIdx.x / kJoinRows) * kCols;
+    auto part_of = [&](int cta) {
+        return a.partials + (static_cast<long long>(2 * cta + (cta == c0)) * 2 + x) * kPart;
+    };
+    auto stat = [&](int cta) { return __ldcg(reinterpret_cast<const float2*>(part_of(cta) + D * kChunkRows) + row); };
+    float most = -INFINITY, total = 0.f;
+#pragma unroll 4
+    for (int cta = c0; cta <= c1; ++cta) most = fmaxf(most, stat(cta).x);
+    float4 v[kCols];
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int cta = c0; cta <= c1; ++cta) {
+        const float2 ml = stat(cta);  // l = 0: saw no key
+        const float f = ml.y == 0.f ? 0.f : ex2_approx(ml.x - most);
+        total += ml.y * f;
+        const float4* o = reinterpret_cast<const float4*>(part_of(cta));
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) {
+            const float4 y = __ldcg(o + (c + k) * kChunkRows + row);
+            v[k].x += y.x * f, v[k].y += y.y * f, v[k].z += y.z * f, v[k].w += y.w * f;
+        }
+    }
+    const float scale = total != 0.f ? 1.0f / total : 0.f;
+    const long long out_row = entry.y + x * a.half_tokens + token;
+    const int out_head = entry.w * a.group + head;
+    T* out = static_cast<T*>(a.out) + out_row * a.out_stride + out_head * D + 4 * c;
+#pragma unroll
+    for (int k = 0; k < kCols; k += 2)
+        *reinterpret_cast<uint4*>(out + 4 * k) =
+            make_uint4(Pair<T>::pack(v[k].x * scale, v[k].y * scale), Pair<T>::pack(v[k].z * scale, v[k].w * scale),
+                       Pair<T>::pack(v[k + 1].x * scale, v[k + 1].y * scale),
+                       Pair<T>::pack(v[k + 1].z * scale, v[k + 1].w * scale));
+    if (a.lse != nullptr && c == 0)
+        a.lse[out_row * a.heads + out_head] =
+            total == 0.f ? -INFINITY : (most - kFewOffset) * 0.6931471805599453f + logf(total);
 }
 
 // A layer's pages [pages * kv_heads][page_size][D] as a 5-D tensor map (value,
@@ -765,8 +769,19 @@ static int launch_chunk(AttendArgs a, const h4b_paged_kv* kv, int sms, cudaStrea
     if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.q_stride) || !paged_kv_map(&kmap, a.k_pages, kv) ||
         !paged_kv_map(&vmap, a.v_pages, kv))
         return H4B_EUNSUPPORTED;
+    a.half_tokens = kChunkRows / a.group;
     paged_attention_chunk_kernel<T, D><<<sms, kChunkThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
     H4B_CUDA_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms, 2 * kChunkRows / kJoinRows);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // it waits in the kernel
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    H4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a));
     return 0;
 }
 
