@@ -229,6 +229,33 @@ def test_captured_graph_follows_the_tables():
     assert ((out.double() - want).abs() <= bound).all()
 
 
+def test_captured_chunks():
+    """Long chunks, some of them across CTAs, replay to the same bits (two launches a call)."""
+    batch = Batch([300, 1, 64], [3000, 90, 9000], heads=8, kv_heads=2, dim=128, page=16, dtype=torch.bfloat16)
+    workspace = ops.paged_workspace()
+    want = [t.clone() for t in batch.call(workspace=workspace)]
+    out, lse = torch.zeros_like(want[0]), torch.zeros_like(want[1])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        batch.call(workspace=workspace, out=out, lse=lse)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", SHAPES)
+def test_few_long_chunks_among_many_short(heads, kv_heads, dim, page, dtype):
+    """The short sequences of such a step go through a launch of their own; two
+    to four new tokens are on either side of that bound."""
+    new = [1] * 12 + [200] + [2, 3, 4] * 4 + [0, 90] + [1] * 6
+    total = [17 * i + n for i, n in enumerate(new)]
+    Batch(new, total, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype, window=150, sinks=5,
+          seed=11).check()
+
+
 def test_runs_on_the_current_stream():
     batch = Batch([1, 30], [500, 300], heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16)
     want, _ = batch.call()
