@@ -542,7 +542,7 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // products only. Keys that no row sees are zero-filled by the copy, so what
 // such a slot holds cannot reach a sum.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 64;
-constexpr int kFewExtra = 2;  // an item's start and join, in units (1 or 3: up to 5 % slower)
+constexpr int kFewExtra = 2;  // an item's start and join, in units (1: up to 5 % slower, 3 and 4: within 3 %)
 constexpr int kFewLeast = 1;  // a part is 4 KB beside 32 KB of keys
 constexpr float kFewOffset = 8.f, kFewSlack = 7.f;
 
