@@ -78,10 +78,12 @@ class PagedCache:
         return sequence
 
     def fork(self, sequence: int) -> int:
-        """A new sequence with the same tokens, sharing every page."""
-        table, length = self._tables[sequence], self._lengths[sequence]
+        """A new sequence with the same tokens, sharing every page that holds
+        some (room that `sequence` has reserved beyond them stays its own)."""
+        length = self._lengths[sequence]
+        table = self._tables[sequence][:-(-length // self.page_size)]
         new = self.new_sequence()
-        self._tables[new], self._lengths[new] = list(table), length
+        self._tables[new], self._lengths[new] = table, length
         for page in table:
             if page >= 0:
                 self._shared[page] += 1
