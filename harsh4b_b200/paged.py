@@ -55,6 +55,7 @@ class PagedCache:
         self._shared = np.zeros(pages, dtype=np.int32)  # sequences that hold a page
         self._tables: dict[int, list[int]] = {}         # page ids; -1 where trimmed
         self._lengths: dict[int, int] = {}
+        self._trimmed: set[int] = set()                 # sequences with a -1 in their table
         self._next = 0
 
     @classmethod
@@ -84,6 +85,8 @@ class PagedCache:
         table = self._tables[sequence][:-(-length // self.page_size)]
         new = self.new_sequence()
         self._tables[new], self._lengths[new] = table, length
+        if sequence in self._trimmed:
+            self._trimmed.add(new)
         for page in table:
             if page >= 0:
                 self._shared[page] += 1
@@ -93,9 +96,11 @@ class PagedCache:
         for page in self._tables.pop(sequence):
             self._drop(page)
         del self._lengths[sequence]
+        self._trimmed.discard(sequence)
 
     def truncate(self, sequence: int, length: int) -> None:
-        """Forget the tokens from `length` on."""
+        """Forget the tokens from `length` on. What `trim` gave back does not
+        return with an earlier end: see check_visible."""
         if not 0 <= length <= self._lengths[sequence]:
             raise ValueError("length must be within the sequence")
         table = self._tables[sequence]
@@ -117,7 +122,21 @@ class PagedCache:
                 self._drop(table[index])
                 table[index] = -1
                 dropped += 1
+        if dropped:
+            self._trimmed.add(sequence)
         return dropped
+
+    def check_visible(self, sequence: int, window: int = 0, sinks: int = 0) -> None:
+        """RuntimeError if the next token would see, under (window, sinks),
+        tokens whose pages `trim` gave back (after a truncation, or when the
+        window is wider than the one trimmed for): they would read as zeros."""
+        length, size = self._lengths[sequence], self.page_size
+        if sequence not in self._trimmed or length == 0:
+            return
+        table, first = self._tables[sequence], max(0, length + 1 - window) if window else 0
+        seen = table[first // size:-(-length // size)] if first < length else []
+        if -1 in seen or -1 in table[:-(-min(sinks, length) // size)]:
+            raise RuntimeError(f"sequence {sequence} sees tokens whose pages were given back")
 
     def reserve(self, wanted: dict[int, int]) -> None:
         """Room for `wanted[sequence]` more tokens of each sequence; what they
@@ -257,6 +276,8 @@ class PagedRunner:
         cache, model = self.cache, self.model
         if max(cache.length(s) + n for s, n in zip(sequences, new)) > model.max_pos:
             raise ValueError(f"a sequence would pass the model's {model.max_pos} positions")
+        for s in sequences:
+            cache.check_visible(s, self.window, self.sinks)
         cache.reserve(dict(zip(sequences, new)))
         table, offsets, lengths = (torch.from_numpy(a).to(cache.device) for a in cache.batch_tables(sequences, new))
         self.tokens[:total].copy_(torch.from_numpy(ids))

@@ -47,3 +47,69 @@ def test_reserved_room_outlives_a_fork(cache, length):  # noqa: F811
     assert read(cache, a) == list(range(length + 30))
     assert read(cache, b) == list(range(length)) + [p + 100 * b for p in range(length, length + 20)]
     consistent(cache)
+
+
+# ---- what a window has passed ---------------------------------------------------
+def seen_pages(length, window, sinks):
+    """Pages of the tokens that the next one (at `length`) sees, by the definition."""
+    return {j // 16 for j in range(length) if not window or j > length - window or j < sinks}
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (20, 4), (40, 0), (40, 17), (100, 0)])
+@pytest.mark.parametrize("trimmed,kept", [(40, 0), (20, 4), (100, 33)])
+@pytest.mark.parametrize("forked", [False, True])
+def test_tokens_given_back_are_not_seen_again(cache, window, sinks, trimmed, kept, forked):  # noqa: F811
+    a = cache.new_sequence()
+    grow(cache, a, 160)
+    cache.trim(a, trimmed, kept)
+    for length in (160, 159, 144, 143, 130, 96, 48, 16, 1, 0):
+        cache.truncate(a, length)
+        s = cache.fork(a) if forked else a
+        missing = [p for p in seen_pages(length, window, sinks) if cache.table(s)[p] < 0]
+        if missing:
+            with pytest.raises(RuntimeError, match="given back"):
+                cache.check_visible(s, window, sinks)
+        else:
+            cache.check_visible(s, window, sinks)
+        if forked:
+            cache.free(s)
+
+
+def cpu_runner(monkeypatch, cache, **kwargs):  # noqa: F811
+    """A runner whose model step and workspace are stand-ins."""
+    from types import SimpleNamespace
+
+    from harsh4b_b200 import paged
+
+    monkeypatch.setattr(paged.ops, "paged_workspace", lambda *a: torch.zeros(16, dtype=torch.uint8))
+    monkeypatch.setattr(paged, "lib", lambda: SimpleNamespace(h4b_forward_paged=lambda *a: 0))
+    monkeypatch.setattr(paged.torch.cuda, "current_stream", lambda *a: SimpleNamespace(cuda_stream=0))
+    model = SimpleNamespace(n_layers=2, kv_heads=2, head_dim=64, hidden=8, intermediate=8, q_size=128, kv_size=128,
+                            vocab=50, max_pos=4096, desc=paged.PagedStepDesc())
+    return paged.PagedRunner(model, cache, max_tokens=64, **kwargs)
+
+
+def test_a_step_behind_its_window_is_refused(cache, monkeypatch):  # noqa: F811
+    runner = cpu_runner(monkeypatch, cache, window=40)
+    a = cache.new_sequence()
+    for _ in range(10):
+        runner.step({a: [1] * 16})  # gives back what the window passes
+    runner.step({a: [1]})
+    cache.truncate(a, 152)  # the next token sees 113 and later, which are there
+    before = cache.table(a), cache.free_pages
+    cache.truncate(a, 144)  # and here 105 and later: page 6 is gone
+    before = cache.table(a), cache.free_pages
+    with pytest.raises(RuntimeError, match="given back"):
+        runner.step({a: [1]})
+    assert (cache.table(a), cache.free_pages) == before and cache.length(a) == 144
+    cache.truncate(a, 0)
+    runner.step({a: [1] * 20})
+    assert cache.length(a) == 20
+
+
+def test_an_unwindowed_step_over_a_trimmed_sequence_is_refused(cache, monkeypatch):  # noqa: F811
+    a = cache.new_sequence()
+    grow(cache, a, 60)
+    cache.trim(a, 20)
+    with pytest.raises(RuntimeError, match="given back"):
+        cpu_runner(monkeypatch, cache).step({a: [1]})
