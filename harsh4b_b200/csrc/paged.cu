@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 
 #include <climits>
+#include <cmath>
 
 namespace h4b {
 
@@ -1167,6 +1168,9 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     if (!paged_view(kv, &a.p) || heads < 1 || heads % kv->kv_heads || window < 0 || sinks < 0 ||
         (sinks > 0 && window == 0) || max_query < 1)
         return H4B_EINVAL;
+    // Both kernels take the maxima before the scale and mask with -infinity.
+    const float base2_scale = scale * 1.4426950408889634f;
+    if (!(base2_scale > 0.f) || !std::isfinite(base2_scale)) return H4B_EINVAL;
     if (!paged_shape_supported(kv) || heads / kv->kv_heads > kFewMaxRows ||
         static_cast<long long>(kv->pages) * kv->kv_heads > 0x7fffffffll)
         return H4B_EUNSUPPORTED;
@@ -1183,7 +1187,7 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     if (const int rc = paged_sm_count(&sms)) return rc;
     a.q = q, a.k_pages = kv->k_pages, a.v_pages = kv->v_pages, a.out = out, a.lse = lse;
     a.q_stride = q_stride, a.out_stride = out_stride, a.heads = heads, a.group = heads / kv->kv_heads;
-    a.window = window < kMaxLength ? window : kMaxLength, a.sinks = sinks, a.scale = scale * 1.4426950408889634f;
+    a.window = window < kMaxLength ? window : kMaxLength, a.sinks = sinks, a.scale = base2_scale;
     a.counters = static_cast<unsigned int*>(workspace);
     a.entries = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
     a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes + kEntryBytes);

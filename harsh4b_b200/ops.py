@@ -337,9 +337,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     hold the new tokens already (paged_append). `window` > 0: a token sees the
     last `window` keys (itself among them) and the first `sinks`. `max_query`
     is the longest chunk to expect (it picks the kernel; by default 1 when
-    there are no more rows than sequences, else all rows). `lse`, if given,
-    receives the float32 [tokens][heads] log-sum-exp. `workspace`: from
-    paged_workspace, kept between calls (one is made per call otherwise)."""
+    there are no more rows than sequences, else all rows). `scale` is positive
+    (1 / sqrt(head_dim) by default). `lse`, if given, receives the float32
+    [tokens][heads] log-sum-exp. `workspace`: from paged_workspace, kept between
+    calls (one is made per call otherwise)."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens][heads][head_dim]")
     tokens, heads, head_dim = shape = q.shape

@@ -492,7 +492,8 @@ int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, lon
  * apart (multiples of 8); q head h reads kv head h / (heads / kv_heads), at
  * most 32 heads to a kv head. A token at position p sees the keys j <= p; with
  * window > 0 only j > p - window or j < sinks. lse (may be null): float
- * [tokens][heads], the natural logarithm of each row's sum of exp(scale q.k).
+ * [tokens][heads], the natural logarithm of each row's sum of exp(scale q.k);
+ * scale is positive, and scale * log2(e) a finite fp32 above zero.
  * A row that sees no key gets zeros and lse -inf. max_query is the longest
  * chunk that the caller expects: it picks the kernel, and a longer chunk is
  * computed as well, only slower. workspace: zeroed when it is created, left
