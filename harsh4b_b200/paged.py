@@ -314,6 +314,8 @@ class PagedRunner:
         while any(len(o) < steps for o in out.values()):
             feed, left = {}, self.max_tokens
             for s, rest in pending.items():
+                if len(feed) == self.max_sequences:
+                    break
                 if len(out[s]) >= steps:
                     continue
                 take = 1 if out[s] else min(chunk, len(rest), left)

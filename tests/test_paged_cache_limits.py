@@ -113,3 +113,55 @@ def test_an_unwindowed_step_over_a_trimmed_sequence_is_refused(cache, monkeypatc
     cache.trim(a, 20)
     with pytest.raises(RuntimeError, match="given back"):
         cpu_runner(monkeypatch, cache).step({a: [1]})
+
+
+# ---- generate -------------------------------------------------------------------
+def generating(monkeypatch, cache, **kwargs):  # noqa: F811
+    """A runner whose greedy token is the number of rows fed so far, and its record of steps."""
+    runner = cpu_runner(monkeypatch, cache, **kwargs)
+    plain, runner.feeds = runner.step, []
+
+    def step(feed):
+        logits = plain(feed)
+        runner.feeds.append({s: list(t) for s, t in feed.items()})
+        runner.next_tokens[:len(feed)] = torch.tensor([cache.length(s) % 50 for s in feed], dtype=torch.int32)
+        return logits
+
+    runner.step = step
+    return runner
+
+
+def test_generate_refuses_before_its_first_step(cache, monkeypatch):  # noqa: F811
+    runner = generating(monkeypatch, cache)
+    a, b = cache.new_sequence(), cache.new_sequence()
+    for prompts, chunk in (({a: [1, 2], b: []}, 512), ({a: [1]}, 0), ({a: [1]}, -3)):
+        with pytest.raises(ValueError):
+            runner.generate(prompts, 3, chunk=chunk)
+    with pytest.raises(KeyError):
+        runner.generate({a: [1], 77: [2]}, 3)
+    assert runner.feeds == [] and cache.length(a) == cache.length(b) == 0
+    assert runner.generate({a: [1], b: [2]}, 0) == {a: [], b: []} and runner.generate({}, 4) == {}
+
+
+@pytest.mark.parametrize("most", [1, 2, 3, 5])
+@pytest.mark.parametrize("chunk", [1, 3, 512])
+def test_generate_more_prompts_than_a_step_holds(cache, monkeypatch, most, chunk):  # noqa: F811
+    runner = generating(monkeypatch, cache, max_sequences=most)
+    prompts = {cache.new_sequence(): [7] * n for n in (5, 1, 20, 3, 9)}
+    out = runner.generate(prompts, 4, chunk=chunk)
+    for s, prompt in prompts.items():
+        assert out[s] == [len(prompt) + i for i in range(4)]
+        fed = [t for feed in runner.feeds for t in feed.get(s, [])]
+        assert fed == prompt + out[s][:3] and cache.length(s) == len(fed)
+    assert max(len(feed) for feed in runner.feeds) == most
+
+
+def test_generate_checks_ids_and_positions_first(cache, monkeypatch):  # noqa: F811
+    runner = generating(monkeypatch, cache)
+    runner.model.max_pos = 30
+    a, b = cache.new_sequence(), cache.new_sequence()
+    for prompt, steps in (([-1], 2), ([50], 2), ([1] * 31, 1), ([1] * 28, 4)):
+        with pytest.raises(ValueError):
+            runner.generate({a: [1], b: prompt}, steps, chunk=8)
+    assert runner.feeds == []
+    assert len(runner.generate({b: [1] * 28}, 3, chunk=8)[b]) == 3
