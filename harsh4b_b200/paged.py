@@ -308,8 +308,16 @@ class PagedRunner:
     def generate(self, prompts: dict[int, list[int]], steps: int, chunk: int = 512) -> dict[int, list[int]]:
         """Greedy tokens of every sequence: prompts go in `chunk` tokens at a
         time while the others already decode (each step holds the chunks and
-        the decoding sequences' single tokens)."""
-        pending = {s: list(p) for s, p in prompts.items()}
+        the decoding sequences' single tokens; sequences that a step has no
+        room for wait). Prompts are checked before the first step."""
+        pending = {s: [int(t) for t in p] for s, p in prompts.items()}
+        if chunk < 1:
+            raise ValueError("chunk must be positive")
+        for s, rest in pending.items():
+            if not rest or min(rest) < 0 or max(rest) >= self.model.vocab:
+                raise ValueError("every prompt needs a token, and its IDs must be in the vocabulary")
+            if self.cache.length(s) + len(rest) + max(steps, 1) - 1 > self.model.max_pos:
+                raise ValueError(f"a sequence would pass the model's {self.model.max_pos} positions")
         out: dict[int, list[int]] = {s: [] for s in prompts}
         while any(len(o) < steps for o in out.values()):
             feed, left = {}, self.max_tokens
