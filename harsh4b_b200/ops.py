@@ -249,6 +249,15 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _here(*tensors) -> int:
+    """The current device, where the library launches: every tensor has to be there."""
+    index = torch.cuda.current_device()
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != index:
+            raise ValueError(f"every tensor must be on the current device, cuda:{index}, got {tensor.device}")
+    return index
+
+
 def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> PagedKvDesc:
     """The h4b_paged_kv of one layer's pages and a batch's tables."""
     dtype = k_pages.dtype
@@ -303,10 +312,12 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             raise ValueError("rope_cos and rope_sin must be [positions][head_dim / 2]")
         positions = rope_cos.shape[0]
         cos, sin = _dev(rope_cos, torch.float32, "rope_cos"), _dev(rope_sin, torch.float32, "rope_sin")
-    check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, source, "qkv"), 0 if source is torch.float32 else kv.dtype,
+    source_rows, out_rows = _rows(qkv, source, "qkv"), _rows(out, dtype, "out")
+    device = _here(qkv, k_pages, v_pages, page_table, q_offsets, kv_lens, norm_q, norm_k, rope_cos, rope_sin, out)
+    check(lib().h4b_paged_append(ctypes.byref(kv), source_rows, 0 if source is torch.float32 else kv.dtype,
                                  qkv.stride(0) if tokens > 1 else width, heads, weights[0], weights[1], eps, cos, sin,
-                                 positions, _rows(out, dtype, "out"), out.stride(0) if tokens > 1 else heads * head_dim,
-                                 _raw_stream(qkv.device.index)), "h4b_paged_append")
+                                 positions, out_rows, out.stride(0) if tokens > 1 else heads * head_dim,
+                                 _raw_stream(device)), "h4b_paged_append")
     return out
 
 
@@ -360,12 +371,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         workspace = paged_workspace(head_dim, q.device)
     width = heads * head_dim
     several = tokens > 1
-    check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, dtype, "q"), q.stride(0) if several else width, heads,
-                                    head_dim ** -0.5 if scale is None else scale, window, sinks, max_query,
-                                    _rows(out, dtype, "out"), out.stride(0) if several else width,
-                                    None if lse is None else _dev(lse, torch.float32, "lse"),
-                                    _dev(workspace, torch.uint8, "workspace"), workspace.numel(),
-                                    _raw_stream(q.device.index)), "h4b_paged_attention")
+    q_rows, out_rows = _rows(q, dtype, "q"), _rows(out, dtype, "out")
+    sums, scratch = None if lse is None else _dev(lse, torch.float32, "lse"), _dev(workspace, torch.uint8, "workspace")
+    device = _here(q, k_pages, v_pages, page_table, q_offsets, kv_lens, out, lse, workspace)
+    check(lib().h4b_paged_attention(ctypes.byref(kv), q_rows, q.stride(0) if several else width, heads,
+                                    head_dim ** -0.5 if scale is None else scale, window, sinks, max_query, out_rows,
+                                    out.stride(0) if several else width, sums, scratch, workspace.numel(),
+                                    _raw_stream(device)), "h4b_paged_attention")
     return out
 
 
@@ -380,8 +392,9 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     if count != dst.numel():
         raise ValueError("src and dst must hold as many page ids")
     pages, kv_heads, page_size, head_dim = shape[-4:]
-    check(lib().h4b_pages_copy(_dev(k_pages, dtype, "k_pages"), _dev(v_pages, dtype, "v_pages"),
-                               shape[0] if len(shape) == 5 else 1, pages,
-                               kv_heads * page_size * head_dim * k_pages.element_size(),
-                               _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst"), count,
-                               _raw_stream(k_pages.device.index)), "h4b_pages_copy")
+    buffers = _dev(k_pages, dtype, "k_pages"), _dev(v_pages, dtype, "v_pages")
+    ids = _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst")
+    device = _here(k_pages, v_pages, src, dst)
+    check(lib().h4b_pages_copy(*buffers, shape[0] if len(shape) == 5 else 1, pages,
+                               kv_heads * page_size * head_dim * k_pages.element_size(), *ids, count,
+                               _raw_stream(device)), "h4b_pages_copy")

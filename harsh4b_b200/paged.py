@@ -21,6 +21,7 @@ any number of sequences in one step.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 
 import numpy as np
 import torch
@@ -29,6 +30,11 @@ from . import ops
 from ._lib import STATUS_BAD_PAGE, PagedKvDesc, PagedStepDesc, check, device_status, lib
 
 CACHE_DTYPES = {"float16": torch.float16, "bfloat16": torch.bfloat16}
+
+
+def on_device(device: torch.device):
+    """Makes a CUDA device current (the library launches there)."""
+    return torch.cuda.device(device) if device.type == "cuda" else nullcontext()
 
 
 class PagedCache:
@@ -50,7 +56,7 @@ class PagedCache:
         shape = (layers, pages, kv_heads, page_size, head_dim)
         self.k_pages = torch.zeros(shape, dtype=CACHE_DTYPES[dtype], device=device)
         self.v_pages = torch.zeros(shape, dtype=CACHE_DTYPES[dtype], device=device)
-        self.page_size, self.pages, self.device = page_size, pages, device
+        self.page_size, self.pages, self.device = page_size, pages, self.k_pages.device
         self._free = list(range(pages - 1, -1, -1))  # the lowest page is taken next
         self._shared = np.zeros(pages, dtype=np.int32)  # sequences that hold a page
         self._tables: dict[int, list[int]] = {}         # page ids; -1 where trimmed
@@ -225,7 +231,8 @@ class PagedCache:
         if not moves:
             return
         ids = torch.tensor(moves, dtype=torch.int32).T.contiguous().to(self.device)
-        ops.copy_pages(self.k_pages, self.v_pages, ids[0], ids[1])
+        with on_device(self.device):
+            ops.copy_pages(self.k_pages, self.v_pages, ids[0], ids[1])
 
 
 class PagedRunner:
@@ -242,6 +249,8 @@ class PagedRunner:
         layers, _, kv_heads, _, head_dim = cache.k_pages.shape
         if (layers, kv_heads, head_dim) != (model.n_layers, model.kv_heads, model.head_dim):
             raise ValueError("the cache does not have the model's layers and heads")
+        if cache.device != model.embedding.device:
+            raise ValueError("the cache is not on the model's device")
         self.model, self.cache, self.max_tokens, self.max_sequences = model, cache, max_tokens, max_sequences
         self.window, self.sinks = window, sinks
         dev = cache.device
@@ -289,8 +298,9 @@ class PagedRunner:
         step = PagedStepDesc(kv, cache.k_pages[0].numel() * 2, self.window, self.sinks, max(new), *[t.data_ptr() for t in (
             self.tokens, self.x, self.x8, self.act_scale, self.act_sum, self.qkv, self.q, self.attended16, self.attended,
             self.gate_up, self.act, self.last, self.logits, self.next_tokens, self.workspace)], self.workspace.numel())
-        check(lib().h4b_forward_paged(ctypes.byref(model.desc), ctypes.byref(step),
-                                      torch.cuda.current_stream(cache.device).cuda_stream), "h4b_forward_paged")
+        with on_device(cache.device):
+            check(lib().h4b_forward_paged(ctypes.byref(model.desc), ctypes.byref(step),
+                                          torch.cuda.current_stream(cache.device).cuda_stream), "h4b_forward_paged")
         for s, n in zip(sequences, new):
             cache.advance(s, n)
             if self.window:
@@ -299,7 +309,8 @@ class PagedRunner:
 
     def status(self) -> None:
         """Raise if a kernel met a page, offset or length out of range."""
-        code = device_status()
+        with on_device(self.cache.device):
+            code = device_status()
         if code & STATUS_BAD_PAGE:
             raise RuntimeError("a page id, row offset or length was out of range")
         if code:

@@ -40,3 +40,16 @@ def test_scales_that_are_refused(new, total, scale):
     batch = Batch(new, total, heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16)
     with pytest.raises(ValueError, match="scale|invalid argument"):
         batch.call(scale=scale)
+
+
+# ---- devices ----------------------------------------------------------------------
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    batch = Batch([1], [40], heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16)
+    workspace, ids = ops.paged_workspace(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    args = batch.k_pages, batch.v_pages, batch.table, batch.offsets, batch.lens
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: ops.paged_attention(batch.q, *args, workspace=workspace),
+                 lambda: ops.paged_append(torch.zeros(1, 12 * 128, device="cuda:0"), *args, heads=8),
+                 lambda: ops.copy_pages(*args[:2], ids, ids + 1)):
+        with pytest.raises(ValueError, match="current device, cuda:1"):
+            call()

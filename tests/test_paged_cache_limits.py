@@ -85,7 +85,7 @@ def cpu_runner(monkeypatch, cache, **kwargs):  # noqa: F811
     monkeypatch.setattr(paged, "lib", lambda: SimpleNamespace(h4b_forward_paged=lambda *a: 0))
     monkeypatch.setattr(paged.torch.cuda, "current_stream", lambda *a: SimpleNamespace(cuda_stream=0))
     model = SimpleNamespace(n_layers=2, kv_heads=2, head_dim=64, hidden=8, intermediate=8, q_size=128, kv_size=128,
-                            vocab=50, max_pos=4096, desc=paged.PagedStepDesc())
+                            vocab=50, max_pos=4096, desc=paged.PagedStepDesc(), embedding=cache.k_pages)
     return paged.PagedRunner(model, cache, max_tokens=64, **kwargs)
 
 
@@ -165,3 +165,53 @@ def test_generate_checks_ids_and_positions_first(cache, monkeypatch):  # noqa: F
             runner.generate({a: [1], b: prompt}, steps, chunk=8)
     assert runner.feeds == []
     assert len(runner.generate({b: [1] * 28}, 3, chunk=8)[b]) == 3
+
+
+# ---- devices --------------------------------------------------------------------
+def test_every_tensor_must_be_on_the_current_device(monkeypatch):
+    from types import SimpleNamespace
+
+    from harsh4b_b200 import ops
+
+    def on(index):
+        return SimpleNamespace(get_device=lambda: index, device=f"cuda:{index}")
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    assert ops._here(on(1), None, on(1)) == 1
+    for tensors in ((on(0), on(0)), (on(1), on(0)), (on(1), None, on(2))):
+        with pytest.raises(ValueError, match="current device, cuda:1"):
+            ops._here(*tensors)
+
+
+def test_steps_and_copies_make_the_caches_device_current(cache, monkeypatch):  # noqa: F811
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+
+    from harsh4b_b200 import paged
+
+    current, seen = [], []
+
+    @contextmanager
+    def device(index):
+        current.append(index)
+        yield
+        current.pop()
+
+    runner = cpu_runner(monkeypatch, cache)
+    monkeypatch.setattr(paged, "on_device", device)
+    monkeypatch.setattr(paged, "lib", lambda: SimpleNamespace(h4b_forward_paged=lambda *a: seen.append(list(current)) or 0))
+    copy = paged.ops.copy_pages
+    monkeypatch.setattr(paged.ops, "copy_pages", lambda *a: (seen.append(list(current)), copy(*a)))
+    a = cache.new_sequence()
+    runner.step({a: [1] * 20})
+    runner.step({cache.fork(a): [2]})  # a copy and a step
+    assert seen == [[cache.device]] * 3
+
+
+def test_a_cache_on_another_device_is_refused(cache, monkeypatch):  # noqa: F811
+    from types import SimpleNamespace
+
+    runner = cpu_runner(monkeypatch, cache)
+    runner.model.embedding = SimpleNamespace(device=torch.device("cuda", 1))
+    with pytest.raises(ValueError, match="model's device"):
+        type(runner)(runner.model, cache)
