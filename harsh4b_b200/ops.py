@@ -236,11 +236,21 @@ def residual_acc(x: torch.Tensor, acc: torch.Tensor, absmax: torch.Tensor, scale
 _PAGED_DTYPES = {torch.float16: 1, torch.bfloat16: 2}  # H4B_FP16, H4B_BF16
 
 
-def _rows(tensor: torch.Tensor, dtype: torch.dtype, name: str) -> int:
-    """Data pointer of a CUDA tensor whose rows (dim 0) may be strided."""
-    if tensor.is_cuda and tensor.dtype == dtype and (tensor.is_contiguous() or tensor[:1].squeeze(0).is_contiguous()):
+def _on(tensor: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> int:
+    """Data pointer of a contiguous tensor on CUDA device `device`."""
+    if isinstance(tensor, torch.Tensor) and tensor.get_device() == device >= 0 and tensor.dtype == dtype \
+            and tensor.is_contiguous():
         return tensor.data_ptr()
     _dev(tensor, dtype, name)
+    raise ValueError(f"{name} must be on the device of the other tensors, cuda:{device}, got {tensor.device}")
+
+
+def _rows(tensor: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> int:
+    """Data pointer of a tensor on CUDA device `device` whose rows (dim 0) may be strided."""
+    if isinstance(tensor, torch.Tensor) and tensor.get_device() == device >= 0 and tensor.dtype == dtype \
+            and (tensor.is_contiguous() or tensor[:1].squeeze(0).is_contiguous()):
+        return tensor.data_ptr()
+    _on(tensor[:1].squeeze(0) if isinstance(tensor, torch.Tensor) else tensor, dtype, name, device)
     raise ValueError(f"{name} must be contiguous within each row")
 
 
@@ -249,13 +259,13 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _here(*tensors) -> int:
-    """The current device, where the library launches: every tensor has to be there."""
-    index = torch.cuda.current_device()
-    for tensor in tensors:
-        if tensor is not None and tensor.get_device() != index:
-            raise ValueError(f"every tensor must be on the current device, cuda:{index}, got {tensor.device}")
-    return index
+def _here(device: int) -> int:
+    """The current stream of the tensors' device, which has to be the current
+    one: the library launches there."""
+    current = torch.cuda.current_device()
+    if device != current:
+        raise ValueError(f"the tensors must be on the current device, cuda:{current}, not cuda:{device}")
+    return _raw_stream(device)
 
 
 def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> PagedKvDesc:
@@ -270,9 +280,11 @@ def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> Pag
     sequences = kv_lens.numel()
     if len(table) != 2 or table[0] != sequences or q_offsets.numel() != sequences + 1:
         raise ValueError("page_table must be [sequences][pages each], q_offsets [sequences + 1], kv_lens [sequences]")
-    return PagedKvDesc(_dev(k_pages, dtype, "k_pages"), _dev(v_pages, dtype, "v_pages"),
-                       _dev(page_table, torch.int32, "page_table"), _dev(q_offsets, torch.int32, "q_offsets"),
-                       _dev(kv_lens, torch.int32, "kv_lens"), code, shape[0], shape[2], shape[1], shape[3],
+    device = k_pages.get_device()
+    return PagedKvDesc(_on(k_pages, dtype, "k_pages", device), _on(v_pages, dtype, "v_pages", device),
+                       _on(page_table, torch.int32, "page_table", device),
+                       _on(q_offsets, torch.int32, "q_offsets", device),
+                       _on(kv_lens, torch.int32, "kv_lens", device), code, shape[0], shape[2], shape[1], shape[3],
                        sequences, table[1], tokens)
 
 
@@ -287,7 +299,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     `norm_q` / `norm_k` and rotated with `rope_cos` / `rope_sin` where given.
     Returns q [tokens][heads][head_dim] in the cache's type."""
     tokens, width = qkv.shape if qkv.dim() == 2 else (0, -1)
-    dtype, source = k_pages.dtype, qkv.dtype
+    dtype, source, device = k_pages.dtype, qkv.dtype, k_pages.get_device()
     kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
     head_dim = kv.head_dim
     if width != (heads + 2 * kv.kv_heads) * head_dim:
@@ -303,7 +315,7 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         if norm is not None:
             if norm.numel() != head_dim:
                 raise ValueError(f"{name} must hold head_dim values")
-            weights[k] = _dev(norm, torch.float32, name)
+            weights[k] = _on(norm, torch.float32, name, device)
     cos = sin = None
     positions = 0
     if rope_cos is not None or rope_sin is not None:
@@ -311,13 +323,11 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                 or rope_cos.shape[1] != head_dim // 2:
             raise ValueError("rope_cos and rope_sin must be [positions][head_dim / 2]")
         positions = rope_cos.shape[0]
-        cos, sin = _dev(rope_cos, torch.float32, "rope_cos"), _dev(rope_sin, torch.float32, "rope_sin")
-    source_rows, out_rows = _rows(qkv, source, "qkv"), _rows(out, dtype, "out")
-    device = _here(qkv, k_pages, v_pages, page_table, q_offsets, kv_lens, norm_q, norm_k, rope_cos, rope_sin, out)
-    check(lib().h4b_paged_append(ctypes.byref(kv), source_rows, 0 if source is torch.float32 else kv.dtype,
-                                 qkv.stride(0) if tokens > 1 else width, heads, weights[0], weights[1], eps, cos, sin,
-                                 positions, out_rows, out.stride(0) if tokens > 1 else heads * head_dim,
-                                 _raw_stream(device)), "h4b_paged_append")
+        cos, sin = _on(rope_cos, torch.float32, "rope_cos", device), _on(rope_sin, torch.float32, "rope_sin", device)
+    check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, source, "qkv", device),
+                                 0 if source is torch.float32 else kv.dtype, qkv.stride(0) if tokens > 1 else width, heads, weights[0], weights[1], eps, cos, sin,
+                                 positions, _rows(out, dtype, "out", device),
+                                 out.stride(0) if tokens > 1 else heads * head_dim, _here(device)), "h4b_paged_append")
     return out
 
 
@@ -355,7 +365,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.dim() != 3:
         raise ValueError("q must be [tokens][heads][head_dim]")
     tokens, heads, head_dim = shape = q.shape
-    dtype = k_pages.dtype
+    dtype, device = k_pages.dtype, k_pages.get_device()
     kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
     if head_dim != kv.head_dim or heads % kv.kv_heads:
         raise ValueError("q must have the cache's head_dim and a multiple of its kv heads")
@@ -371,13 +381,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         workspace = paged_workspace(head_dim, q.device)
     width = heads * head_dim
     several = tokens > 1
-    q_rows, out_rows = _rows(q, dtype, "q"), _rows(out, dtype, "out")
-    sums, scratch = None if lse is None else _dev(lse, torch.float32, "lse"), _dev(workspace, torch.uint8, "workspace")
-    device = _here(q, k_pages, v_pages, page_table, q_offsets, kv_lens, out, lse, workspace)
-    check(lib().h4b_paged_attention(ctypes.byref(kv), q_rows, q.stride(0) if several else width, heads,
-                                    head_dim ** -0.5 if scale is None else scale, window, sinks, max_query, out_rows,
-                                    out.stride(0) if several else width, sums, scratch, workspace.numel(),
-                                    _raw_stream(device)), "h4b_paged_attention")
+    check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, dtype, "q", device), q.stride(0) if several else width,
+                                    heads, head_dim ** -0.5 if scale is None else scale, window, sinks, max_query,
+                                    _rows(out, dtype, "out", device), out.stride(0) if several else width,
+                                    None if lse is None else _on(lse, torch.float32, "lse", device),
+                                    _on(workspace, torch.uint8, "workspace", device), workspace.numel(),
+                                    _here(device)), "h4b_paged_attention")
     return out
 
 
@@ -386,15 +395,14 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     [layers][pages][kv_heads][page_size][head_dim] (or one layer's [pages]...)
     caches of any type; int32 ids on the device. No page may be the
     destination of two moves, nor a source and a destination."""
-    shape, dtype, count = k_pages.shape, k_pages.dtype, src.numel()
+    shape, dtype, count, device = k_pages.shape, k_pages.dtype, src.numel(), k_pages.get_device()
     if shape != v_pages.shape or len(shape) not in (4, 5):
         raise ValueError("k_pages and v_pages must be [layers][pages][kv_heads][page_size][head_dim]")
     if count != dst.numel():
         raise ValueError("src and dst must hold as many page ids")
     pages, kv_heads, page_size, head_dim = shape[-4:]
-    buffers = _dev(k_pages, dtype, "k_pages"), _dev(v_pages, dtype, "v_pages")
-    ids = _dev(src, torch.int32, "src"), _dev(dst, torch.int32, "dst")
-    device = _here(k_pages, v_pages, src, dst)
-    check(lib().h4b_pages_copy(*buffers, shape[0] if len(shape) == 5 else 1, pages,
-                               kv_heads * page_size * head_dim * k_pages.element_size(), *ids, count,
-                               _raw_stream(device)), "h4b_pages_copy")
+    check(lib().h4b_pages_copy(_on(k_pages, dtype, "k_pages", device), _on(v_pages, dtype, "v_pages", device),
+                               shape[0] if len(shape) == 5 else 1, pages,
+                               kv_heads * page_size * head_dim * k_pages.element_size(),
+                               _on(src, torch.int32, "src", device), _on(dst, torch.int32, "dst", device), count,
+                               _here(device)), "h4b_pages_copy")

@@ -169,18 +169,27 @@ def test_generate_checks_ids_and_positions_first(cache, monkeypatch):  # noqa: F
 
 # ---- devices --------------------------------------------------------------------
 def test_every_tensor_must_be_on_the_current_device(monkeypatch):
-    from types import SimpleNamespace
-
     from harsh4b_b200 import ops
 
-    def on(index):
-        return SimpleNamespace(get_device=lambda: index, device=f"cuda:{index}")
+    class On(torch.Tensor):  # a CPU tensor that says it lies on CUDA device 1
+        is_cuda, device = True, "cuda:1"
+
+        def get_device(self):
+            return 1
 
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
-    assert ops._here(on(1), None, on(1)) == 1
-    for tensors in ((on(0), on(0)), (on(1), on(0)), (on(1), None, on(2))):
-        with pytest.raises(ValueError, match="current device, cuda:1"):
-            ops._here(*tensors)
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 100 + index)
+    assert ops._here(1) == 101
+    with pytest.raises(ValueError, match="current device, cuda:1, not cuda:0"):
+        ops._here(0)
+    tensor = torch.zeros(4, 4).as_subclass(On)
+    for pointer in (ops._on, ops._rows):
+        assert pointer(tensor, torch.float32, "x", 1) == tensor.data_ptr()
+        for device in (0, 2):
+            with pytest.raises(ValueError, match="x must be on the device of the other tensors"):
+                pointer(tensor, torch.float32, "x", device)
+        with pytest.raises(ValueError, match="x must be a CUDA tensor"):
+            pointer(torch.zeros(4, 4), torch.float32, "x", -1)
 
 
 def test_steps_and_copies_make_the_caches_device_current(cache, monkeypatch):  # noqa: F811
