@@ -325,8 +325,8 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         positions = rope_cos.shape[0]
         cos, sin = _on(rope_cos, torch.float32, "rope_cos", device), _on(rope_sin, torch.float32, "rope_sin", device)
     check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, source, "qkv", device),
-                                 0 if source is torch.float32 else kv.dtype, qkv.stride(0) if tokens > 1 else width, heads, weights[0], weights[1], eps, cos, sin,
-                                 positions, _rows(out, dtype, "out", device),
+                                 0 if source is torch.float32 else kv.dtype, qkv.stride(0) if tokens > 1 else width, heads,
+                                 weights[0], weights[1], eps, cos, sin, positions, _rows(out, dtype, "out", device),
                                  out.stride(0) if tokens > 1 else heads * head_dim, _here(device)), "h4b_paged_append")
     return out
 
