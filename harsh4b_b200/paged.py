@@ -21,7 +21,7 @@ any number of sequences in one step.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
+from contextlib import contextmanager, nullcontext
 
 import numpy as np
 import torch
@@ -40,7 +40,13 @@ def on_device(device: torch.device):
 class PagedCache:
     """Pages [layers][pages][kv_heads][page_size][head_dim] of K and V, and the
     sequences that hold them. Lengths count tokens; `reserve` makes room (and
-    private) what the next append writes."""
+    private) what the next append writes.
+
+    Pages that are given back may be taken again while kernels that read them
+    are still queued, so all work on the pages is in one order: the cache's
+    copies and its runners' steps follow those before them, whichever streams
+    they are on. Launches of one's own belong into ``with cache.ordered():``
+    where several streams use the cache."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, page_size: int = 16,
                  dtype: str = "float16", device=None):
@@ -63,6 +69,28 @@ class PagedCache:
         self._lengths: dict[int, int] = {}
         self._trimmed: set[int] = set()                 # sequences with a -1 in their table
         self._next = 0
+        # the end of the latest work on the pages (none on a CPU) and its stream
+        self._event = torch.cuda.Event() if self.device.type == "cuda" else None
+        self._stream = None
+        with self.ordered():
+            pass  # the pages are zeroed here
+
+    @contextmanager
+    def ordered(self):
+        """Work on the pages that is launched in here, on the current stream,
+        runs after all such work before it and before all that follows."""
+        with on_device(self.device):
+            if self._event is None:
+                yield
+                return
+            stream = torch.cuda.current_stream(self.device)
+            if self._stream is not None and stream != self._stream:
+                stream.wait_event(self._event)
+            try:
+                yield
+            finally:
+                self._event.record(stream)
+                self._stream = stream
 
     @classmethod
     def for_model(cls, model, pages: int, page_size: int = 16, dtype: str = "float16") -> "PagedCache":
@@ -231,7 +259,7 @@ class PagedCache:
         if not moves:
             return
         ids = torch.tensor(moves, dtype=torch.int32).T.contiguous().to(self.device)
-        with on_device(self.device):
+        with self.ordered():
             ops.copy_pages(self.k_pages, self.v_pages, ids[0], ids[1])
 
 
@@ -253,7 +281,12 @@ class PagedRunner:
             raise ValueError("the cache is not on the model's device")
         self.model, self.cache, self.max_tokens, self.max_sequences = model, cache, max_tokens, max_sequences
         self.window, self.sinks = window, sinks
-        dev = cache.device
+        with cache.ordered():  # its first step may be on another stream
+            self._allocate()
+
+    def _allocate(self) -> None:
+        model, cache = self.model, self.cache
+        dev, max_tokens, max_sequences = cache.device, self.max_tokens, self.max_sequences
         H, I, Q, KV = model.hidden, model.intermediate, model.q_size, model.kv_size
         M, B, either = max_tokens, max_sequences, max(max_tokens, max_sequences)
         f32, i32 = dict(dtype=torch.float32, device=dev), dict(dtype=torch.int32, device=dev)
@@ -287,7 +320,17 @@ class PagedRunner:
             raise ValueError(f"a sequence would pass the model's {model.max_pos} positions")
         for s in sequences:
             cache.check_visible(s, self.window, self.sinks)
-        cache.reserve(dict(zip(sequences, new)))
+        with cache.ordered():
+            cache.reserve(dict(zip(sequences, new)))
+            self._launch(sequences, new, ids)
+        for s, n in zip(sequences, new):
+            cache.advance(s, n)
+            if self.window:
+                cache.trim(s, self.window, self.sinks)
+        return {s: self.logits[b] for b, s in enumerate(sequences)}
+
+    def _launch(self, sequences, new, ids: np.ndarray) -> None:
+        cache, model, total = self.cache, self.model, len(ids)
         table, offsets, lengths = (torch.from_numpy(a).to(cache.device) for a in cache.batch_tables(sequences, new))
         self.tokens[:total].copy_(torch.from_numpy(ids))
         layers, pages, kv_heads, page_size, head_dim = cache.k_pages.shape
@@ -298,14 +341,8 @@ class PagedRunner:
         step = PagedStepDesc(kv, cache.k_pages[0].numel() * 2, self.window, self.sinks, max(new), *[t.data_ptr() for t in (
             self.tokens, self.x, self.x8, self.act_scale, self.act_sum, self.qkv, self.q, self.attended16, self.attended,
             self.gate_up, self.act, self.last, self.logits, self.next_tokens, self.workspace)], self.workspace.numel())
-        with on_device(cache.device):
-            check(lib().h4b_forward_paged(ctypes.byref(model.desc), ctypes.byref(step),
-                                          torch.cuda.current_stream(cache.device).cuda_stream), "h4b_forward_paged")
-        for s, n in zip(sequences, new):
-            cache.advance(s, n)
-            if self.window:
-                cache.trim(s, self.window, self.sinks)
-        return {s: self.logits[b] for b, s in enumerate(sequences)}
+        check(lib().h4b_forward_paged(ctypes.byref(model.desc), ctypes.byref(step),
+                                      torch.cuda.current_stream(cache.device).cuda_stream), "h4b_forward_paged")
 
     def status(self) -> None:
         """Raise if a kernel met a page, offset or length out of range."""

@@ -84,6 +84,14 @@ def cpu_runner(monkeypatch, cache, **kwargs):  # noqa: F811
     monkeypatch.setattr(paged.ops, "paged_workspace", lambda *a: torch.zeros(16, dtype=torch.uint8))
     monkeypatch.setattr(paged, "lib", lambda: SimpleNamespace(h4b_forward_paged=lambda *a: 0))
     monkeypatch.setattr(paged.torch.cuda, "current_stream", lambda *a: SimpleNamespace(cuda_stream=0))
+    return cpu_runner_over(cache, **kwargs)
+
+
+def cpu_runner_over(cache, **kwargs):  # noqa: F811
+    from types import SimpleNamespace
+
+    from harsh4b_b200 import paged
+
     model = SimpleNamespace(n_layers=2, kv_heads=2, head_dim=64, hidden=8, intermediate=8, q_size=128, kv_size=128,
                             vocab=50, max_pos=4096, desc=paged.PagedStepDesc(), embedding=cache.k_pages)
     return paged.PagedRunner(model, cache, max_tokens=64, **kwargs)
@@ -214,7 +222,7 @@ def test_steps_and_copies_make_the_caches_device_current(cache, monkeypatch):  #
     a = cache.new_sequence()
     runner.step({a: [1] * 20})
     runner.step({cache.fork(a): [2]})  # a copy and a step
-    assert seen == [[cache.device]] * 3
+    assert [devices[-1:] for devices in seen] == [[cache.device]] * 3
 
 
 def test_a_cache_on_another_device_is_refused(cache, monkeypatch):  # noqa: F811
@@ -224,3 +232,57 @@ def test_a_cache_on_another_device_is_refused(cache, monkeypatch):  # noqa: F811
     runner.model.embedding = SimpleNamespace(device=torch.device("cuda", 1))
     with pytest.raises(ValueError, match="model's device"):
         type(runner)(runner.model, cache)
+
+
+# ---- streams --------------------------------------------------------------------
+class Streams:
+    """Stand-ins for CUDA streams and the cache's event: what waits for what."""
+
+    def __init__(self, monkeypatch, cache):  # noqa: F811
+        from types import SimpleNamespace
+
+        from harsh4b_b200 import paged
+
+        self.log, self.now = [], None
+        self.made = {name: SimpleNamespace(name=name, cuda_stream=0, wait_event=lambda e, name=name: self.log.append(f"{name} waits"))
+                     for name in "AB"}
+        cache._event = SimpleNamespace(record=lambda stream: self.log.append(f"{stream.name} records"))
+        monkeypatch.setattr(paged.torch.cuda, "current_stream", lambda *a: self.made[self.now])
+
+    def on(self, name):
+        self.now = name
+        self.log.clear()
+
+
+def test_work_on_another_stream_waits(cache, monkeypatch):  # noqa: F811
+    runner, other = cpu_runner(monkeypatch, cache, window=20), cpu_runner(monkeypatch, cache)
+    streams = Streams(monkeypatch, cache)
+    a, b = cache.new_sequence(), cache.new_sequence()
+    streams.on("A")
+    runner.step({a: [1] * 60})  # gives pages back while its kernels may still read them
+    assert streams.log[-1] == "A records"
+    streams.on("A")
+    runner.step({a: [1]})
+    assert "A waits" not in streams.log and streams.log[-1] == "A records"
+    streams.on("B")
+    other.step({b: [1] * 40})
+    assert streams.log[0] == "B waits" and streams.log[-1] == "B records"
+    cache.free(a)
+    streams.on("A")
+    assert cache.compact() > 0
+    assert streams.log == ["A waits", "A records"]
+    streams.on("B")
+    cache.reserve({cache.fork(b): 1})  # the copy of a shared page
+    assert streams.log == ["B waits", "B records"]
+
+
+def test_a_runner_follows_its_caches_streams(cache, monkeypatch):  # noqa: F811
+    """Its scratch is zeroed on the stream that makes it."""
+    cpu_runner(monkeypatch, cache)
+    streams = Streams(monkeypatch, cache)
+    streams.on("A")
+    runner = cpu_runner_over(cache)
+    assert streams.log[-1] == "A records"
+    streams.on("B")
+    runner.step({cache.new_sequence(): [1]})
+    assert streams.log[0] == "B waits"
