@@ -181,9 +181,12 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const A
             }
         }
     }
-    float4 cos = make_float4(1.f, 1.f, 1.f, 1.f), sin = make_float4(0.f, 0.f, 0.f, 0.f);
+    // (not by an angle of zero where there is none: that would add 0 times the
+    // partner, which need not be finite)
+    float4 cos{}, sin{};
+    const bool rotated = a.cos != nullptr && position >= 0 && position < a.max_pos;
     if (a.cos != nullptr && position >= 0) {
-        if (position < a.max_pos) {
+        if (rotated) {
             cos = __ldg(reinterpret_cast<const float4*>(a.cos + static_cast<long long>(position) * (D / 2)) + i);
             sin = __ldg(reinterpret_cast<const float4*>(a.sin + static_cast<long long>(position) * (D / 2)) + i);
         } else if (lane == 0) {
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const A
                     w = scaled(w, inv, __ldg(weight + kLanes));
                 }
             }
-            if (!is_v) {
+            if (!is_v && rotated) {
                 const float4 t = u;
                 u = turned(t, cos, w, minus);
                 w = turned(w, cos, t, sin);

@@ -53,3 +53,35 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
                  lambda: ops.copy_pages(*args[:2], ids, ids + 1)):
         with pytest.raises(ValueError, match="current device, cuda:1"):
             call()
+
+
+# ---- append: values that are not rotated ---------------------------------------------
+@pytest.mark.parametrize("source", ["fp32", "same"])
+@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("past", [False, True])
+def test_unrotated_values_do_not_meet_their_partners(source, normed, past):
+    """Without a rotation (none asked for, or a position past its rows) dim d's
+    value is its own: an infinity or NaN in dim d + D / 2 does not reach it."""
+    batch = Batch([3, 1], [40, 9], heads=4, kv_heads=2, dim=128, page=16, dtype=torch.float16, stale=5.0)
+    qkv = torch.randn(4, 8, 128, device="cuda")
+    qkv[0, 0, 70] = qkv[1, 4, 3] = math.inf
+    qkv[2, 5, 127], qkv[3, 1, 64] = math.nan, -math.inf
+    qkv[3, 7, 10] = math.nan  # a v head
+    qkv = qkv if source == "fp32" else qkv.half()
+    extra, want = {}, qkv.double()
+    if normed:
+        ones = torch.ones(128, device="cuda")
+        extra.update(norm_q=ones, norm_k=ones)
+        want[:, :6] = want[:, :6] / (want[:, :6].pow(2).mean(-1, keepdim=True) + 1e-6).sqrt()
+    if past:
+        extra.update(rope_cos=torch.zeros(8, 64, device="cuda"), rope_sin=torch.ones(8, 64, device="cuda"))
+    q = ops.paged_append(qkv.view(4, -1), batch.k_pages, batch.v_pages, batch.table, batch.offsets, batch.lens, heads=4,
+                         **extra)
+    position, row = torch.tensor([37, 38, 39, 8], device="cuda"), torch.tensor([0, 0, 0, 1], device="cuda")
+    held, slot = batch.table[row, position // 16].long(), position % 16
+    got = torch.cat([q, batch.k_pages[held, :, slot], batch.v_pages[held, :, slot]], 1).double()
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[~finite].nan_to_num(7.0), want[~finite].nan_to_num(7.0))
+    assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -18 * 4)[finite].all()
+    assert _lib.device_status() == (_lib.STATUS_BAD_POSITION if past else 0)
