@@ -1005,8 +1005,11 @@ static bool paged_view(const h4b_paged_kv* kv, PagedView* out) {
     return true;
 }
 
-static bool paged_shape_supported(const h4b_paged_kv* kv) {
-    return (kv->dtype == H4B_FP16 || kv->dtype == H4B_BF16) && (kv->head_dim == 64 || kv->head_dim == 128);
+// The kernels count the values of a page and of a row (of row_heads heads) in 32 bits.
+static bool paged_shape_supported(const h4b_paged_kv* kv, long long row_heads) {
+    return (kv->dtype == H4B_FP16 || kv->dtype == H4B_BF16) && (kv->head_dim == 64 || kv->head_dim == 128) &&
+           static_cast<long long>(kv->kv_heads) * kv->page_size <= INT_MAX / kv->head_dim &&
+           row_heads <= INT_MAX / kv->head_dim;
 }
 
 static int paged_sm_count(int* sms) {
@@ -1105,14 +1108,15 @@ extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv
     using namespace h4b;
     AppendArgs a{};
     if (!paged_view(kv, &a.p) || heads < 0) return H4B_EINVAL;
-    if (!paged_shape_supported(kv) || (qkv_dtype != H4B_FP32 && qkv_dtype != kv->dtype)) return H4B_EUNSUPPORTED;
+    const long long row_heads = heads + 2ll * kv->kv_heads;
+    if (!paged_shape_supported(kv, row_heads) || (qkv_dtype != H4B_FP32 && qkv_dtype != kv->dtype)) return H4B_EUNSUPPORTED;
     if ((norm_q == nullptr) != (norm_k == nullptr) || (rope_cos == nullptr) != (rope_sin == nullptr) ||
         (rope_cos != nullptr && max_pos < 1))
         return H4B_EINVAL;
     if (kv->tokens == 0 || kv->sequences == 0) return 0;
     if (qkv == nullptr || (heads > 0 && q_out == nullptr)) return H4B_EINVAL;
     const auto misaligned = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
-    if (qkv_stride < static_cast<long long>(heads + 2 * kv->kv_heads) * kv->head_dim || (qkv_stride & 3) ||
+    if (qkv_stride < row_heads * kv->head_dim || (qkv_stride & 3) ||
         (heads > 0 && (q_stride < static_cast<long long>(heads) * kv->head_dim || (q_stride & 3))))
         return H4B_EINVAL;
     if (misaligned(qkv, qkv_dtype == H4B_FP32 ? 16 : 8) || misaligned(rope_cos, 16) || misaligned(rope_sin, 16) ||
@@ -1174,7 +1178,7 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     // Both kernels take the maxima before the scale and mask with -infinity.
     const float base2_scale = scale * 1.4426950408889634f;
     if (!(base2_scale > 0.f) || !std::isfinite(base2_scale)) return H4B_EINVAL;
-    if (!paged_shape_supported(kv) || heads / kv->kv_heads > kFewMaxRows ||
+    if (!paged_shape_supported(kv, heads) || heads / kv->kv_heads > kFewMaxRows ||
         static_cast<long long>(kv->pages) * kv->kv_heads > 0x7fffffffll)
         return H4B_EUNSUPPORTED;
     if (kv->tokens == 0 || kv->sequences == 0) return 0;

@@ -455,7 +455,8 @@ int h4b_prefill_tp_stage(const h4b_model *model, const h4b_state *state, const h
  * memory and read on the device: a captured graph follows their contents.
  *
  * page_size is a power of two in 16..1024, head_dim 64 or 128, buffers
- * 16-byte aligned. Page ids of places that no call reads may be anything
+ * 16-byte aligned; a page and a row of qkv, q or out hold fewer than 2^31
+ * values. Page ids of places that no call reads may be anything
  * (-1 for freed pages). A page id that is needed and out of range reads as
  * zeros and is not written, a sequence with an offset or a length out of
  * range counts as empty, and both set status bit 8. */
