@@ -379,6 +379,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         max_query = 1 if tokens <= kv.sequences else tokens
     if workspace is None:
         workspace = paged_workspace(head_dim, q.device)
+    if max(window, sinks, max_query) > 0x7fffffff or min(window, sinks, max_query) < -0x80000000:
+        raise ValueError("window, sinks and max_query must fit 32 bits")
     width = heads * head_dim
     several = tokens > 1
     check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, dtype, "q", device), q.stride(0) if several else width,

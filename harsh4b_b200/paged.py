@@ -274,6 +274,8 @@ class PagedRunner:
             raise ValueError("max_tokens and max_sequences must be positive")
         if window < 0 or sinks < 0 or (sinks and not window):
             raise ValueError("sinks need a window, and neither is negative")
+        if max(window, sinks) > 0x7fffffff:
+            raise ValueError("window and sinks must fit 32 bits")
         layers, _, kv_heads, _, head_dim = cache.k_pages.shape
         if (layers, kv_heads, head_dim) != (model.n_layers, model.kv_heads, model.head_dim):
             raise ValueError("the cache does not have the model's layers and heads")

@@ -85,3 +85,14 @@ def test_unrotated_values_do_not_meet_their_partners(source, normed, past):
     assert torch.equal(got[~finite].nan_to_num(7.0), want[~finite].nan_to_num(7.0))
     assert ((got - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -18 * 4)[finite].all()
     assert _lib.device_status() == (_lib.STATUS_BAD_POSITION if past else 0)
+
+
+# ---- integers past 32 bits --------------------------------------------------------------
+@pytest.mark.parametrize("name", ["window", "sinks", "max_query"])
+@pytest.mark.parametrize("value", [1 << 31, (1 << 32) + 1, (1 << 32) + 16, -(1 << 32) + 1, 1 << 70])
+def test_integers_past_32_bits_are_refused(name, value):
+    batch = Batch([1], [40], heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16)
+    options = {"window": 8, "sinks": 1, "max_query": 1, name: value}
+    batch.window, batch.sinks = options["window"], options["sinks"]
+    with pytest.raises(ValueError, match="32 bits|invalid argument"):
+        batch.call(max_query=options["max_query"])

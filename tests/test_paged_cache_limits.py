@@ -286,3 +286,9 @@ def test_a_runner_follows_its_caches_streams(cache, monkeypatch):  # noqa: F811
     streams.on("B")
     runner.step({cache.new_sequence(): [1]})
     assert streams.log[0] == "B waits"
+
+
+@pytest.mark.parametrize("options", [{"window": (1 << 32) + 8}, {"window": 8, "sinks": 1 << 31}])
+def test_windows_past_32_bits_are_refused(cache, monkeypatch, options):  # noqa: F811
+    with pytest.raises(ValueError, match="32 bits"):
+        cpu_runner(monkeypatch, cache, **options)
