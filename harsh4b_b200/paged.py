@@ -211,6 +211,8 @@ class PagedCache:
 
     def advance(self, sequence: int, count: int) -> None:
         """`count` tokens were appended to the reserved room."""
+        if count < 0:
+            raise ValueError("tokens are taken back with truncate")
         length = self._lengths[sequence] + count
         if length > len(self._tables[sequence]) * self.page_size:
             raise ValueError("more tokens than were reserved")

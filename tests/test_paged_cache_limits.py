@@ -292,3 +292,12 @@ def test_a_runner_follows_its_caches_streams(cache, monkeypatch):  # noqa: F811
 def test_windows_past_32_bits_are_refused(cache, monkeypatch, options):  # noqa: F811
     with pytest.raises(ValueError, match="32 bits"):
         cpu_runner(monkeypatch, cache, **options)
+
+
+def test_advance_goes_forward_only(cache):  # noqa: F811
+    a = cache.new_sequence()
+    grow(cache, a, 20)
+    with pytest.raises(ValueError):
+        cache.advance(a, -1)
+    assert cache.length(a) == 20
+    cache.advance(a, 0)
