@@ -96,3 +96,40 @@ def test_integers_past_32_bits_are_refused(name, value):
     batch.window, batch.sinks = options["window"], options["sinks"]
     with pytest.raises(ValueError, match="32 bits|invalid argument"):
         batch.call(max_query=options["max_query"])
+
+
+# ---- append: long chunks, two warps a token, several passes over the heads --------------
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(32, 8, 128, torch.float16), (24, 8, 64, torch.bfloat16),
+                                                      (40, 1, 128, torch.bfloat16), (3, 1, 128, torch.float16)])
+@pytest.mark.parametrize("source", ["fp32", "same"])
+def test_append_long_chunks(heads, kv_heads, dim, dtype, source):
+    """1024 tokens and more, with norms and rotation. The bound is that of
+    test_gpu_paged.py's append: one rounding of a few fp32 operations."""
+    new, total = [1, 1030, 0, 200, 1], [40, 1100, 7, 200, 1]
+    batch = Batch(new, total, heads=heads, kv_heads=kv_heads, dim=dim, page=32, dtype=dtype, stale=5.0)
+    g = torch.Generator("cuda").manual_seed(5)
+    qkv = torch.empty(batch.rows, (heads + 2 * kv_heads) * dim, device="cuda").normal_(generator=g) * 3
+    qkv = qkv if source == "fp32" else qkv.to(dtype)
+    norm_q, norm_k = (1 + 0.1 * torch.empty(dim, device="cuda").normal_(generator=g) for _ in range(2))
+    angles = torch.rand(1100, dim // 2, generator=g, device="cuda") * 6
+    cos, sin = angles.cos(), angles.sin()
+    q = ops.paged_append(qkv, batch.k_pages, batch.v_pages, batch.table, batch.offsets, batch.lens, heads=heads,
+                         norm_q=norm_q, norm_k=norm_k, eps=1e-5, rope_cos=cos, rope_sin=sin)
+    x = qkv.double().view(batch.rows, heads + 2 * kv_heads, dim)
+    position = torch.cat([torch.arange(t - n, t, device="cuda") for n, t in zip(new, total)])
+    row = torch.repeat_interleave(torch.arange(len(new), device="cuda"), torch.tensor(new, device="cuda"))
+
+    def turned(t, weight):
+        t = t / (t.pow(2).mean(-1, keepdim=True) + 1e-5).sqrt() * weight.double()
+        a, b = t.chunk(2, -1)
+        c, s = cos.double()[position][:, None], sin.double()[position][:, None]
+        return torch.cat((a * c - b * s, b * c + a * s), -1)
+
+    held, slot = batch.table[row, position // 32].long(), position % 32
+    unit = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -8
+    for got, want in ((q, turned(x[:, :heads], norm_q)),
+                      (batch.k_pages[held, :, slot], turned(x[:, heads:heads + kv_heads], norm_k)),
+                      (batch.v_pages[held, :, slot], x[:, heads + kv_heads:])):
+        bound = unit * want.abs() + 2.0 ** -18 * want.abs().amax(-1, keepdim=True) + 2.0 ** -25
+        assert ((got.double() - want).abs() <= bound).all()
+    assert _lib.device_status() == 0
