@@ -28,6 +28,7 @@ struct Pair;  // two 16-bit values of a 32-bit word
 template <>
 struct Pair<__half> {
     static constexpr bool kBf16 = false;
+    static constexpr uint32_t kExponent = 0x7C007C00u, kExponentOne = 0x04000400u;
     __device__ static uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -37,6 +38,7 @@ struct Pair<__half> {
 template <>
 struct Pair<__nv_bfloat16> {
     static constexpr bool kBf16 = true;
+    static constexpr uint32_t kExponent = 0x7F807F80u, kExponentOne = 0x00800080u;
     __device__ static uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -45,6 +47,16 @@ struct Pair<__nv_bfloat16> {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     }
 };
+
+// Nonzero where one of a word's two values is an infinity or a NaN: its
+// exponent, all ones, carries into the value's top bit.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    return ((w & Pair<T>::kExponent) + Pair<T>::kExponentOne) & 0x80008000u;
+}
+
+// All bits of the values that not_finite marks.
+__device__ __forceinline__ uint32_t halves_of(uint32_t marks) { return (marks >> 15) * 0xffffu; }
 
 // The batch as the kernels see it (h4b_paged_kv without its pointers' types).
 struct PagedView {
@@ -544,7 +556,11 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // m + 7 (p < 2^15 fits fp16; the 8 keeps small p clear of fp16's subnormals);
 // l is summed from the fp32 p, which is rounded to 16 bits for the p v
 // products only. Keys that no row sees are zero-filled by the copy, so what
-// such a slot holds cannot reach a sum.
+// such a slot holds cannot reach a sum. Keys that some rows see have weight 0
+// in the others, and 0 times an infinity or NaN would reach those: a piece
+// with such a key is searched for them (only where a tile has several tokens,
+// at their own positions and at the window's edge); those found are added to
+// the rows that see them and taken out of the piece before its product.
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 64;
 constexpr int kFewExtra = 2;  // an item's start and join, in units (1: up to 5 % slower, 3 and 4: within 3 %)
 constexpr int kFewLeast = 1;  // a part is 4 KB beside 32 KB of keys
@@ -806,6 +822,44 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                     l[mt][half] += (p[0] + p[1]) + (p[2] + p[3]);
                     pf[mt][half] = Pair<T>::pack(p[0], p[1]);
                     pf[mt][2 + half] = Pair<T>::pack(p[2], p[3]);
+                }
+            }
+            if (!all && t.tokens > 1) {
+                uint8_t* piece = few_smem + (vbase - smem_addr(few_smem));
+                uint4* v = reinterpret_cast<uint4*>(piece) + lane;
+                uint32_t bad = 0;
+#pragma unroll
+                for (int c = 0; c < C::kPiece / 16; c += 32)
+                    bad |= not_finite<T>(v[c].x) | not_finite<T>(v[c].y) | not_finite<T>(v[c].z) | not_finite<T>(v[c].w);
+                if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll 1
+                    for (int j = 0; j < 16; ++j) {
+#pragma unroll
+                        for (int n = 0; n < kCols; ++n) {
+                            const uint32_t w = *reinterpret_cast<const uint32_t*>(piece + piece_at<D>(j, n) + (lane & 3) * 4);
+                            const uint32_t which = not_finite<T>(w);
+                            if (which == 0) continue;
+                            const float2 x = Pair<T>::unpack(w & halves_of(which));
+#pragma unroll
+                            for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                                for (int half = 0; half < C::kHalves; ++half) {
+                                    const int p = pos[mt][half];
+                                    if (key + j > p || (a.window > 0 && key + j <= p - a.window && key + j >= a.sinks)) continue;
+                                    o[mt][n][half * 2] += x.x;
+                                    o[mt][n][half * 2 + 1] += x.y;
+                                }
+                        }
+                    }
+                    __syncwarp();
+#pragma unroll 1
+                    for (int c = 0; c < C::kPiece / 16; c += 32) {
+                        uint4 x = v[c];
+                        x.x &= ~halves_of(not_finite<T>(x.x)), x.y &= ~halves_of(not_finite<T>(x.y));
+                        x.z &= ~halves_of(not_finite<T>(x.z)), x.w &= ~halves_of(not_finite<T>(x.w));
+                        v[c] = x;
+                    }
+                    __syncwarp();
                 }
             }
 #pragma unroll

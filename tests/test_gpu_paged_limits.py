@@ -133,3 +133,52 @@ def test_append_long_chunks(heads, kv_heads, dim, dtype, source):
         bound = unit * want.abs() + 2.0 ** -18 * want.abs().amax(-1, keepdim=True) + 2.0 ** -25
         assert ((got.double() - want).abs() <= bound).all()
     assert _lib.device_status() == 0
+
+
+# ---- values that are not finite reach the rows that see them, and no others --------------
+SPECIAL = [math.inf, -math.inf, math.nan]
+
+
+def check_reach(new, total, hint, *, heads, kv_heads, dim, page, dtype, window=0, sinks=0, seed=0):
+    """v values that are not finite in every seventh key or so: a row's dims
+    are finite where no key that it sees has one there, and within the bound."""
+    batch = Batch(new, total, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype, window=window, sinks=sinks,
+                  seed=seed)
+    clean, _, bound = batch.expected()
+    g = torch.Generator().manual_seed(seed)
+    reached = torch.zeros(batch.rows, heads, dim, dtype=torch.bool, device="cuda")
+    group, at, wild = heads // kv_heads, 0, 0
+    for b, (n, t) in enumerate(zip(new, total)):
+        p = torch.arange(t - n, t, device="cuda")
+        # mostly where the chunk's rows see different keys: its own tokens, the window's edge; a few elsewhere
+        keys = [j for j in range(max(0, t - n), t, 5)] + [j for j in range(max(0, t - n - window), max(0, t - window), 3)]
+        for j in set(keys) if window else set(keys[:len(keys) // 2]):
+            held = int(batch.table[b, j // page])
+            if held < 0:
+                continue
+            h, d = int(torch.randint(kv_heads, (1,), generator=g)), int(torch.randint(dim, (1,), generator=g))
+            batch.v_pages[held, h, j % page, d] = SPECIAL[wild % 3]
+            wild += 1
+            seen = j <= p
+            if window:
+                seen &= (j > p - window) | (j < sinks)
+            reached[at:at + n, h * group:(h + 1) * group, d] |= seen[:, None]
+        at += n
+    out, lse = batch.call(max_query=hint)
+    assert torch.equal(torch.isfinite(out), ~reached)
+    assert ((out.double() - clean).abs() <= bound)[~reached].all()
+    assert torch.isfinite(lse).all() and wild > 0 and reached.any()
+    assert _lib.device_status() == 0
+
+
+REACH = [dict(heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16),
+         dict(heads=6, kv_heads=2, dim=64, page=64, dtype=torch.bfloat16),
+         dict(heads=5, kv_heads=1, dim=128, page=256, dtype=torch.bfloat16),
+         dict(heads=32, kv_heads=1, dim=64, page=16, dtype=torch.float16)]
+
+
+@pytest.mark.parametrize("shape", REACH)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 5), (3, 0)])
+def test_values_reach_the_rows_that_see_them_few_rows(shape, window, sinks):
+    check_reach([4, 2, 7, 3], [200, 2, 70, 129], 1, window=window, sinks=sinks, seed=1, **shape)
+    check_reach([3], [5000], 1, window=window, sinks=sinks, seed=2, **shape)
