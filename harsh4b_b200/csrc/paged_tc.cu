@@ -44,8 +44,12 @@
 // Keys that no row of the item sees (past its last token, before its window)
 // may lie in slots that hold anything: their scores are selected away, and
 // their V rows are zeroed in shared memory before the product, since 0 * NaN
-// would reach the sum: such a V tile lands on a barrier of its own, warp 11
-// zeroes the rows and then completes the tile's barrier in the loads' place.
+// would reach the sum. For the same reason infinities and NaN are taken out of
+// the V rows that some rows of the item see and others do not (its own tokens,
+// the window's edge); where there are any, the rows that see them get them
+// added at the item's end, from the pages. A V tile with keys of either kind
+// lands on a barrier of its own, warp 11 goes over it and then completes the
+// tile's barrier in the loads' place.
 //
 // Every wait is bounded (mbar_wait). A role whose wait runs out marks the CTA
 // as failed and stops; the load warp waits for the copies it issued, the MMA
@@ -161,10 +165,13 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t y) {
     const float2 v = unpack2(y);
     return pack2(ex2_approx(v.x), ex2_approx(v.y));
 }
-// Whether the block of keys from `key` on has one that no row of the tile sees.
-__device__ __forceinline__ bool has_unseen_keys(const Tile& t, int window, int sinks, int key) {
-    const int end = key + kChunkKeys - 1;
-    return !(end <= t.p1 && (window <= 0 || key > t.p0 - window || end < sinks));
+// Whether every row of the tile sees keys `key` .. `end`.
+__device__ __forceinline__ bool tile_all_see(const Tile& t, int window, int sinks, int key, int end) {
+    return end <= t.p0 && (window <= 0 || key > t.p1 - window || end < sinks);
+}
+// Whether the block of keys from `key` on has one that some row of the tile does not see.
+__device__ __forceinline__ bool has_hidden_keys(const Tile& t, int window, int sinks, int key) {
+    return !tile_all_see(t, window, sinks, key, key + kChunkKeys - 1);
 }
 
 // Bits 0 .. n - 1, of 32.
@@ -193,6 +200,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint64_t* mma_done = o_free + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* wild = failed + 1;  // values that are not finite were taken out of a V tile
     volatile uint32_t* flags = reinterpret_cast<volatile uint32_t*>(smem + C::kFlagOff);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -225,6 +233,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         mbar_init(mma_done, 2);
         *failed = wait_failed_before() ? 1 : 0;
+        *wild = 0;
         fence_mbar_init();
     }
     if (warp == kChunkMmaWarp) {
@@ -290,7 +299,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 const int key = w.tile.block(w.unit) * kChunkKeys;
                 const int y = boxes > 1 ? 0 : key & (page_size - 1);
                 const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
-                const bool unclean = has_unseen_keys(w.tile, a.window, a.sinks, key);
+                const bool unclean = has_hidden_keys(w.tile, a.window, a.sinks, key);
                 uint32_t flag = (tiles == 2 ? kStepTwo : 0u) | (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u);
                 // the next step's page ids are on their way while this step's copies are issued
                 new_item = w.part_ends();
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (issued >= C::kStages)
                         ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&empty[stage], phase(issued - C::kStages)));
                     if (!ok) break;
-                    // a V tile with unseen keys goes through the cleaning warp
+                    // a V tile with hidden keys goes through the cleaning warp
                     uint64_t* bar = v == 1 && unclean ? &raw[stage] : &full[stage];
                     if (lane == 0) {
                         if (v == 0) flags[stage] = flag;
@@ -329,13 +338,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
             __syncwarp();
         } else if (warp == kChunkCleanWarp) {
-            // V rows of keys that no row of the item sees: zeros
+            // V rows of keys that no row of the item sees: zeros; values that are
+            // not finite in rows of keys that only some rows see: out
             Walk<kChunkKeys> w;
             uint32_t n = 0, raw_phase = 0;
             bool more = w.start(a, *shared_range, tile_tokens);
             for (; more; more = w.next(a, tile_tokens), ++n) {
                 const int key = w.tile.block(w.unit) * kChunkKeys;
-                if (!has_unseen_keys(w.tile, a.window, a.sinks, key)) continue;
+                if (!has_hidden_keys(w.tile, a.window, a.sinks, key)) continue;
                 const uint32_t stage = (2 * n + 1) % C::kStages;
                 if (!__all_sync(0xffffffffu, !*failed && mbar_wait(&raw[stage], (raw_phase >> stage) & 1u))) {
                     *failed = 1;
@@ -343,12 +353,55 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
                 raw_phase ^= 1u << stage;
                 uint8_t* tile = ring(2 * n + 1);
-                for (int r = lane; r < kChunkKeys; r += 32)
-                    if (!tile_sees(w.tile, a.window, a.sinks, key + r))
+                // (eight lanes a row's 128 bytes: no two lanes in one bank)
+                auto at = [&](int r, int slab) {
+                    return reinterpret_cast<uint4*>(tile + (r >> 3) * C::kGroup + slab * 1024 + (r & 7) * 128 + (lane & 7) * 16);
+                };
+                // Keys by intervals: no row sees those past the last token, nor those
+                // before the first row's window that are not first tokens; some rows
+                // see the item's own tokens but the first, and those that the window
+                // leaves from row to row.
+                const Tile& t = w.tile;
+                const bool windowed = a.window > 0;
+                auto zero = [&](int from, int to) {
+                    for (int r = max(from - key, 0) + (lane >> 3); r < min(to - key, kChunkKeys); r += 4)
 #pragma unroll
-                        for (int c = 0; c < 2 * D; c += 16)
-                            *reinterpret_cast<uint4*>(tile + (r >> 3) * C::kGroup + (c >> 7) * 1024 + (r & 7) * 128 +
-                                                      (c & 127)) = make_uint4(0u, 0u, 0u, 0u);
+                        for (int slab = 0; slab < C::kSlabs; ++slab) *at(r, slab) = make_uint4(0u, 0u, 0u, 0u);
+                };
+                uint32_t bad = 0;
+                auto search = [&](int from, int to) {
+                    const int end = min(to - key, kChunkKeys);
+#pragma unroll 1
+                    for (int r = max(from - key, 0) + (lane >> 3); r < end; r += 16) {
+                        uint4 v[4 * C::kSlabs];  // four rows' loads in flight (one past the end is its lane's first again)
+#pragma unroll
+                        for (int k = 0; k < 4 * C::kSlabs; ++k)
+                            v[k] = *at(r + 4 * (k / C::kSlabs) < end ? r + 4 * (k / C::kSlabs) : r, k % C::kSlabs);
+#pragma unroll
+                        for (int k = 0; k < 4 * C::kSlabs; ++k)
+                            bad |= not_finite<T>(v[k].x) | not_finite<T>(v[k].y) | not_finite<T>(v[k].z) | not_finite<T>(v[k].w);
+                    }
+                };
+                zero(t.p1 + 1, INT_MAX);
+                search(t.p0 + 1, t.p1 + 1);
+                if (windowed) {
+                    zero(a.sinks, t.p0 - a.window + 1);
+                    search(max(t.p0 - a.window + 1, a.sinks), t.p1 - a.window + 1);
+                }
+                if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll 1
+                    for (int r = lane >> 3; r < kChunkKeys; r += 4) {
+                        if (tile_all_see(w.tile, a.window, a.sinks, key + r, key + r)) continue;
+#pragma unroll
+                        for (int slab = 0; slab < C::kSlabs; ++slab) {
+                            uint4 v = *at(r, slab);
+                            v.x &= ~halves_of(not_finite<T>(v.x)), v.y &= ~halves_of(not_finite<T>(v.y));
+                            v.z &= ~halves_of(not_finite<T>(v.z)), v.w &= ~halves_of(not_finite<T>(v.w));
+                            *at(r, slab) = v;
+                        }
+                    }
+                    *wild = 1;
+                }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[stage]);
@@ -609,12 +662,42 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             float4* part = reinterpret_cast<float4*>(
                 a.partials + (static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * 2 + x) * kPart);
             const float inv = 1.0f / l;
+            // Columns c .. c + 31 of the values that the cleaning warp took out of
+            // the blocks of this part, from the pages, where the row sees their key.
+            auto add_wild = [&](float (&v)[32], int c) {
+                const Range& r = *shared_range;
+                const long long first = r.end - w.left - w.unit;  // place of the item's unit 0
+                for (int u = static_cast<int>(max(r.begin - first, 0ll)); u <= w.unit; ++u) {
+                    const int block = w.tile.block(u) * kChunkKeys;
+                    for (int j = block; j < block + kChunkKeys; ++j) {
+                        if (!tile_sees(w.tile, a.window, a.sinks, j) || tile_all_see(w.tile, a.window, a.sinks, j, j)) continue;
+                        const int page = a.p.table[static_cast<long long>(w.b) * a.p.table_stride + (j >> a.p.page_shift)];
+                        if (page < 0 || page >= a.p.pages) continue;
+                        const long long at = ((static_cast<long long>(page) * a.p.kv_heads + w.h) << a.p.page_shift) +
+                                             (j & ((1 << a.p.page_shift) - 1));
+                        const uint32_t* x = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v_pages) + at * D + c);
+                        const bool sees = valid && j <= pos && (a.window <= 0 || j > pos - a.window || j < a.sinks);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const uint32_t word = __ldg(x + k), which = not_finite<T>(word);
+                            if (which == 0 || !sees) continue;
+                            const float2 y = Pair<T>::unpack(word & halves_of(which));
+                            v[2 * k] += y.x, v[2 * k + 1] += y.y;
+                        }
+                    }
+                }
+            };
+            const bool any_wild = __any_sync(0xffffffffu, *wild != 0);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float v[32];
                 tmem_ld16_nowait(o_col + c, v, 0);
                 tmem_ld16_nowait(o_col + c + 16, v, 16);
                 tmem_wait_regs(v);
+                if (any_wild) {
+                    add_wild(v, c);
+                    __syncwarp();
+                }
                 if (whole) {
                     uint32_t o16[16];
 #pragma unroll

@@ -500,10 +500,8 @@ int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, lon
  * computed as well, only slower. workspace: zeroed when it is created, left
  * ready for the next call; h4b_paged_attention_workspace_bytes bytes (zero it
  * again after a call that set status bit 1). Calls that may overlap on the
- * GPU need workspaces of their own. What lies in a key that no row of a chunk
- * sees reaches no result; a v that is not finite in a key that some rows of a
- * chunk see reaches up to 256 / (heads / kv_heads) tokens before it, too
- * (0 * inf). */
+ * GPU need workspaces of their own. What lies in a key reaches the rows that
+ * see it and no others, whatever its values. */
 int h4b_paged_attention(const h4b_paged_kv *kv, const void *q, long long q_stride, int heads, float scale, int window,
                         int sinks, int max_query, void *out, long long out_stride, float *lse, void *workspace,
                         long long workspace_bytes, void *stream);

@@ -182,3 +182,29 @@ REACH = [dict(heads=8, kv_heads=2, dim=128, page=16, dtype=torch.float16),
 def test_values_reach_the_rows_that_see_them_few_rows(shape, window, sinks):
     check_reach([4, 2, 7, 3], [200, 2, 70, 129], 1, window=window, sinks=sinks, seed=1, **shape)
     check_reach([3], [5000], 1, window=window, sinks=sinks, seed=2, **shape)
+
+
+@pytest.mark.parametrize("shape", REACH)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 5), (300, 130), (3, 0)])
+def test_values_reach_the_rows_that_see_them_long_chunks(shape, window, sinks):
+    check_reach([150, 2, 64, 300], [200, 2, 70, 900], 1000, window=window, sinks=sinks, seed=1, **shape)
+    check_reach([90], [6000], 1000, window=window, sinks=sinks, seed=2, **shape)  # items across CTAs
+
+
+def test_values_reach_the_rows_that_see_them_mixed_step():
+    """Chunks and decoded tokens in one step, each kernel with its share of them."""
+    check_reach([1] * 20 + [200, 90], [50 + i for i in range(20)] + [500, 90], 200, window=60, sinks=3, seed=3, **REACH[0])
+
+
+def test_an_item_after_such_values_is_as_before():
+    """Where one sequence's v values are not finite, the others keep their bits."""
+    batch = Batch([200] * 8, [1000] * 8, heads=32, kv_heads=8, dim=128, page=16, dtype=torch.float16, seed=4)
+    want, want_lse = batch.call()
+    batch.v_pages[int(batch.table[2, 60]), :, 3, ::7] = math.nan  # token 963 of sequence 2: rows from 163 on
+    out, lse = batch.call()
+    same = torch.ones(batch.rows, dtype=torch.bool, device="cuda")
+    same[2 * 200 + 163:3 * 200] = False
+    assert torch.equal(out[same], want[same]) and torch.equal(lse, want_lse)
+    assert torch.isnan(out[~same][..., ::7]).all()
+    rest = torch.arange(128, device="cuda") % 7 != 0
+    assert torch.equal(out[~same][..., rest], want[~same][..., rest])
