@@ -1138,11 +1138,15 @@ static int launch_attention(AttendArgs a, const h4b_paged_kv* kv, int max_query,
     if (rows > kMost) {
         // A step of few long chunks among many short ones (the mean is under
         // half of the longest): the short ones go to the kernel of few rows, in
-        // a launch of its own. Three 255-token chunks and 5, 21 or 61 decoding
-        // sequences, 24 / 8 heads of 64: one launch 42, 66 and 139 us, two
-        // launches 47, 61 and 98.
+        // a launch of its own, where they are many enough to pay for it. Three
+        // 255-token chunks among 16, 20, 24, 32 and 64 sequences of 1000 to 2000
+        // tokens, one launch against two: 24 / 8 heads of 64 61-66, 72-76, 74-74,
+        // 82-78 and 129-98 us; 32 / 8 of 128 70-80, 80-92, 82-92, 92-96 and
+        // 143-137 (40: 107-109). The same with 100 to 8000 tokens and one or
+        // eight chunks, within 8 sequences; of 20 to 200 tokens two launches pay
+        // from about 50 (24: 33-39, 64: 47-43).
         const int few_rows = a.group <= 8 ? 8 : (a.group <= 16 ? 16 : 32);
-        if (few_rows <= kMost && a.p.sequences >= 20 &&
+        if (few_rows <= kMost && a.p.sequences >= (D == 64 ? 20 : 40) &&
             2ll * a.p.tokens < static_cast<long long>(a.p.sequences) * max_query) {
             a.most = few_rows / a.group;
             if (const int rc = launch_few_rows<T, D>(a, few_rows, sms, stream)) return rc;

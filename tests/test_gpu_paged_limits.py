@@ -208,3 +208,13 @@ def test_an_item_after_such_values_is_as_before():
     assert torch.isnan(out[~same][..., ::7]).all()
     rest = torch.arange(128, device="cuda") % 7 != 0
     assert torch.equal(out[~same][..., rest], want[~same][..., rest])
+
+
+# ---- steps of few long chunks among many short sequences: one launch or two -------------
+@pytest.mark.parametrize("sequences", [19, 20, 39, 40, 70])
+@pytest.mark.parametrize("shape", REACH + [dict(heads=32, kv_heads=8, dim=128, page=16, dtype=torch.bfloat16)])
+def test_mixed_steps_on_both_sides_of_the_rule(sequences, shape):
+    new = [1] * 6 + [130] + [2] * 3 + [0, 70] + [1] * (sequences - 12)
+    total = [n + (37 * i) % 400 for i, n in enumerate(new)]
+    Batch(new, total, window=150, sinks=5, seed=13, **shape).check()
+    assert check_reach(new, total, None, window=150, sinks=5, seed=13, **shape) is None
