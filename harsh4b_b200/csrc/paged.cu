@@ -101,8 +101,8 @@ __device__ __forceinline__ SequenceSpan sequence_span(const PagedView& p, int b)
 // lanes: lane i holds dims 4i .. 4i + 3 and their partners D/2 further, so the
 // rotation needs no exchange.
 // Bound by HBM: (heads + 2 kv_heads) D (source + 2) bytes a token (8192 tokens
-// of 48 heads of 128 from fp32: 52 us, 5.9 TB/s); a decode step by its chain of
-// lookups (64 tokens: 3 us).
+// of 48 heads of 128 from fp32: 52 to 55 us, 5.6 to 5.9 TB/s; from fp16 45);
+// a decode step by its chain of lookups (64 tokens: 3 us).
 struct AppendArgs {
     PagedView p;
     const void* qkv;
@@ -539,8 +539,8 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // ---- attention of few rows -----------------------------------------------------
 // For decode and short chunks the keys are read once and each takes part in
 // few products, so HBM is the bound: 4 D kv_heads bytes a key (32 sequences of
-// 32768 tokens, 8 kv heads of 128: 625 us, 6.87 TB/s; 64 ragged ones up to 2100:
-// 61 us, 5.5 TB/s, of which 6 us pass before the first keys arrive). The products
+// 32768 tokens, 8 kv heads of 128: 613 to 636 us, 6.8 to 7.0 TB/s; 64 ragged ones
+// up to 2100: 63 us, 5.3 TB/s, of which 6 pass before the first keys arrive). The products
 // run on mma.sync (m16n8k16): its 16 rows hold the item's rows, and its
 // operands come from shared memory without the tensor-memory allocation, the
 // MMA-issuing thread and the 128-row tiles that tcgen05 asks for.
@@ -555,7 +555,13 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // Softmax in base 2: p = 2^(s - m + 8), m moves only when a score passes
 // m + 7 (p < 2^15 fits fp16; the 8 keeps small p clear of fp16's subnormals);
 // l is summed from the fp32 p, which is rounded to 16 bits for the p v
-// products only. Keys that no row sees are zero-filled by the copy, so what
+// products only: the tensor cores take both operands in the cache's type, and a
+// second product for the rest of p would be a quarter more instructions in a
+// loop whose instruction count shows under the power cap (505 -> 361 a piece:
+// 704 -> 625 us). The rounding is to 2^-12 of a weight (bf16 2^-9), independent
+// from key to key, so its part of a sum is below the result's own rounding: the
+// error against 64 bits is 2.2 to 2.9e-4 in fp16, 2.2 to 2.3e-3 in bf16, with
+// fp32 weights 2.1e-4 and 1.7e-3. Keys that no row sees are zero-filled by the copy, so what
 // such a slot holds cannot reach a sum. Keys that some rows see have weight 0
 // in the others, and 0 times an infinity or NaN would reach those: a piece
 // with such a key is searched for them (only where a tile has several tokens,
@@ -1128,9 +1134,10 @@ static int launch_few_rows(const AttendArgs& a, int rows, int sms, cudaStream_t 
 template <typename T, int D>
 static int launch_attention(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     // Few rows: up to 16 (32 at head_dim 64, where the registers last): 32 x
-    // 32768 tokens of 8 kv heads in 625 us with 4 rows, 632 with 8, 639 with 16,
-    // 1883 with 32 (spilled), the chunk kernel 804 to 863. At head_dim 64 64
-    // ragged sequences with 32 rows: 78 us, the chunk kernel 99.
+    // 32768 tokens of 8 kv heads in 636 us with 4 rows, 638 with 8, 656 with 16,
+    // 1883 with 32 (spilled), the chunk kernel 986 to 1021 (820 to 853 before the
+    // power cap). At head_dim 64 64 ragged sequences of 4 kv heads with 32 rows:
+    // 39 us, the chunk kernel 50.
     constexpr int kMost = D == 64 ? 32 : 16;
     const long long rows = static_cast<long long>(max_query) * a.group;
     a.fewest = 1;

@@ -4,8 +4,12 @@
 // of the prefill (prefill.cu) -- RMSNorm + quantisation, the tensor-core int4
 // GEMMs, SwiGLU in the quantisation of its rows -- with the append and the
 // attention of paged.cu in between; the LM head runs on each sequence's last
-// new row. q, k, v and the attended rows are 16-bit here, so the logits are
-// those of the fp16-cache paths within 16-bit rounding, not their bits.
+// new row. q, k, v and the attended rows are 16-bit here: they are the paged
+// operators' tensors, and halve what they move. The attended rows' int8 codes
+// (a step is max / 127) mostly do not see the difference, so the logits are those
+// of the fp16-cache paths within what the flips of a few codes make of it (2 % of
+// a row's norm in the tests, 5 % at most), not their bits. Where those bits matter
+// the sessions of one contiguous cache have attention="exact".
 
 namespace h4b {
 

@@ -7,10 +7,12 @@
 // rows (128 / group tokens each, row = token * group + q head) that share
 // every K/V tile of 128 keys. While the tensor cores work for one tile the
 // softmax of the other runs. B is left out where A holds all tokens.
-// Measured: an 8192-token prompt, 32 / 8 heads of 128, 500 us (1100 TFLOP/s), 577
-// once the power cap holds the clock at 1.65 GHz; over 8K of history 1195
-// TFLOP/s, and 1604 with the softmax taken out: what bounds it is how well one
-// tile's softmax hides under the other's MMAs.
+// Measured: an 8192-token prompt, 32 / 8 heads of 128, 588 us (935 TFLOP/s) with
+// the clock at the 1.65 GHz that the power cap leaves, 519 in a burst of a dozen;
+// over 8K of history 1670 us (988 TFLOP/s), 1450 in a burst. Of the prompt's
+// cycles the tensor pipe works in 53 %, the exponentials' unit in 54 %, and a
+// first version without the softmax ran at 1604 TFLOP/s: what bounds it is how
+// well one tile's softmax hides under the other's MMAs.
 //
 // Warps: 0-3 and 4-7 are the softmax of A and B (thread = query row, TMEM lane
 // = thread), 8 issues the loads, 9 and 10 the MMAs of A and B, 11 cleans V
@@ -39,7 +41,11 @@
 // group tokens.
 //
 // Softmax in base 2 with a lazily moved reference, as in the kernel of few
-// rows: p = 2^(s - m + 8), m moves when a score passes m + 7.
+// rows: p = 2^(s - m + 8), m moves when a score passes m + 7. P is rounded to
+// the cache's type, which the MMA asks of an operand beside such a V; two halves
+// a weight, as prompts over the other caches have them, would make the P V
+// products twice as many where the tensor pipe is the longer half already. What
+// the rounding does to the result is stated in paged.cu.
 //
 // Keys that no row of the item sees (past its last token, before its window)
 // may lie in slots that hold anything: their scores are selected away, and
@@ -747,8 +753,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 // slice) the item that begins last in CTA c, if it goes on in others, in the
 // order of the CTAs. A launch of its own, on all SMs: one SM that reads an
 // item's parts (64 KB a tile at head_dim 128) took as long as the products (64
-// tokens over 16000: 60 us with the join in the CTA that ends last, 47 so; an
-// 8192-token prompt 506 and 501).
+// tokens over 16000: 60 us with the join in the CTA that ends last, 47 to 50
+// so; an 8192-token prompt within 1 %).
 constexpr int kJoinRows = 16, kJoinThreads = 128;
 
 template <typename T, int D>

@@ -501,7 +501,10 @@ int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, lon
  * ready for the next call; h4b_paged_attention_workspace_bytes bytes (zero it
  * again after a call that set status bit 1). Calls that may overlap on the
  * GPU need workspaces of their own. What lies in a key reaches the rows that
- * see it and no others, whatever its values. */
+ * see it and no others, whatever its values. Arithmetic: q, the pages, the
+ * weights of the v products and out have the cache's 16 bits; scores, maxima,
+ * sums and accumulators are fp32 (a score past 2^23 has no fraction left there,
+ * and past 2^24 its weight may be infinite). */
 int h4b_paged_attention(const h4b_paged_kv *kv, const void *q, long long q_stride, int heads, float scale, int window,
                         int sinks, int max_query, void *out, long long out_stride, float *lse, void *workspace,
                         long long workspace_bytes, void *stream);
