@@ -552,8 +552,10 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // own copies only, and the ring runs on over the item boundaries. Each warp
 // keeps its own (o, m, l); at an item's end (or the range's) the warps join
 // theirs through shared memory.
-// Softmax in base 2: p = 2^(s - m + 8), m moves only when a score passes
-// m + 7 (p < 2^15 fits fp16; the 8 keeps small p clear of fp16's subnormals);
+// Softmax in base 2: p = 2^(s - m) with m 8 below a score that was the largest
+// (so that small p keep clear of fp16's subnormals); m moves only when a score
+// passes it by 15 (2^15 fits fp16). Where a score's unit is more than 1, m is
+// the score itself: 8 less might round to more than 15 less.
 // l is summed from the fp32 p, which is rounded to 16 bits for the p v
 // products only: the tensor cores take both operands in the cache's type, and a
 // second product for the rest of p would be a quarter more instructions in a
@@ -570,7 +572,8 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps, kFewKeys = 64;
 constexpr int kFewExtra = 2;  // an item's start and join, in units (1: up to 5 % slower, 3 and 4: within 3 %)
 constexpr int kFewLeast = 1;  // a part is 4 KB beside 32 KB of keys
-constexpr float kFewOffset = 8.f, kFewSlack = 7.f;
+constexpr float kMostExponent = 15.f;
+__device__ __forceinline__ float softmax_reference(float top) { return fabsf(top) < 16777216.f ? top - 8.f : top; }
 
 template <int D, int ROWS>
 struct FewCfg {
@@ -781,23 +784,30 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                                     s[mt][n][half * 2 + e] = -INFINITY;
                             }
             }
-            // (the scale is positive: maxima can be taken before it)
+            // (scaled on their own: s - m is then exact near m, whatever their size)
+#pragma unroll
+            for (int mt = 0; mt < C::kTiles; ++mt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2 * C::kHalves; ++e) s[mt][n][e] = __fmul_rn(s[mt][n][e], a.scale);
             bool grow = false;
 #pragma unroll
             for (int mt = 0; mt < C::kTiles; ++mt)
 #pragma unroll
                 for (int half = 0; half < C::kHalves; ++half)
-                    grow |= a.scale * fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
-                                            fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1])) > m[mt][half] + kFewSlack;
+                    grow |= fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
+                                  fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1])) - m[mt][half] > kMostExponent;
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int mt = 0; mt < C::kTiles; ++mt)
 #pragma unroll
                     for (int half = 0; half < C::kHalves; ++half) {
-                        float top = a.scale * fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
-                                                    fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1]));
+                        float top = fmaxf(fmaxf(s[mt][0][half * 2], s[mt][0][half * 2 + 1]),
+                                          fmaxf(s[mt][1][half * 2], s[mt][1][half * 2 + 1]));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        top = softmax_reference(top);
                         if (top > m[mt][half]) {
                             const float f = ex2_approx(m[mt][half] - top);  // 0 for the first keys
                             m[mt][half] = top;
@@ -819,12 +829,12 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                         pf[mt][half] = pf[mt][2 + half] = 0u;
                         continue;
                     }
-                    const float base = m[mt][half] == -INFINITY ? 0.f : kFewOffset - m[mt][half];
+                    const float base = m[mt][half] == -INFINITY ? 0.f : m[mt][half];
                     float p[4];
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) p[n * 2 + e] = ex2_approx(__fmaf_rn(s[mt][n][half * 2 + e], a.scale, base));
+                        for (int e = 0; e < 2; ++e) p[n * 2 + e] = ex2_approx(__fsub_rn(s[mt][n][half * 2 + e], base));
                     l[mt][half] += (p[0] + p[1]) + (p[2] + p[3]);
                     pf[mt][half] = Pair<T>::pack(p[0], p[1]);
                     pf[mt][2 + half] = Pair<T>::pack(p[2], p[3]);
@@ -975,7 +985,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                             a.lse[static_cast<long long>(now.tile.first + i) * a.heads + head] =
                                 l[mt][half] == 0.f
                                     ? -INFINITY
-                                    : (m[mt][half] - kFewOffset) * 0.6931471805599453f + logf(l[mt][half]);
+                                    : m[mt][half] * 0.6931471805599453f + logf(l[mt][half]);
                     } else {
                         if ((lane & 3) == 0) {
                             __stcg(part + ROWS * D + 2 * r, m[mt][half]);
@@ -1028,7 +1038,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                         make_uint2(Pair<T>::pack(v.x * inv, v.y * inv), Pair<T>::pack(v.z * inv, v.w * inv));
                     if (a.lse != nullptr && c == 0)
                         a.lse[static_cast<long long>(now.tile.first + i) * a.heads + head] =
-                            sum == 0.f ? -INFINITY : (top - kFewOffset) * 0.6931471805599453f + logf(sum);
+                            sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
                 }
             }
             __syncthreads();

@@ -41,7 +41,9 @@
 // group tokens.
 //
 // Softmax in base 2 with a lazily moved reference, as in the kernel of few
-// rows: p = 2^(s - m + 8), m moves when a score passes m + 7. P is rounded to
+// rows: p = 2^(s - m). The scale is applied in one step with the subtraction;
+// scores of 2^20 and more, where the rounding of m against that exact product
+// would reach the exponent, take a slower way, scaled before it. P is rounded to
 // the cache's type, which the MMA asks of an operand beside such a V; two halves
 // a weight, as prompts over the other caches have them, would make the P V
 // products twice as many where the tensor pipe is the longer half already. What
@@ -180,15 +182,111 @@ __device__ __forceinline__ bool has_hidden_keys(const Tile& t, int window, int s
     return !tile_all_see(t, window, sinks, key, key + kChunkKeys - 1);
 }
 
+// Whether scores near this one need their product with the scale rounded on its own.
+__device__ __forceinline__ bool is_huge(float score) { return fabsf(score) >= 1048576.f; }
+
 // Bits 0 .. n - 1, of 32.
 __device__ __forceinline__ uint32_t bits_below(int n) {
     return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
 }
 
+// A row's O times f. (P V of every earlier block has completed: see above.)
+template <int D>
+__device__ __forceinline__ void rescale_row(uint32_t o_col, float f) {
+#pragma unroll 1
+    for (int c = 0; c < D; c += 16) {  // rare: few registers beside the scores
+        float v[16];
+        tmem_ld16_nowait(o_col + c, v, 0);
+        tmem_wait_regs(v);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] *= f;
+        tmem_st16(o_col + c, v, 0);
+    }
+}
+
+// The softmax of a tile's row from a block on whose scores are huge for some row
+// of the warp, to the end of the part: scaled before the subtraction, 32 at a
+// time, the maximum first and then p. A call of its own, which leaves the usual
+// way its registers. The first block's scores have come and its turn is taken.
+struct HugeRow {
+    Walk<kChunkKeys> w;
+    float m, l;
+    uint32_t s_count, turns;
+    int pos;                  // -1: no row
+    uint32_t s_col, o_col;
+    bool ok;
+};
+template <typename T, int D>
+__device__ __noinline__ void huge_scores(const AttendArgs& a, HugeRow& row, int half_tokens, uint64_t* s_full,
+                                         uint64_t* p_half, uint64_t* p_full, uint64_t* my_turn, uint64_t* other_turn) {
+    HugeRow r = row;
+    const int lane = threadIdx.x & 31;
+    const bool two = r.w.tile.tokens > half_tokens;
+    const bool second = threadIdx.x >= 128;  // tile B, whose turns start one later
+    while (true) {
+        const int key = r.w.tile.block(r.w.unit) * kChunkKeys;
+        auto scaled = [&](float (&v)[32], int c) {
+            tmem_ld16_nowait(r.s_col + c, v, 0);
+            tmem_ld16_nowait(r.s_col + c + 16, v, 16);
+            tmem_wait_regs(v);
+            uint32_t seen = bits_below(r.pos - key - c + 1);
+            if (a.window > 0) seen &= ~bits_below(r.pos - a.window - key - c + 1) | bits_below(a.sinks - key - c);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] = (seen >> k) & 1u ? __fmul_rn(v[k], a.scale) : -INFINITY;
+        };
+        float v[32], mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < kChunkKeys; c += 32) {
+            scaled(v, c);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
+        }
+        const bool move = mx - r.m > kMostExponent;
+        if (__any_sync(0xffffffffu, move && r.m != -INFINITY)) {
+            const float f = move ? ex2_approx(r.m - softmax_reference(mx)) : 1.f;
+            r.l *= f;
+            rescale_row<D>(r.o_col, f);
+        }
+        if (move) r.m = softmax_reference(mx);
+        const float base = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll 1
+        for (int c = 0; c < kChunkKeys; c += 32) {
+            scaled(v, c);
+            uint32_t p16[16];
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+                const float p0 = ex2_approx(__fsub_rn(v[k], base)), p1 = ex2_approx(__fsub_rn(v[k + 1], base));
+                r.l += p0 + p1;
+                p16[k / 2] = Pair<T>::pack(p0, p1);
+            }
+            tmem_st16u(r.s_col + c / 2, p16, 0);  // (over scores that are read already)
+            if (c == kChunkKeys / 2 - 32 || c == kChunkKeys - 32) {
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(c < kChunkKeys / 2 ? p_half : p_full);
+            }
+        }
+        if (lane == 0 && two) mbar_arrive(other_turn);
+        if (r.w.part_ends()) break;
+        r.w.next(a, 2 * half_tokens);
+        r.ok = warp_wait(s_full, r.s_count & 1);
+        if (!r.ok) break;
+        ++r.s_count;
+        tc_fence_after();
+        if (two) {
+            r.ok = warp_wait(my_turn, (r.turns - 1 + (second ? 1 : 0)) & 1);
+            if (!r.ok) break;
+            ++r.turns;
+        }
+    }
+    row = r;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     paged_attention_chunk_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                                 const __grid_constant__ CUtensorMap vmap, const AttendArgs a) {
+                                 const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttendArgs a) {
     using C = ChunkCfg<D>;
     extern __shared__ uint8_t chunk_smem_raw[];
     uint8_t* smem = chunk_smem_raw + ((1024u - (smem_addr(chunk_smem_raw) & 1023u)) & 1023u);
@@ -575,7 +673,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
                 uint64_t sum[2] = {0ull, 0ull};
                 auto weights = [&](const float (&v)[kHalf], int column) {  // p of 64 keys, to the P columns
-                    const float base = m == -INFINITY ? 0.f : kFewOffset - m;
+                    const float base = m == -INFINITY ? 0.f : -m;
                     const uint64_t scale2 = pack2(a.scale, a.scale), base2 = pack2(base, base);
 #pragma unroll
                     for (int c = 0; c < kHalf; c += 32) {
@@ -603,30 +701,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 };
                 // The first half's p with the m of the blocks before, while the
                 // second half's scores arrive and the maximum is found beside
-                // it. Where that passes m + slack (always at a row's first
+                // it. Where that passes m too far (always at a row's first
                 // keys) m moves and they are formed anew.
                 weights(s1, 0);
                 const float mx1 = largest(s1);
                 tmem_wait_regs(s2);
                 if (masked) mask(s2, key + kHalf);
                 const float mx = a.scale * fmaxf(mx1, largest(s2));
-                const bool move = valid && mx > m + kFewSlack;
+                const bool move = valid && mx - m > kMostExponent;
                 if (__any_sync(0xffffffffu, move)) {
-                    if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
-                        // P V of every earlier block has completed (see above)
-                        const float f = move ? ex2_approx(m - mx) : 1.f;  // 0 for m = -inf, whose l and O are 0
-                        l *= f;
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {  // rare: few registers beside the scores
-                            float v[16];
-                            tmem_ld16_nowait(o_col + c, v, 0);
-                            tmem_wait_regs(v);
+                    if (__any_sync(0xffffffffu, move && is_huge(mx))) {
+                        // this block, with its scores put back, and the others go another way
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) v[k] *= f;
-                            tmem_st16(o_col + c, v, 0);
-                        }
+                        for (int c = 0; c < kHalf; c += 16) tmem_st16(s_col + c, s1, c);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        HugeRow row{w, m, l, s_count, turns, pos, s_col, o_col, true};
+                        huge_scores<T, D>(a, row, half_tokens, s_full + x, p_half + x, p_full + x, turn + 4 * x + (warp & 3),
+                                          turn + 4 * (x ^ 1) + (warp & 3));
+                        w = row.w, m = row.m, l = row.l, s_count = row.s_count, turns = row.turns, ok = row.ok;
+                        done = w.item_ends();
+                        break;
                     }
-                    if (move) m = mx;
+                    if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
+                        const float f = move ? ex2_approx(m - softmax_reference(mx)) : 1.f;  // 0 for m = -inf, whose l and O are 0
+                        l *= f;
+                        rescale_row<D>(o_col, f);
+                    }
+                    if (move) m = softmax_reference(mx);
                     sum[0] = sum[1] = 0ull;
                     weights(s1, 0);
                 }
@@ -727,7 +829,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (whole) {
                 if (valid && a.lse != nullptr)
                     a.lse[out_row * a.heads + out_head] =
-                        l == 0.f ? -INFINITY : (m - kFewOffset) * 0.6931471805599453f + logf(l);
+                        l == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(l);
             } else {
                 if (valid)
                     __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
@@ -803,7 +905,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendAr
                        Pair<T>::pack(v[k + 1].z * scale, v[k + 1].w * scale));
     if (a.lse != nullptr && c == 0)
         a.lse[out_row * a.heads + out_head] =
-            total == 0.f ? -INFINITY : (most - kFewOffset) * 0.6931471805599453f + logf(total);
+            total == 0.f ? -INFINITY : most * 0.6931471805599453f + logf(total);
 }
 
 // A layer's pages [pages * kv_heads][page_size][D] as a 5-D tensor map (value,

@@ -503,8 +503,7 @@ int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, lon
  * GPU need workspaces of their own. What lies in a key reaches the rows that
  * see it and no others, whatever its values. Arithmetic: q, the pages, the
  * weights of the v products and out have the cache's 16 bits; scores, maxima,
- * sums and accumulators are fp32 (a score past 2^23 has no fraction left there,
- * and past 2^24 its weight may be infinite). */
+ * sums and accumulators are fp32. */
 int h4b_paged_attention(const h4b_paged_kv *kv, const void *q, long long q_stride, int heads, float scale, int window,
                         int sinks, int max_query, void *out, long long out_stride, float *lse, void *workspace,
                         long long workspace_bytes, void *stream);

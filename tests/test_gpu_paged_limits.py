@@ -218,3 +218,38 @@ def test_mixed_steps_on_both_sides_of_the_rule(sequences, shape):
     total = [n + (37 * i) % 400 for i, n in enumerate(new)]
     Batch(new, total, window=150, sinks=5, seed=13, **shape).check()
     assert check_reach(new, total, None, window=150, sinks=5, seed=13, **shape) is None
+
+
+# ---- scores far past fp32's fractions ----------------------------------------------------
+@pytest.mark.parametrize("hint", [1, 1000])
+@pytest.mark.parametrize("dim,dtype,power", [(128, torch.float16, 8), (128, torch.float16, 12), (64, torch.float16, 13),
+                                             (128, torch.float16, 14), (64, torch.float16, 15), (128, torch.bfloat16, 12),
+                                             (128, torch.bfloat16, 16), (64, torch.bfloat16, 20), (128, torch.bfloat16, 60)])
+@pytest.mark.parametrize("below", [False, True])
+def test_huge_scores(hint, dim, dtype, power, below):
+    """q and k of one dim each, of few bits: their products are exact in fp32
+    and equal scores stay equal, so the weights are known whatever their size."""
+    new, total = [1, 3, 60, 130], [700, 65, 500, 130]
+    batch = Batch(new, total, heads=8, kv_heads=2, dim=dim, page=16, dtype=dtype, seed=31)
+    batch.q.zero_()
+    batch.q[:, :, 5] = 1.375 * 2.0 ** power
+    g = torch.Generator().manual_seed(power)
+    for b, t in enumerate(total):
+        k = torch.zeros_like(batch.k[b])
+        # rising by factors of two along the sequence, each with many equal and some opposite ones
+        size = torch.arange(t, device="cuda").float().mul(4.0 / t).floor() - 3
+        sign = torch.randint(-1, 2, (t,), generator=g).float().cuda()
+        sign[0] = 1
+        if below:  # none but hugely negative ones
+            sign = -torch.ones_like(sign)
+        k[:, :, 5] = (sign * 1.625 * torch.exp2(size + power))[:, None].to(dtype)
+        batch.k[b] = k
+        for j in range(t):
+            batch.k_pages[int(batch.table[b, j // 16]), :, j % 16] = k[j]
+    out, lse = batch.call(max_query=hint)
+    want, want_lse, bound = batch.expected()
+    assert torch.isfinite(out).all()
+    assert ((out.double() - want).abs() <= bound).all()
+    # a score's own rounding, and the product with the scale's
+    assert ((lse.double() - want_lse).abs() <= 2e-4 + 2.0 ** -22 * want_lse.abs()).all()
+    assert _lib.device_status() == 0
