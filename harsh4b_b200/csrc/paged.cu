@@ -539,8 +539,8 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // ---- attention of few rows -----------------------------------------------------
 // For decode and short chunks the keys are read once and each takes part in
 // few products, so HBM is the bound: 4 D kv_heads bytes a key (32 sequences of
-// 32768 tokens, 8 kv heads of 128: 613 to 636 us, 6.8 to 7.0 TB/s; 64 ragged ones
-// up to 2100: 63 us, 5.3 TB/s, of which 6 pass before the first keys arrive). The products
+// 32768 tokens, 8 kv heads of 128: 615 to 636 us, 6.8 to 7.0 TB/s; 64 ragged ones
+// up to 2100: 64 us, 5.3 TB/s, of which 6 pass before the first keys arrive). The products
 // run on mma.sync (m16n8k16): its 16 rows hold the item's rows, and its
 // operands come from shared memory without the tensor-memory allocation, the
 // MMA-issuing thread and the 128-row tiles that tcgen05 asks for.
@@ -1144,8 +1144,8 @@ static int launch_few_rows(const AttendArgs& a, int rows, int sms, cudaStream_t 
 template <typename T, int D>
 static int launch_attention(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     // Few rows: up to 16 (32 at head_dim 64, where the registers last): 32 x
-    // 32768 tokens of 8 kv heads in 636 us with 4 rows, 638 with 8, 656 with 16,
-    // 1883 with 32 (spilled), the chunk kernel 986 to 1021 (820 to 853 before the
+    // 32768 tokens of 8 kv heads in 615 us with 4 rows, 615 with 8, 623 with 16,
+    // 1883 with 32 (spilled), the chunk kernel 926 to 958 (816 to 824 before the
     // power cap). At head_dim 64 64 ragged sequences of 4 kv heads with 32 rows:
     // 39 us, the chunk kernel 50.
     constexpr int kMost = D == 64 ? 32 : 16;

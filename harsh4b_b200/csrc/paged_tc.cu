@@ -7,10 +7,10 @@
 // rows (128 / group tokens each, row = token * group + q head) that share
 // every K/V tile of 128 keys. While the tensor cores work for one tile the
 // softmax of the other runs. B is left out where A holds all tokens.
-// Measured: an 8192-token prompt, 32 / 8 heads of 128, 588 us (935 TFLOP/s) with
-// the clock at the 1.65 GHz that the power cap leaves, 519 in a burst of a dozen;
-// over 8K of history 1670 us (988 TFLOP/s), 1450 in a burst. Of the prompt's
-// cycles the tensor pipe works in 53 %, the exponentials' unit in 54 %, and a
+// Measured: an 8192-token prompt, 32 / 8 heads of 128, 588 to 602 us (913 to 935
+// TFLOP/s) with the clock at the 1.65 GHz that the power cap leaves, 537 in a
+// burst of a dozen; over 8K of history 1664 us (991 TFLOP/s), 1449 in a burst. Of
+// the prompt's cycles the tensor pipe works in 52 %, the exponentials' unit in 53 %, and a
 // first version without the softmax ran at 1604 TFLOP/s: what bounds it is how
 // well one tile's softmax hides under the other's MMAs.
 //
@@ -43,7 +43,9 @@
 // Softmax in base 2 with a lazily moved reference, as in the kernel of few
 // rows: p = 2^(s - m). The scale is applied in one step with the subtraction;
 // scores of 2^20 and more, where the rounding of m against that exact product
-// would reach the exponent, take a slower way, scaled before it. P is rounded to
+// would reach the exponent, take a slower way, scaled before it (a call, so that
+// the usual way keeps its registers: the prompt 592 -> 602 us; with that code in
+// the loop 612 to 688). P is rounded to
 // the cache's type, which the MMA asks of an operand beside such a V; two halves
 // a weight, as prompts over the other caches have them, would make the P V
 // products twice as many where the tensor pipe is the longer half already. What

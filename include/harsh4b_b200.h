@@ -495,7 +495,8 @@ int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, lon
  * window > 0 only j > p - window or j < sinks. lse (may be null): float
  * [tokens][heads], the natural logarithm of each row's sum of exp(scale q.k);
  * scale is positive, and scale * log2(e) a finite fp32 above zero.
- * A row that sees no key gets zeros and lse -inf. max_query is the longest
+ * A row that sees no key gets zeros and lse -inf; rows that q_offsets gives to
+ * no sequence are not written. max_query is the longest
  * chunk that the caller expects: it picks the kernel, and a longer chunk is
  * computed as well, only slower. workspace: zeroed when it is created, left
  * ready for the next call; h4b_paged_attention_workspace_bytes bytes (zero it
