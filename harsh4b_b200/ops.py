@@ -238,16 +238,18 @@ _PAGED_DTYPES = {torch.float16: 1, torch.bfloat16: 2}  # H4B_FP16, H4B_BF16
 
 def _on(tensor: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> int:
     """Data pointer of a contiguous tensor on CUDA device `device`."""
-    if isinstance(tensor, torch.Tensor) and tensor.get_device() == device >= 0 and tensor.dtype == dtype \
-            and tensor.is_contiguous():
-        return tensor.data_ptr()
+    try:
+        if tensor.get_device() == device and tensor.dtype is dtype and tensor.is_contiguous() and device >= 0:
+            return tensor.data_ptr()
+    except AttributeError:  # not a tensor
+        pass
     _dev(tensor, dtype, name)
     raise ValueError(f"{name} must be on the device of the other tensors, cuda:{device}, got {tensor.device}")
 
 
 def _rows(tensor: torch.Tensor, dtype: torch.dtype, name: str, device: int) -> int:
     """Data pointer of a tensor on CUDA device `device` whose rows (dim 0) may be strided."""
-    if isinstance(tensor, torch.Tensor) and tensor.get_device() == device >= 0 and tensor.dtype == dtype \
+    if isinstance(tensor, torch.Tensor) and tensor.get_device() == device >= 0 and tensor.dtype is dtype \
             and (tensor.is_contiguous() or tensor[:1].squeeze(0).is_contiguous()):
         return tensor.data_ptr()
     _on(tensor[:1].squeeze(0) if isinstance(tensor, torch.Tensor) else tensor, dtype, name, device)
