@@ -539,7 +539,7 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // ---- attention of few rows -----------------------------------------------------
 // For decode and short chunks the keys are read once and each takes part in
 // few products, so HBM is the bound: 4 D kv_heads bytes a key (32 sequences of
-// 32768 tokens, 8 kv heads of 128: 615 to 636 us, 6.8 to 7.0 TB/s; 64 ragged ones
+// 32768 tokens, 8 kv heads of 128: 615 to 646 us, 6.6 to 7.0 TB/s; 64 ragged ones
 // up to 2100: 64 us, 5.3 TB/s, of which 6 pass before the first keys arrive). The products
 // run on mma.sync (m16n8k16): its 16 rows hold the item's rows, and its
 // operands come from shared memory without the tensor-memory allocation, the
@@ -558,9 +558,9 @@ __device__ __forceinline__ bool tile_sees(const Tile& t, int window, int sinks, 
 // the score itself: 8 less might round to more than 15 less.
 // l is summed from the fp32 p, which is rounded to 16 bits for the p v
 // products only: the tensor cores take both operands in the cache's type, and a
-// second product for the rest of p would be a quarter more instructions in a
-// loop whose instruction count shows under the power cap (505 -> 361 a piece:
-// 704 -> 625 us). The rounding is to 2^-12 of a weight (bf16 2^-9), independent
+// second product for the rest of p costs 3 to 4 % (646 -> 674 us for the 32 x
+// 32768 tokens, 64.6 -> 66.3 for the 64 ragged ones: the instruction count shows
+// under the power cap). The rounding is to 2^-12 of a weight (bf16 2^-9), independent
 // from key to key, so its part of a sum is below the result's own rounding: the
 // error against 64 bits is 2.2 to 2.9e-4 in fp16, 2.2 to 2.3e-3 in bf16, with
 // fp32 weights 2.1e-4 and 1.7e-3. Keys that no row sees are zero-filled by the copy, so what
