@@ -20,6 +20,8 @@ STATUS_BAD_TOKEN = 2
 STATUS_BAD_POSITION = 4
 STATUS_BAD_PAGE = 8
 
+TREE_NODES = 256  # H4B_TREE_NODES
+
 _vp, _i32, _f32, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
 
@@ -146,6 +148,14 @@ _SIGNATURES = {
                             _i64, _vp],
     "h4b_paged_attention_workspace_bytes": [_i32],
     "h4b_forward_paged": [ctypes.POINTER(ModelDesc), ctypes.POINTER(PagedStepDesc), _vp],
+    "h4b_paged_append_tree": [ctypes.POINTER(PagedKvDesc), _vp, _vp, _i32, _i64, _i32, _vp, _vp, _f32, _vp, _vp, _i32, _vp,
+                              _i64, _vp],
+    "h4b_paged_tree_attention": [ctypes.POINTER(PagedKvDesc), _vp, _vp, _i64, _i32, _f32, _i32, _i32, _i32, _vp, _i64, _vp,
+                                 _vp, _i64, _vp],
+    "h4b_tree_accept": [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
+    "h4b_tree_accept_workspace_bytes": [_i32, _i32],
+    "h4b_tree_keep": [ctypes.POINTER(PagedKvDesc), _i32, _i64, _vp, _i32, _vp, _vp, _vp],
+    "h4b_rmsnorm_quantize_rows": [_vp, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _f32, _vp, _vp, _vp, _i32, _i32, _vp],
     "h4b_pages_copy": [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i32, _vp],
     "h4b_lattice_scratch_bytes": [_i32],
     "h4b_lattice_to_int4": [ctypes.POINTER(LatticeProjectionDesc), _vp, _vp, _vp, ctypes.POINTER(_i32), _vp],
@@ -153,7 +163,7 @@ _SIGNATURES = {
 }
 _RESTYPES = {"h4b_persistent_exchange_words": ctypes.c_longlong, "h4b_sample_scratch_bytes": ctypes.c_longlong,
              "h4b_tp_buffer_bytes": ctypes.c_longlong, "h4b_lattice_scratch_bytes": ctypes.c_longlong,
-             "h4b_paged_attention_workspace_bytes": ctypes.c_longlong}
+             "h4b_paged_attention_workspace_bytes": ctypes.c_longlong, "h4b_tree_accept_workspace_bytes": ctypes.c_longlong}
 
 
 def exported_symbols() -> list[str]:

@@ -78,9 +78,14 @@ constexpr int kMaxLength = 1 << 30;  // keeps position - window in 32 bits
 struct SequenceSpan {
     int first, count, base;  // first row, new tokens, position of the first one
 };
+// Nodes of a drafted tree, at most (a row's ancestors are kept as bits). A
+// sequence with more, or with more than its length, counts as out of range.
+constexpr int kTreeNodes = H4B_TREE_NODES, kTreeWords = kTreeNodes / 32;
+template <bool TREE = false>
 __device__ __forceinline__ SequenceSpan checked_span(const PagedView& p, const RawSpan& r) {
-    const bool good = r.first >= 0 && r.end >= r.first && r.end <= p.tokens && r.len >= 0 &&
-                      r.len <= kMaxLength && r.len <= static_cast<long long>(p.table_stride) << p.page_shift;
+    bool good = r.first >= 0 && r.end >= r.first && r.end <= p.tokens && r.len >= 0 &&
+                r.len <= kMaxLength && r.len <= static_cast<long long>(p.table_stride) << p.page_shift;
+    if constexpr (TREE) good = good && r.end - r.first <= min(kTreeNodes, r.len);
     if (!good) {
         report(kStatusBadPage);
         // its rows, as far as they exist, still get an (empty) answer
@@ -89,8 +94,33 @@ __device__ __forceinline__ SequenceSpan checked_span(const PagedView& p, const R
     }
     return SequenceSpan{r.first, r.end - r.first, r.len - (r.end - r.first)};
 }
+template <bool TREE = false>
 __device__ __forceinline__ SequenceSpan sequence_span(const PagedView& p, int b) {
-    return checked_span(p, raw_span(p, b));
+    return checked_span<TREE>(p, raw_span(p, b));
+}
+
+// A drafted tree: parents[first + i] is node i's parent within its sequence,
+// -1 where the node follows the tokens before the tree, and less than i. One
+// that is not counts as -1 and sets status bit 8, so every walk ends.
+__device__ __forceinline__ int checked_parent(int parent, int node) {
+    if (parent >= -1 && parent < node) return parent;
+    report(kStatusBadPage);
+    return -1;
+}
+// Parent by parent up to the root: node `i`'s depth, and in `sight` (kTreeWords
+// words, may be null) the nodes that it sees, itself among them: with a window
+// those less than `window` above it, or at positions below `sinks`.
+__device__ __forceinline__ int walk_tree(const int32_t* parents, int i, int base, int window, int sinks, uint32_t* sight) {
+    int depth = 0;
+    for (int j = checked_parent(parents[i], i); j >= 0; j = checked_parent(parents[j], j)) ++depth;
+    if (sight != nullptr) {
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w) sight[w] = 0u;
+        int up = 0;
+        for (int j = i; j >= 0; j = checked_parent(parents[j], j), ++up)
+            if (window <= 0 || up < window || base + depth - up < sinks) sight[j >> 5] |= 1u << (j & 31);
+    }
+    return depth;
 }
 
 // ---- append ---------------------------------------------------------------
@@ -113,6 +143,7 @@ struct AppendArgs {
     float eps;
     void *q_out, *k_pages, *v_pages;
     long long q_stride;
+    const int32_t* parents;  // of a tree's nodes, or null
 };
 
 // Warps that share a token of a long chunk, and turns a warp has in flight
@@ -142,7 +173,7 @@ __device__ __forceinline__ float4 turned(const float4& a, const float4& c, const
     return make_float4(a.x * c.x + b.x * s.x, a.y * c.y + b.y * s.y, a.z * c.z + b.z * s.z, a.w * c.w + b.w * s.w);
 }
 
-template <typename S, typename T, int D>
+template <typename S, typename T, int D, bool TREE>
 __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const AppendArgs a) {
     using Raw = typename RawQuad<S>::type;
     constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes;  // heads a warp holds in its lanes
@@ -177,10 +208,13 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const A
         b += __popc(__ballot_sync(0xffffffffu, before));
     }
     T *k_row = nullptr, *v_row = nullptr;  // of the token, kv head 0
-    int position = -1;
+    int position = -1;  // its place in the cache, and below its position
+    int depth = -1;     // of a tree's node, less its index
     if (b >= 0) {
-        const SequenceSpan s = sequence_span(a.p, b);
+        const SequenceSpan s = sequence_span<TREE>(a.p, b);
         position = token < s.first + s.count ? s.base + token - s.first : -1;
+        if constexpr (TREE)
+            if (position >= 0) depth = walk_tree(a.parents + s.first, token - s.first, 0, 0, 0, nullptr) - (token - s.first);
         if (position >= 0) {
             const int page = a.p.table[static_cast<long long>(b) * a.p.table_stride + (position >> a.p.page_shift)];
             if (page >= 0 && page < a.p.pages) {
@@ -193,6 +227,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const A
             }
         }
     }
+    if constexpr (TREE) position = position >= 0 ? position + depth : -1;
     // (not by an angle of zero where there is none: that would add 0 times the
     // partner, which need not be finite)
     float4 cos{}, sin{};
@@ -305,19 +340,23 @@ struct AttendArgs {
     unsigned int* counters;   // [CTAs], zero between calls (few-row kernel)
     int4* entries;            // [CTAs] the item that begins last in each (chunk kernel)
     int half_tokens;          // new tokens of each of an item's two tiles (chunk kernel)
+    const int32_t* parents;   // of a tree's nodes (TREE)
 };
 
 // A sequence as this kernel's share of the batch has it: without new tokens if
 // it is another kernel's.
+template <bool TREE>
 __device__ __forceinline__ SequenceSpan own_span(const AttendArgs& a, const RawSpan& r) {
-    SequenceSpan s = checked_span(a.p, r);
+    SequenceSpan s = checked_span<TREE>(a.p, r);
     if (s.count < a.fewest || s.count > a.most) s.count = 0;
     return s;
 }
 
+// Of a tree (TREE) the new tokens lie at base .. base + count - 1 too, but a
+// row sees of these its ancestors and itself only, and stands at its depth.
 struct Tile {  // one tile of new tokens of a sequence
     int first, tokens;        // first row (token index in the batch), tokens
-    int p0, p1;               // positions of its first and last token
+    int p0, p1;               // positions of its first and last token (TREE: base, place of its last node)
     int low, high, sink_blocks;
     __device__ __forceinline__ int units() const { return high - low + sink_blocks; }
     __device__ __forceinline__ int block(int unit) const {
@@ -325,13 +364,13 @@ struct Tile {  // one tile of new tokens of a sequence
     }
 };
 
-template <int KEYS>
+template <int KEYS, bool TREE>
 __device__ __forceinline__ Tile make_tile(const SequenceSpan& s, int t, int tile_tokens, int window, int sinks) {
     Tile x;
     x.first = s.first + t * tile_tokens;
     x.tokens = min(tile_tokens, s.count - t * tile_tokens);
-    x.p0 = s.base + t * tile_tokens;
-    x.p1 = x.p0 + x.tokens - 1;
+    x.p0 = TREE ? s.base : s.base + t * tile_tokens;
+    x.p1 = s.base + t * tile_tokens + x.tokens - 1;
     const int end = max(x.p1 + 1, 0);
     const int from = window > 0 ? max(x.p0 - window + 1, 0) : 0;
     x.high = max((end + KEYS - 1) / KEYS, 1);
@@ -340,27 +379,27 @@ __device__ __forceinline__ Tile make_tile(const SequenceSpan& s, int t, int tile
     return x;
 }
 
-template <int KEYS>
+template <int KEYS, bool TREE>
 __device__ __forceinline__ int item_places(const AttendArgs& a, const SequenceSpan& s, int t, int tile_tokens) {
-    return a.extra + make_tile<KEYS>(s, t, tile_tokens, a.window, a.sinks).units();
+    return a.extra + make_tile<KEYS, TREE>(s, t, tile_tokens, a.window, a.sinks).units();
 }
 
 // Places of one kv head of every lane's sequence. The whole warp takes part: a
 // lane sums a few tiles by itself, a long chunk's are summed by all lanes.
-template <int KEYS>
+template <int KEYS, bool TREE>
 __device__ __forceinline__ long long warp_places(const AttendArgs& a, const SequenceSpan& s, int tile_tokens) {
     const int lane = threadIdx.x & 31;
     long long n = 0;
     const bool is_long = s.count > 4 * tile_tokens;
     if (!is_long)
-        for (int t = 0; t * tile_tokens < s.count; ++t) n += item_places<KEYS>(a, s, t, tile_tokens);
+        for (int t = 0; t * tile_tokens < s.count; ++t) n += item_places<KEYS, TREE>(a, s, t, tile_tokens);
     for (unsigned todo = __ballot_sync(0xffffffffu, is_long); todo; todo &= todo - 1) {
         const int who = __ffs(todo) - 1;
         const SequenceSpan x{__shfl_sync(0xffffffffu, s.first, who), __shfl_sync(0xffffffffu, s.count, who),
                              __shfl_sync(0xffffffffu, s.base, who)};
         long long sum = 0;
         for (int t = lane; static_cast<long long>(t) * tile_tokens < x.count; t += 32)
-            sum += item_places<KEYS>(a, x, t, tile_tokens);
+            sum += item_places<KEYS, TREE>(a, x, t, tile_tokens);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == who) n = sum;
@@ -385,7 +424,7 @@ __device__ __forceinline__ int range_owner(long long total, long long place, int
 // and a Range. Each thread has a share of the sequences, a prefix sum over
 // the threads follows, and the thread whose sequences hold place `begin`
 // finds it.
-template <int THREADS, int KEYS>
+template <int THREADS, int KEYS, bool TREE = false>
 __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens, void* shared) {
     long long* warp_sums = static_cast<long long*>(shared);
     Range* found = reinterpret_cast<Range*>(warp_sums + THREADS / 32);
@@ -393,8 +432,8 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     const int each = (a.p.sequences + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
     auto places_of = [&](int e) {  // of the thread's e-th sequence, all kv heads
         SequenceSpan s{0, 0, 0};
-        if (b0 + e < a.p.sequences) s = own_span(a, raw_span(a.p, b0 + e));
-        return a.p.kv_heads * warp_places<KEYS>(a, s, tile_tokens);
+        if (b0 + e < a.p.sequences) s = own_span<TREE>(a, raw_span(a.p, b0 + e));
+        return a.p.kv_heads * warp_places<KEYS, TREE>(a, s, tile_tokens);
     };
     long long mine = 0;
     for (int e = 0; e < each; ++e) mine += places_of(e);
@@ -443,7 +482,7 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
 }
 
 // A walk over the CTA's units, item by item.
-template <int KEYS>
+template <int KEYS, bool TREE = false>
 struct Walk {
     SequenceSpan span;
     RawSpan following;        // of sequence b + 1, requested when b was entered
@@ -460,13 +499,13 @@ struct Walk {
         const int lane = threadIdx.x & 31;
         b = r.sequence;
         left = static_cast<int>(min(r.end - r.begin, static_cast<long long>(INT_MAX)));
-        span = own_span(a, raw_span(a.p, b));
+        span = own_span<TREE>(a, raw_span(a.p, b));
         request(a);
         long long skip = r.skip;
         for (int t0 = 0;; t0 += 32) {
             long long n = 0;
             if (static_cast<long long>(t0 + lane) * tile_tokens < span.count)
-                n = item_places<KEYS>(a, span, t0 + lane, tile_tokens) * static_cast<long long>(a.p.kv_heads);
+                n = item_places<KEYS, TREE>(a, span, t0 + lane, tile_tokens) * static_cast<long long>(a.p.kv_heads);
             long long upto = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -482,7 +521,7 @@ struct Walk {
             }
             skip -= __shfl_sync(0xffffffffu, upto, 31);
         }
-        tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
+        tile = make_tile<KEYS, TREE>(span, t, tile_tokens, a.window, a.sinks);
         const int places = a.extra + tile.units();
         h = static_cast<int>(skip / places);
         unit = static_cast<int>(skip % places) - a.extra;
@@ -501,10 +540,10 @@ struct Walk {
         while (t * tile_tokens >= span.count) {
             t = 0;
             ++b;
-            span = own_span(a, following);
+            span = own_span<TREE>(a, following);
             request(a);
         }
-        tile = make_tile<KEYS>(span, t, tile_tokens, a.window, a.sinks);
+        tile = make_tile<KEYS, TREE>(span, t, tile_tokens, a.window, a.sinks);
     }
     __device__ __forceinline__ bool item_ends() const { return unit + 1 >= tile.units(); }
     // Whether this unit is the last of the item in this range, or of all.
@@ -524,8 +563,8 @@ struct Walk {
 
 // The CTAs that hold units of an item, given one of its units (walk state of
 // the CTA of `range`): from its first unit's to its last's.
-template <int KEYS>
-__device__ __forceinline__ int2 item_owners(const Range& range, const Walk<KEYS>& w) {
+template <int KEYS, bool TREE>
+__device__ __forceinline__ int2 item_owners(const Range& range, const Walk<KEYS, TREE>& w) {
     const long long first = range.end - w.left - w.unit;
     return make_int2(range_owner(range.total, first, range.ctas),
                      range_owner(range.total, first + w.tile.units() - 1, range.ctas));
@@ -586,6 +625,9 @@ struct FewCfg {
     static constexpr int kJoinOff = kRing;
     static constexpr int kStatOff = kJoinOff + 2 * kJoin;
     static constexpr int kSmem = kStatOff + 2 * (ROWS < 16 ? 16 : ROWS) * 2 * 4 + 256;
+    // of a tree's tile: the nodes that each of its nodes sees, and its position
+    static constexpr int kSightOff = kStatOff + 2 * (ROWS < 16 ? 16 : ROWS) * 2 * 4;
+    static constexpr int kTreeSmem = kSightOff + ROWS * (kTreeWords + 1) * 4;
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -630,14 +672,14 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) {
     return static_cast<uint32_t>(r * (D * 2) + ((c ^ (r & 7)) * 16));
 }
 
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool TREE>
 __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(const AttendArgs a) {
     using C = FewCfg<D, ROWS>;
     constexpr int kSteps = D / 16, kCols = D / 8;
     extern __shared__ __align__(128) uint8_t few_smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tile_tokens = ROWS / a.group;
-    const Range range = find_range<kFewThreads, kFewKeys>(a, tile_tokens, few_smem + C::kStatOff);
+    const Range range = find_range<kFewThreads, kFewKeys, TREE>(a, tile_tokens, few_smem + C::kStatOff);
     if (range.begin >= range.end) return;
     __syncthreads();  // the range's scratch is reused below
 
@@ -646,7 +688,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     const int page_mask = (1 << a.p.page_shift) - 1;
 
     // Page of the walk's piece: -1 when no row sees any key of it.
-    auto page_of = [&](const Walk<kFewKeys>& w) -> int {
+    auto page_of = [&](const Walk<kFewKeys, TREE>& w) -> int {
         const int key = w.tile.block(w.unit) * kFewKeys + warp * 16;
         const Tile& t = w.tile;
         const bool seen = key <= t.p1 && (a.window <= 0 || key + 15 > t.p0 - a.window || key < a.sinks);
@@ -663,7 +705,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     constexpr int kChunks = D / 8, kRowsStep = 32 / kChunks;  // 16-byte chunks a row, rows a pass
     const int r0 = lane / kChunks;
     const uint32_t from = r0 * D + (lane % kChunks) * 8, to = piece_at<D>(r0, lane % kChunks);
-    auto load = [&](const Walk<kFewKeys>& w, int page, int stage) {
+    auto load = [&](const Walk<kFewKeys, TREE>& w, int page, int stage) {
         if (page == -1) return;
         const int key = w.tile.block(w.unit) * kFewKeys + warp * 16;
         const long long row = (static_cast<long long>(max(page, 0)) * a.p.kv_heads + w.h) * head_rows + (key & page_mask);
@@ -671,7 +713,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
         const T* k = static_cast<const T*>(a.k_pages) + row * D + from;
         const T* v = static_cast<const T*>(a.v_pages) + row * D + from;
         if (page >= 0 && key + 15 <= w.tile.p1 &&
-            (a.window <= 0 || key > w.tile.p0 - a.window || key + 15 < a.sinks)) {  // the usual: every key is seen
+            (a.window <= 0 || key > w.tile.p0 - a.window || key + 15 < a.sinks)) {  // the usual: some row sees every key
 #pragma unroll
             for (int r = 0; r < 16; r += kRowsStep) {
                 const uint32_t at = dst + (to ^ ((r & 7) << 4)) + r * (D * 2);
@@ -693,7 +735,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     const uint32_t k_at = piece_at<D>((lane >> 4) * 8 + (lane & 7), (lane >> 3) & 1);
     const uint32_t v_at = piece_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), lane >> 4);
 
-    Walk<kFewKeys> now, ahead;
+    Walk<kFewKeys, TREE> now, ahead;
     if (!now.start(a, range, tile_tokens)) return;
     ahead = now;
     // the ring's first stages; `page` belongs to the piece `ahead` stands at, and
@@ -719,9 +761,26 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
     int stage = 0;
     bool begun = now.unit == 0;  // the item's first unit is in this range
     bool fresh = true;
+    uint32_t* sight = reinterpret_cast<uint32_t*>(few_smem + C::kSightOff);  // [tile tokens][kTreeWords], then positions
+    int sight_b = -1, sight_t = 0;  // the tile that it holds
     while (true) {
         if (fresh) {  // a new item: its q fragments and empty sums
             fresh = false;
+            if constexpr (TREE) {
+                if (now.b != sight_b || now.t != sight_t) {  // (the same for every kv head; all warps are at the same item)
+                    sight_b = now.b, sight_t = now.t;
+                    const int i = threadIdx.x;
+                    if (i < now.tile.tokens) {
+                        const int node = now.tile.first - now.span.first + i;
+                        const bool some = now.span.base >= 0;  // else the sequence counts as empty
+                        const int depth = some ? walk_tree(a.parents + now.span.first, node, now.span.base, a.window, a.sinks,
+                                                           sight + i * kTreeWords)
+                                               : 0;
+                        sight[ROWS * kTreeWords + i] = some ? now.span.base + depth : -1;
+                    }
+                    __syncthreads();
+                }
+            }
 #pragma unroll
             for (int mt = 0; mt < C::kTiles; ++mt) {
 #pragma unroll
@@ -729,7 +788,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                     const int r = mt * 16 + half * 8 + lane / 4;
                     const int i = r / a.group;
                     const bool valid = (half < C::kHalves) && i < now.tile.tokens;
-                    pos[mt][half] = valid ? now.tile.p0 + i : -1;
+                    if constexpr (TREE)
+                        pos[mt][half] = valid ? static_cast<int>(sight[ROWS * kTreeWords + i]) : -1;
+                    else
+                        pos[mt][half] = valid ? now.tile.p0 + i : -1;
                     m[mt][half] = -INFINITY;
                     l[mt][half] = 0.f;
                     const T* q = static_cast<const T*>(a.q) + (now.tile.first + (valid ? i : 0)) * a.q_stride +
@@ -746,6 +808,18 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                     for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
             }
         }
+        // Whether the row of m16 tile mt, half `half` sees key j (of those up to the tile's last).
+        auto sees = [&](int mt, int half, int j) {
+            const int p = pos[mt][half];
+            if constexpr (TREE) {
+                const int node = j - now.tile.p0;
+                if (node >= 0) {
+                    const int i = (mt * 16 + half * 8 + lane / 4) / a.group;
+                    return p >= 0 && j <= now.tile.p1 && ((sight[i * kTreeWords + (node >> 5)] >> (node & 31)) & 1u) != 0u;
+                }
+            }
+            return !(j > p || (a.window > 0 && j <= p - a.window && j >= a.sinks));
+        };
         async_copy_wait_prior<C::kStages - 2>();
         __syncwarp();
         if (live & 1u) {
@@ -769,7 +843,8 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
             }
             const int key = now.tile.block(now.unit) * kFewKeys + warp * 16;
             const Tile& t = now.tile;
-            const bool all = key + 15 <= t.p0 && (a.window <= 0 || key > t.p1 - a.window || key + 15 < a.sinks);
+            const bool all = key + 15 <= t.p0 - (TREE ? 1 : 0) &&
+                             (a.window <= 0 || key > t.p1 - a.window || key + 15 < a.sinks);
             if (!all) {
 #pragma unroll
                 for (int mt = 0; mt < C::kTiles; ++mt)
@@ -779,9 +854,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                         for (int n = 0; n < 2; ++n)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const int j = key + n * 8 + (lane & 3) * 2 + e, p = pos[mt][half];
-                                if (j > p || (a.window > 0 && j <= p - a.window && j >= a.sinks))
-                                    s[mt][n][half * 2 + e] = -INFINITY;
+                                if (!sees(mt, half, key + n * 8 + (lane & 3) * 2 + e)) s[mt][n][half * 2 + e] = -INFINITY;
                             }
             }
             // (scaled on their own: s - m is then exact near m, whatever their size)
@@ -840,7 +913,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                     pf[mt][2 + half] = Pair<T>::pack(p[2], p[3]);
                 }
             }
-            if (!all && t.tokens > 1) {
+            if (!all && (TREE || t.tokens > 1)) {
                 uint8_t* piece = few_smem + (vbase - smem_addr(few_smem));
                 uint4* v = reinterpret_cast<uint4*>(piece) + lane;
                 uint32_t bad = 0;
@@ -860,8 +933,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
                             for (int mt = 0; mt < C::kTiles; ++mt)
 #pragma unroll
                                 for (int half = 0; half < C::kHalves; ++half) {
-                                    const int p = pos[mt][half];
-                                    if (key + j > p || (a.window > 0 && key + j <= p - a.window && key + j >= a.sinks)) continue;
+                                    if (!sees(mt, half, key + j)) continue;
                                     o[mt][n][half * 2] += x.x;
                                     o[mt][n][half * 2 + 1] += x.y;
                                 }
@@ -1101,7 +1173,7 @@ static int paged_sm_count(int* sms) {
 constexpr int kFewCtasPerSm = 2, kFewMaxRows = 32;
 constexpr long long kCounterBytes = 4096, kEntryBytes = 4096;
 
-template <typename S, typename T, int D>
+template <typename S, typename T, int D, bool TREE>
 static int launch_append(AppendArgs a, cudaStream_t stream) {
     // Few tokens: a token's heads are spread over as many warps as it takes;
     // many: kAppendShare warps walk them, which look up the token's place once
@@ -1110,35 +1182,47 @@ static int launch_append(AppendArgs a, cudaStream_t stream) {
     a.parts = a.p.tokens >= 1024 && most > kAppendShare ? kAppendShare : most;
     const long long ctas = (static_cast<long long>(a.p.tokens) * a.parts + kAppendWarps - 1) / kAppendWarps;
     if (ctas > INT_MAX / kAppendWarps) return H4B_EUNSUPPORTED;
-    paged_append_kernel<S, T, D><<<static_cast<unsigned>(ctas), 32 * kAppendWarps, 0, stream>>>(a);
+    paged_append_kernel<S, T, D, TREE><<<static_cast<unsigned>(ctas), 32 * kAppendWarps, 0, stream>>>(a);
     H4B_CUDA_TRY(cudaGetLastError());
     return 0;
 }
 
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool TREE = false>
 static int launch_few(AttendArgs a, int sms, cudaStream_t stream) {
     using C = FewCfg<D, ROWS>;
+    constexpr int kSmem = TREE ? C::kTreeSmem : C::kSmem;
     a.extra = kFewExtra;
     a.least = kFewLeast;
     static std::atomic<bool> opted_in[kMaxDevices];
     int dev = 0;
     H4B_CUDA_TRY(cudaGetDevice(&dev));
     if (!opted_in[dev].load(std::memory_order_acquire)) {
-        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_few_kernel<T, D, ROWS>,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_few_kernel<T, D, ROWS, TREE>,
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         opted_in[dev].store(true, std::memory_order_release);
     }
-    paged_attention_few_kernel<T, D, ROWS><<<kFewCtasPerSm * sms, kFewThreads, C::kSmem, stream>>>(a);
+    paged_attention_few_kernel<T, D, ROWS, TREE><<<kFewCtasPerSm * sms, kFewThreads, kSmem, stream>>>(a);
     H4B_CUDA_TRY(cudaGetLastError());
     return 0;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TREE = false>
 static int launch_few_rows(const AttendArgs& a, int rows, int sms, cudaStream_t stream) {
-    if (rows <= 8) return launch_few<T, D, 8>(a, sms, stream);
+    if (rows <= 8) return launch_few<T, D, 8, TREE>(a, sms, stream);
     if constexpr (D == 64)
-        if (rows > 16) return launch_few<T, D, 32>(a, sms, stream);
-    return launch_few<T, D, 16>(a, sms, stream);
+        if (rows > 16) return launch_few<T, D, 32, TREE>(a, sms, stream);
+    return launch_few<T, D, 16, TREE>(a, sms, stream);
+}
+
+// A tile holds a token's whole group, so a group of more than 16 takes the 32
+// rows, also at head_dim 128 (where they spill).
+template <typename T, int D>
+static int launch_tree(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
+    a.fewest = 1;
+    a.most = INT_MAX;
+    const long long rows = static_cast<long long>(max_query) * a.group;
+    if (a.group > 16) return launch_few<T, D, 32, true>(a, sms, stream);
+    return launch_few_rows<T, D, true>(a, static_cast<int>(rows < 32 ? rows : 32), sms, stream);
 }
 
 template <typename T, int D>
@@ -1175,12 +1259,23 @@ static int launch_attention(AttendArgs a, const h4b_paged_kv* kv, int max_query,
     return launch_few_rows<T, D>(a, static_cast<int>(rows), sms, stream);
 }
 
-}  // namespace h4b
+template <bool TREE>
+static int launch_append_types(const AppendArgs& a, const h4b_paged_kv* kv, int qkv_dtype, cudaStream_t s) {
+    const bool wide = kv->head_dim == 128, from32 = qkv_dtype == H4B_FP32;
+    if (kv->dtype == H4B_FP16) {
+        if (from32) return wide ? launch_append<float, __half, 128, TREE>(a, s) : launch_append<float, __half, 64, TREE>(a, s);
+        return wide ? launch_append<__half, __half, 128, TREE>(a, s) : launch_append<__half, __half, 64, TREE>(a, s);
+    }
+    using B16 = __nv_bfloat16;
+    if (from32) return wide ? launch_append<float, B16, 128, TREE>(a, s) : launch_append<float, B16, 64, TREE>(a, s);
+    return wide ? launch_append<B16, B16, 128, TREE>(a, s) : launch_append<B16, B16, 64, TREE>(a, s);
+}
 
-extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv_dtype, long long qkv_stride, int heads,
-                                const float* norm_q, const float* norm_k, float eps, const float* rope_cos,
-                                const float* rope_sin, int max_pos, void* q_out, long long q_stride, void* stream) {
-    using namespace h4b;
+// `parents`: the new tokens are a tree's nodes (null: one after the other).
+static int paged_append(const h4b_paged_kv* kv, const int32_t* parents, const void* qkv, int qkv_dtype,
+                        long long qkv_stride, int heads, const float* norm_q, const float* norm_k, float eps,
+                        const float* rope_cos, const float* rope_sin, int max_pos, void* q_out, long long q_stride,
+                        void* stream) {
     AppendArgs a{};
     if (!paged_view(kv, &a.p) || heads < 0) return H4B_EINVAL;
     const long long row_heads = heads + 2ll * kv->kv_heads;
@@ -1200,16 +1295,27 @@ extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv
     a.qkv = qkv, a.qkv_stride = qkv_stride, a.norm_q = norm_q, a.norm_k = norm_k, a.cos = rope_cos, a.sin = rope_sin;
     a.max_pos = max_pos, a.heads = heads, a.eps = eps, a.q_out = q_out, a.q_stride = q_stride;
     a.k_pages = kv->k_pages, a.v_pages = kv->v_pages;
+    a.parents = parents;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool wide = kv->head_dim == 128, from32 = qkv_dtype == H4B_FP32;
-    if (kv->dtype == H4B_FP16) {
-        if (from32) return wide ? launch_append<float, __half, 128>(a, s) : launch_append<float, __half, 64>(a, s);
-        return wide ? launch_append<__half, __half, 128>(a, s) : launch_append<__half, __half, 64>(a, s);
-    }
-    if (from32)
-        return wide ? launch_append<float, __nv_bfloat16, 128>(a, s) : launch_append<float, __nv_bfloat16, 64>(a, s);
-    return wide ? launch_append<__nv_bfloat16, __nv_bfloat16, 128>(a, s)
-                : launch_append<__nv_bfloat16, __nv_bfloat16, 64>(a, s);
+    return parents == nullptr ? launch_append_types<false>(a, kv, qkv_dtype, s) : launch_append_types<true>(a, kv, qkv_dtype, s);
+}
+
+}  // namespace h4b
+
+extern "C" int h4b_paged_append(const h4b_paged_kv* kv, const void* qkv, int qkv_dtype, long long qkv_stride, int heads,
+                                const float* norm_q, const float* norm_k, float eps, const float* rope_cos,
+                                const float* rope_sin, int max_pos, void* q_out, long long q_stride, void* stream) {
+    return h4b::paged_append(kv, nullptr, qkv, qkv_dtype, qkv_stride, heads, norm_q, norm_k, eps, rope_cos, rope_sin,
+                             max_pos, q_out, q_stride, stream);
+}
+
+extern "C" int h4b_paged_append_tree(const h4b_paged_kv* kv, const int32_t* parents, const void* qkv, int qkv_dtype,
+                                     long long qkv_stride, int heads, const float* norm_q, const float* norm_k, float eps,
+                                     const float* rope_cos, const float* rope_sin, int max_pos, void* q_out,
+                                     long long q_stride, void* stream) {
+    if (parents == nullptr && kv != nullptr && kv->tokens > 0) return H4B_EINVAL;
+    return h4b::paged_append(kv, parents, qkv, qkv_dtype, qkv_stride, heads, norm_q, norm_k, eps, rope_cos, rope_sin,
+                             max_pos, q_out, q_stride, stream);
 }
 
 extern "C" int h4b_pages_copy(void* k_pages, void* v_pages, int layers, int pages, long long page_bytes,
@@ -1242,10 +1348,12 @@ extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
     return kCounterBytes + kEntryBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
 }
 
-extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long long q_stride, int heads, float scale,
-                                   int window, int sinks, int max_query, void* out, long long out_stride, float* lse,
-                                   void* workspace, long long workspace_bytes, void* stream) {
-    using namespace h4b;
+namespace h4b {
+
+// `parents`: the new tokens are a tree's nodes (null: one after the other).
+static int paged_attention(const h4b_paged_kv* kv, const int32_t* parents, const void* q, long long q_stride, int heads,
+                           float scale, int window, int sinks, int max_query, void* out, long long out_stride, float* lse,
+                           void* workspace, long long workspace_bytes, void* stream) {
     AttendArgs a{};
     if (!paged_view(kv, &a.p) || heads < 1 || heads % kv->kv_heads || window < 0 || sinks < 0 ||
         (sinks > 0 && window == 0) || max_query < 1)
@@ -1273,11 +1381,35 @@ extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long l
     a.counters = static_cast<unsigned int*>(workspace);
     a.entries = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
     a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes + kEntryBytes);
+    a.parents = parents;
     const int longest = max_query < kv->tokens ? max_query : kv->tokens;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool wide = kv->head_dim == 128;
+    using B16 = __nv_bfloat16;
+    if (parents != nullptr) {
+        if (kv->dtype == H4B_FP16)
+            return wide ? launch_tree<__half, 128>(a, kv, longest, sms, s) : launch_tree<__half, 64>(a, kv, longest, sms, s);
+        return wide ? launch_tree<B16, 128>(a, kv, longest, sms, s) : launch_tree<B16, 64>(a, kv, longest, sms, s);
+    }
     if (kv->dtype == H4B_FP16)
         return wide ? launch_attention<__half, 128>(a, kv, longest, sms, s) : launch_attention<__half, 64>(a, kv, longest, sms, s);
-    return wide ? launch_attention<__nv_bfloat16, 128>(a, kv, longest, sms, s)
-                : launch_attention<__nv_bfloat16, 64>(a, kv, longest, sms, s);
+    return wide ? launch_attention<B16, 128>(a, kv, longest, sms, s) : launch_attention<B16, 64>(a, kv, longest, sms, s);
+}
+
+}  // namespace h4b
+
+extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long long q_stride, int heads, float scale,
+                                   int window, int sinks, int max_query, void* out, long long out_stride, float* lse,
+                                   void* workspace, long long workspace_bytes, void* stream) {
+    return h4b::paged_attention(kv, nullptr, q, q_stride, heads, scale, window, sinks, max_query, out, out_stride, lse,
+                                workspace, workspace_bytes, stream);
+}
+
+extern "C" int h4b_paged_tree_attention(const h4b_paged_kv* kv, const int32_t* parents, const void* q, long long q_stride,
+                                        int heads, float scale, int window, int sinks, int max_query, void* out,
+                                        long long out_stride, float* lse, void* workspace, long long workspace_bytes,
+                                        void* stream) {
+    if (parents == nullptr && kv != nullptr && kv->tokens > 0) return H4B_EINVAL;
+    return h4b::paged_attention(kv, parents, q, q_stride, heads, scale, window, sinks, max_query, out, out_stride, lse,
+                                workspace, workspace_bytes, stream);
 }

@@ -11,7 +11,7 @@ from functools import lru_cache
 
 import torch
 
-from ._lib import PagedKvDesc, check, lib, stream_handle
+from ._lib import TREE_NODES, PagedKvDesc, check, lib, stream_handle
 
 
 def _dev(tensor: torch.Tensor, dtype: torch.dtype, name: str) -> int:
@@ -166,6 +166,41 @@ def quantize_rows(values: torch.Tensor):
     return x8, scales, sums
 
 
+def rmsnorm_quantize_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, *, delta: torch.Tensor | None = None,
+                          out: torch.Tensor | None = None):
+    """h4b_rmsnorm_quantize_rows: the residual addition s = x + delta, its
+    RMSNorm and per-token int8 quantisation in one pass over rows [M, K] (fp32,
+    fp16 or bf16 each, rows may be strided; s and the norm are fp32). s, rounded
+    to x's type, goes to `out` (x itself by default; unused without `delta`).
+    Returns (x8, scales[M], sums[M]) for int4_gemm; fp32 rows have the bits of
+    rmsnorm and quantize_rows."""
+    if x.dim() != 2 or weight.numel() != x.shape[1]:
+        raise ValueError("x must be [rows][width], weight [width]")
+    (rows, width), dtype, device = x.shape, x.dtype, x.get_device()
+    code = _VALUE_DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"x must be float32, float16 or bfloat16, got {dtype}")
+    several = rows > 1
+    add, add_code, add_stride, to, to_stride = None, 0, 0, None, 0
+    if delta is not None:
+        add_code = _VALUE_DTYPES.get(delta.dtype)
+        if add_code is None:
+            raise ValueError(f"delta must be float32, float16 or bfloat16, got {delta.dtype}")
+        out = x if out is None else out
+        if delta.shape != x.shape or out.shape != x.shape:
+            raise ValueError("delta and out must have x's shape")
+        add, add_stride = _rows(delta, delta.dtype, "delta", device), delta.stride(0) if several else width
+        to, to_stride = _rows(out, dtype, "out", device), out.stride(0) if several else width
+    x8 = torch.empty((rows, width), dtype=torch.int8, device=x.device)
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    sums = torch.empty(rows, dtype=torch.int32, device=x.device)
+    check(lib().h4b_rmsnorm_quantize_rows(_rows(x, dtype, "x", device), code, x.stride(0) if several else width, add, add_code,
+                                          add_stride, to, to_stride, _on(weight, torch.float32, "weight", device), eps,
+                                          x8.data_ptr(), scales.data_ptr(), sums.data_ptr(), rows, width, _here(device)),
+          "h4b_rmsnorm_quantize_rows")
+    return x8, scales, sums
+
+
 GEMM_KERNELS = {"auto": 0, "tcgen05": 1, "mma_sync": 2}
 
 
@@ -290,16 +325,27 @@ def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> Pag
                        sequences, table[1], tokens)
 
 
+def _parents(parents, tokens: int, device: int) -> int:
+    """Data pointer of the parents of `tokens` nodes."""
+    at = _on(parents, torch.int32, "parents", device)
+    if parents.numel() != tokens:
+        raise ValueError(f"parents must hold one index a token, {tokens}, got {parents.numel()}")
+    return at
+
+
 def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                  q_offsets: torch.Tensor, kv_lens: torch.Tensor, *, heads: int, norm_q: torch.Tensor | None = None,
                  norm_k: torch.Tensor | None = None, eps: float = 1e-6, rope_cos: torch.Tensor | None = None,
-                 rope_sin: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                 rope_sin: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                 parents: torch.Tensor | None = None) -> torch.Tensor:
     """h4b_paged_append: the new tokens' k and v into one layer's pages, their
     q heads back. `qkv` holds `heads` q heads, the k heads and the v heads of
     every new token ([tokens][(heads + 2 kv_heads) * head_dim], fp32 or the
     cache's type, rows may be strided); q and k are RMS-normalised with
     `norm_q` / `norm_k` and rotated with `rope_cos` / `rope_sin` where given.
-    Returns q [tokens][heads][head_dim] in the cache's type."""
+    With `parents` (int32 [tokens]) the new tokens are nodes of drafted trees
+    (paged_tree_attention) and stand at their depths. Returns q
+    [tokens][heads][head_dim] in the cache's type."""
     tokens, width = qkv.shape if qkv.dim() == 2 else (0, -1)
     dtype, source, device = k_pages.dtype, qkv.dtype, k_pages.get_device()
     kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens)
@@ -326,10 +372,14 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
             raise ValueError("rope_cos and rope_sin must be [positions][head_dim / 2]")
         positions = rope_cos.shape[0]
         cos, sin = _on(rope_cos, torch.float32, "rope_cos", device), _on(rope_sin, torch.float32, "rope_sin", device)
-    check(lib().h4b_paged_append(ctypes.byref(kv), _rows(qkv, source, "qkv", device),
-                                 0 if source is torch.float32 else kv.dtype, qkv.stride(0) if tokens > 1 else width, heads,
-                                 weights[0], weights[1], eps, cos, sin, positions, _rows(out, dtype, "out", device),
-                                 out.stride(0) if tokens > 1 else heads * head_dim, _here(device)), "h4b_paged_append")
+    rest = (_rows(qkv, source, "qkv", device), 0 if source is torch.float32 else kv.dtype,
+            qkv.stride(0) if tokens > 1 else width, heads, weights[0], weights[1], eps, cos, sin, positions,
+            _rows(out, dtype, "out", device), out.stride(0) if tokens > 1 else heads * head_dim, _here(device))
+    if parents is None:
+        check(lib().h4b_paged_append(ctypes.byref(kv), *rest), "h4b_paged_append")
+    else:
+        check(lib().h4b_paged_append_tree(ctypes.byref(kv), _parents(parents, tokens, device), *rest),
+              "h4b_paged_append_tree")
     return out
 
 
@@ -364,6 +414,34 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (1 / sqrt(head_dim) by default). `lse`, if given, receives the float32
     [tokens][heads] log-sum-exp. `workspace`: from paged_workspace, kept between
     calls (one is made per call otherwise)."""
+    return _attend(q, k_pages, v_pages, page_table, q_offsets, kv_lens, None, max_query, window, sinks, scale, out, lse,
+                   workspace)
+
+
+def paged_tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                         q_offsets: torch.Tensor, kv_lens: torch.Tensor, parents: torch.Tensor, *,
+                         max_query: int | None = None, window: int = 0, sinks: int = 0, scale: float | None = None,
+                         out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """h4b_paged_tree_attention: paged_attention where the new tokens of each
+    sequence are the nodes of a drafted tree (at most 256): `parents` (int32
+    [tokens]) holds a node's parent within its sequence, less than the node's
+    own index, or -1 where it follows the sequence's kv_lens[b] - nodes earlier
+    tokens. Node i lies in the cache behind these, at place i (paged_append with
+    the same `parents` wrote it there), and stands at their number + its depth.
+    It sees the earlier tokens, its ancestors and itself; with `window` > 0 those
+    of them that stand less than `window` before it, or among the first `sinks`.
+    `max_query` is the largest tree to expect (it sets the tiles; by default all
+    rows, at most 256)."""
+    if max_query is None:
+        max_query = max(1, min(q.shape[0], TREE_NODES))
+    return _attend(q, k_pages, v_pages, page_table, q_offsets, kv_lens, parents, max_query, window, sinks, scale, out, lse,
+                   workspace)
+
+
+def _attend(q, k_pages, v_pages, page_table, q_offsets, kv_lens, parents, max_query, window, sinks, scale, out, lse,
+            workspace) -> torch.Tensor:
+    """Both attentions' checks, and the call: of a tree's nodes with `parents`."""
     if q.dim() != 3:
         raise ValueError("q must be [tokens][heads][head_dim]")
     tokens, heads, head_dim = shape = q.shape
@@ -385,12 +463,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("window, sinks and max_query must fit 32 bits")
     width = heads * head_dim
     several = tokens > 1
-    check(lib().h4b_paged_attention(ctypes.byref(kv), _rows(q, dtype, "q", device), q.stride(0) if several else width,
-                                    heads, head_dim ** -0.5 if scale is None else scale, window, sinks, max_query,
-                                    _rows(out, dtype, "out", device), out.stride(0) if several else width,
-                                    None if lse is None else _on(lse, torch.float32, "lse", device),
-                                    _on(workspace, torch.uint8, "workspace", device), workspace.numel(),
-                                    _here(device)), "h4b_paged_attention")
+    rest = (_rows(q, dtype, "q", device), q.stride(0) if several else width, heads,
+            head_dim ** -0.5 if scale is None else scale, window, sinks, max_query, _rows(out, dtype, "out", device),
+            out.stride(0) if several else width, None if lse is None else _on(lse, torch.float32, "lse", device),
+            _on(workspace, torch.uint8, "workspace", device), workspace.numel(), _here(device))
+    if parents is None:
+        check(lib().h4b_paged_attention(ctypes.byref(kv), *rest), "h4b_paged_attention")
+    else:
+        check(lib().h4b_paged_tree_attention(ctypes.byref(kv), _parents(parents, tokens, device), *rest),
+              "h4b_paged_tree_attention")
     return out
 
 
@@ -410,3 +491,98 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
                                kv_heads * page_size * head_dim * k_pages.element_size(),
                                _on(src, torch.int32, "src", device), _on(dst, torch.int32, "dst", device), count,
                                _here(device)), "h4b_pages_copy")
+
+
+# ---- drafted token trees -----------------------------------------------------------
+_VALUE_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # H4B_FP32, H4B_FP16, H4B_BF16
+
+
+def accept_workspace(rows: int, sequences: int, device=None) -> torch.Tensor:
+    """A workspace for accept_tree calls of up to so many rows and sequences
+    that follow each other (one stream): zeroed once, every call leaves it ready
+    for the next."""
+    nbytes = int(lib().h4b_tree_accept_workspace_bytes(rows, sequences))
+    if nbytes < 0:
+        check(nbytes, "h4b_tree_accept_workspace_bytes")
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+
+
+def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, q_offsets: torch.Tensor, logits: torch.Tensor | None = None,
+                *, targets: torch.Tensor | None = None, max_path: int | None = None,
+                workspace: torch.Tensor | None = None):
+    """h4b_tree_accept: the branch of each sequence's drafted tree that agrees
+    with the model. Node 0 (row q_offsets[b]) is the token that was decided
+    before; an accepted node is followed by its first child whose token
+    (tokens[row]) is the node's target: the first maximum of its logits
+    ([rows][vocab], fp32, fp16 or bf16, rows may be strided; a NaN counts as the
+    largest), or, without logits, `targets` (int32 [rows], for example sampled).
+    Returns (path, counts, next_tokens, targets): the accepted nodes' indices
+    [sequences][max_path], -1 behind them (by default max_path is the number of
+    rows, at most 256), how many they are, the last one's target, and all rows'.
+    `workspace`: from accept_workspace, kept between calls (one is made per call
+    otherwise)."""
+    rows, sequences, device = tokens.numel(), q_offsets.numel() - 1, tokens.get_device()
+    if sequences < 0:
+        raise ValueError("q_offsets must be [sequences + 1]")
+    if (logits is None) == (targets is None):
+        raise ValueError("accept_tree takes either logits or targets")
+    if max_path is None:
+        max_path = max(1, min(rows, TREE_NODES))
+    if not 1 <= max_path <= 0x7fffffff:
+        raise ValueError("max_path must be positive and fit 32 bits")
+    at = _on(tokens, torch.int32, "tokens", device), _parents(parents, rows, device), _on(q_offsets, torch.int32, "q_offsets",
+                                                                                         device)
+    vocab, code, data, stride = 0, 0, None, 0
+    if logits is None:
+        if targets.numel() != rows:
+            raise ValueError("targets must hold one token a row")
+    else:
+        if logits.dim() != 2 or logits.shape[0] != rows:
+            raise ValueError("logits must be [rows][vocab]")
+        code = _VALUE_DTYPES.get(logits.dtype)
+        if code is None:
+            raise ValueError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+        vocab = logits.shape[1]
+        data, stride = _rows(logits, logits.dtype, "logits", device), logits.stride(0) if rows > 1 else vocab
+        if workspace is None:
+            workspace = accept_workspace(rows, sequences, tokens.device)
+        targets = torch.empty(rows, dtype=torch.int32, device=tokens.device)
+    path = torch.empty((sequences, max_path), dtype=torch.int32, device=tokens.device)
+    counts, following = torch.empty((2, sequences), dtype=torch.int32, device=tokens.device)
+    check(lib().h4b_tree_accept(data, code, stride, vocab, *at, rows, sequences, max_path,
+                                _on(targets, torch.int32, "targets", device), path.data_ptr(), counts.data_ptr(),
+                                following.data_ptr(),
+                                None if workspace is None else _on(workspace, torch.uint8, "workspace", device),
+                                0 if workspace is None else workspace.numel(), _here(device)), "h4b_tree_accept")
+    return path, counts, following, targets
+
+
+def keep_tokens(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, q_offsets: torch.Tensor,
+                kv_lens: torch.Tensor, path: torch.Tensor, counts: torch.Tensor,
+                lengths: torch.Tensor | None = None) -> torch.Tensor:
+    """h4b_tree_keep: the K and V of the accepted nodes path[b][:counts[b]]
+    (accept_tree), moved behind the tokens before the tree, in every layer of
+    [layers][pages][kv_heads][page_size][head_dim] (or one layer's [pages]...)
+    caches. Returns the new lengths (int32 [sequences]; `lengths`, if given,
+    overlaps neither kv_lens nor counts)."""
+    layered = k_pages.dim() == 5
+    if (not layered and k_pages.dim() != 4) or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must be [layers][pages][kv_heads][page_size][head_dim]")
+    device, sequences, layers = k_pages.get_device(), kv_lens.numel(), k_pages.shape[0] if layered else 1
+    _on(k_pages, k_pages.dtype, "k_pages", device), _on(v_pages, k_pages.dtype, "v_pages", device)
+    if layers == 0:
+        raise ValueError("k_pages and v_pages must hold a layer")
+    if path.dim() != 2 or path.shape[0] != sequences or path.shape[1] < 1 or counts.numel() != sequences:
+        raise ValueError("path must be [sequences][nodes], counts [sequences]")
+    if lengths is None:
+        lengths = torch.empty(sequences, dtype=torch.int32, device=kv_lens.device)
+    elif lengths.numel() != sequences:
+        raise ValueError("lengths must hold one length a sequence")
+    kv = _paged(k_pages[0] if layered else k_pages, v_pages[0] if layered else v_pages, page_table, q_offsets, kv_lens,
+                0x7fffffff)
+    check(lib().h4b_tree_keep(ctypes.byref(kv), layers, k_pages.stride(0) * k_pages.element_size() if layered else 0,
+                              _on(path, torch.int32, "path", device), path.shape[1],
+                              _on(counts, torch.int32, "counts", device), _on(lengths, torch.int32, "lengths", device),
+                              _here(device)), "h4b_tree_keep")
+    return lengths

@@ -30,8 +30,8 @@ extern "C" {
 #define H4B_ETOOBIG (-3)      /* request exceeds the library's static scratch */
 
 /* Device-side status word (bit 1: a bounded wait gave up; bit 2: token id
- * out of range; bit 4: position beyond capacity; bit 8: page id, row offset
- * or length of a paged batch out of range). Reads and clears it; the
+ * out of range; bit 4: position beyond capacity; bit 8: page id, row offset,
+ * length, parent or path of a paged batch out of range). Reads and clears it; the
  * read synchronises with the device. */
 int h4b_get_status(int *host_status);
 
@@ -520,6 +520,64 @@ long long h4b_paged_attention_workspace_bytes(int head_dim);
 int h4b_pages_copy(void *k_pages, void *v_pages, int layers, int pages, long long page_bytes, const int32_t *src,
                    const int32_t *dst, int count, void *stream);
 
+/* ---- drafted token trees over a paged cache --------------------------------------
+ * No counterpart in the reference, which decodes token by token
+ * (cpu_lightspark.py:424-468). One step verifies a tree of drafted tokens for
+ * each sequence: its new rows are the tree's nodes, at most H4B_TREE_NODES of
+ * them, and parents[row] (device memory, [tokens]) is a node's parent within
+ * its sequence, less than the node's own index, or -1 where the node follows
+ * the sequence's kv_lens[b] - nodes earlier tokens. Node i lies in the cache
+ * behind those at place i and stands at their number + its depth. A
+ * sequence of more nodes, or more than kv_lens[b], counts as empty, a parent out
+ * of range as -1; both set status bit 8. */
+#define H4B_TREE_NODES 256
+
+/* h4b_paged_append of a tree's nodes: rotated by their positions, written to
+ * their places. */
+int h4b_paged_append_tree(const h4b_paged_kv *kv, const int32_t *parents, const void *qkv, int qkv_dtype,
+                          long long qkv_stride, int heads, const float *norm_q, const float *norm_k, float eps,
+                          const float *rope_cos, const float *rope_sin, int max_pos, void *q_out, long long q_stride,
+                          void *stream);
+
+/* h4b_paged_attention of a tree's nodes: a node sees the tokens before the
+ * tree, its ancestors and itself; with window > 0 those of them at positions
+ * past its own - window, or below sinks. max_query is the largest tree to expect
+ * (it sets the tiles; a larger one is computed as well, only slower).
+ * Everything else, the workspace among it, is as there. */
+int h4b_paged_tree_attention(const h4b_paged_kv *kv, const int32_t *parents, const void *q, long long q_stride,
+                             int heads, float scale, int window, int sinks, int max_query, void *out,
+                             long long out_stride, float *lse, void *workspace, long long workspace_bytes, void *stream);
+
+/* The branch of each tree that agrees with the model. targets[row] is the token
+ * that the model chooses after a node: found here, as the first maximum of its
+ * logits (rows of `vocab` values, logits_stride apart, H4B_FP32, H4B_FP16 or
+ * H4B_BF16; a NaN counts as the largest), or given, where logits is null. Node 0 is
+ * the token that was decided before; each accepted node is followed by its first
+ * child whose token (tokens[row]) is its target, up to max_path nodes.
+ * path: int32 [sequences][max_path], the accepted nodes and then -1; counts
+ * [sequences]; next_tokens [sequences], the target of the last accepted node. A
+ * sequence without rows gets count 0 and token -1; offsets that do not ascend
+ * within the rows leave all sequences so (with logits) and set status bit 8.
+ * targets of rows that belong to no sequence are not written. workspace (with
+ * logits only): zeroed when it is created, left ready for the next call, 16-byte
+ * aligned; calls that may overlap on the GPU need workspaces of their own. */
+int h4b_tree_accept(const void *logits, int logits_dtype, long long logits_stride, int vocab, const int32_t *tokens,
+                    const int32_t *parents, const int32_t *q_offsets, int rows, int sequences, int max_path,
+                    int32_t *targets, int32_t *path, int32_t *counts, int32_t *next_tokens, void *workspace,
+                    long long workspace_bytes, void *stream);
+/* Workspace bytes of h4b_tree_accept for so many rows and sequences. */
+long long h4b_tree_accept_workspace_bytes(int rows, int sequences);
+
+/* Moves the accepted nodes' K and V behind the tokens before the tree: node
+ * path[b][i] to place i, i < counts[b], in every layer (kv.k_pages / v_pages are
+ * layer 0's, layer l's lie l * layer_bytes further). lengths[b] = the tokens
+ * before the tree + counts[b]; it may overlap neither kv_lens nor counts. A path
+ * that does not ascend within the tree's nodes leaves its sequence as it was
+ * (lengths[b] = kv_lens[b]) and sets status bit 8. The places written must not
+ * be shared with other sequences. */
+int h4b_tree_keep(const h4b_paged_kv *kv, int layers, long long layer_bytes, const int32_t *path, int max_path,
+                  const int32_t *counts, int32_t *lengths, void *stream);
+
 /* One step of the model over a paged cache: sequence b of kv feeds its rows
  * of `tokens` (a prompt's chunk, one decoded token, none), which are appended
  * and attended in every layer; the reference runs one token of one sequence
@@ -549,6 +607,20 @@ typedef struct h4b_paged_step {
     long long workspace_bytes;
 } h4b_paged_step;
 int h4b_forward_paged(const h4b_model *model, const h4b_paged_step *step, void *stream);
+
+/* Residual addition, RMSNorm and int8 rows in one call, the input of
+ * h4b_int4_gemm: s = x + delta, y = (s / sqrt(mean(s^2) + eps)) * weight,
+ * x8 = clamp(rint(y * 127/m), -127, 127) with m = max(absmax(y), 1e-5), scales = m / 127,
+ * sums = the row's sum of x8 (cpu_lightspark.py:431-433, :445; kernel.add_inplace,
+ * kernel.rmsnorm_into and kernel.quantize_activation of the reference, for rows).
+ * x and delta are H4B_FP32, H4B_FP16 or H4B_BF16, rows x_stride / delta_stride values
+ * apart; s is formed in fp32 and goes, rounded to x's type, to out (which may be
+ * x). delta may be null: out is not used then. x8 [rows][width]. fp32 rows have the bits of
+ * h4b_rmsnorm and h4b_quantize_rows. width and strides are multiples of 8,
+ * pointers 16-byte aligned (x8 8-byte). */
+int h4b_rmsnorm_quantize_rows(const void *x, int x_dtype, long long x_stride, const void *delta, int delta_dtype,
+                              long long delta_stride, void *out, long long out_stride, const float *weight, float eps,
+                              int8_t *x8, float *scales, int32_t *sums, int rows, int width, void *stream);
 
 /* ---- format producer: LATTICE checkpoint -> packed int4 cache ------------- */
 
