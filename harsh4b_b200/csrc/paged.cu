@@ -339,7 +339,7 @@ struct AttendArgs {
     float* partials;          // [2 * CTAs][ROWS * (D + 2)]: a CTA's first and last item
     unsigned int* counters;   // [CTAs], zero between calls (few-row kernel)
     int4* entries;            // [CTAs] the item that begins last in each (chunk kernel)
-    int half_tokens;          // new tokens of each of an item's two tiles (chunk kernel)
+    int half_tokens;          // new tokens of each of an item's two tiles (chunk kernel), or of its one (tree kernel)
     const int32_t* parents;   // of a tree's nodes (TREE)
 };
 
@@ -1125,6 +1125,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) paged_attention_few_kernel(con
 }  // namespace h4b
 
 #include "paged_tc.cu"
+#include "paged_tree.cu"
 
 namespace h4b {
 
@@ -1214,15 +1215,14 @@ static int launch_few_rows(const AttendArgs& a, int rows, int sms, cudaStream_t 
     return launch_few<T, D, 16, TREE>(a, sms, stream);
 }
 
-// A tile holds a token's whole group, so a group of more than 16 takes the 32
-// rows, also at head_dim 128 (where they spill).
 template <typename T, int D>
 static int launch_tree(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     a.fewest = 1;
     a.most = INT_MAX;
+    constexpr int kMost = D == 64 ? 32 : 16;
     const long long rows = static_cast<long long>(max_query) * a.group;
-    if (a.group > 16) return launch_few<T, D, 32, true>(a, sms, stream);
-    return launch_few_rows<T, D, true>(a, static_cast<int>(rows < 32 ? rows : 32), sms, stream);
+    if (rows > kMost) return launch_tree_tiles<T, D>(a, kv, max_query, sms, stream);
+    return launch_few_rows<T, D, true>(a, static_cast<int>(rows), sms, stream);
 }
 
 template <typename T, int D>

@@ -929,15 +929,15 @@ static bool paged_kv_map(CUtensorMap* out, const void* base, const h4b_paged_kv*
 }
 
 // The q rows [tokens][heads][D] with boxes of 64 values x group heads x
-// 128 / group tokens: a tile's rows in their order.
-static bool paged_q_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv, int heads, int group,
+// box_tokens tokens: a tile's rows in their order.
+static bool paged_q_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv, int heads, int group, int box_tokens,
                         long long q_stride) {
     auto encode = tensor_map_encoder();
     if (!encode) return false;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kv->head_dim), static_cast<cuuint64_t>(heads),
                                 static_cast<cuuint64_t>(kv->tokens)};
     const cuuint64_t strides[2] = {kv->head_dim * 2ull, static_cast<cuuint64_t>(q_stride) * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(kChunkRows / group)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(group), static_cast<cuuint32_t>(box_tokens)};
     const cuuint32_t elem[3] = {1, 1, 1};
     return encode(out, kv->dtype == H4B_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                   const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -959,7 +959,7 @@ static int launch_chunk(AttendArgs a, const h4b_paged_kv* kv, int sms, cudaStrea
         opted_in[dev].store(true, std::memory_order_release);
     }
     CUtensorMap qmap, kmap, vmap;
-    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.q_stride) || !paged_kv_map(&kmap, a.k_pages, kv) ||
+    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, kChunkRows / a.group, a.q_stride) || !paged_kv_map(&kmap, a.k_pages, kv) ||
         !paged_kv_map(&vmap, a.v_pages, kv))
         return H4B_EUNSUPPORTED;
     a.half_tokens = kChunkRows / a.group;

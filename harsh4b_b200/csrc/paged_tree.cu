@@ -1,0 +1,707 @@
+// Paged attention of drafted trees of more than a few rows on the 5th-generation
+// tensor cores: tcgen05.mma kind::f16, fp32 accumulators in tensor memory, pages
+// fetched by TMA. The split of the work over the CTAs is that of paged.cu, the
+// layout of the tiles and the operands' descriptors are those of paged_tc.cu.
+//
+// An item is (sequence, up to 128 query rows = nodes x q heads of a kv head, kv
+// head). Its keys are read once for few products each, so HBM is the bound, and
+// what has to hide under the loads is one tile's chain S -> softmax -> P V. So
+// two warpgroups take the item's blocks of 128 keys in turn, block n the one
+// with the number n % 2, each with scores, maximum, sum and output accumulator of
+// its own; they are joined at the item's end, from tensor memory.
+//
+// Warps: 0-3 and 4-7 are the softmax (thread = query row, TMEM lane = thread of
+// its warpgroup), 8 issues the loads, 9 the MMAs, 10 cleans V tiles. For block n,
+// x = n % 2:
+//   MMA:     S_x = Q K_n^T                      -> s_full[x]
+//   softmax: S_x to registers, p; P_x over S_x  -> p_full[x]
+//   MMA:     S of block n + 1, then O_x += P_x V_n
+// S_x of block n + 2 is issued after P V of block n, which reads P_x; the tensor
+// cores run a CTA's MMAs in issue order, and a commit tracks every earlier MMA, so
+// s_full of block n + 2 says that O_x is at rest too and may be rescaled.
+//
+// A node sees the tokens before the tree and, of the tree, the nodes whose bits
+// its walk to the root set (sight); blocks that hold only keys that every row
+// sees need no mask. The scores are taken in their own unit: p = 2^((s - m) scale
+// + 8) with m a score, so equal scores cancel exactly whatever their size; m moves
+// only where a score passes it by 2^7. p is rounded to the cache's type for the
+// product as in the other kernels (see paged.cu), l is its fp32 sum.
+//
+// V rows of keys that no row sees are zeroed and values that are not finite are
+// taken out of rows that only some see, and added at the item's end, as in
+// paged_tc.cu.
+//
+// Every wait is bounded (mbar_wait). A role whose wait runs out marks the CTA as
+// failed and stops; the load warp waits for the copies it issued, the MMA warp
+// commits a last barrier, and the tensor memory is freed on every path.
+
+namespace h4b {
+
+constexpr int kTreeLoadWarp = 8, kTreeMmaWarp = 9, kTreeCleanWarp = 10, kTreeThreads = 352;
+constexpr int kTreeLeast = 2, kTreeExtra = 2;  // as kChunkLeast and kChunkExtra
+
+template <int D>
+struct TreeCfg {
+    using C = ChunkCfg<D>;
+    static constexpr int kSlabs = C::kSlabs, kSlab = C::kSlab, kGroup = C::kGroup, kTile = C::kTile;
+    static constexpr int kStages = D == 128 ? 5 : 10;
+    static constexpr int kQOff = 0, kRingOff = kTile, kBarOff = kRingOff + kStages * kTile;
+    static constexpr int kBars = 3 * kStages + 10;
+    static constexpr int kFlagOff = kBarOff + kBars * 8 + 16;
+    static constexpr int kRangeOff = kFlagOff + (kStages + 1) / 2 * 8;
+    static constexpr int kStatOff = (kRangeOff + static_cast<int>(sizeof(Range)) + 15) / 16 * 16;  // [2][2][128] (m, l)
+    static constexpr int kSightOff = kStatOff + 2 * 2 * kChunkRows * 8;                            // [128][kTreeWords]
+    static constexpr int kPositionOff = kSightOff + kChunkRows * kTreeWords * 4;
+    static constexpr int kParentOff = kPositionOff + kChunkRows * 4;                               // int16 [kTreeNodes]
+    static constexpr int kSmem = kParentOff + kTreeNodes * 2 + 1024;
+    static constexpr uint32_t kSCol = 0, kOCol = 256;  // S_x at 128 x, O_x at 256 + 128 x
+    static_assert(kSmem <= 232448, "shared memory per CTA");
+};
+
+// Whether every row of the tile sees keys `key` .. `end`.
+__device__ __forceinline__ bool tree_all_see(const Tile& t, int window, int sinks, int key, int end) {
+    return end < t.p0 && (window <= 0 || key > t.p1 - window || end < sinks);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTreeThreads, 1)
+    paged_attention_tree_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                                const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttendArgs a) {
+    using C = TreeCfg<D>;
+    using TreeWalk = Walk<kChunkKeys, true>;
+    extern __shared__ uint8_t tree_smem_raw[];
+    uint8_t* smem = tree_smem_raw + ((1024u - (smem_addr(tree_smem_raw) & 1023u)) & 1023u);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* raw = empty + C::kStages;  // a V tile on its way to the cleaning warp
+    uint64_t* q_full = raw + C::kStages;
+    uint64_t* q_empty = q_full + 1;
+    uint64_t* s_full = q_empty + 1;  // [2]
+    uint64_t* p_full = s_full + 2;   // [2]
+    uint64_t* o_full = p_full + 2;
+    uint64_t* o_free = o_full + 1;
+    uint64_t* meet = o_free + 1;     // of the softmax warps
+    uint64_t* mma_done = meet + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+    volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* wild = failed + 1;  // values that are not finite were taken out of a V tile
+    volatile uint32_t* flags = reinterpret_cast<volatile uint32_t*>(smem + C::kFlagOff);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tile_tokens = a.half_tokens;
+    Range* shared_range = reinterpret_cast<Range*>(smem + C::kRangeOff);
+    {
+        const Range r = find_range<kTreeThreads, kChunkKeys, true>(a, tile_tokens, smem);
+        if (threadIdx.x == 0) {
+            *shared_range = r;
+            a.entries[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        }
+        if (r.begin >= r.end) return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+            mbar_init(&raw[s], 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&s_full[x], 1);
+            mbar_init(&p_full[x], 4);
+        }
+        mbar_init(o_full, 1);
+        mbar_init(o_free, 8);
+        mbar_init(meet, 8);
+        mbar_init(mma_done, 1);
+        *failed = wait_failed_before() ? 1 : 0;
+        *wild = 0;
+        fence_mbar_init();
+    }
+    if (warp == kTreeMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_addr(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto ring = [&](uint32_t i) { return smem + C::kRingOff + (i % C::kStages) * C::kTile; };
+    auto phase_of = [&](uint32_t i) { return (i / C::kStages) & 1u; };
+
+    // K of the CTA's block n is tile 2 n of the ring, V tile 2 n + 1. A block's
+    // flags lie beside K's barrier, written before K's copies start.
+    if (warp == kTreeLoadWarp) {
+        TreeWalk w;
+        const int page_size = 1 << a.p.page_shift, box = min(page_size, kChunkKeys);  // a box: keys of one page
+        const int boxes = kChunkKeys / box;
+        const bool mine = lane < boxes;  // each lane one box
+        auto page_of = [&](const TreeWalk& u) -> int {  // -1: read as zeros
+            const int key = u.tile.block(u.unit) * kChunkKeys + lane * box;
+            const Tile& t = u.tile;
+            if (!mine || key > t.p1 || !(a.window <= 0 || key + box - 1 > t.p0 - a.window || key < a.sinks)) return -1;
+            const int page = a.p.table[static_cast<long long>(u.b) * a.p.table_stride + (key >> a.p.page_shift)];
+            if (page >= 0 && page < a.p.pages) return page;
+            report(kStatusBadPage);
+            return -1;
+        };
+        uint32_t issued = 0, raw_open = 0, raw_phase = 0;  // a bit per stage
+        bool ok = !*failed, more = w.start(a, *shared_range, tile_tokens);
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
+        }
+        if (!more && lane == 0) {
+            flags[0] = kStepNone;
+            mbar_arrive(&full[0]);
+        }
+        int page = more ? page_of(w) : -1, items = 0;
+        bool new_item = true;
+        while (ok && more) {
+            if (new_item) {  // the q rows, once the previous item's are no longer read
+                if (items > 0) ok = __all_sync(0xffffffffu, !*failed && mbar_wait(q_empty, (items - 1) & 1));
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(q_full, C::kSlabs * tile_tokens * a.group * 128);
+                __syncwarp();
+                if (lane < C::kSlabs)
+                    tma_load_3d(smem + C::kQOff + lane * C::kSlab, &qmap, lane * 64, w.h * a.group, w.tile.first, q_full);
+                ++items;
+            }
+            const int key = w.tile.block(w.unit) * kChunkKeys;
+            const int y = boxes > 1 ? 0 : key & (page_size - 1);
+            const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
+            const bool unclean = !tree_all_see(w.tile, a.window, a.sinks, key, key + kChunkKeys - 1);
+            uint32_t flag = (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u);
+            // the next block's page ids are on their way while this one's copies are issued
+            new_item = w.part_ends();
+            more = w.next(a, tile_tokens);
+            if (more) page = page_of(w);
+            if (!more) flag |= kStepFinal;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const uint32_t stage = issued % C::kStages;
+                if (issued >= C::kStages)
+                    ok = __all_sync(0xffffffffu, !*failed && mbar_wait(&empty[stage], phase_of(issued - C::kStages)));
+                if (!ok) break;
+                // a V tile with hidden keys goes through the cleaning warp
+                uint64_t* bar = v == 1 && unclean ? &raw[stage] : &full[stage];
+                if (lane == 0) {
+                    if (v == 0) flags[stage] = flag;
+                    mbar_arrive_expect_tx(bar, C::kTile);
+                }
+                __syncwarp();
+                if (mine) tma_load_tile(ring(issued) + lane * box * 2 * D, v ? &vmap : &kmap, y >> 3, z, bar);
+                if (v == 1 && unclean) raw_phase ^= 1u << stage, raw_open |= 1u << stage;
+                else raw_open &= ~(1u << stage);
+                ++issued;
+            }
+        }
+        if (!ok) *failed = 1;
+        // the copies issued must land before the CTA may exit
+        if (items > 0) mbar_wait(q_full, (items - 1) & 1);
+        for (uint32_t i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i) {
+            const uint32_t stage = i % C::kStages;
+            if ((raw_open >> stage) & 1u)
+                mbar_wait(&raw[stage], ((raw_phase >> stage) & 1u) ^ 1u);
+            else
+                mbar_wait(&full[stage], phase_of(i));
+        }
+        __syncwarp();
+    } else if (warp == kTreeCleanWarp) {
+        // V rows of keys that no row of the item sees: zeros; values that are
+        // not finite in rows of keys that only some rows see: out
+        TreeWalk w;
+        uint32_t n = 0, raw_phase = 0;
+        bool more = w.start(a, *shared_range, tile_tokens);
+        for (; more; more = w.next(a, tile_tokens), ++n) {
+            const int key = w.tile.block(w.unit) * kChunkKeys;
+            if (tree_all_see(w.tile, a.window, a.sinks, key, key + kChunkKeys - 1)) continue;
+            const uint32_t stage = (2 * n + 1) % C::kStages;
+            if (!__all_sync(0xffffffffu, !*failed && mbar_wait(&raw[stage], (raw_phase >> stage) & 1u))) {
+                *failed = 1;
+                break;
+            }
+            raw_phase ^= 1u << stage;
+            uint8_t* tile = ring(2 * n + 1);
+            // (eight lanes a row's 128 bytes: no two lanes in one bank)
+            auto at = [&](int r, int slab) {
+                return reinterpret_cast<uint4*>(tile + (r >> 3) * C::kGroup + slab * 1024 + (r & 7) * 128 + (lane & 7) * 16);
+            };
+            // Keys by intervals: no row sees those past the last node, nor those
+            // before the first position's window that are not first tokens; some rows
+            // see the tree's, and those that the window leaves from row to row.
+            const Tile& t = w.tile;
+            auto zero = [&](int from, int to) {
+                for (int r = max(from - key, 0) + (lane >> 3); r < min(to - key, kChunkKeys); r += 4)
+#pragma unroll
+                    for (int slab = 0; slab < C::kSlabs; ++slab) *at(r, slab) = make_uint4(0u, 0u, 0u, 0u);
+            };
+            uint32_t bad = 0;
+            auto search = [&](int from, int to) {
+                const int end = min(to - key, kChunkKeys);
+#pragma unroll 1
+                for (int r = max(from - key, 0) + (lane >> 3); r < end; r += 16) {
+                    uint4 v[4 * C::kSlabs];  // four rows' loads in flight (one past the end is its lane's first again)
+#pragma unroll
+                    for (int k = 0; k < 4 * C::kSlabs; ++k)
+                        v[k] = *at(r + 4 * (k / C::kSlabs) < end ? r + 4 * (k / C::kSlabs) : r, k % C::kSlabs);
+#pragma unroll
+                    for (int k = 0; k < 4 * C::kSlabs; ++k)
+                        bad |= not_finite<T>(v[k].x) | not_finite<T>(v[k].y) | not_finite<T>(v[k].z) | not_finite<T>(v[k].w);
+                }
+            };
+            zero(t.p1 + 1, INT_MAX);
+            search(t.p0, t.p1 + 1);
+            if (a.window > 0) {
+                zero(a.sinks, t.p0 - a.window + 1);
+                search(max(t.p0 - a.window + 1, a.sinks), t.p1 - a.window + 1);
+            }
+            if (__any_sync(0xffffffffu, bad != 0)) {
+#pragma unroll 1
+                for (int r = lane >> 3; r < kChunkKeys; r += 4) {
+                    if (tree_all_see(t, a.window, a.sinks, key + r, key + r)) continue;
+#pragma unroll
+                    for (int slab = 0; slab < C::kSlabs; ++slab) {
+                        uint4 v = *at(r, slab);
+                        v.x &= ~halves_of(not_finite<T>(v.x)), v.y &= ~halves_of(not_finite<T>(v.y));
+                        v.z &= ~halves_of(not_finite<T>(v.z)), v.w &= ~halves_of(not_finite<T>(v.w));
+                        *at(r, slab) = v;
+                    }
+                }
+                *wild = 1;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+        }
+        __syncwarp();
+    } else if (warp == kTreeMmaWarp) {
+        // The whole warp runs the loop on uniform values and one elected lane
+        // issues: the MMAs' operands then stay in uniform registers.
+        const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0) >> 4;
+        constexpr uint64_t common = (1ull << 46) | (2ull << 61);
+        constexpr uint64_t q_major = common | (1ull << 16) | (64ull << 32);
+        constexpr uint64_t k_major = common | (1ull << 16) | (static_cast<uint64_t>(C::kGroup >> 4) << 32);
+        constexpr uint64_t v_major = common | (64ull << 16) | (static_cast<uint64_t>(C::kGroup >> 4) << 32);
+        const uint64_t q_desc = q_major | (base + (C::kQOff >> 4));
+        const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t stage = 0, phase = 0;  // of the ring: K's, then V's
+        uint32_t q_items = 0, parts = 0, p_count0 = 0, p_count1 = 0, x = 0;
+        bool fresh0 = true, fresh1 = true, issued = false;  // O_x has nothing of this part; S of this block is issued
+        bool ok = !*failed && warp_wait(&full[0], 0);
+        uint32_t flag = ok ? flags[0] : 0u;
+        const bool none = (flag & kStepNone) != 0;
+        if (none) ok = false;
+        auto issue_s = [&](uint32_t which, uint32_t k_stage, uint32_t f) {  // K has landed
+            if (f & kStepFirst) {
+                if (!warp_wait(q_full, q_items++ & 1)) return false;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t bd = k_major | (base + ((C::kRingOff + k_stage * C::kTile) >> 4));
+                const uint32_t s_tmem = t0 + C::kSCol + 128 * which;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t in_slab = 2 * (kk & 3), slab = kk >> 2;  // 16 values: 32 bytes
+                    tc_mma_f16(s_tmem, q_desc + slab * (C::kSlab >> 4) + in_slab, bd + slab * 64 + in_slab,
+                               chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                }
+                tc_commit(&s_full[which]);
+                tc_commit(&empty[k_stage]);
+                if (f & kStepLast) tc_commit(q_empty);
+            }
+            __syncwarp();
+            return true;
+        };
+        while (ok) {  // K of this block has landed
+            const uint32_t k_stage = stage;
+            if (++stage == C::kStages) stage = 0, phase ^= 1u;
+            const uint32_t v_stage = stage, v_phase = phase;
+            if (++stage == C::kStages) stage = 0, phase ^= 1u;
+            if (!issued) ok = issue_s(x, k_stage, flag);
+            if (!ok) break;
+            // the next block's S, so that it runs while this one's softmax does
+            uint32_t next_flag = 0;
+            issued = false;
+            if (!(flag & (kStepLast | kStepFinal))) {
+                ok = warp_wait(&full[stage], phase);
+                if (!ok) break;
+                next_flag = flags[stage];
+                ok = issued = issue_s(x ^ 1, stage, next_flag);
+                if (!ok) break;
+            }
+            ok = warp_wait(&full[v_stage], v_phase);
+            if (ok && fresh0 && fresh1 && parts > 0) ok = warp_wait(o_free, (parts - 1) & 1);
+            const uint32_t count = x ? p_count1 : p_count0;
+            ok = ok && warp_wait(&p_full[x], count & 1);
+            if (!ok) break;
+            tc_fence_after();
+            const bool first = x ? fresh1 : fresh0;
+            if (elect_one()) {
+                const uint64_t bd = v_major | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
+                const uint32_t s_tmem = t0 + C::kSCol + 128 * x, o_tmem = t0 + C::kOCol + 128 * x;
+#pragma unroll
+                for (int kk = 0; kk < kChunkKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                    tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * (C::kGroup >> 3), chunk_idesc<T>(D, true),
+                                  !first || kk != 0);
+                tc_commit(&empty[v_stage]);
+                if (flag & kStepLast) tc_commit(o_full);
+            }
+            __syncwarp();
+            if (x) fresh1 = false, ++p_count1;
+            else fresh0 = false, ++p_count0;
+            if (flag & kStepLast) fresh0 = fresh1 = true, ++parts;
+            if (flag & kStepFinal) break;
+            if (!issued) {
+                ok = warp_wait(&full[stage], phase);
+                if (!ok) break;
+                next_flag = flags[stage];
+            }
+            flag = next_flag;
+            x ^= 1;
+        }
+        if (!ok && !none) *failed = 1;
+        if (elect_one()) tc_commit(mma_done);  // arrives once every MMA issued above has completed
+        __syncwarp();
+    } else {
+        TreeWalk w;
+        bool more = w.start(a, *shared_range, tile_tokens);
+        const int x = warp >> 2, row = threadIdx.x & 127, quarter = warp & 3;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+        const uint32_t s_col = lane_base + C::kSCol + 128 * x, o_col = lane_base + C::kOCol;
+        const int node = row / a.group, head = row - node * a.group;
+        float2* stats = reinterpret_cast<float2*>(smem + C::kStatOff);
+        uint32_t* sights = reinterpret_cast<uint32_t*>(smem + C::kSightOff);
+        int* positions = reinterpret_cast<int*>(smem + C::kPositionOff);
+        int16_t* parent = reinterpret_cast<int16_t*>(smem + C::kParentOff);
+        const uint32_t* sight = sights + node * kTreeWords;  // this row's
+        bool ok = !*failed;
+        bool begun = w.unit == 0;  // the item's first unit is in this range
+        uint32_t n = 0, s_count = 0, parts = 0, meets = 0;
+        int sight_b = -1, sight_t = 0;
+        auto meet_all = [&]() {  // of the eight softmax warps
+            __syncwarp();
+            if (lane == 0) mbar_arrive(meet);
+            return warp_wait(meet, meets++ & 1);
+        };
+        while (ok && more) {
+            const Tile tile = w.tile;
+            const int base = tile.p0;
+            if (w.b != sight_b || w.t != sight_t) {  // what the tile's nodes see (the same for every kv head)
+                sight_b = w.b, sight_t = w.t;
+                ok = meet_all();  // no one reads the last one's any more
+                if (!ok) break;
+                const bool some = w.span.base >= 0;  // else the sequence counts as empty
+                if (some && static_cast<int>(threadIdx.x) < w.span.count)
+                    parent[threadIdx.x] = static_cast<int16_t>(checked_parent(a.parents[w.span.first + threadIdx.x], threadIdx.x));
+                ok = meet_all();
+                if (!ok) break;
+                if (static_cast<int>(threadIdx.x) < tile.tokens) {
+                    const int i = threadIdx.x, me = tile.first - w.span.first + i;
+                    uint32_t* bits = sights + i * kTreeWords;
+#pragma unroll
+                    for (int k = 0; k < kTreeWords; ++k) bits[k] = 0u;
+                    int depth = -1;
+                    if (some)
+                        for (int j = me; j >= 0; j = parent[j]) ++depth;
+                    positions[i] = some ? base + depth : -1;
+                    if (some) {
+                        int up = 0;
+                        for (int j = me; j >= 0; j = parent[j], ++up)
+                            if (a.window <= 0 || up < a.window || base + depth - up < a.sinks) bits[j >> 5] |= 1u << (j & 31);
+                    }
+                }
+                ok = meet_all();
+                if (!ok) break;
+            }
+            const bool valid = node < tile.tokens;
+            const bool live = 32 * quarter < tile.tokens * a.group;  // of the warp: it has rows
+            const int pos = valid ? positions[node] : -1;
+            // Bits of the keys first .. first + 31 that the row sees.
+            auto seen_bits = [&](int first) -> uint32_t {
+                if (pos < 0) return 0u;
+                uint32_t earlier = bits_below(base - first);
+                if (a.window > 0) earlier &= ~bits_below(pos - a.window - first + 1) | bits_below(a.sinks - first);
+                const int off = first - base;  // in the tree
+                if (off <= -32 || off >= kTreeNodes) return earlier;
+                if (off < 0) return earlier | (sight[0] << -off);
+                const uint32_t low = sight[off >> 5], high = (off >> 5) + 1 < kTreeWords ? sight[(off >> 5) + 1] : 0u;
+                return earlier | __funnelshift_r(low, high, off & 31);
+            };
+            float m = -INFINITY, l = 0.f;
+            bool done = false;
+            while (true) {
+                if ((n & 1) == static_cast<uint32_t>(x)) {
+                    ok = warp_wait(&s_full[x], s_count & 1);
+                    if (!ok) break;
+                    ++s_count;
+                    tc_fence_after();
+                    if (live) {
+                        const int key = tile.block(w.unit) * kChunkKeys;
+                        const bool masked = !tree_all_see(tile, a.window, a.sinks, key, key + kChunkKeys - 1);
+                        uint32_t seen[4];
+                        if (masked) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) seen[k] = seen_bits(key + 32 * k);
+                        }
+                        auto mask = [&](float (&v)[32], uint32_t bits) {
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[k] = (bits >> k) & 1u ? v[k] : -INFINITY;
+                        };
+                        // the maximum first, then the weights: the scores are read twice, which keeps them out of the registers
+                        float v[32], mx = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            tmem_ld16_nowait(s_col + 32 * k, v, 0);
+                            tmem_ld16_nowait(s_col + 32 * k + 16, v, 16);
+                            tmem_wait_regs(v);
+                            if (masked) mask(v, seen[k]);
+                            float top[2] = {v[0], v[1]};
+#pragma unroll
+                            for (int e = 2; e < 30; e += 4) {
+                                top[0] = fmaxf(fmaxf(top[0], v[e]), v[e + 1]);
+                                top[1] = fmaxf(fmaxf(top[1], v[e + 2]), v[e + 3]);
+                            }
+                            mx = fmaxf(fmaxf(mx, fmaxf(top[0], top[1])), fmaxf(v[30], v[31]));
+                        }
+                        const bool move = valid && (mx - m) * a.scale > 7.f;
+                        if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
+                            const float f = move ? ex2_approx((m - mx) * a.scale) : 1.f;  // 0 for m = -inf, whose l and O are 0
+                            l *= f;
+                            rescale_row<D>(o_col + 128 * x, f);
+                        }
+                        if (move) m = mx;
+                        const float less = m == -INFINITY ? 0.f : -m;
+                        const uint64_t less2 = pack2(less, less), scale2 = pack2(a.scale, a.scale), eight2 = pack2(8.f, 8.f);
+                        uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            tmem_ld16_nowait(s_col + 32 * k, v, 0);
+                            tmem_ld16_nowait(s_col + 32 * k + 16, v, 16);
+                            tmem_wait_regs(v);
+                            if (masked) mask(v, seen[k]);
+                            uint32_t p16[16];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const uint64_t p2 = exp2_pair(fma2(add2(pack2(v[e], v[e + 1]), less2), scale2, eight2));
+                                sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], p2);
+                                const float2 p = unpack2(p2);
+                                p16[e / 2] = Pair<T>::pack(p.x, p.y);
+                            }
+                            tmem_st16u(s_col + 16 * k, p16, 0);  // (over scores that are read already)
+                        }
+                        const float2 sums = unpack2(add2(sum[0], sum[1]));
+                        l += sums.x + sums.y;
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[x]);
+                }
+                ++n;
+                done = w.item_ends();
+                if (w.part_ends()) break;
+                w.next(a, tile_tokens);
+            }
+            if (!ok) break;
+
+            // ---- the two warpgroups' sums joined: each half of the columns ------------
+            float2* stat = stats + (parts & 1) * 2 * kChunkRows;
+            stat[x * kChunkRows + row] = make_float2(m, l);
+            ok = meet_all() && warp_wait(o_full, parts & 1);
+            if (!ok) break;
+            ++parts;
+            tc_fence_after();
+            const float2 s0 = stat[row], s1 = stat[kChunkRows + row];
+            const float top = fmaxf(s0.x, s1.x);
+            // (a side that saw no key has l = 0, and an accumulator that may hold anything)
+            const bool some0 = s0.y != 0.f, some1 = s1.y != 0.f;
+            float f0 = some0 ? ex2_approx((s0.x - top) * a.scale) : 0.f, f1 = some1 ? ex2_approx((s1.x - top) * a.scale) : 0.f;
+            const float total = s0.y * f0 + s1.y * f1;
+            const bool whole = begun && done;
+            if (whole) {
+                const float inv = total != 0.f ? 1.0f / total : 0.f;
+                f0 *= inv, f1 *= inv;
+            }
+            constexpr int kPart = kChunkRows * (D + 2);
+            // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
+            float4* part = reinterpret_cast<float4*>(a.partials + static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * kPart);
+            if (live) {
+                T* out_tile = static_cast<T*>(a.out) + tile.first * a.out_stride + w.h * a.group * D;
+                const long long my_place = valid ? node * a.out_stride + head * D : -1;
+                long long to[4];  // the places of the quad's four rows
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[k] = __shfl_sync(0xffffffffu, my_place, (lane & 28) + k);
+                // Columns c .. c + 31 of the values that the cleaning warp took out of
+                // the blocks of this part, from the pages, where the row sees their key.
+                auto add_wild = [&](float (&v)[32], int c) {
+                    const Range& r = *shared_range;
+                    const long long first = r.end - w.left - w.unit;  // place of the item's unit 0
+                    for (int u = static_cast<int>(max(r.begin - first, 0ll)); u <= w.unit; ++u) {
+                        const int block = tile.block(u) * kChunkKeys;
+                        for (int j = block; j < block + kChunkKeys; ++j) {
+                            if (!tile_sees(tile, a.window, a.sinks, j) || tree_all_see(tile, a.window, a.sinks, j, j)) continue;
+                            const int page = a.p.table[static_cast<long long>(w.b) * a.p.table_stride + (j >> a.p.page_shift)];
+                            if (page < 0 || page >= a.p.pages) continue;
+                            const long long at = ((static_cast<long long>(page) * a.p.kv_heads + w.h) << a.p.page_shift) +
+                                                 (j & ((1 << a.p.page_shift) - 1));
+                            const uint32_t* words = reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v_pages) + at * D + c);
+                            const bool sees = (seen_bits(j) & 1u) != 0u;
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                const uint32_t word = __ldg(words + k), which = not_finite<T>(word);
+                                if (which == 0 || !sees) continue;
+                                const float2 y = Pair<T>::unpack(word & halves_of(which));
+                                v[2 * k] += y.x, v[2 * k + 1] += y.y;
+                            }
+                        }
+                    }
+                };
+                const bool any_wild = __any_sync(0xffffffffu, *wild != 0);
+#pragma unroll 1
+                for (int c = x * (D / 2); c < (x + 1) * (D / 2); c += 32) {
+                    float v[32], u[32];
+                    tmem_ld16_nowait(o_col + c, v, 0);
+                    tmem_ld16_nowait(o_col + c + 16, v, 16);
+                    tmem_ld16_nowait(o_col + 128 + c, u, 0);
+                    tmem_ld16_nowait(o_col + 128 + c + 16, u, 16);
+                    tmem_wait_regs(v);
+                    tmem_wait_regs(u);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = (some0 ? v[k] * f0 : 0.f) + (some1 ? u[k] * f1 : 0.f);
+                    if (any_wild) {
+                        add_wild(v, c);
+                        __syncwarp();
+                    }
+                    if (whole) {
+                        uint32_t o16[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o16[k] = Pair<T>::pack(v[2 * k], v[2 * k + 1]);
+                        quad_transpose(o16);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (to[k] >= 0)
+                                *reinterpret_cast<uint4*>(out_tile + to[k] + c + 8 * (lane & 3)) =
+                                    make_uint4(o16[4 * k], o16[4 * k + 1], o16[4 * k + 2], o16[4 * k + 3]);
+                    } else if (valid) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            __stcg(part + ((c + k) / 4) * kChunkRows + row, make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free);
+            if (x == 0) {
+                if (whole) {
+                    if (valid && a.lse != nullptr)
+                        a.lse[static_cast<long long>(tile.first + node) * a.heads + w.h * a.group + head] =
+                            total == 0.f ? -INFINITY : (top * a.scale - 8.f) * 0.6931471805599453f + logf(total);
+                } else {
+                    if (valid) __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(top, total));
+                    if (threadIdx.x == 0 && begun)  // the item's first part: what the join needs to know
+                        a.entries[blockIdx.x] = make_int4(item_owners(*shared_range, w).y, tile.first, tile.tokens, w.h);
+                }
+            }
+            more = w.next(a, tile_tokens);
+            begun = true;
+        }
+        if (!ok) *failed = 1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kTreeMmaWarp) {
+        // the MMAs must be complete before their tensor memory is released
+        mbar_wait(mma_done, 0);
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Joins the parts of the items that lie across CTAs, as paged_join_kernel does:
+// block (c, slice) rows 16 slice .. of the item that begins last in CTA c, in the
+// order of the CTAs. Maxima are scores, in their own unit.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const AttendArgs a) {
+    constexpr int kPart = kChunkRows * (D + 2), kCols = D / 8 / 4;  // float4s a thread
+    pdl_wait();
+    const int4 entry = a.entries[blockIdx.x];
+    const int c0 = blockIdx.x, c1 = entry.x;
+    if (c1 < 0) return;
+    const int row = blockIdx.y * kJoinRows + (threadIdx.x % kJoinRows);
+    const int node = row / a.group, head = row - node * a.group;
+    if (node >= entry.z) return;
+    const int c = (threadIdx.x / kJoinRows) * kCols;
+    auto part_of = [&](int cta) { return a.partials + static_cast<long long>(2 * cta + (cta == c0)) * kPart; };
+    auto stat = [&](int cta) { return __ldcg(reinterpret_cast<const float2*>(part_of(cta) + D * kChunkRows) + row); };
+    float most = -INFINITY, total = 0.f;
+#pragma unroll 4
+    for (int cta = c0; cta <= c1; ++cta) most = fmaxf(most, stat(cta).x);
+    float4 v[kCols];
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int cta = c0; cta <= c1; ++cta) {
+        const float2 ml = stat(cta);  // l = 0: saw no key
+        const float f = ml.y == 0.f ? 0.f : ex2_approx((ml.x - most) * a.scale);
+        total += ml.y * f;
+        const float4* o = reinterpret_cast<const float4*>(part_of(cta));
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) {
+            const float4 y = __ldcg(o + (c + k) * kChunkRows + row);
+            v[k].x += y.x * f, v[k].y += y.y * f, v[k].z += y.z * f, v[k].w += y.w * f;
+        }
+    }
+    const float scale = total != 0.f ? 1.0f / total : 0.f;
+    const long long out_row = entry.y + node;
+    const int out_head = entry.w * a.group + head;
+    T* out = static_cast<T*>(a.out) + out_row * a.out_stride + out_head * D + 4 * c;
+#pragma unroll
+    for (int k = 0; k < kCols; k += 2)
+        *reinterpret_cast<uint4*>(out + 4 * k) =
+            make_uint4(Pair<T>::pack(v[k].x * scale, v[k].y * scale), Pair<T>::pack(v[k].z * scale, v[k].w * scale),
+                       Pair<T>::pack(v[k + 1].x * scale, v[k + 1].y * scale),
+                       Pair<T>::pack(v[k + 1].z * scale, v[k + 1].w * scale));
+    if (a.lse != nullptr && c == 0)
+        a.lse[out_row * a.heads + out_head] =
+            total == 0.f ? -INFINITY : (most * a.scale - 8.f) * 0.6931471805599453f + logf(total);
+}
+
+template <typename T, int D>
+static int launch_tree_tiles(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
+    using C = TreeCfg<D>;
+    a.extra = kTreeExtra;
+    a.least = kTreeLeast;
+    a.half_tokens = std::min(kChunkRows / a.group, max_query);  // of a tile
+    static std::atomic<bool> opted_in[kMaxDevices];
+    int dev = 0;
+    H4B_CUDA_TRY(cudaGetDevice(&dev));
+    if (!opted_in[dev].load(std::memory_order_acquire)) {
+        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_tree_kernel<T, D>,
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        opted_in[dev].store(true, std::memory_order_release);
+    }
+    CUtensorMap qmap, kmap, vmap;
+    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.half_tokens, a.q_stride) || !paged_kv_map(&kmap, a.k_pages, kv) ||
+        !paged_kv_map(&vmap, a.v_pages, kv))
+        return H4B_EUNSUPPORTED;
+    paged_attention_tree_kernel<T, D><<<sms, kTreeThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
+    H4B_CUDA_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sms, (a.half_tokens * a.group + kJoinRows - 1) / kJoinRows);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // it waits in the kernel
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    H4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a));
+    return 0;
+}
+
+}  // namespace h4b
