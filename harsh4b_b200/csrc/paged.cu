@@ -1172,7 +1172,7 @@ static int paged_sm_count(int* sms) {
 // The few-row kernel's CTAs an SM and largest tile; as many q heads may share a
 // kv head (a token's group stays in one tile of either kernel).
 constexpr int kFewCtasPerSm = 2, kFewMaxRows = 32;
-constexpr long long kCounterBytes = 4096, kEntryBytes = 4096;
+constexpr long long kCounterBytes = 4096, kEntryBytes = 8192;
 
 template <typename S, typename T, int D, bool TREE>
 static int launch_append(AppendArgs a, cudaStream_t stream) {
@@ -1344,7 +1344,8 @@ extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
     // two parts a CTA: an SM's rows of the few-row kernel are fewer than
     // the 256 of the chunk kernel's CTA
     static_assert(kFewCtasPerSm * kFewMaxRows <= 2 * kChunkRows, "the chunk kernel's parts are the larger");
-    if (kFewCtasPerSm * sms * 4 > kCounterBytes || sms * 16 > kEntryBytes) return H4B_EUNSUPPORTED;
+    static_assert(kTreeCtasPerSm * kChunkRows <= 2 * kChunkRows, "and than the tree kernel's");
+    if (kFewCtasPerSm * sms * 4 > kCounterBytes || kTreeCtasPerSm * sms * 16 > kEntryBytes) return H4B_EUNSUPPORTED;
     return kCounterBytes + kEntryBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
 }
 

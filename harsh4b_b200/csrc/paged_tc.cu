@@ -911,12 +911,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendAr
 }
 
 // A layer's pages [pages * kv_heads][page_size][D] as a 5-D tensor map (value,
-// row of its group of 8, slab of 64 values, group, page and head).
-static bool paged_kv_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv) {
+// row of its group of 8, slab of 64 values, group, page and head), with boxes of
+// one page's part of a tile of `keys`.
+static bool paged_kv_map(CUtensorMap* out, const void* base, const h4b_paged_kv* kv, int keys = kChunkKeys) {
     auto encode = tensor_map_encoder();
     if (!encode) return false;
     const cuuint64_t row = kv->head_dim * 2ull;
-    const cuuint32_t slabs = kv->head_dim / 64, box_rows = kv->page_size < kChunkKeys ? kv->page_size : kChunkKeys;
+    const cuuint32_t slabs = kv->head_dim / 64, box_rows = kv->page_size < keys ? kv->page_size : keys;
     const cuuint64_t dims[5] = {64, 8, slabs, static_cast<cuuint64_t>(kv->page_size) / 8,
                                 static_cast<cuuint64_t>(kv->pages) * kv->kv_heads};
     const cuuint64_t strides[4] = {row, 128, 8 * row, kv->page_size * row};

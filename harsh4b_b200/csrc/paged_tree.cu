@@ -5,20 +5,20 @@
 //
 // An item is (sequence, up to 128 query rows = nodes x q heads of a kv head, kv
 // head). Its keys are read once for few products each, so HBM is the bound, and
-// what has to hide under the loads is one tile's chain S -> softmax -> P V. So
-// two warpgroups take the item's blocks of 128 keys in turn, block n the one
-// with the number n % 2, each with scores, maximum, sum and output accumulator of
-// its own; they are joined at the item's end, from tensor memory.
+// what has to hide under the loads is the chain S -> softmax -> P V of a block of
+// 64 keys, and an item's start and end. So two CTAs share an SM, each with half of
+// its tensor memory and shared memory: what one waits for the other fills. (One
+// CTA with two warpgroups that took an item's blocks of 128 keys in turn: 64 trees
+// of 16 nodes over ragged 2100 tokens 100 us, now 71; 16 x 32 nodes over 32768
+// 386, now 375; over 16-token pages 570, now 402.)
 //
-// Warps: 0-3 and 4-7 are the softmax (thread = query row, TMEM lane = thread of
-// its warpgroup), 8 issues the loads, 9 the MMAs, 10 cleans V tiles. For block n,
-// x = n % 2:
+// Warps: 0-3 are the softmax (thread = query row = TMEM lane), 4 issues the loads,
+// 5 the MMAs, 6 cleans V tiles. For block n, x = n % 2:
 //   MMA:     S_x = Q K_n^T                      -> s_full[x]
 //   softmax: S_x to registers, p; P_x over S_x  -> p_full[x]
-//   MMA:     S of block n + 1, then O_x += P_x V_n
-// S_x of block n + 2 is issued after P V of block n, which reads P_x; the tensor
-// cores run a CTA's MMAs in issue order, and a commit tracks every earlier MMA, so
-// s_full of block n + 2 says that O_x is at rest too and may be rescaled.
+//   MMA:     S of block n + 1, then O += P_x V_n, whichever's operands come first
+// S_x of block n + 2 is issued after P V of block n, which reads P_x: the tensor
+// cores run a CTA's MMAs in issue order.
 //
 // A node sees the tokens before the tree and, of the tree, the nodes whose bits
 // its walk to the root set (sight); blocks that hold only keys that every row
@@ -31,44 +31,62 @@
 // taken out of rows that only some see, and added at the item's end, as in
 // paged_tc.cu.
 //
-// Every wait is bounded (mbar_wait). A role whose wait runs out marks the CTA as
-// failed and stops; the load warp waits for the copies it issued, the MMA warp
-// commits a last barrier, and the tensor memory is freed on every path.
+// Every wait is bounded (mbar_wait, or a loop with its limit). A role whose wait
+// runs out marks the CTA as failed and stops; the load warp waits for the copies
+// it issued, the MMA warp commits a last barrier, and the tensor memory is freed
+// on every path.
 
 namespace h4b {
 
-constexpr int kTreeLoadWarp = 8, kTreeMmaWarp = 9, kTreeCleanWarp = 10, kTreeThreads = 352;
-constexpr int kTreeLeast = 2, kTreeExtra = 2;  // as kChunkLeast and kChunkExtra
+constexpr int kTreeKeys = 64;
+constexpr int kTreeLoadWarp = 4, kTreeMmaWarp = 5, kTreeCleanWarp = 6, kTreeThreads = 224, kTreeCtasPerSm = 2;
+constexpr int kTreeLeast = 2, kTreeExtra = 4;  // as kChunkLeast and kChunkExtra, of 64 keys
 
-template <int D>
+// ROWS: query rows of a tile that there is room for; the MMAs take 128 all the same,
+// and what they make of the others' lanes goes nowhere.
+template <int D, int ROWS>
 struct TreeCfg {
-    using C = ChunkCfg<D>;
-    static constexpr int kSlabs = C::kSlabs, kSlab = C::kSlab, kGroup = C::kGroup, kTile = C::kTile;
-    static constexpr int kStages = D == 128 ? 5 : 10;
-    static constexpr int kQOff = 0, kRingOff = kTile, kBarOff = kRingOff + kStages * kTile;
-    static constexpr int kBars = 3 * kStages + 10;
+    static constexpr int kSlabs = D / 64;                        // 64 values of head_dim each
+    static constexpr int kSlab = ROWS * 128;                     // of Q
+    static constexpr int kGroup = kSlabs * 1024;                 // of K or V: 8 keys, all slabs
+    static constexpr int kTile = kTreeKeys / 8 * kGroup;
+    static constexpr int kStages = (ROWS == 128 ? 4 : ROWS == 64 ? 5 : 6) * (128 / D);
+    static constexpr int kQOff = 0, kRingOff = kSlabs * kSlab, kBarOff = kRingOff + kStages * kTile;
+    static constexpr int kBars = 3 * kStages + 11;
     static constexpr int kFlagOff = kBarOff + kBars * 8 + 16;
     static constexpr int kRangeOff = kFlagOff + (kStages + 1) / 2 * 8;
-    static constexpr int kStatOff = (kRangeOff + static_cast<int>(sizeof(Range)) + 15) / 16 * 16;  // [2][2][128] (m, l)
-    static constexpr int kSightOff = kStatOff + 2 * 2 * kChunkRows * 8;                            // [128][kTreeWords]
-    static constexpr int kPositionOff = kSightOff + kChunkRows * kTreeWords * 4;
-    static constexpr int kParentOff = kPositionOff + kChunkRows * 4;                               // int16 [kTreeNodes]
+    static constexpr int kSightOff = (kRangeOff + static_cast<int>(sizeof(Range)) + 15) / 16 * 16;  // [ROWS][kTreeWords]
+    static constexpr int kPositionOff = kSightOff + ROWS * kTreeWords * 4;
+    static constexpr int kParentOff = kPositionOff + ROWS * 4;                                      // int16 [kTreeNodes]
     static constexpr int kSmem = kParentOff + kTreeNodes * 2 + 1024;
-    static constexpr uint32_t kSCol = 0, kOCol = 256;  // S_x at 128 x, O_x at 256 + 128 x
-    static_assert(kSmem <= 232448, "shared memory per CTA");
+    static constexpr uint32_t kColumns = 256, kSCol = 0, kOCol = 128;  // S_x at 64 x
+    // (Q's 128 rows of the MMAs lie within the tiles' memory)
+    static_assert(kQOff + (kSlabs - 1) * kSlab + 128 * 128 <= kBarOff, "rows that the MMAs read");
+    static_assert(kTreeCtasPerSm * (kSmem + 1024) <= 233472, "shared memory per SM");
 };
+
+// Whether the phase with the given parity has completed, without a wait.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool warp_test(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_test(bar, parity));
+}
 
 // Whether every row of the tile sees keys `key` .. `end`.
 __device__ __forceinline__ bool tree_all_see(const Tile& t, int window, int sinks, int key, int end) {
     return end < t.p0 && (window <= 0 || key > t.p1 - window || end < sinks);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kTreeThreads, 1)
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     paged_attention_tree_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                                 const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttendArgs a) {
-    using C = TreeCfg<D>;
-    using TreeWalk = Walk<kChunkKeys, true>;
+    using C = TreeCfg<D, ROWS>;
+    using TreeWalk = Walk<kTreeKeys, true>;
     extern __shared__ uint8_t tree_smem_raw[];
     uint8_t* smem = tree_smem_raw + ((1024u - (smem_addr(tree_smem_raw) & 1023u)) & 1023u);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
@@ -78,9 +96,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     uint64_t* q_empty = q_full + 1;
     uint64_t* s_full = q_empty + 1;  // [2]
     uint64_t* p_full = s_full + 2;   // [2]
-    uint64_t* o_full = p_full + 2;
-    uint64_t* o_free = o_full + 1;
-    uint64_t* meet = o_free + 1;     // of the softmax warps
+    uint64_t* pv_done = p_full + 2;  // [2], of blocks n % 2
+    uint64_t* o_full = pv_done + 2;
+    uint64_t* meet = o_full + 1;     // of the softmax warps
     uint64_t* mma_done = meet + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -91,7 +109,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     const int tile_tokens = a.half_tokens;
     Range* shared_range = reinterpret_cast<Range*>(smem + C::kRangeOff);
     {
-        const Range r = find_range<kTreeThreads, kChunkKeys, true>(a, tile_tokens, smem);
+        const Range r = find_range<kTreeThreads, kTreeKeys, true>(a, tile_tokens, smem);
         if (threadIdx.x == 0) {
             *shared_range = r;
             a.entries[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -110,10 +128,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         for (int x = 0; x < 2; ++x) {
             mbar_init(&s_full[x], 1);
             mbar_init(&p_full[x], 4);
+            mbar_init(&pv_done[x], 1);
         }
         mbar_init(o_full, 1);
-        mbar_init(o_free, 8);
-        mbar_init(meet, 8);
+        mbar_init(meet, 4);
         mbar_init(mma_done, 1);
         *failed = wait_failed_before() ? 1 : 0;
         *wild = 0;
@@ -121,7 +139,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     }
     if (warp == kTreeMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_addr(tmem_slot)), "r"(512u) : "memory");
+                     ::"r"(smem_addr(tmem_slot)), "r"(C::kColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -135,11 +153,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     // flags lie beside K's barrier, written before K's copies start.
     if (warp == kTreeLoadWarp) {
         TreeWalk w;
-        const int page_size = 1 << a.p.page_shift, box = min(page_size, kChunkKeys);  // a box: keys of one page
-        const int boxes = kChunkKeys / box;
+        const int page_size = 1 << a.p.page_shift, box = min(page_size, kTreeKeys);  // a box: keys of one page
+        const int boxes = kTreeKeys / box;
         const bool mine = lane < boxes;  // each lane one box
         auto page_of = [&](const TreeWalk& u) -> int {  // -1: read as zeros
-            const int key = u.tile.block(u.unit) * kChunkKeys + lane * box;
+            const int key = u.tile.block(u.unit) * kTreeKeys + lane * box;
             const Tile& t = u.tile;
             if (!mine || key > t.p1 || !(a.window <= 0 || key + box - 1 > t.p0 - a.window || key < a.sinks)) return -1;
             const int page = a.p.table[static_cast<long long>(u.b) * a.p.table_stride + (key >> a.p.page_shift)];
@@ -170,10 +188,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     tma_load_3d(smem + C::kQOff + lane * C::kSlab, &qmap, lane * 64, w.h * a.group, w.tile.first, q_full);
                 ++items;
             }
-            const int key = w.tile.block(w.unit) * kChunkKeys;
+            const int key = w.tile.block(w.unit) * kTreeKeys;
             const int y = boxes > 1 ? 0 : key & (page_size - 1);
             const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
-            const bool unclean = !tree_all_see(w.tile, a.window, a.sinks, key, key + kChunkKeys - 1);
+            const bool unclean = !tree_all_see(w.tile, a.window, a.sinks, key, key + kTreeKeys - 1);
             uint32_t flag = (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u);
             // the next block's page ids are on their way while this one's copies are issued
             new_item = w.part_ends();
@@ -217,8 +235,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         uint32_t n = 0, raw_phase = 0;
         bool more = w.start(a, *shared_range, tile_tokens);
         for (; more; more = w.next(a, tile_tokens), ++n) {
-            const int key = w.tile.block(w.unit) * kChunkKeys;
-            if (tree_all_see(w.tile, a.window, a.sinks, key, key + kChunkKeys - 1)) continue;
+            const int key = w.tile.block(w.unit) * kTreeKeys;
+            if (tree_all_see(w.tile, a.window, a.sinks, key, key + kTreeKeys - 1)) continue;
             const uint32_t stage = (2 * n + 1) % C::kStages;
             if (!__all_sync(0xffffffffu, !*failed && mbar_wait(&raw[stage], (raw_phase >> stage) & 1u))) {
                 *failed = 1;
@@ -235,13 +253,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             // see the tree's, and those that the window leaves from row to row.
             const Tile& t = w.tile;
             auto zero = [&](int from, int to) {
-                for (int r = max(from - key, 0) + (lane >> 3); r < min(to - key, kChunkKeys); r += 4)
+                for (int r = max(from - key, 0) + (lane >> 3); r < min(to - key, kTreeKeys); r += 4)
 #pragma unroll
                     for (int slab = 0; slab < C::kSlabs; ++slab) *at(r, slab) = make_uint4(0u, 0u, 0u, 0u);
             };
             uint32_t bad = 0;
             auto search = [&](int from, int to) {
-                const int end = min(to - key, kChunkKeys);
+                const int end = min(to - key, kTreeKeys);
 #pragma unroll 1
                 for (int r = max(from - key, 0) + (lane >> 3); r < end; r += 16) {
                     uint4 v[4 * C::kSlabs];  // four rows' loads in flight (one past the end is its lane's first again)
@@ -261,7 +279,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             }
             if (__any_sync(0xffffffffu, bad != 0)) {
 #pragma unroll 1
-                for (int r = lane >> 3; r < kChunkKeys; r += 4) {
+                for (int r = lane >> 3; r < kTreeKeys; r += 4) {
                     if (tree_all_see(t, a.window, a.sinks, key + r, key + r)) continue;
 #pragma unroll
                     for (int slab = 0; slab < C::kSlabs; ++slab) {
@@ -289,79 +307,85 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         const uint64_t q_desc = q_major | (base + (C::kQOff >> 4));
         const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t stage = 0, phase = 0;  // of the ring: K's, then V's
-        uint32_t q_items = 0, parts = 0, p_count0 = 0, p_count1 = 0, x = 0;
-        bool fresh0 = true, fresh1 = true, issued = false;  // O_x has nothing of this part; S of this block is issued
+        uint32_t n = 0, q_items = 0;
+        bool fresh = true, issued = false;  // O has nothing of this part; S of this block is issued
         bool ok = !*failed && warp_wait(&full[0], 0);
         uint32_t flag = ok ? flags[0] : 0u;
         const bool none = (flag & kStepNone) != 0;
         if (none) ok = false;
-        auto issue_s = [&](uint32_t which, uint32_t k_stage, uint32_t f) {  // K has landed
-            if (f & kStepFirst) {
-                if (!warp_wait(q_full, q_items++ & 1)) return false;
-            }
+        auto issue_s = [&](uint32_t x, uint32_t k_stage, uint32_t f) {  // K and Q have landed
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t bd = k_major | (base + ((C::kRingOff + k_stage * C::kTile) >> 4));
-                const uint32_t s_tmem = t0 + C::kSCol + 128 * which;
+                const uint32_t s_tmem = t0 + C::kSCol + kTreeKeys * x;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     const uint32_t in_slab = 2 * (kk & 3), slab = kk >> 2;  // 16 values: 32 bytes
                     tc_mma_f16(s_tmem, q_desc + slab * (C::kSlab >> 4) + in_slab, bd + slab * 64 + in_slab,
-                               chunk_idesc<T>(kChunkKeys, false), kk != 0);
+                               chunk_idesc<T>(kTreeKeys, false), kk != 0);
                 }
-                tc_commit(&s_full[which]);
+                tc_commit(&s_full[x]);
                 tc_commit(&empty[k_stage]);
                 if (f & kStepLast) tc_commit(q_empty);
             }
             __syncwarp();
-            return true;
         };
         while (ok) {  // K of this block has landed
-            const uint32_t k_stage = stage;
+            const uint32_t x = n & 1, k_stage = stage;
             if (++stage == C::kStages) stage = 0, phase ^= 1u;
             const uint32_t v_stage = stage, v_phase = phase;
             if (++stage == C::kStages) stage = 0, phase ^= 1u;
-            if (!issued) ok = issue_s(x, k_stage, flag);
-            if (!ok) break;
-            // the next block's S, so that it runs while this one's softmax does
-            uint32_t next_flag = 0;
-            issued = false;
-            if (!(flag & (kStepLast | kStepFinal))) {
-                ok = warp_wait(&full[stage], phase);
+            if (!issued) {
+                if (flag & kStepFirst) ok = warp_wait(q_full, q_items++ & 1);
                 if (!ok) break;
-                next_flag = flags[stage];
-                ok = issued = issue_s(x ^ 1, stage, next_flag);
-                if (!ok) break;
+                issue_s(x, k_stage, flag);
             }
-            ok = warp_wait(&full[v_stage], v_phase);
-            if (ok && fresh0 && fresh1 && parts > 0) ok = warp_wait(o_free, (parts - 1) & 1);
-            const uint32_t count = x ? p_count1 : p_count0;
-            ok = ok && warp_wait(&p_full[x], count & 1);
+            // the next block's S as soon as its operands are there, and this one's P V
+            uint32_t next_flag = 0, rounds = 0;
+            bool landed = false;  // the next block's K
+            issued = false;
+            PollClock clock;
+            while (true) {
+                if (!issued && !(flag & kStepFinal)) {
+                    if (!landed && warp_test(&full[stage], phase)) {
+                        landed = true;
+                        next_flag = flags[stage];
+                    }
+                    if (landed && (!(next_flag & kStepFirst) || warp_test(q_full, q_items & 1))) {
+                        if (next_flag & kStepFirst) ++q_items;
+                        issue_s(x ^ 1, stage, next_flag);
+                        issued = true;
+                    }
+                }
+                if (warp_test(&p_full[x], (n >> 1) & 1) && warp_test(&full[v_stage], v_phase)) break;
+                if ((++rounds & 63) == 0 && __any_sync(0xffffffffu, *failed || poll_expired(clock))) {
+                    ok = false;
+                    break;
+                }
+            }
             if (!ok) break;
             tc_fence_after();
-            const bool first = x ? fresh1 : fresh0;
             if (elect_one()) {
                 const uint64_t bd = v_major | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
-                const uint32_t s_tmem = t0 + C::kSCol + 128 * x, o_tmem = t0 + C::kOCol + 128 * x;
+                const uint32_t s_tmem = t0 + C::kSCol + kTreeKeys * x, o_tmem = t0 + C::kOCol;
 #pragma unroll
-                for (int kk = 0; kk < kChunkKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                for (int kk = 0; kk < kTreeKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
                     tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * (C::kGroup >> 3), chunk_idesc<T>(D, true),
-                                  !first || kk != 0);
+                                  !fresh || kk != 0);
                 tc_commit(&empty[v_stage]);
+                tc_commit(&pv_done[x]);
                 if (flag & kStepLast) tc_commit(o_full);
             }
             __syncwarp();
-            if (x) fresh1 = false, ++p_count1;
-            else fresh0 = false, ++p_count0;
-            if (flag & kStepLast) fresh0 = fresh1 = true, ++parts;
+            fresh = (flag & kStepLast) != 0;
             if (flag & kStepFinal) break;
-            if (!issued) {
+            if (!landed) {
                 ok = warp_wait(&full[stage], phase);
                 if (!ok) break;
                 next_flag = flags[stage];
             }
             flag = next_flag;
-            x ^= 1;
+            ++n;
         }
         if (!ok && !none) *failed = 1;
         if (elect_one()) tc_commit(mma_done);  // arrives once every MMA issued above has completed
@@ -369,20 +393,19 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     } else {
         TreeWalk w;
         bool more = w.start(a, *shared_range, tile_tokens);
-        const int x = warp >> 2, row = threadIdx.x & 127, quarter = warp & 3;
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-        const uint32_t s_col = lane_base + C::kSCol + 128 * x, o_col = lane_base + C::kOCol;
+        const int row = threadIdx.x;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+        const uint32_t o_col = lane_base + C::kOCol;
         const int node = row / a.group, head = row - node * a.group;
-        float2* stats = reinterpret_cast<float2*>(smem + C::kStatOff);
         uint32_t* sights = reinterpret_cast<uint32_t*>(smem + C::kSightOff);
         int* positions = reinterpret_cast<int*>(smem + C::kPositionOff);
         int16_t* parent = reinterpret_cast<int16_t*>(smem + C::kParentOff);
         const uint32_t* sight = sights + node * kTreeWords;  // this row's
         bool ok = !*failed;
         bool begun = w.unit == 0;  // the item's first unit is in this range
-        uint32_t n = 0, s_count = 0, parts = 0, meets = 0;
+        uint32_t n = 0, parts = 0, meets = 0;
         int sight_b = -1, sight_t = 0;
-        auto meet_all = [&]() {  // of the eight softmax warps
+        auto meet_all = [&]() {  // of the softmax warps
             __syncwarp();
             if (lane == 0) mbar_arrive(meet);
             return warp_wait(meet, meets++ & 1);
@@ -395,8 +418,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 ok = meet_all();  // no one reads the last one's any more
                 if (!ok) break;
                 const bool some = w.span.base >= 0;  // else the sequence counts as empty
-                if (some && static_cast<int>(threadIdx.x) < w.span.count)
-                    parent[threadIdx.x] = static_cast<int16_t>(checked_parent(a.parents[w.span.first + threadIdx.x], threadIdx.x));
+                if (some)
+                    for (int i = threadIdx.x; i < w.span.count; i += 128)
+                        parent[i] = static_cast<int16_t>(checked_parent(a.parents[w.span.first + i], i));
                 ok = meet_all();
                 if (!ok) break;
                 if (static_cast<int>(threadIdx.x) < tile.tokens) {
@@ -418,7 +442,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 if (!ok) break;
             }
             const bool valid = node < tile.tokens;
-            const bool live = 32 * quarter < tile.tokens * a.group;  // of the warp: it has rows
+            const bool live = 32 * warp < tile.tokens * a.group;  // of the warp: it has rows
             const int pos = valid ? positions[node] : -1;
             // Bits of the keys first .. first + 31 that the row sees.
             auto seen_bits = [&](int first) -> uint32_t {
@@ -434,73 +458,65 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             float m = -INFINITY, l = 0.f;
             bool done = false;
             while (true) {
-                if ((n & 1) == static_cast<uint32_t>(x)) {
-                    ok = warp_wait(&s_full[x], s_count & 1);
-                    if (!ok) break;
-                    ++s_count;
-                    tc_fence_after();
-                    if (live) {
-                        const int key = tile.block(w.unit) * kChunkKeys;
-                        const bool masked = !tree_all_see(tile, a.window, a.sinks, key, key + kChunkKeys - 1);
-                        uint32_t seen[4];
-                        if (masked) {
+                const uint32_t x = n & 1, s_col = lane_base + C::kSCol + kTreeKeys * x;
+                ok = warp_wait(&s_full[x], (n >> 1) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (live) {
+                    float v[kTreeKeys];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) seen[k] = seen_bits(key + 32 * k);
+                    for (int c = 0; c < kTreeKeys; c += 16) tmem_ld16_nowait(s_col + c, v, c);
+                    tmem_wait_regs(v);
+                    const int key = tile.block(w.unit) * kTreeKeys;
+                    if (!tree_all_see(tile, a.window, a.sinks, key, key + kTreeKeys - 1)) {
+#pragma unroll
+                        for (int c = 0; c < kTreeKeys; c += 32) {
+                            const uint32_t bits = seen_bits(key + c);
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[c + k] = (bits >> k) & 1u ? v[c + k] : -INFINITY;
                         }
-                        auto mask = [&](float (&v)[32], uint32_t bits) {
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = (bits >> k) & 1u ? v[k] : -INFINITY;
-                        };
-                        // the maximum first, then the weights: the scores are read twice, which keeps them out of the registers
-                        float v[32], mx = -INFINITY;
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            tmem_ld16_nowait(s_col + 32 * k, v, 0);
-                            tmem_ld16_nowait(s_col + 32 * k + 16, v, 16);
-                            tmem_wait_regs(v);
-                            if (masked) mask(v, seen[k]);
-                            float top[2] = {v[0], v[1]};
-#pragma unroll
-                            for (int e = 2; e < 30; e += 4) {
-                                top[0] = fmaxf(fmaxf(top[0], v[e]), v[e + 1]);
-                                top[1] = fmaxf(fmaxf(top[1], v[e + 2]), v[e + 3]);
-                            }
-                            mx = fmaxf(fmaxf(mx, fmaxf(top[0], top[1])), fmaxf(v[30], v[31]));
-                        }
-                        const bool move = valid && (mx - m) * a.scale > 7.f;
-                        if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
-                            const float f = move ? ex2_approx((m - mx) * a.scale) : 1.f;  // 0 for m = -inf, whose l and O are 0
-                            l *= f;
-                            rescale_row<D>(o_col + 128 * x, f);
-                        }
-                        if (move) m = mx;
-                        const float less = m == -INFINITY ? 0.f : -m;
-                        const uint64_t less2 = pack2(less, less), scale2 = pack2(a.scale, a.scale), eight2 = pack2(8.f, 8.f);
-                        uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            tmem_ld16_nowait(s_col + 32 * k, v, 0);
-                            tmem_ld16_nowait(s_col + 32 * k + 16, v, 16);
-                            tmem_wait_regs(v);
-                            if (masked) mask(v, seen[k]);
-                            uint32_t p16[16];
-#pragma unroll
-                            for (int e = 0; e < 32; e += 2) {
-                                const uint64_t p2 = exp2_pair(fma2(add2(pack2(v[e], v[e + 1]), less2), scale2, eight2));
-                                sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], p2);
-                                const float2 p = unpack2(p2);
-                                p16[e / 2] = Pair<T>::pack(p.x, p.y);
-                            }
-                            tmem_st16u(s_col + 16 * k, p16, 0);  // (over scores that are read already)
-                        }
-                        const float2 sums = unpack2(add2(sum[0], sum[1]));
-                        l += sums.x + sums.y;
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[x]);
+                    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                    for (int c = 4; c < kTreeKeys - 4; c += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top[k] = fmaxf(fmaxf(top[k], v[c + k]), v[c + k + 4]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], v[kTreeKeys - 4 + k]);
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    const bool move = valid && (mx - m) * a.scale > 7.f;
+                    if (__any_sync(0xffffffffu, move && m != -INFINITY)) {
+                        // O at rest: P V of the block before (those before that were done before this S)
+                        ok = warp_wait(&pv_done[x ^ 1], ((n - 1) >> 1) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const float f = move ? ex2_approx((m - mx) * a.scale) : 1.f;  // 0 for m = -inf, whose l and O are 0
+                        l *= f;
+                        rescale_row<D>(o_col, f);
+                    }
+                    if (move) m = mx;
+                    const float less = m == -INFINITY ? 0.f : -m;
+                    const uint64_t less2 = pack2(less, less), scale2 = pack2(a.scale, a.scale), eight2 = pack2(8.f, 8.f);
+                    uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int c = 0; c < kTreeKeys; c += 32) {
+                        uint32_t p16[16];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            const uint64_t p2 = exp2_pair(fma2(add2(pack2(v[c + k], v[c + k + 1]), less2), scale2, eight2));
+                            sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], p2);
+                            const float2 p = unpack2(p2);
+                            p16[k / 2] = Pair<T>::pack(p.x, p.y);
+                        }
+                        tmem_st16u(s_col + c / 2, p16, 0);  // (over scores that are read already)
+                    }
+                    const float2 sums = unpack2(add2(sum[0], sum[1]));
+                    l += sums.x + sums.y;
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
                 ++n;
                 done = w.item_ends();
                 if (w.part_ends()) break;
@@ -508,24 +524,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             }
             if (!ok) break;
 
-            // ---- the two warpgroups' sums joined: each half of the columns ------------
-            float2* stat = stats + (parts & 1) * 2 * kChunkRows;
-            stat[x * kChunkRows + row] = make_float2(m, l);
-            ok = meet_all() && warp_wait(o_full, parts & 1);
+            // ---- the item's result, or this CTA's part of it -----------------------
+            ok = warp_wait(o_full, parts & 1);
             if (!ok) break;
             ++parts;
             tc_fence_after();
-            const float2 s0 = stat[row], s1 = stat[kChunkRows + row];
-            const float top = fmaxf(s0.x, s1.x);
-            // (a side that saw no key has l = 0, and an accumulator that may hold anything)
-            const bool some0 = s0.y != 0.f, some1 = s1.y != 0.f;
-            float f0 = some0 ? ex2_approx((s0.x - top) * a.scale) : 0.f, f1 = some1 ? ex2_approx((s1.x - top) * a.scale) : 0.f;
-            const float total = s0.y * f0 + s1.y * f1;
             const bool whole = begun && done;
-            if (whole) {
-                const float inv = total != 0.f ? 1.0f / total : 0.f;
-                f0 *= inv, f1 *= inv;
-            }
+            const float f = l == 0.f ? 0.f : whole ? 1.0f / l : 1.f;  // l = 0: saw no key
             constexpr int kPart = kChunkRows * (D + 2);
             // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
             float4* part = reinterpret_cast<float4*>(a.partials + static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * kPart);
@@ -541,8 +546,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     const Range& r = *shared_range;
                     const long long first = r.end - w.left - w.unit;  // place of the item's unit 0
                     for (int u = static_cast<int>(max(r.begin - first, 0ll)); u <= w.unit; ++u) {
-                        const int block = tile.block(u) * kChunkKeys;
-                        for (int j = block; j < block + kChunkKeys; ++j) {
+                        const int block = tile.block(u) * kTreeKeys;
+                        for (int j = block; j < block + kTreeKeys; ++j) {
                             if (!tile_sees(tile, a.window, a.sinks, j) || tree_all_see(tile, a.window, a.sinks, j, j)) continue;
                             const int page = a.p.table[static_cast<long long>(w.b) * a.p.table_stride + (j >> a.p.page_shift)];
                             if (page < 0 || page >= a.p.pages) continue;
@@ -562,16 +567,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                 };
                 const bool any_wild = __any_sync(0xffffffffu, *wild != 0);
 #pragma unroll 1
-                for (int c = x * (D / 2); c < (x + 1) * (D / 2); c += 32) {
-                    float v[32], u[32];
+                for (int c = 0; c < D; c += 32) {
+                    float v[32];
                     tmem_ld16_nowait(o_col + c, v, 0);
                     tmem_ld16_nowait(o_col + c + 16, v, 16);
-                    tmem_ld16_nowait(o_col + 128 + c, u, 0);
-                    tmem_ld16_nowait(o_col + 128 + c + 16, u, 16);
                     tmem_wait_regs(v);
-                    tmem_wait_regs(u);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) v[k] = (some0 ? v[k] * f0 : 0.f) + (some1 ? u[k] * f1 : 0.f);
+                    for (int k = 0; k < 32; ++k) v[k] *= f;
                     if (any_wild) {
                         add_wild(v, c);
                         __syncwarp();
@@ -593,19 +595,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                     }
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(o_free);
-            if (x == 0) {
-                if (whole) {
-                    if (valid && a.lse != nullptr)
-                        a.lse[static_cast<long long>(tile.first + node) * a.heads + w.h * a.group + head] =
-                            total == 0.f ? -INFINITY : (top * a.scale - 8.f) * 0.6931471805599453f + logf(total);
-                } else {
-                    if (valid) __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(top, total));
-                    if (threadIdx.x == 0 && begun)  // the item's first part: what the join needs to know
-                        a.entries[blockIdx.x] = make_int4(item_owners(*shared_range, w).y, tile.first, tile.tokens, w.h);
-                }
+            tc_fence_before();  // (the next item's first P V follows this warp's next P)
+            if (whole) {
+                if (valid && a.lse != nullptr)
+                    a.lse[static_cast<long long>(tile.first + node) * a.heads + w.h * a.group + head] =
+                        l == 0.f ? -INFINITY : (m * a.scale - 8.f) * 0.6931471805599453f + logf(l);
+            } else {
+                if (valid) __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
+                if (threadIdx.x == 0 && begun)  // the item's first part: what the join needs to know
+                    a.entries[blockIdx.x] = make_int4(item_owners(*shared_range, w).y, tile.first, tile.tokens, w.h);
             }
             more = w.next(a, tile_tokens);
             begun = true;
@@ -618,7 +616,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         // the MMAs must be complete before their tensor memory is released
         mbar_wait(mma_done, 0);
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kColumns) : "memory");
     }
 }
 
@@ -671,28 +669,28 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const AttendArg
             total == 0.f ? -INFINITY : (most * a.scale - 8.f) * 0.6931471805599453f + logf(total);
 }
 
-template <typename T, int D>
-static int launch_tree_tiles(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
-    using C = TreeCfg<D>;
+template <typename T, int D, int ROWS>
+static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
+    using C = TreeCfg<D, ROWS>;
     a.extra = kTreeExtra;
     a.least = kTreeLeast;
-    a.half_tokens = std::min(kChunkRows / a.group, max_query);  // of a tile
+    a.half_tokens = std::min(ROWS / a.group, max_query);  // of a tile
     static std::atomic<bool> opted_in[kMaxDevices];
     int dev = 0;
     H4B_CUDA_TRY(cudaGetDevice(&dev));
     if (!opted_in[dev].load(std::memory_order_acquire)) {
-        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_tree_kernel<T, D>,
+        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_tree_kernel<T, D, ROWS>,
                                           cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         opted_in[dev].store(true, std::memory_order_release);
     }
     CUtensorMap qmap, kmap, vmap;
-    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.half_tokens, a.q_stride) || !paged_kv_map(&kmap, a.k_pages, kv) ||
-        !paged_kv_map(&vmap, a.v_pages, kv))
+    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.half_tokens, a.q_stride) ||
+        !paged_kv_map(&kmap, a.k_pages, kv, kTreeKeys) || !paged_kv_map(&vmap, a.v_pages, kv, kTreeKeys))
         return H4B_EUNSUPPORTED;
-    paged_attention_tree_kernel<T, D><<<sms, kTreeThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
+    paged_attention_tree_kernel<T, D, ROWS><<<kTreeCtasPerSm * sms, kTreeThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
     H4B_CUDA_TRY(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(sms, (a.half_tokens * a.group + kJoinRows - 1) / kJoinRows);
+    cfg.gridDim = dim3(kTreeCtasPerSm * sms, (a.half_tokens * a.group + kJoinRows - 1) / kJoinRows);
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -702,6 +700,16 @@ static int launch_tree_tiles(AttendArgs a, const h4b_paged_kv* kv, int max_query
     cfg.numAttrs = 1;
     H4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a));
     return 0;
+}
+
+// Tiles with room for the rows of the largest tree, for the deeper ring of K and V
+// that the smaller ones leave room for.
+template <typename T, int D>
+static int launch_tree_tiles(const AttendArgs& a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
+    const long long rows = static_cast<long long>(max_query) * a.group;
+    if (rows <= 32) return launch_tree_rows<T, D, 32>(a, kv, max_query, sms, stream);
+    if (rows <= 64) return launch_tree_rows<T, D, 64>(a, kv, max_query, sms, stream);
+    return launch_tree_rows<T, D, 128>(a, kv, max_query, sms, stream);
 }
 
 }  // namespace h4b
