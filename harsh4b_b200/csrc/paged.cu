@@ -413,11 +413,18 @@ struct Range {
     long long skip;               // places of its sequence before `begin`
     int sequence;                 // of place `begin`
     int ctas;                     // that have a range: every one of them has a place at least
+    SequenceSpan span;            // of that sequence (trees only: the others look it up)
 };
-__device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
+// n / d of numbers that are not negative, in 32 bits where they fit: a 64-bit division
+// is a long piece of code, and what runs once a launch runs cold.
+__device__ __forceinline__ long long quotient(long long n, long long d) {
+    if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+    return n / d;
+}
+__device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return quotient(total * cta, ctas); }
 // The CTA that holds a place: the largest c with range_begin(c) <= place.
 __device__ __forceinline__ int range_owner(long long total, long long place, int ctas) {
-    return static_cast<int>(((place + 1) * ctas - 1) / total);
+    return static_cast<int>(quotient((place + 1) * ctas - 1, total));
 }
 
 // Every thread of the CTA takes part; `shared` holds THREADS / 32 long longs
@@ -430,8 +437,9 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     Range* found = reinterpret_cast<Range*>(warp_sums + THREADS / 32);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int each = (a.p.sequences + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
+    SequenceSpan s{0, 0, 0};
     auto places_of = [&](int e) {  // of the thread's e-th sequence, all kv heads
-        SequenceSpan s{0, 0, 0};
+        s = SequenceSpan{0, 0, 0};
         if (b0 + e < a.p.sequences) s = own_span<TREE>(a, raw_span(a.p, b0 + e));
         return a.p.kv_heads * warp_places<KEYS, TREE>(a, s, tile_tokens);
     };
@@ -468,6 +476,7 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
             if (open && r.begin < at + n) {
                 found->sequence = b0 + e;
                 found->skip = r.begin - at;
+                if constexpr (TREE) found->span = s;
                 open = false;
             }
             at += n;
@@ -477,6 +486,7 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     if (r.begin < r.end) {
         r.sequence = found->sequence;
         r.skip = found->skip;
+        if constexpr (TREE) r.span = found->span;
     }
     return r;
 }
@@ -499,7 +509,10 @@ struct Walk {
         const int lane = threadIdx.x & 31;
         b = r.sequence;
         left = static_cast<int>(min(r.end - r.begin, static_cast<long long>(INT_MAX)));
-        span = own_span<TREE>(a, raw_span(a.p, b));
+        if constexpr (TREE)
+            span = r.span;
+        else
+            span = own_span<TREE>(a, raw_span(a.p, b));
         request(a);
         long long skip = r.skip;
         for (int t0 = 0;; t0 += 32) {
@@ -523,8 +536,8 @@ struct Walk {
         }
         tile = make_tile<KEYS, TREE>(span, t, tile_tokens, a.window, a.sinks);
         const int places = a.extra + tile.units();
-        h = static_cast<int>(skip / places);
-        unit = static_cast<int>(skip % places) - a.extra;
+        h = static_cast<int>(quotient(skip, places));
+        unit = static_cast<int>(skip - static_cast<long long>(h) * places) - a.extra;
         if (unit < 0) {
             left += unit;
             unit = 0;
@@ -546,6 +559,8 @@ struct Walk {
         tile = make_tile<KEYS, TREE>(span, t, tile_tokens, a.window, a.sinks);
     }
     __device__ __forceinline__ bool item_ends() const { return unit + 1 >= tile.units(); }
+    // Whether this unit is the last of the range.
+    __device__ __forceinline__ bool range_ends(const AttendArgs& a) const { return left <= (item_ends() ? 1 + a.extra : 1); }
     // Whether this unit is the last of the item in this range, or of all.
     __device__ __forceinline__ bool part_ends() const { return item_ends() || left <= 1; }
     // To the next unit; false past the range's end.

@@ -50,15 +50,14 @@ struct TreeCfg {
     static constexpr int kSlab = ROWS * 128;                     // of Q
     static constexpr int kGroup = kSlabs * 1024;                 // of K or V: 8 keys, all slabs
     static constexpr int kTile = kTreeKeys / 8 * kGroup;
-    static constexpr int kStages = (ROWS == 128 ? 4 : ROWS == 64 ? 5 : 6) * (128 / D);
+    static constexpr int kStages = (ROWS == 128 ? 4 : 5) * (128 / D);
     static constexpr int kQOff = 0, kRingOff = kSlabs * kSlab, kBarOff = kRingOff + kStages * kTile;
-    static constexpr int kBars = 3 * kStages + 11;
+    static constexpr int kBars = 3 * kStages + 12;
     static constexpr int kFlagOff = kBarOff + kBars * 8 + 16;
     static constexpr int kRangeOff = kFlagOff + (kStages + 1) / 2 * 8;
-    static constexpr int kSightOff = (kRangeOff + static_cast<int>(sizeof(Range)) + 15) / 16 * 16;  // [ROWS][kTreeWords]
-    static constexpr int kPositionOff = kSightOff + ROWS * kTreeWords * 4;
-    static constexpr int kParentOff = kPositionOff + ROWS * 4;                                      // int16 [kTreeNodes]
-    static constexpr int kSmem = kParentOff + kTreeNodes * 2 + 1024;
+    static constexpr int kSightOff = (kRangeOff + static_cast<int>(sizeof(Range)) + 15) / 16 * 16;  // [kTreeNodes][kTreeWords]
+    static constexpr int kDepthOff = kSightOff + kTreeNodes * kTreeWords * 4;                       // int16 [kTreeNodes]
+    static constexpr int kSmem = kDepthOff + kTreeNodes * 2 + 1024;
     static constexpr uint32_t kColumns = 256, kSCol = 0, kOCol = 128;  // S_x at 64 x
     // (Q's 128 rows of the MMAs lie within the tiles' memory)
     static_assert(kQOff + (kSlabs - 1) * kSlab + 128 * 128 <= kBarOff, "rows that the MMAs read");
@@ -74,6 +73,51 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 }
 __device__ __forceinline__ bool warp_test(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_test(bar, parity));
+}
+
+// What each of a sequence's first `nodes` nodes sees of the tree, as bits, and its
+// depth. By one warp, 32 nodes at a time, whose parents are among them or earlier:
+// within the 32 by doubling the step (a node's set joins that of the node its step
+// leads to), then the set of the earlier node that the topmost one hangs from. So
+// a chain takes no longer than a bush. With a window (of fewer than all nodes) what
+// lies too far above is taken out at the end.
+__device__ __forceinline__ void find_sights(const int (&parent)[kTreeWords], int nodes, int base, int window, int sinks,
+                                            uint32_t* sights, int16_t* depths) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < kTreeWords; ++k) {
+        if (32 * k >= nodes) break;
+        const int i = 32 * k + lane;
+        const int p = i < nodes ? checked_parent(parent[k], i) : -1;
+        uint32_t mine = 1u << lane;
+        int to = p >= 32 * k ? p & 31 : lane;  // where the step leads: itself at the top
+#pragma unroll
+        for (int r = 0; r < 5; ++r) {
+            mine |= __shfl_sync(0xffffffffu, mine, to);
+            to = __shfl_sync(0xffffffffu, to, to);
+        }
+        const int above = __shfl_sync(0xffffffffu, p, to);  // of the topmost: an earlier node, or -1
+        uint32_t* bits = sights + i * kTreeWords;
+#pragma unroll
+        for (int w = 0; w < kTreeWords; ++w) bits[w] = w < k ? (above >= 0 ? sights[above * kTreeWords + w] : 0u) : w == k ? mine : 0u;
+        depths[i] = static_cast<int16_t>(__popc(mine) - 1 + (above >= 0 ? depths[above] + 1 : 0));
+        __syncwarp();
+    }
+    if (window <= 0 || window >= nodes) return;
+#pragma unroll 1
+    for (int i = lane; i < nodes; i += 32) {
+        const int depth = depths[i];
+#pragma unroll 1
+        for (int w = 0; w <= i >> 5; ++w) {
+            uint32_t bits = sights[i * kTreeWords + w], left = bits;
+            for (; left != 0u; left &= left - 1) {
+                const int up = depths[32 * w + __ffs(left) - 1];
+                if (depth - up >= window && base + up >= sinks) bits &= ~(left & (0u - left));
+            }
+            sights[i * kTreeWords + w] = bits;
+        }
+    }
+    __syncwarp();
 }
 
 // Whether every row of the tile sees keys `key` .. `end`.
@@ -98,8 +142,9 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     uint64_t* p_full = s_full + 2;   // [2]
     uint64_t* pv_done = p_full + 2;  // [2], of blocks n % 2
     uint64_t* o_full = pv_done + 2;
-    uint64_t* meet = o_full + 1;     // of the softmax warps
-    uint64_t* mma_done = meet + 1;
+    uint64_t* sight_full = o_full + 1;
+    uint64_t* sight_free = sight_full + 1;
+    uint64_t* mma_done = sight_free + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
     volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* wild = failed + 1;  // values that are not finite were taken out of a V tile
@@ -108,16 +153,13 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile_tokens = a.half_tokens;
     Range* shared_range = reinterpret_cast<Range*>(smem + C::kRangeOff);
-    {
-        const Range r = find_range<kTreeThreads, kTreeKeys, true>(a, tile_tokens, smem);
-        if (threadIdx.x == 0) {
-            *shared_range = r;
-            a.entries[blockIdx.x] = make_int4(-1, 0, 0, 0);
-        }
-        if (r.begin >= r.end) return;
+    // barriers and tensor memory first: their cost hides behind the range's look-ups
+    if (warp == kTreeMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_addr(tmem_slot)), "r"(C::kColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 32 * kTreeLoadWarp) {
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -131,28 +173,39 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             mbar_init(&pv_done[x], 1);
         }
         mbar_init(o_full, 1);
-        mbar_init(meet, 4);
+        mbar_init(sight_full, 1);
+        mbar_init(sight_free, 4);
         mbar_init(mma_done, 1);
         *failed = wait_failed_before() ? 1 : 0;
         *wild = 0;
         fence_mbar_init();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
     }
-    if (warp == kTreeMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_addr(tmem_slot)), "r"(C::kColumns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    pdl_trigger();  // the join waits for this grid's end in its kernel
+    {
+        const Range r = find_range<kTreeThreads, kTreeKeys, true>(a, tile_tokens, smem);
+        if (threadIdx.x == 0) {
+            *shared_range = r;
+            a.entries[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    uint32_t* sights = reinterpret_cast<uint32_t*>(smem + C::kSightOff);  // of the tile's sequence, up to its last node
+    int16_t* depths = reinterpret_cast<int16_t*>(smem + C::kDepthOff);
+    // One walk for all roles, in code that they share: each role's own would run cold.
+    TreeWalk w;
+    bool more = shared_range->begin < shared_range->end && w.start(a, *shared_range, tile_tokens);
     auto ring = [&](uint32_t i) { return smem + C::kRingOff + (i % C::kStages) * C::kTile; };
     auto phase_of = [&](uint32_t i) { return (i / C::kStages) & 1u; };
 
     // K of the CTA's block n is tile 2 n of the ring, V tile 2 n + 1. A block's
     // flags lie beside K's barrier, written before K's copies start.
     if (warp == kTreeLoadWarp) {
-        TreeWalk w;
         const int page_size = 1 << a.p.page_shift, box = min(page_size, kTreeKeys);  // a box: keys of one page
         const int boxes = kTreeKeys / box;
         const bool mine = lane < boxes;  // each lane one box
@@ -166,12 +219,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             return -1;
         };
         uint32_t issued = 0, raw_open = 0, raw_phase = 0;  // a bit per stage
-        bool ok = !*failed, more = w.start(a, *shared_range, tile_tokens);
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&kmap)) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&vmap)) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&qmap)) : "memory");
-        }
+        bool ok = !*failed;
         if (!more && lane == 0) {
             flags[0] = kStepNone;
             mbar_arrive(&full[0]);
@@ -192,12 +240,8 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             const int y = boxes > 1 ? 0 : key & (page_size - 1);
             const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
             const bool unclean = !tree_all_see(w.tile, a.window, a.sinks, key, key + kTreeKeys - 1);
-            uint32_t flag = (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u);
-            // the next block's page ids are on their way while this one's copies are issued
-            new_item = w.part_ends();
-            more = w.next(a, tile_tokens);
-            if (more) page = page_of(w);
-            if (!more) flag |= kStepFinal;
+            const uint32_t flag = (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u) |
+                                  (w.range_ends(a) ? kStepFinal : 0u);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 const uint32_t stage = issued % C::kStages;
@@ -216,6 +260,9 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
                 else raw_open &= ~(1u << stage);
                 ++issued;
             }
+            new_item = w.part_ends();
+            more = w.next(a, tile_tokens);
+            if (more) page = page_of(w);
         }
         if (!ok) *failed = 1;
         // the copies issued must land before the CTA may exit
@@ -229,12 +276,29 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
         }
         __syncwarp();
     } else if (warp == kTreeCleanWarp) {
-        // V rows of keys that no row of the item sees: zeros; values that are
-        // not finite in rows of keys that only some rows see: out
-        TreeWalk w;
-        uint32_t n = 0, raw_phase = 0;
-        bool more = w.start(a, *shared_range, tile_tokens);
+        // What the nodes of a tile see; V rows of keys that no row of the item sees:
+        // zeros; values that are not finite in rows of keys that only some rows see: out
+        uint32_t n = 0, raw_phase = 0, tiles = 0;
+        int sight_b = -1, sight_t = 0;
         for (; more; more = w.next(a, tile_tokens), ++n) {
+            if (w.b != sight_b || w.t != sight_t) {  // (the same for every kv head)
+                sight_b = w.b, sight_t = w.t;
+                const int nodes = w.span.base >= 0 ? w.tile.first - w.span.first + w.tile.tokens : 0;  // else it counts as empty
+                int parent[kTreeWords];
+#pragma unroll
+                for (int k = 0; k < kTreeWords; ++k) {
+                    const int i = 32 * k + lane;
+                    parent[k] = i < nodes ? a.parents[w.span.first + i] : -1;
+                }
+                // (once the tile before is done with)
+                if (tiles > 0 && !__all_sync(0xffffffffu, !*failed && mbar_wait(sight_free, (tiles - 1) & 1))) {
+                    *failed = 1;
+                    break;
+                }
+                ++tiles;
+                find_sights(parent, nodes, w.span.base, a.window, a.sinks, sights, depths);
+                if (lane == 0) mbar_arrive(sight_full);
+            }
             const int key = w.tile.block(w.unit) * kTreeKeys;
             if (tree_all_see(w.tile, a.window, a.sinks, key, key + kTreeKeys - 1)) continue;
             const uint32_t stage = (2 * n + 1) % C::kStages;
@@ -391,59 +455,30 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
         if (elect_one()) tc_commit(mma_done);  // arrives once every MMA issued above has completed
         __syncwarp();
     } else {
-        TreeWalk w;
-        bool more = w.start(a, *shared_range, tile_tokens);
         const int row = threadIdx.x;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * warp) << 16);
         const uint32_t o_col = lane_base + C::kOCol;
         const int node = row / a.group, head = row - node * a.group;
-        uint32_t* sights = reinterpret_cast<uint32_t*>(smem + C::kSightOff);
-        int* positions = reinterpret_cast<int*>(smem + C::kPositionOff);
-        int16_t* parent = reinterpret_cast<int16_t*>(smem + C::kParentOff);
-        const uint32_t* sight = sights + node * kTreeWords;  // this row's
         bool ok = !*failed;
-        bool begun = w.unit == 0;  // the item's first unit is in this range
-        uint32_t n = 0, parts = 0, meets = 0;
+        bool begun = more && w.unit == 0;  // the item's first unit is in this range
+        uint32_t n = 0, parts = 0, tiles = 0;
         int sight_b = -1, sight_t = 0;
-        auto meet_all = [&]() {  // of the softmax warps
-            __syncwarp();
-            if (lane == 0) mbar_arrive(meet);
-            return warp_wait(meet, meets++ & 1);
-        };
+        bool sighted = false;  // the tile's sights have come
+        int pos = -1;
         while (ok && more) {
             const Tile tile = w.tile;
-            const int base = tile.p0;
-            if (w.b != sight_b || w.t != sight_t) {  // what the tile's nodes see (the same for every kv head)
+            const int base = tile.p0, first_node = tile.first - w.span.first;
+            const uint32_t* sight = sights + (first_node + node) * kTreeWords;  // this row's
+            if (w.b != sight_b || w.t != sight_t) {  // (the same for every kv head)
+                __syncwarp();
+                if (tiles > 0 && lane == 0) mbar_arrive(sight_free);
                 sight_b = w.b, sight_t = w.t;
-                ok = meet_all();  // no one reads the last one's any more
-                if (!ok) break;
-                const bool some = w.span.base >= 0;  // else the sequence counts as empty
-                if (some)
-                    for (int i = threadIdx.x; i < w.span.count; i += 128)
-                        parent[i] = static_cast<int16_t>(checked_parent(a.parents[w.span.first + i], i));
-                ok = meet_all();
-                if (!ok) break;
-                if (static_cast<int>(threadIdx.x) < tile.tokens) {
-                    const int i = threadIdx.x, me = tile.first - w.span.first + i;
-                    uint32_t* bits = sights + i * kTreeWords;
-#pragma unroll
-                    for (int k = 0; k < kTreeWords; ++k) bits[k] = 0u;
-                    int depth = -1;
-                    if (some)
-                        for (int j = me; j >= 0; j = parent[j]) ++depth;
-                    positions[i] = some ? base + depth : -1;
-                    if (some) {
-                        int up = 0;
-                        for (int j = me; j >= 0; j = parent[j], ++up)
-                            if (a.window <= 0 || up < a.window || base + depth - up < a.sinks) bits[j >> 5] |= 1u << (j & 31);
-                    }
-                }
-                ok = meet_all();
-                if (!ok) break;
+                ++tiles;
+                sighted = false;
+                pos = -1;
             }
             const bool valid = node < tile.tokens;
             const bool live = 32 * warp < tile.tokens * a.group;  // of the warp: it has rows
-            const int pos = valid ? positions[node] : -1;
             // Bits of the keys first .. first + 31 that the row sees.
             auto seen_bits = [&](int first) -> uint32_t {
                 if (pos < 0) return 0u;
@@ -469,6 +504,12 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
                     tmem_wait_regs(v);
                     const int key = tile.block(w.unit) * kTreeKeys;
                     if (!tree_all_see(tile, a.window, a.sinks, key, key + kTreeKeys - 1)) {
+                        if (!sighted) {
+                            ok = warp_wait(sight_full, (tiles - 1) & 1);
+                            if (!ok) break;
+                            sighted = true;
+                            pos = valid && w.span.base >= 0 ? base + depths[first_node + node] : -1;
+                        }
 #pragma unroll
                         for (int c = 0; c < kTreeKeys; c += 32) {
                             const uint32_t bits = seen_bits(key + c);
@@ -621,49 +662,76 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
 }
 
 // Joins the parts of the items that lie across CTAs, as paged_join_kernel does:
-// block (c, slice) rows 16 slice .. of the item that begins last in CTA c, in the
-// order of the CTAs. Maxima are scores, in their own unit.
+// block (c, slice) rows 16 slice .. of the item that begins last in CTA c. A warp
+// holds 16 rows twice, for every other part each, and an eighth of the columns;
+// the statistics and values of up to kJoinAhead parts are on their way together. The
+// order of the sums is that of the CTAs, whichever came last. Maxima are scores.
+constexpr int kTreeJoinThreads = 256, kJoinAhead = 2;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const AttendArgs a) {
     constexpr int kPart = kChunkRows * (D + 2), kCols = D / 8 / 4;  // float4s a thread
     pdl_wait();
     const int4 entry = a.entries[blockIdx.x];
     const int c0 = blockIdx.x, c1 = entry.x;
     if (c1 < 0) return;
-    const int row = blockIdx.y * kJoinRows + (threadIdx.x % kJoinRows);
+    const int lane = threadIdx.x & 31, side = lane >> 4, c = (threadIdx.x >> 5) * kCols;
+    const int row = blockIdx.y * kJoinRows + (lane & 15);
     const int node = row / a.group, head = row - node * a.group;
-    if (node >= entry.z) return;
-    const int c = (threadIdx.x / kJoinRows) * kCols;
-    auto part_of = [&](int cta) { return a.partials + static_cast<long long>(2 * cta + (cta == c0)) * kPart; };
-    auto stat = [&](int cta) { return __ldcg(reinterpret_cast<const float2*>(part_of(cta) + D * kChunkRows) + row); };
-    float most = -INFINITY, total = 0.f;
-#pragma unroll 4
-    for (int cta = c0; cta <= c1; ++cta) most = fmaxf(most, stat(cta).x);
+    const bool valid = node < entry.z;  // (rows past the tile's: within the part's memory, and not written)
+    float top = -INFINITY, total = 0.f;
     float4 v[kCols];
 #pragma unroll
     for (int k = 0; k < kCols; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int cta = c0; cta <= c1; ++cta) {
-        const float2 ml = stat(cta);  // l = 0: saw no key
-        const float f = ml.y == 0.f ? 0.f : ex2_approx((ml.x - most) * a.scale);
-        total += ml.y * f;
-        const float4* o = reinterpret_cast<const float4*>(part_of(cta));
+    for (int cta = c0 + side; cta <= c1; cta += 2 * kJoinAhead) {
+        float2 ml[kJoinAhead];
+        float4 y[kJoinAhead][kCols];
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) {
-            const float4 y = __ldcg(o + (c + k) * kChunkRows + row);
-            v[k].x += y.x * f, v[k].y += y.y * f, v[k].z += y.z * f, v[k].w += y.w * f;
+        for (int u = 0; u < kJoinAhead; ++u) {
+            const int which = cta + 2 * u;
+            ml[u] = make_float2(-INFINITY, 0.f);
+            if (which > c1 || !valid) continue;
+            const float* part = a.partials + static_cast<long long>(2 * which + (which == c0)) * kPart;
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(part + D * kChunkRows) + row);
+#pragma unroll
+            for (int k = 0; k < kCols; ++k) y[u][k] = __ldcg(reinterpret_cast<const float4*>(part) + (c + k) * kChunkRows + row);
+        }
+#pragma unroll
+        for (int u = 0; u < kJoinAhead; ++u) {
+            if (ml[u].y == 0.f) continue;  // saw no key
+            const float most = fmaxf(top, ml[u].x);
+            const float f = total == 0.f ? 0.f : ex2_approx((top - most) * a.scale), g = ex2_approx((ml[u].x - most) * a.scale);
+            top = most;
+            total = total * f + ml[u].y * g;
+#pragma unroll
+            for (int k = 0; k < kCols; ++k) {
+                v[k].x = v[k].x * f + y[u][k].x * g, v[k].y = v[k].y * f + y[u][k].y * g;
+                v[k].z = v[k].z * f + y[u][k].z * g, v[k].w = v[k].w * f + y[u][k].w * g;
+            }
         }
     }
+    // the two sides
+    const float top1 = __shfl_down_sync(0xffffffffu, top, 16), total1 = __shfl_down_sync(0xffffffffu, total, 16);
+    const float most = fmaxf(top, top1);
+    const float f = total == 0.f ? 0.f : ex2_approx((top - most) * a.scale);
+    const float g = total1 == 0.f ? 0.f : ex2_approx((top1 - most) * a.scale);
+    total = total * f + total1 * g;
     const float scale = total != 0.f ? 1.0f / total : 0.f;
+    uint32_t words[2 * kCols];
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) {
+        const float4 w = make_float4(__shfl_down_sync(0xffffffffu, v[k].x, 16), __shfl_down_sync(0xffffffffu, v[k].y, 16),
+                                     __shfl_down_sync(0xffffffffu, v[k].z, 16), __shfl_down_sync(0xffffffffu, v[k].w, 16));
+        words[2 * k] = Pair<T>::pack((v[k].x * f + w.x * g) * scale, (v[k].y * f + w.y * g) * scale);
+        words[2 * k + 1] = Pair<T>::pack((v[k].z * f + w.z * g) * scale, (v[k].w * f + w.w * g) * scale);
+    }
+    if (side != 0 || !valid) return;
     const long long out_row = entry.y + node;
     const int out_head = entry.w * a.group + head;
     T* out = static_cast<T*>(a.out) + out_row * a.out_stride + out_head * D + 4 * c;
 #pragma unroll
-    for (int k = 0; k < kCols; k += 2)
-        *reinterpret_cast<uint4*>(out + 4 * k) =
-            make_uint4(Pair<T>::pack(v[k].x * scale, v[k].y * scale), Pair<T>::pack(v[k].z * scale, v[k].w * scale),
-                       Pair<T>::pack(v[k + 1].x * scale, v[k + 1].y * scale),
-                       Pair<T>::pack(v[k + 1].z * scale, v[k + 1].w * scale));
+    for (int k = 0; k < 2 * kCols; k += 4)
+        *reinterpret_cast<uint4*>(out + 2 * k) = make_uint4(words[k], words[k + 1], words[k + 2], words[k + 3]);
     if (a.lse != nullptr && c == 0)
         a.lse[out_row * a.heads + out_head] =
             total == 0.f ? -INFINITY : (most * a.scale - 8.f) * 0.6931471805599453f + logf(total);
@@ -691,7 +759,7 @@ static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int max_query,
     H4B_CUDA_TRY(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kTreeCtasPerSm * sms, (a.half_tokens * a.group + kJoinRows - 1) / kJoinRows);
-    cfg.blockDim = dim3(kJoinThreads);
+    cfg.blockDim = dim3(kTreeJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // it waits in the kernel
@@ -702,12 +770,11 @@ static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int max_query,
     return 0;
 }
 
-// Tiles with room for the rows of the largest tree, for the deeper ring of K and V
-// that the smaller ones leave room for.
+// Tiles with room for the rows of the largest tree: up to 64 leave room for a deeper
+// ring of K and V.
 template <typename T, int D>
 static int launch_tree_tiles(const AttendArgs& a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     const long long rows = static_cast<long long>(max_query) * a.group;
-    if (rows <= 32) return launch_tree_rows<T, D, 32>(a, kv, max_query, sms, stream);
     if (rows <= 64) return launch_tree_rows<T, D, 64>(a, kv, max_query, sms, stream);
     return launch_tree_rows<T, D, 128>(a, kv, max_query, sms, stream);
 }
