@@ -1222,22 +1222,29 @@ static int launch_few(AttendArgs a, int sms, cudaStream_t stream) {
     return 0;
 }
 
-template <typename T, int D, bool TREE = false>
+template <typename T, int D>
 static int launch_few_rows(const AttendArgs& a, int rows, int sms, cudaStream_t stream) {
-    if (rows <= 8) return launch_few<T, D, 8, TREE>(a, sms, stream);
+    if (rows <= 8) return launch_few<T, D, 8>(a, sms, stream);
     if constexpr (D == 64)
-        if (rows > 16) return launch_few<T, D, 32, TREE>(a, sms, stream);
-    return launch_few<T, D, 16, TREE>(a, sms, stream);
+        if (rows > 16) return launch_few<T, D, 32>(a, sms, stream);
+    return launch_few<T, D, 16>(a, sms, stream);
 }
 
+// Trees of few rows in the few-row kernel, others on tcgen05. In us, the few-row
+// kernel and the other one: 8 rows of head_dim 128 324 and 321 (16 x 32768 tokens),
+// 57 and 59 (64 ragged trees up to 2100), 10.9 and 12.8 (one over 1000), 132 and 136
+// (windows of 4096); 16 rows 329 and 324, 68 and 59, 13.9 and 13.1, 140 and 138. 16
+// rows of 64 201 and 210, 51 and 49, 10.9 and 11.3, 96 and 98; 32 rows 249 and 212,
+// 80 and 50, 20.4 and 11.4, 128 and 98.
 template <typename T, int D>
 static int launch_tree(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
     a.fewest = 1;
     a.most = INT_MAX;
-    constexpr int kMost = D == 64 ? 32 : 16;
     const long long rows = static_cast<long long>(max_query) * a.group;
-    if (rows > kMost) return launch_tree_tiles<T, D>(a, kv, max_query, sms, stream);
-    return launch_few_rows<T, D, true>(a, static_cast<int>(rows), sms, stream);
+    if (rows <= 8) return launch_few<T, D, 8, true>(a, sms, stream);
+    if constexpr (D == 64)
+        if (rows <= 16) return launch_few<T, D, 16, true>(a, sms, stream);
+    return launch_tree_tiles<T, D>(a, kv, max_query, sms, stream);
 }
 
 template <typename T, int D>
@@ -1359,8 +1366,8 @@ extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
     // two parts a CTA: an SM's rows of the few-row kernel are fewer than
     // the 256 of the chunk kernel's CTA
     static_assert(kFewCtasPerSm * kFewMaxRows <= 2 * kChunkRows, "the chunk kernel's parts are the larger");
-    static_assert(kTreeCtasPerSm * kChunkRows <= 2 * kChunkRows, "and than the tree kernel's");
-    if (kFewCtasPerSm * sms * 4 > kCounterBytes || kTreeCtasPerSm * sms * 16 > kEntryBytes) return H4B_EUNSUPPORTED;
+    // (the tree kernel's are as many rows an SM: two CTAs of 128 or one of 256)
+    if (kFewCtasPerSm * sms * 4 > kCounterBytes || 2 * sms * 16 > kEntryBytes) return H4B_EUNSUPPORTED;
     return kCounterBytes + kEntryBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
 }
 

@@ -39,29 +39,34 @@
 namespace h4b {
 
 constexpr int kTreeKeys = 64;
-constexpr int kTreeLoadWarp = 4, kTreeMmaWarp = 5, kTreeCleanWarp = 6, kTreeThreads = 224, kTreeCtasPerSm = 2;
 constexpr int kTreeLeast = 2, kTreeExtra = 4;  // as kChunkLeast and kChunkExtra, of 64 keys
 
-// ROWS: query rows of a tile that there is room for; the MMAs take 128 all the same,
-// and what they make of the others' lanes goes nowhere.
-template <int D, int ROWS>
+// TILES x ROWS: the query rows of an item that there is room for, in tiles of up to
+// 128 that share the keys; the MMAs take 128 all the same, and what they make of
+// the others' lanes goes nowhere.
+template <int D, int ROWS, int TILES>
 struct TreeCfg {
+    static constexpr int kCtasPerSm = 2 / TILES;
+    static constexpr int kLoadWarp = 4 * TILES, kMmaWarp = kLoadWarp + 1, kCleanWarp = kLoadWarp + 2;
+    static constexpr int kThreads = 32 * (kLoadWarp + 3);
     static constexpr int kSlabs = D / 64;                        // 64 values of head_dim each
     static constexpr int kSlab = ROWS * 128;                     // of Q
     static constexpr int kGroup = kSlabs * 1024;                 // of K or V: 8 keys, all slabs
     static constexpr int kTile = kTreeKeys / 8 * kGroup;
-    static constexpr int kStages = (ROWS == 128 ? 4 : 5) * (128 / D);
-    static constexpr int kQOff = 0, kRingOff = kSlabs * kSlab, kBarOff = kRingOff + kStages * kTile;
-    static constexpr int kBars = 3 * kStages + 12;
+    static constexpr int kStages = (TILES == 2 ? 9 : ROWS == 128 ? 4 : 5) * (128 / D);
+    static constexpr int kQOff = 0, kQTile = kSlabs * kSlab, kRingOff = TILES * kQTile, kBarOff = kRingOff + kStages * kTile;
+    static constexpr int kBars = 3 * kStages + 5 + 7 * TILES;
     static constexpr int kFlagOff = kBarOff + kBars * 8 + 16;
-    static constexpr int kRangeOff = kFlagOff + (kStages + 1) / 2 * 8;
+    static constexpr int kRangeOff = (kFlagOff + kStages * 4 + 7) / 8 * 8;
     static constexpr int kSightOff = (kRangeOff + static_cast<int>(sizeof(Range)) + 15) / 16 * 16;  // [kTreeNodes][kTreeWords]
     static constexpr int kDepthOff = kSightOff + kTreeNodes * kTreeWords * 4;                       // int16 [kTreeNodes]
     static constexpr int kSmem = kDepthOff + kTreeNodes * 2 + 1024;
-    static constexpr uint32_t kColumns = 256, kSCol = 0, kOCol = 128;  // S_x at 64 x
+    // S of tile t, block n at 64 (2 t + n % 2), O of tile t at kOCol + 128 t
+    static constexpr uint32_t kColumns = 256 * TILES, kSCol = 0, kOCol = 128 * TILES;
     // (Q's 128 rows of the MMAs lie within the tiles' memory)
-    static_assert(kQOff + (kSlabs - 1) * kSlab + 128 * 128 <= kBarOff, "rows that the MMAs read");
-    static_assert(kTreeCtasPerSm * (kSmem + 1024) <= 233472, "shared memory per SM");
+    static_assert(kQOff + TILES * kQTile - kSlab + 128 * 128 <= kBarOff, "rows that the MMAs read");
+    static_assert(kCtasPerSm * (kSmem + 1024) <= 233472 && kSmem <= 232448, "shared memory per SM");
+    static_assert(kStages <= 32, "a bit per stage");
 };
 
 // Whether the phase with the given parity has completed, without a wait.
@@ -125,11 +130,11 @@ __device__ __forceinline__ bool tree_all_see(const Tile& t, int window, int sink
     return end < t.p0 && (window <= 0 || key > t.p1 - window || end < sinks);
 }
 
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
+template <typename T, int D, int ROWS, int TILES>
+__global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, ROWS, TILES>::kCtasPerSm)
     paged_attention_tree_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                                 const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttendArgs a) {
-    using C = TreeCfg<D, ROWS>;
+    using C = TreeCfg<D, ROWS, TILES>;
     using TreeWalk = Walk<kTreeKeys, true>;
     extern __shared__ uint8_t tree_smem_raw[];
     uint8_t* smem = tree_smem_raw + ((1024u - (smem_addr(tree_smem_raw) & 1023u)) & 1023u);
@@ -138,11 +143,11 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     uint64_t* raw = empty + C::kStages;  // a V tile on its way to the cleaning warp
     uint64_t* q_full = raw + C::kStages;
     uint64_t* q_empty = q_full + 1;
-    uint64_t* s_full = q_empty + 1;  // [2]
-    uint64_t* p_full = s_full + 2;   // [2]
-    uint64_t* pv_done = p_full + 2;  // [2], of blocks n % 2
-    uint64_t* o_full = pv_done + 2;
-    uint64_t* sight_full = o_full + 1;
+    uint64_t* s_full = q_empty + 1;            // [TILES][2], of blocks n % 2
+    uint64_t* p_full = s_full + 2 * TILES;     // [TILES][2]
+    uint64_t* pv_done = p_full + 2 * TILES;    // [TILES][2]
+    uint64_t* o_full = pv_done + 2 * TILES;    // [TILES]
+    uint64_t* sight_full = o_full + TILES;
     uint64_t* sight_free = sight_full + 1;
     uint64_t* mma_done = sight_free + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
@@ -151,15 +156,15 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     volatile uint32_t* flags = reinterpret_cast<volatile uint32_t*>(smem + C::kFlagOff);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile_tokens = a.half_tokens;
+    const int half_tokens = a.half_tokens, tile_tokens = TILES * half_tokens;  // of a tile, of an item
     Range* shared_range = reinterpret_cast<Range*>(smem + C::kRangeOff);
     // barriers and tensor memory first: their cost hides behind the range's look-ups
-    if (warp == kTreeMmaWarp) {
+    if (warp == C::kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_addr(tmem_slot)), "r"(C::kColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (threadIdx.x == 32 * kTreeLoadWarp) {
+    if (threadIdx.x == 32 * C::kLoadWarp) {
         for (int s = 0; s < C::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -167,14 +172,14 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
         }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < 2 * TILES; ++x) {
             mbar_init(&s_full[x], 1);
             mbar_init(&p_full[x], 4);
             mbar_init(&pv_done[x], 1);
         }
-        mbar_init(o_full, 1);
+        for (int t = 0; t < TILES; ++t) mbar_init(&o_full[t], 1);
         mbar_init(sight_full, 1);
-        mbar_init(sight_free, 4);
+        mbar_init(sight_free, 4 * TILES);
         mbar_init(mma_done, 1);
         *failed = wait_failed_before() ? 1 : 0;
         *wild = 0;
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     }
     pdl_trigger();  // the join waits for this grid's end in its kernel
     {
-        const Range r = find_range<kTreeThreads, kTreeKeys, true>(a, tile_tokens, smem);
+        const Range r = find_range<C::kThreads, kTreeKeys, true>(a, tile_tokens, smem);
         if (threadIdx.x == 0) {
             *shared_range = r;
             a.entries[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
 
     // K of the CTA's block n is tile 2 n of the ring, V tile 2 n + 1. A block's
     // flags lie beside K's barrier, written before K's copies start.
-    if (warp == kTreeLoadWarp) {
+    if (warp == C::kLoadWarp) {
         const int page_size = 1 << a.p.page_shift, box = min(page_size, kTreeKeys);  // a box: keys of one page
         const int boxes = kTreeKeys / box;
         const bool mine = lane < boxes;  // each lane one box
@@ -230,10 +235,12 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             if (new_item) {  // the q rows, once the previous item's are no longer read
                 if (items > 0) ok = __all_sync(0xffffffffu, !*failed && mbar_wait(q_empty, (items - 1) & 1));
                 if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(q_full, C::kSlabs * tile_tokens * a.group * 128);
+                const int boxes_q = (w.tile.tokens > half_tokens ? TILES : 1) * C::kSlabs;
+                if (lane == 0) mbar_arrive_expect_tx(q_full, boxes_q * half_tokens * a.group * 128);
                 __syncwarp();
-                if (lane < C::kSlabs)
-                    tma_load_3d(smem + C::kQOff + lane * C::kSlab, &qmap, lane * 64, w.h * a.group, w.tile.first, q_full);
+                if (lane < boxes_q)
+                    tma_load_3d(smem + C::kQOff + lane * C::kSlab, &qmap, (lane % C::kSlabs) * 64, w.h * a.group,
+                                w.tile.first + lane / C::kSlabs * half_tokens, q_full);
                 ++items;
             }
             const int key = w.tile.block(w.unit) * kTreeKeys;
@@ -241,7 +248,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             const int z = page < 0 ? -1 : page * a.p.kv_heads + w.h;
             const bool unclean = !tree_all_see(w.tile, a.window, a.sinks, key, key + kTreeKeys - 1);
             const uint32_t flag = (new_item ? kStepFirst : 0u) | (w.part_ends() ? kStepLast : 0u) |
-                                  (w.range_ends(a) ? kStepFinal : 0u);
+                                  (w.range_ends(a) ? kStepFinal : 0u) | (w.tile.tokens > half_tokens ? kStepTwo : 0u);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
                 const uint32_t stage = issued % C::kStages;
@@ -275,7 +282,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
                 mbar_wait(&full[stage], phase_of(i));
         }
         __syncwarp();
-    } else if (warp == kTreeCleanWarp) {
+    } else if (warp == C::kCleanWarp) {
         // What the nodes of a tile see; V rows of keys that no row of the item sees:
         // zeros; values that are not finite in rows of keys that only some rows see: out
         uint32_t n = 0, raw_phase = 0, tiles = 0;
@@ -360,7 +367,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             if (lane == 0) mbar_arrive(&full[stage]);
         }
         __syncwarp();
-    } else if (warp == kTreeMmaWarp) {
+    } else if (warp == C::kMmaWarp) {
         // The whole warp runs the loop on uniform values and one elected lane
         // issues: the MMAs' operands then stay in uniform registers.
         const uint32_t base = __shfl_sync(0xffffffffu, smem_addr(smem), 0) >> 4;
@@ -371,42 +378,47 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
         const uint64_t q_desc = q_major | (base + (C::kQOff >> 4));
         const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t stage = 0, phase = 0;  // of the ring: K's, then V's
-        uint32_t n = 0, q_items = 0;
-        bool fresh = true, issued = false;  // O has nothing of this part; S of this block is issued
+        uint32_t c0 = 0, c1 = 0, q_items = 0;  // blocks of each tile so far
+        bool fresh = true, issued = false;     // O has nothing of this part; S of this block is issued
         bool ok = !*failed && warp_wait(&full[0], 0);
         uint32_t flag = ok ? flags[0] : 0u;
         const bool none = (flag & kStepNone) != 0;
         if (none) ok = false;
-        auto issue_s = [&](uint32_t x, uint32_t k_stage, uint32_t f) {  // K and Q have landed
+        auto issue_s = [&](uint32_t i0, uint32_t i1, uint32_t k_stage, uint32_t f) {  // K and Q have landed
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t bd = k_major | (base + ((C::kRingOff + k_stage * C::kTile) >> 4));
-                const uint32_t s_tmem = t0 + C::kSCol + kTreeKeys * x;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t in_slab = 2 * (kk & 3), slab = kk >> 2;  // 16 values: 32 bytes
-                    tc_mma_f16(s_tmem, q_desc + slab * (C::kSlab >> 4) + in_slab, bd + slab * 64 + in_slab,
-                               chunk_idesc<T>(kTreeKeys, false), kk != 0);
+                for (int t = 0; t < TILES; ++t) {
+                    if (t == 1 && !(f & kStepTwo)) break;
+                    const uint32_t x = 2 * t + ((t ? i1 : i0) & 1), s_tmem = t0 + C::kSCol + kTreeKeys * x;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t in_slab = 2 * (kk & 3), slab = kk >> 2;  // 16 values: 32 bytes
+                        tc_mma_f16(s_tmem, q_desc + t * (C::kQTile >> 4) + slab * (C::kSlab >> 4) + in_slab,
+                                   bd + slab * 64 + in_slab, chunk_idesc<T>(kTreeKeys, false), kk != 0);
+                    }
+                    tc_commit(&s_full[x]);
                 }
-                tc_commit(&s_full[x]);
                 tc_commit(&empty[k_stage]);
                 if (f & kStepLast) tc_commit(q_empty);
             }
             __syncwarp();
         };
         while (ok) {  // K of this block has landed
-            const uint32_t x = n & 1, k_stage = stage;
+            const uint32_t k_stage = stage, n1 = c1 + (flag & kStepTwo ? 1 : 0);
             if (++stage == C::kStages) stage = 0, phase ^= 1u;
             const uint32_t v_stage = stage, v_phase = phase;
             if (++stage == C::kStages) stage = 0, phase ^= 1u;
             if (!issued) {
                 if (flag & kStepFirst) ok = warp_wait(q_full, q_items++ & 1);
                 if (!ok) break;
-                issue_s(x, k_stage, flag);
+                issue_s(c0, c1, k_stage, flag);
             }
             // the next block's S as soon as its operands are there, and this one's P V
             uint32_t next_flag = 0, rounds = 0;
-            bool landed = false;  // the next block's K
+            bool landed = false, v_landed = false;  // the next block's K; this one's V
+            uint32_t todo = TILES == 2 && (flag & kStepTwo) ? 3u : 1u;
             issued = false;
             PollClock clock;
             while (true) {
@@ -417,30 +429,37 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
                     }
                     if (landed && (!(next_flag & kStepFirst) || warp_test(q_full, q_items & 1))) {
                         if (next_flag & kStepFirst) ++q_items;
-                        issue_s(x ^ 1, stage, next_flag);
+                        issue_s(c0 + 1, n1, stage, next_flag);
                         issued = true;
                     }
                 }
-                if (warp_test(&p_full[x], (n >> 1) & 1) && warp_test(&full[v_stage], v_phase)) break;
+                if (!v_landed) v_landed = warp_test(&full[v_stage], v_phase);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    const uint32_t c = t ? c1 : c0, x = 2 * t + (c & 1);
+                    if (!v_landed || !(todo & (1u << t)) || !warp_test(&p_full[x], (c >> 1) & 1)) continue;
+                    todo &= ~(1u << t);
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t bd = v_major | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
+                        const uint32_t s_tmem = t0 + C::kSCol + kTreeKeys * x, o_tmem = t0 + C::kOCol + 128 * t;
+#pragma unroll
+                        for (int kk = 0; kk < kTreeKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
+                            tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * (C::kGroup >> 3), chunk_idesc<T>(D, true),
+                                          !fresh || kk != 0);
+                        if (todo == 0) tc_commit(&empty[v_stage]);
+                        tc_commit(&pv_done[x]);
+                        if (flag & kStepLast) tc_commit(&o_full[t]);
+                    }
+                    __syncwarp();
+                }
+                if (todo == 0) break;
                 if ((++rounds & 63) == 0 && __any_sync(0xffffffffu, *failed || poll_expired(clock))) {
                     ok = false;
                     break;
                 }
             }
             if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint64_t bd = v_major | (base + ((C::kRingOff + v_stage * C::kTile) >> 4));
-                const uint32_t s_tmem = t0 + C::kSCol + kTreeKeys * x, o_tmem = t0 + C::kOCol;
-#pragma unroll
-                for (int kk = 0; kk < kTreeKeys / 16; ++kk)  // 16 keys: 8 columns of P, two 8-row groups of V
-                    tc_mma_f16_ts(o_tmem, s_tmem + 8 * kk, bd + kk * (C::kGroup >> 3), chunk_idesc<T>(D, true),
-                                  !fresh || kk != 0);
-                tc_commit(&empty[v_stage]);
-                tc_commit(&pv_done[x]);
-                if (flag & kStepLast) tc_commit(o_full);
-            }
-            __syncwarp();
             fresh = (flag & kStepLast) != 0;
             if (flag & kStepFinal) break;
             if (!landed) {
@@ -449,15 +468,16 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
                 next_flag = flags[stage];
             }
             flag = next_flag;
-            ++n;
+            ++c0;
+            c1 = n1;
         }
         if (!ok && !none) *failed = 1;
         if (elect_one()) tc_commit(mma_done);  // arrives once every MMA issued above has completed
         __syncwarp();
     } else {
-        const int row = threadIdx.x;
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * warp) << 16);
-        const uint32_t o_col = lane_base + C::kOCol;
+        const int t = TILES == 1 ? 0 : warp >> 2, row = threadIdx.x & 127, quarter = warp & 3;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+        const uint32_t o_col = lane_base + C::kOCol + 128 * t;
         const int node = row / a.group, head = row - node * a.group;
         bool ok = !*failed;
         bool begun = more && w.unit == 0;  // the item's first unit is in this range
@@ -467,7 +487,8 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
         int pos = -1;
         while (ok && more) {
             const Tile tile = w.tile;
-            const int base = tile.p0, first_node = tile.first - w.span.first;
+            const int base = tile.p0, first_row = tile.first + t * half_tokens, first_node = first_row - w.span.first;
+            const int my_tokens = min(half_tokens, tile.tokens - t * half_tokens);
             const uint32_t* sight = sights + (first_node + node) * kTreeWords;  // this row's
             if (w.b != sight_b || w.t != sight_t) {  // (the same for every kv head)
                 __syncwarp();
@@ -477,8 +498,14 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
                 sighted = false;
                 pos = -1;
             }
-            const bool valid = node < tile.tokens;
-            const bool live = 32 * warp < tile.tokens * a.group;  // of the warp: it has rows
+            if (TILES == 2 && my_tokens <= 0) {  // the second tile has nothing to do for this item
+                while (!w.part_ends()) w.next(a, tile_tokens);
+                more = w.next(a, tile_tokens);
+                begun = true;
+                continue;
+            }
+            const bool valid = node < my_tokens;
+            const bool live = 32 * quarter < my_tokens * a.group;  // of the warp: it has rows
             // Bits of the keys first .. first + 31 that the row sees.
             auto seen_bits = [&](int first) -> uint32_t {
                 if (pos < 0) return 0u;
@@ -493,7 +520,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             float m = -INFINITY, l = 0.f;
             bool done = false;
             while (true) {
-                const uint32_t x = n & 1, s_col = lane_base + C::kSCol + kTreeKeys * x;
+                const uint32_t x = 2 * t + (n & 1), s_col = lane_base + C::kSCol + kTreeKeys * x;
                 ok = warp_wait(&s_full[x], (n >> 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
@@ -566,7 +593,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             if (!ok) break;
 
             // ---- the item's result, or this CTA's part of it -----------------------
-            ok = warp_wait(o_full, parts & 1);
+            ok = warp_wait(&o_full[t], parts & 1);
             if (!ok) break;
             ++parts;
             tc_fence_after();
@@ -574,9 +601,9 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             const float f = l == 0.f ? 0.f : whole ? 1.0f / l : 1.f;  // l = 0: saw no key
             constexpr int kPart = kChunkRows * (D + 2);
             // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
-            float4* part = reinterpret_cast<float4*>(a.partials + static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * kPart);
+            float4* part = reinterpret_cast<float4*>(a.partials + static_cast<long long>((2 * blockIdx.x + (begun ? 1 : 0)) * TILES + t) * kPart);
             if (live) {
-                T* out_tile = static_cast<T*>(a.out) + tile.first * a.out_stride + w.h * a.group * D;
+                T* out_tile = static_cast<T*>(a.out) + first_row * a.out_stride + w.h * a.group * D;
                 const long long my_place = valid ? node * a.out_stride + head * D : -1;
                 long long to[4];  // the places of the quad's four rows
 #pragma unroll
@@ -639,7 +666,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
             tc_fence_before();  // (the next item's first P V follows this warp's next P)
             if (whole) {
                 if (valid && a.lse != nullptr)
-                    a.lse[static_cast<long long>(tile.first + node) * a.heads + w.h * a.group + head] =
+                    a.lse[static_cast<long long>(first_row + node) * a.heads + w.h * a.group + head] =
                         l == 0.f ? -INFINITY : (m * a.scale - 8.f) * 0.6931471805599453f + logf(l);
             } else {
                 if (valid) __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
@@ -653,7 +680,7 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == kTreeMmaWarp) {
+    if (warp == C::kMmaWarp) {
         // the MMAs must be complete before their tensor memory is released
         mbar_wait(mma_done, 0);
         tc_fence_after();
@@ -662,13 +689,13 @@ __global__ void __launch_bounds__(kTreeThreads, kTreeCtasPerSm)
 }
 
 // Joins the parts of the items that lie across CTAs, as paged_join_kernel does:
-// block (c, slice) rows 16 slice .. of the item that begins last in CTA c. A warp
+// block (c, tile * slices + slice) rows 16 slice .. of that tile of the item that begins last in CTA c. A warp
 // holds 16 rows twice, for every other part each, and an eighth of the columns;
 // the statistics and values of up to kJoinAhead parts are on their way together. The
 // order of the sums is that of the CTAs, whichever came last. Maxima are scores.
 constexpr int kTreeJoinThreads = 256, kJoinAhead = 2;
 
-template <typename T, int D>
+template <typename T, int D, int TILES>
 __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const AttendArgs a) {
     constexpr int kPart = kChunkRows * (D + 2), kCols = D / 8 / 4;  // float4s a thread
     pdl_wait();
@@ -676,9 +703,10 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
     const int c0 = blockIdx.x, c1 = entry.x;
     if (c1 < 0) return;
     const int lane = threadIdx.x & 31, side = lane >> 4, c = (threadIdx.x >> 5) * kCols;
-    const int row = blockIdx.y * kJoinRows + (lane & 15);
+    const int slices = gridDim.y / TILES, t = TILES == 1 ? 0 : blockIdx.y / slices;
+    const int row = (blockIdx.y - t * slices) * kJoinRows + (lane & 15);
     const int node = row / a.group, head = row - node * a.group;
-    const bool valid = node < entry.z;  // (rows past the tile's: within the part's memory, and not written)
+    const bool valid = node < min(a.half_tokens, entry.z - t * a.half_tokens);
     float top = -INFINITY, total = 0.f;
     float4 v[kCols];
 #pragma unroll
@@ -691,7 +719,7 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
             const int which = cta + 2 * u;
             ml[u] = make_float2(-INFINITY, 0.f);
             if (which > c1 || !valid) continue;
-            const float* part = a.partials + static_cast<long long>(2 * which + (which == c0)) * kPart;
+            const float* part = a.partials + static_cast<long long>((2 * which + (which == c0)) * TILES + t) * kPart;
             ml[u] = __ldcg(reinterpret_cast<const float2*>(part + D * kChunkRows) + row);
 #pragma unroll
             for (int k = 0; k < kCols; ++k) y[u][k] = __ldcg(reinterpret_cast<const float4*>(part) + (c + k) * kChunkRows + row);
@@ -726,7 +754,7 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
         words[2 * k + 1] = Pair<T>::pack((v[k].z * f + w.z * g) * scale, (v[k].w * f + w.w * g) * scale);
     }
     if (side != 0 || !valid) return;
-    const long long out_row = entry.y + node;
+    const long long out_row = entry.y + t * a.half_tokens + node;
     const int out_head = entry.w * a.group + head;
     T* out = static_cast<T*>(a.out) + out_row * a.out_stride + out_head * D + 4 * c;
 #pragma unroll
@@ -737,28 +765,29 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
             total == 0.f ? -INFINITY : (most * a.scale - 8.f) * 0.6931471805599453f + logf(total);
 }
 
-template <typename T, int D, int ROWS>
-static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
-    using C = TreeCfg<D, ROWS>;
+template <typename T, int D, int ROWS, int TILES>
+static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int tile_tokens, int sms, cudaStream_t stream) {
+    using C = TreeCfg<D, ROWS, TILES>;
     a.extra = kTreeExtra;
     a.least = kTreeLeast;
-    a.half_tokens = std::min(ROWS / a.group, max_query);  // of a tile
+    a.half_tokens = tile_tokens;
     static std::atomic<bool> opted_in[kMaxDevices];
     int dev = 0;
     H4B_CUDA_TRY(cudaGetDevice(&dev));
     if (!opted_in[dev].load(std::memory_order_acquire)) {
-        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_tree_kernel<T, D, ROWS>,
+        H4B_CUDA_TRY(cudaFuncSetAttribute(paged_attention_tree_kernel<T, D, ROWS, TILES>,
                                           cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         opted_in[dev].store(true, std::memory_order_release);
     }
     CUtensorMap qmap, kmap, vmap;
-    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, a.half_tokens, a.q_stride) ||
+    if (!paged_q_map(&qmap, a.q, kv, a.heads, a.group, tile_tokens, a.q_stride) ||
         !paged_kv_map(&kmap, a.k_pages, kv, kTreeKeys) || !paged_kv_map(&vmap, a.v_pages, kv, kTreeKeys))
         return H4B_EUNSUPPORTED;
-    paged_attention_tree_kernel<T, D, ROWS><<<kTreeCtasPerSm * sms, kTreeThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
+    const int ctas = C::kCtasPerSm * sms;
+    paged_attention_tree_kernel<T, D, ROWS, TILES><<<ctas, C::kThreads, C::kSmem, stream>>>(qmap, kmap, vmap, a);
     H4B_CUDA_TRY(cudaGetLastError());
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kTreeCtasPerSm * sms, (a.half_tokens * a.group + kJoinRows - 1) / kJoinRows);
+    cfg.gridDim = dim3(ctas, TILES * ((tile_tokens * a.group + kJoinRows - 1) / kJoinRows));
     cfg.blockDim = dim3(kTreeJoinThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -766,17 +795,23 @@ static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int max_query,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    H4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D>, a));
+    H4B_CUDA_TRY(cudaLaunchKernelEx(&cfg, tree_join_kernel<T, D, TILES>, a));
     return 0;
 }
 
 // Tiles with room for the rows of the largest tree: up to 64 leave room for a deeper
-// ring of K and V.
+// ring of K and V; from 129 on, at head_dim 128, two tiles share the keys (trees of 64
+// nodes and 4 q heads a kv head: 8 x 32768 tokens 370 -> 309 us, 64 ragged ones up to
+// 2100 130 -> 108, one over 8000 29 -> 29; at head_dim 64 243 and 244, 93 and 90, and
+// windowed trees 56 and 69).
 template <typename T, int D>
 static int launch_tree_tiles(const AttendArgs& a, const h4b_paged_kv* kv, int max_query, int sms, cudaStream_t stream) {
+    const int most = kChunkRows / a.group;  // tokens of a tile
     const long long rows = static_cast<long long>(max_query) * a.group;
-    if (rows <= 64) return launch_tree_rows<T, D, 64>(a, kv, max_query, sms, stream);
-    return launch_tree_rows<T, D, 128>(a, kv, max_query, sms, stream);
+    if (rows <= 64) return launch_tree_rows<T, D, 64, 1>(a, kv, max_query, sms, stream);
+    if constexpr (D == 128)
+        if (max_query > most) return launch_tree_rows<T, D, 128, 2>(a, kv, most, sms, stream);
+    return launch_tree_rows<T, D, 128, 1>(a, kv, std::min(most, max_query), sms, stream);
 }
 
 }  // namespace h4b
