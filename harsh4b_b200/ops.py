@@ -191,9 +191,8 @@ def rmsnorm_quantize_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, *, 
             raise ValueError("delta and out must have x's shape")
         add, add_stride = _rows(delta, delta.dtype, "delta", device), delta.stride(0) if several else width
         to, to_stride = _rows(out, dtype, "out", device), out.stride(0) if several else width
-    x8 = torch.empty((rows, width), dtype=torch.int8, device=x.device)
-    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    sums = torch.empty(rows, dtype=torch.int32, device=x.device)
+    x8, sums = x.new_empty((rows, width), dtype=torch.int8), x.new_empty(rows, dtype=torch.int32)
+    scales = weight.new_empty(rows)
     check(lib().h4b_rmsnorm_quantize_rows(_rows(x, dtype, "x", device), code, x.stride(0) if several else width, add, add_code,
                                           add_stride, to, to_stride, _on(weight, torch.float32, "weight", device), eps,
                                           x8.data_ptr(), scales.data_ptr(), sums.data_ptr(), rows, width, _here(device)),
@@ -305,15 +304,17 @@ def _here(device: int) -> int:
     return _raw_stream(device)
 
 
-def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int) -> PagedKvDesc:
-    """The h4b_paged_kv of one layer's pages and a batch's tables."""
+def _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, tokens: int, layered: bool = False) -> PagedKvDesc:
+    """The h4b_paged_kv of one layer's pages (`layered`: of all layers', the first one's) and a batch's tables."""
     dtype = k_pages.dtype
     code = _PAGED_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"k_pages must be float16 or bfloat16, got {dtype}")
     shape, table = k_pages.shape, page_table.shape
-    if len(shape) != 4 or shape != v_pages.shape:
+    if len(shape) != 4 + layered or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must be [pages][kv_heads][page_size][head_dim]")
+    if layered:
+        shape = shape[1:]
     sequences = kv_lens.numel()
     if len(table) != 2 or table[0] != sequences or q_offsets.numel() != sequences + 1:
         raise ValueError("page_table must be [sequences][pages each], q_offsets [sequences + 1], kv_lens [sequences]")
@@ -355,15 +356,16 @@ def paged_append(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if source is not torch.float32 and source is not dtype:
         raise ValueError(f"qkv must be float32 or {dtype}, got {source}")
     if out is None:
-        out = torch.empty((tokens, heads, head_dim), dtype=dtype, device=qkv.device)
+        out = qkv.new_empty((tokens, heads, head_dim), dtype=dtype)
     elif out.shape != (tokens, heads, head_dim):
         raise ValueError("out must be [tokens][heads][head_dim]")
     weights = [None, None]
-    for k, (name, norm) in enumerate((("norm_q", norm_q), ("norm_k", norm_k))):
-        if norm is not None:
-            if norm.numel() != head_dim:
-                raise ValueError(f"{name} must hold head_dim values")
-            weights[k] = _on(norm, torch.float32, name, device)
+    if norm_q is not None or norm_k is not None:
+        for k, (name, norm) in enumerate((("norm_q", norm_q), ("norm_k", norm_k))):
+            if norm is not None:
+                if norm.numel() != head_dim:
+                    raise ValueError(f"{name} must hold head_dim values")
+                weights[k] = _on(norm, torch.float32, name, device)
     cos = sin = None
     positions = 0
     if rope_cos is not None or rope_sin is not None:
@@ -547,9 +549,8 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, q_offsets: torch.Te
         data, stride = _rows(logits, logits.dtype, "logits", device), logits.stride(0) if rows > 1 else vocab
         if workspace is None:
             workspace = accept_workspace(rows, sequences, tokens.device)
-        targets = torch.empty(rows, dtype=torch.int32, device=tokens.device)
-    path = torch.empty((sequences, max_path), dtype=torch.int32, device=tokens.device)
-    counts, following = torch.empty((2, sequences), dtype=torch.int32, device=tokens.device)
+        targets = tokens.new_empty(rows)
+    path, counts, following = tokens.new_empty((sequences, max_path)), tokens.new_empty(sequences), tokens.new_empty(sequences)
     check(lib().h4b_tree_accept(data, code, stride, vocab, *at, rows, sequences, max_path,
                                 _on(targets, torch.int32, "targets", device), path.data_ptr(), counts.data_ptr(),
                                 following.data_ptr(),
@@ -566,23 +567,19 @@ def keep_tokens(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.
     [layers][pages][kv_heads][page_size][head_dim] (or one layer's [pages]...)
     caches. Returns the new lengths (int32 [sequences]; `lengths`, if given,
     overlaps neither kv_lens nor counts)."""
-    layered = k_pages.dim() == 5
-    if (not layered and k_pages.dim() != 4) or k_pages.shape != v_pages.shape:
-        raise ValueError("k_pages and v_pages must be [layers][pages][kv_heads][page_size][head_dim]")
-    device, sequences, layers = k_pages.get_device(), kv_lens.numel(), k_pages.shape[0] if layered else 1
-    _on(k_pages, k_pages.dtype, "k_pages", device), _on(v_pages, k_pages.dtype, "v_pages", device)
+    layers, layered = (k_pages.shape[0], True) if k_pages.dim() == 5 else (1, False)
+    kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, 0x7fffffff, layered)
+    device, sequences, shape = k_pages.get_device(), kv.sequences, path.shape
     if layers == 0:
         raise ValueError("k_pages and v_pages must hold a layer")
-    if path.dim() != 2 or path.shape[0] != sequences or path.shape[1] < 1 or counts.numel() != sequences:
+    if len(shape) != 2 or shape[0] != sequences or shape[1] < 1 or counts.numel() != sequences:
         raise ValueError("path must be [sequences][nodes], counts [sequences]")
     if lengths is None:
-        lengths = torch.empty(sequences, dtype=torch.int32, device=kv_lens.device)
+        lengths = torch.empty_like(kv_lens)
     elif lengths.numel() != sequences:
         raise ValueError("lengths must hold one length a sequence")
-    kv = _paged(k_pages[0] if layered else k_pages, v_pages[0] if layered else v_pages, page_table, q_offsets, kv_lens,
-                0x7fffffff)
-    check(lib().h4b_tree_keep(ctypes.byref(kv), layers, k_pages.stride(0) * k_pages.element_size() if layered else 0,
-                              _on(path, torch.int32, "path", device), path.shape[1],
+    check(lib().h4b_tree_keep(ctypes.byref(kv), layers, 2 * kv.pages * kv.kv_heads * kv.page_size * kv.head_dim,
+                              _on(path, torch.int32, "path", device), shape[1],
                               _on(counts, torch.int32, "counts", device), _on(lengths, torch.int32, "lengths", device),
                               _here(device)), "h4b_tree_keep")
     return lengths
