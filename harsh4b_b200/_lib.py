@@ -156,6 +156,7 @@ _SIGNATURES = {
     "h4b_tree_accept_workspace_bytes": [_i32, _i32],
     "h4b_tree_keep": [ctypes.POINTER(PagedKvDesc), _i32, _i64, _vp, _i32, _vp, _vp, _vp],
     "h4b_rmsnorm_quantize_rows": [_vp, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp, _f32, _vp, _vp, _vp, _i32, _i32, _vp],
+    "h4b_forward_paged_tree": [ctypes.POINTER(ModelDesc), ctypes.POINTER(PagedStepDesc), _vp, _vp],
     "h4b_pages_copy": [_vp, _vp, _i32, _i32, _i64, _vp, _vp, _i32, _vp],
     "h4b_lattice_scratch_bytes": [_i32],
     "h4b_lattice_to_int4": [ctypes.POINTER(LatticeProjectionDesc), _vp, _vp, _vp, ctypes.POINTER(_i32), _vp],

@@ -10,6 +10,9 @@
 // of the fp16-cache paths within what the flips of a few codes make of it (2 % of
 // a row's norm in the tests, 5 % at most), not their bits. Where those bits matter
 // the sessions of one contiguous cache have attention="exact".
+//
+// With `parents` the new rows are the nodes of drafted trees: they are appended
+// and attended as such, and the LM head runs on every row.
 
 namespace h4b {
 
@@ -55,7 +58,7 @@ int validate_paged_step(const h4b_model* m, const h4b_paged_step* s) {
     return 0;
 }
 
-int forward_paged(const h4b_model* m, const h4b_paged_step* s, cudaStream_t stream) {
+int forward_paged(const h4b_model* m, const h4b_paged_step* s, const int32_t* parents, cudaStream_t stream) {
     int rc = validate_paged_step(m, s);
     if (rc) return rc;
     const int M = s->kv.tokens, B = s->kv.sequences, H = m->hidden, I = m->intermediate, d = m->head_dim;
@@ -79,12 +82,12 @@ int forward_paged(const h4b_model* m, const h4b_paged_step* s, cudaStream_t stre
         if ((rc = gemm(m->w_qkv + static_cast<size_t>(l) * qkv_rows * (H / 2),
                        m->s_qkv + static_cast<size_t>(l) * qkv_rows, s->qkv, M, qkv_rows, H, false)))
             return rc;
-        if ((rc = h4b_paged_append(&kv, s->qkv, H4B_FP32, qkv_rows, m->heads, m->norm_q + static_cast<size_t>(l) * d,
-                                   m->norm_k + static_cast<size_t>(l) * d, m->eps, m->rope_cos, m->rope_sin, m->max_pos,
-                                   s->q, q_size, stream)))
+        if ((rc = paged_append(&kv, parents, s->qkv, H4B_FP32, qkv_rows, m->heads, m->norm_q + static_cast<size_t>(l) * d,
+                               m->norm_k + static_cast<size_t>(l) * d, m->eps, m->rope_cos, m->rope_sin, m->max_pos, s->q,
+                               q_size, stream)))
             return rc;
-        if ((rc = h4b_paged_attention(&kv, s->q, q_size, m->heads, scale, s->window, s->sinks, s->max_query,
-                                      s->attended16, q_size, nullptr, s->workspace, s->workspace_bytes, stream)))
+        if ((rc = paged_attention(&kv, parents, s->q, q_size, m->heads, scale, s->window, s->sinks, s->max_query,
+                                  s->attended16, q_size, nullptr, s->workspace, s->workspace_bytes, stream)))
             return rc;
         const long long eights = static_cast<long long>(M) * q_size / 8;
         const int grid = static_cast<int>(std::min((eights + 255) / 256, 148ll * 8));
@@ -110,6 +113,10 @@ int forward_paged(const h4b_model* m, const h4b_paged_step* s, cudaStream_t stre
                        H, I, true)))
             return rc;
     }
+    if (parents != nullptr) {
+        if ((rc = norm_quant(s->x, m->norm_final, M))) return rc;
+        return gemm(m->w_embed, m->s_embed, s->logits, M, m->vocab, H, false);
+    }
     last_rows_kernel<<<B, 256, 0, stream>>>(s->x, s->kv.q_offsets, M, H, s->last);
     H4B_CUDA_TRY(cudaGetLastError());
     if ((rc = norm_quant(s->last, m->norm_final, B))) return rc;
@@ -122,5 +129,11 @@ int forward_paged(const h4b_model* m, const h4b_paged_step* s, cudaStream_t stre
 }  // namespace h4b
 
 extern "C" int h4b_forward_paged(const h4b_model* model, const h4b_paged_step* step, void* stream) {
-    return h4b::forward_paged(model, step, static_cast<cudaStream_t>(stream));
+    return h4b::forward_paged(model, step, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int h4b_forward_paged_tree(const h4b_model* model, const h4b_paged_step* step, const int32_t* parents,
+                                      void* stream) {
+    if (parents == nullptr) return H4B_EINVAL;
+    return h4b::forward_paged(model, step, parents, static_cast<cudaStream_t>(stream));
 }

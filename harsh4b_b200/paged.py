@@ -17,6 +17,9 @@ any number of sequences in one step.
     logits = runner.step({first: prompt_ids})[first]
     second = cache.fork(first)                      # shares the prompt's pages
     logits = runner.step({first: [a], second: [b]})
+
+``verify`` runs a drafted tree of tokens for each sequence in one step and keeps
+the branch that agrees with the model's greedy tokens.
 """
 from __future__ import annotations
 
@@ -27,7 +30,7 @@ import numpy as np
 import torch
 
 from . import ops
-from ._lib import STATUS_BAD_PAGE, PagedKvDesc, PagedStepDesc, check, device_status, lib
+from ._lib import STATUS_BAD_PAGE, TREE_NODES, PagedKvDesc, PagedStepDesc, check, device_status, lib
 
 CACHE_DTYPES = {"float16": torch.float16, "bfloat16": torch.bfloat16}
 
@@ -303,25 +306,17 @@ class PagedRunner:
         self.gate_up, self.act = torch.zeros(M, 2 * I, **f32), torch.zeros(M, I, **f32)
         self.last, self.logits = torch.zeros(B, H, **f32), torch.zeros(B, model.vocab, **f32)
         self.workspace = ops.paged_workspace(model.head_dim, dev)
+        self.node_logits = self.accept_workspace = None  # verify's
 
     def step(self, feed: dict[int, list[int]]) -> dict[int, torch.Tensor]:
         """Append feed[sequence] (token ids, at least one each) to each sequence
         and return the logits after its last one (views, overwritten by the
         next step)."""
         sequences = list(feed)
-        rows = [[int(t) for t in feed[s]] for s in sequences]
-        new = [len(r) for r in rows]
-        total = sum(new)
-        if not sequences or min(new) < 1:
-            raise ValueError("every sequence of a step needs a token")
-        if total > self.max_tokens or len(sequences) > self.max_sequences:
-            raise ValueError(f"a step holds {self.max_tokens} tokens of {self.max_sequences} sequences")
-        ids = np.fromiter((t for r in rows for t in r), dtype=np.int32, count=total)
-        if ids.min() < 0 or ids.max() >= self.model.vocab:
-            raise ValueError("token ID outside the vocabulary")
-        cache, model = self.cache, self.model
-        if max(cache.length(s) + n for s, n in zip(sequences, new)) > model.max_pos:
-            raise ValueError(f"a sequence would pass the model's {model.max_pos} positions")
+        ids, new = self._checked([[int(t) for t in feed[s]] for s in sequences])
+        cache = self.cache
+        if max(cache.length(s) + n for s, n in zip(sequences, new)) > self.model.max_pos:
+            raise ValueError(f"a sequence would pass the model's {self.model.max_pos} positions")
         for s in sequences:
             cache.check_visible(s, self.window, self.sinks)
         with cache.ordered():
@@ -333,9 +328,68 @@ class PagedRunner:
                 cache.trim(s, self.window, self.sinks)
         return {s: self.logits[b] for b, s in enumerate(sequences)}
 
-    def _launch(self, sequences, new, ids: np.ndarray) -> None:
+    def verify(self, drafts: dict[int, tuple[list[int], list[int]]]) -> dict[int, list[int]]:
+        """One step over a drafted tree of tokens for each sequence:
+        drafts[sequence] = (token ids, parents), node 0 the token that follows
+        the sequence's cached ones (decided before, parent -1), every other
+        node a child of an earlier one; at most 256 nodes. Node 0 and the
+        branch that agrees with the model's greedy tokens stay in the cache.
+        Returns the greedy tokens that follow node 0: the accepted branch's
+        and the one after it, of which the last is not in the cache (node 0 of
+        the next tree). The nodes' logits are `node_logits` until the next
+        call."""
+        sequences = list(drafts)
+        ids, new = self._checked([[int(t) for t in drafts[s][0]] for s in sequences])
+        trees = [[int(p) for p in drafts[s][1]] for s in sequences]
+        cache, model = self.cache, self.model
+        for s, tree, n in zip(sequences, trees, new):
+            if len(tree) != n or n > TREE_NODES:
+                raise ValueError(f"a tree has a parent for each of its nodes, at most {TREE_NODES}")
+            if tree[0] != -1 or not all(0 <= p < i for i, p in enumerate(tree) if i):
+                raise ValueError("a tree's node 0 is its root, the others have earlier parents")
+            if cache.length(s) + n > model.max_pos:
+                raise ValueError(f"a sequence would pass the model's {model.max_pos} positions")
+            cache.check_visible(s, self.window, self.sinks)
+        total = len(ids)
+        with cache.ordered():
+            cache.reserve(dict(zip(sequences, new)))
+            if self.node_logits is None or self.node_logits.shape[0] < total:
+                self.node_logits = None  # (given back first)
+                self.node_logits = torch.empty(total, model.vocab, dtype=torch.float32, device=cache.device)
+            if self.accept_workspace is None:
+                self.accept_workspace = ops.accept_workspace(self.max_tokens, self.max_sequences, cache.device)
+            parents = torch.tensor([p for tree in trees for p in tree], dtype=torch.int32).to(cache.device)
+            table, offsets, lengths = self._launch(sequences, new, ids, parents)
+            path, counts, _, targets = ops.accept_tree(self.tokens[:total], parents, offsets, self.node_logits[:total],
+                                                       max_path=max(new), workspace=self.accept_workspace)
+            ops.keep_tokens(cache.k_pages, cache.v_pages, table, offsets, lengths, path, counts)
+            path, counts, targets = path.tolist(), counts.tolist(), targets.tolist()
+        result, first = {}, 0
+        for b, (s, n) in enumerate(zip(sequences, new)):
+            result[s] = [targets[first + node] for node in path[b][:counts[b]]]
+            first += n
+            cache.advance(s, counts[b])
+            if self.window:
+                cache.trim(s, self.window, self.sinks)
+        return result
+
+    def _checked(self, rows: list[list[int]]) -> tuple[np.ndarray, list[int]]:
+        """A step's token ids, one sequence after the other, and how many each has."""
+        new = [len(r) for r in rows]
+        total = sum(new)
+        if not rows or min(new) < 1:
+            raise ValueError("every sequence of a step needs a token")
+        if total > self.max_tokens or len(rows) > self.max_sequences:
+            raise ValueError(f"a step holds {self.max_tokens} tokens of {self.max_sequences} sequences")
+        ids = np.fromiter((t for r in rows for t in r), dtype=np.int32, count=total)
+        if ids.min() < 0 or ids.max() >= self.model.vocab:
+            raise ValueError("token ID outside the vocabulary")
+        return ids, new
+
+    def _launch(self, sequences, new, ids: np.ndarray, parents: torch.Tensor | None = None):
         cache, model, total = self.cache, self.model, len(ids)
-        table, offsets, lengths = (torch.from_numpy(a).to(cache.device) for a in cache.batch_tables(sequences, new))
+        tables = table, offsets, lengths = tuple(torch.from_numpy(a).to(cache.device)
+                                                 for a in cache.batch_tables(sequences, new))
         self.tokens[:total].copy_(torch.from_numpy(ids))
         layers, pages, kv_heads, page_size, head_dim = cache.k_pages.shape
         code = 1 if cache.k_pages.dtype == torch.float16 else 2
@@ -344,9 +398,15 @@ class PagedRunner:
                          total)
         step = PagedStepDesc(kv, cache.k_pages[0].numel() * 2, self.window, self.sinks, max(new), *[t.data_ptr() for t in (
             self.tokens, self.x, self.x8, self.act_scale, self.act_sum, self.qkv, self.q, self.attended16, self.attended,
-            self.gate_up, self.act, self.last, self.logits, self.next_tokens, self.workspace)], self.workspace.numel())
-        check(lib().h4b_forward_paged(ctypes.byref(model.desc), ctypes.byref(step),
-                                      torch.cuda.current_stream(cache.device).cuda_stream), "h4b_forward_paged")
+            self.gate_up, self.act, self.last, self.logits if parents is None else self.node_logits, self.next_tokens,
+            self.workspace)], self.workspace.numel())
+        stream = torch.cuda.current_stream(cache.device).cuda_stream
+        if parents is None:
+            check(lib().h4b_forward_paged(ctypes.byref(model.desc), ctypes.byref(step), stream), "h4b_forward_paged")
+        else:
+            check(lib().h4b_forward_paged_tree(ctypes.byref(model.desc), ctypes.byref(step), parents.data_ptr(), stream),
+                  "h4b_forward_paged_tree")
+        return tables
 
     def status(self) -> None:
         """Raise if a kernel met a page, offset or length out of range."""

@@ -608,6 +608,11 @@ typedef struct h4b_paged_step {
 } h4b_paged_step;
 int h4b_forward_paged(const h4b_model *model, const h4b_paged_step *step, void *stream);
 
+/* The same where each sequence's rows are the nodes of a drafted tree (parents:
+ * int32 [T], as above): logits [T][vocab] belong to every row, for
+ * h4b_tree_accept. `last` and next_tokens are not used (but given). */
+int h4b_forward_paged_tree(const h4b_model *model, const h4b_paged_step *step, const int32_t *parents, void *stream);
+
 /* Residual addition, RMSNorm and int8 rows in one call, the input of
  * h4b_int4_gemm: s = x + delta, y = (s / sqrt(mean(s^2) + eps)) * weight,
  * x8 = clamp(rint(y * 127/m), -127, 127) with m = max(absmax(y), 1e-5), scales = m / 127,
