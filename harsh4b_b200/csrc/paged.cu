@@ -108,17 +108,45 @@ __device__ __forceinline__ int checked_parent(int parent, int node) {
     return -1;
 }
 // Parent by parent up to the root: node `i`'s depth, and in `sight` (kTreeWords
-// words, may be null) the nodes that it sees, itself among them: with a window
-// those less than `window` above it, or at positions below `sinks`.
+// words) the nodes that it sees, itself among them: with a window those less than
+// `window` above it, or at positions below `sinks`.
 __device__ __forceinline__ int walk_tree(const int32_t* parents, int i, int base, int window, int sinks, uint32_t* sight) {
     int depth = 0;
     for (int j = checked_parent(parents[i], i); j >= 0; j = checked_parent(parents[j], j)) ++depth;
-    if (sight != nullptr) {
 #pragma unroll
-        for (int w = 0; w < kTreeWords; ++w) sight[w] = 0u;
-        int up = 0;
-        for (int j = i; j >= 0; j = checked_parent(parents[j], j), ++up)
-            if (window <= 0 || up < window || base + depth - up < sinks) sight[j >> 5] |= 1u << (j & 31);
+    for (int w = 0; w < kTreeWords; ++w) sight[w] = 0u;
+    int up = 0;
+    for (int j = i; j >= 0; j = checked_parent(parents[j], j), ++up)
+        if (window <= 0 || up < window || base + depth - up < sinks) sight[j >> 5] |= 1u << (j & 31);
+    return depth;
+}
+// By a whole warp, for 32 consecutive nodes from `first` on (parent: this lane's, of
+// node first + lane, -1 past the last): the nodes of these that the lane's node
+// descends from, as bits, and the parent of the topmost of them (an earlier node,
+// or -1). By doubling the step: a node's set joins that of the node its step leads
+// to, so a chain takes no longer than a bush.
+__device__ __forceinline__ uint32_t descent(int parent, int first, int* above) {
+    const int lane = threadIdx.x & 31;
+    uint32_t set = 1u << lane;
+    int to = parent >= first ? parent & 31 : lane;  // where the step leads: itself at the top
+#pragma unroll
+    for (int r = 0; r < 5; ++r) {
+        set |= __shfl_sync(0xffffffffu, set, to);
+        to = __shfl_sync(0xffffffffu, to, to);
+    }
+    *above = __shfl_sync(0xffffffffu, parent, to);
+    return set;
+}
+// Node `i`'s depth, by a whole warp.
+__device__ __forceinline__ int node_depth(const int32_t* parents, int i) {
+    const int lane = threadIdx.x & 31;
+    int depth = -1;
+    while (i >= 0) {
+        const int first = i & ~31, j = first + lane;
+        int above;
+        const uint32_t set = descent(j <= i ? checked_parent(parents[j], j) : -1, first, &above);
+        depth += __popc(__shfl_sync(0xffffffffu, set, i & 31));
+        i = __shfl_sync(0xffffffffu, above, i & 31);
     }
     return depth;
 }
@@ -214,7 +242,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const A
         const SequenceSpan s = sequence_span<TREE>(a.p, b);
         position = token < s.first + s.count ? s.base + token - s.first : -1;
         if constexpr (TREE)
-            if (position >= 0) depth = walk_tree(a.parents + s.first, token - s.first, 0, 0, 0, nullptr) - (token - s.first);
+            if (position >= 0) depth = node_depth(a.parents + s.first, token - s.first) - (token - s.first);
         if (position >= 0) {
             const int page = a.p.table[static_cast<long long>(b) * a.p.table_stride + (position >> a.p.page_shift)];
             if (page >= 0 && page < a.p.pages) {
@@ -415,16 +443,20 @@ struct Range {
     int ctas;                     // that have a range: every one of them has a place at least
     SequenceSpan span;            // of that sequence (trees only: the others look it up)
 };
-// n / d of numbers that are not negative, in 32 bits where they fit: a 64-bit division
-// is a long piece of code, and what runs once a launch runs cold.
+// n / d of numbers that are not negative, with SHORT in 32 bits where they fit: a
+// 64-bit division is a long piece of code, and what runs once a launch runs cold (a
+// tree's items take many roles' warps to their start).
+template <bool SHORT>
 __device__ __forceinline__ long long quotient(long long n, long long d) {
-    if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+    if (SHORT && ((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
     return n / d;
 }
-__device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return quotient(total * cta, ctas); }
+template <bool SHORT>
+__device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return quotient<SHORT>(total * cta, ctas); }
 // The CTA that holds a place: the largest c with range_begin(c) <= place.
+template <bool SHORT>
 __device__ __forceinline__ int range_owner(long long total, long long place, int ctas) {
-    return static_cast<int>(quotient((place + 1) * ctas - 1, total));
+    return static_cast<int>(quotient<SHORT>((place + 1) * ctas - 1, total));
 }
 
 // Every thread of the CTA takes part; `shared` holds THREADS / 32 long longs
@@ -464,8 +496,8 @@ __device__ __forceinline__ Range find_range(const AttendArgs& a, int tile_tokens
     r.ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + a.least - 1) / a.least));
     r.begin = r.end = 0;
     if (static_cast<int>(blockIdx.x) < r.ctas) {
-        r.begin = range_begin(total, blockIdx.x, r.ctas);
-        r.end = range_begin(total, blockIdx.x + 1, r.ctas);
+        r.begin = range_begin<TREE>(total, blockIdx.x, r.ctas);
+        r.end = range_begin<TREE>(total, blockIdx.x + 1, r.ctas);
     }
     const bool here = r.begin < r.end && r.begin >= before && r.begin < before + mine;
     if (__any_sync(0xffffffffu, here)) {
@@ -536,7 +568,7 @@ struct Walk {
         }
         tile = make_tile<KEYS, TREE>(span, t, tile_tokens, a.window, a.sinks);
         const int places = a.extra + tile.units();
-        h = static_cast<int>(quotient(skip, places));
+        h = static_cast<int>(quotient<TREE>(skip, places));
         unit = static_cast<int>(skip - static_cast<long long>(h) * places) - a.extra;
         if (unit < 0) {
             left += unit;
@@ -581,8 +613,8 @@ struct Walk {
 template <int KEYS, bool TREE>
 __device__ __forceinline__ int2 item_owners(const Range& range, const Walk<KEYS, TREE>& w) {
     const long long first = range.end - w.left - w.unit;
-    return make_int2(range_owner(range.total, first, range.ctas),
-                     range_owner(range.total, first + w.tile.units() - 1, range.ctas));
+    return make_int2(range_owner<TREE>(range.total, first, range.ctas),
+                     range_owner<TREE>(range.total, first + w.tile.units() - 1, range.ctas));
 }
 
 // Whether some row of the tile sees key j.

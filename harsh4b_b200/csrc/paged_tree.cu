@@ -22,10 +22,14 @@
 //
 // A node sees the tokens before the tree and, of the tree, the nodes whose bits
 // its walk to the root set (sight); blocks that hold only keys that every row
-// sees need no mask. The scores are taken in their own unit: p = 2^((s - m) scale
-// + 8) with m a score, so equal scores cancel exactly whatever their size; m moves
-// only where a score passes it by 2^7. p is rounded to the cache's type for the
-// product as in the other kernels (see paged.cu), l is its fp32 sum.
+// sees need no mask. p = 2^(s scale - b + 8) with b the product m scale of a score m,
+// rounded on its own: what the rounding adds to b it adds to all weights of the row
+// alike, and the log-sum-exp takes it off again. m moves only where a score passes it
+// by 2^7. From |b| = 2^20 on, where the rounding would reach p's exponent, p = 2^((s - m)
+// scale + 8), in which equal scores cancel whatever their size: one more operation a
+// pair, which costs nothing in time but, under the power cap, clock (16 x 32 nodes
+// over 32768 tokens, sustained: 420 -> 411 us without it). p is rounded to the cache's
+// type for the product as in the other kernels (see paged.cu), l is its fp32 sum.
 //
 // V rows of keys that no row sees are zeroed and values that are not finite are
 // taken out of rows that only some see, and added at the item's end, as in
@@ -82,10 +86,9 @@ __device__ __forceinline__ bool warp_test(uint64_t* bar, uint32_t parity) {
 
 // What each of a sequence's first `nodes` nodes sees of the tree, as bits, and its
 // depth. By one warp, 32 nodes at a time, whose parents are among them or earlier:
-// within the 32 by doubling the step (a node's set joins that of the node its step
-// leads to), then the set of the earlier node that the topmost one hangs from. So
-// a chain takes no longer than a bush. With a window (of fewer than all nodes) what
-// lies too far above is taken out at the end.
+// its descent within the 32, and the set of the earlier node that the topmost of
+// them hangs from. With a window (of fewer than all nodes) what lies too far above
+// is taken out at the end.
 __device__ __forceinline__ void find_sights(const int (&parent)[kTreeWords], int nodes, int base, int window, int sinks,
                                             uint32_t* sights, int16_t* depths) {
     const int lane = threadIdx.x & 31;
@@ -94,14 +97,8 @@ __device__ __forceinline__ void find_sights(const int (&parent)[kTreeWords], int
         if (32 * k >= nodes) break;
         const int i = 32 * k + lane;
         const int p = i < nodes ? checked_parent(parent[k], i) : -1;
-        uint32_t mine = 1u << lane;
-        int to = p >= 32 * k ? p & 31 : lane;  // where the step leads: itself at the top
-#pragma unroll
-        for (int r = 0; r < 5; ++r) {
-            mine |= __shfl_sync(0xffffffffu, mine, to);
-            to = __shfl_sync(0xffffffffu, to, to);
-        }
-        const int above = __shfl_sync(0xffffffffu, p, to);  // of the topmost: an earlier node, or -1
+        int above;
+        const uint32_t mine = descent(p, 32 * k, &above);
         uint32_t* bits = sights + i * kTreeWords;
 #pragma unroll
         for (int w = 0; w < kTreeWords; ++w) bits[w] = w < k ? (above >= 0 ? sights[above * kTreeWords + w] : 0u) : w == k ? mine : 0u;
@@ -123,6 +120,13 @@ __device__ __forceinline__ void find_sights(const int (&parent)[kTreeWords], int
         }
     }
     __syncwarp();
+}
+
+// What weights relative to score m are worth relative to `top`, the way the weights
+// were formed (see above).
+__device__ __forceinline__ float reference_factor(float m, float top, float scale) {
+    const float b = __fmul_rn(top, scale);
+    return is_huge(b) ? ex2_approx((m - top) * scale) : ex2_approx(__fsub_rn(__fmul_rn(m, scale), b));
 }
 
 // Whether every row of the tile sees keys `key` .. `end`.
@@ -517,8 +521,8 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
                 const uint32_t low = sight[off >> 5], high = (off >> 5) + 1 < kTreeWords ? sight[(off >> 5) + 1] : 0u;
                 return earlier | __funnelshift_r(low, high, off & 31);
             };
-            float m = -INFINITY, l = 0.f;
-            bool done = false;
+            float m = -INFINITY, l = 0.f, offset = 8.f;  // offset: 8 - b
+            bool done = false, huge = false;
             while (true) {
                 const uint32_t x = 2 * t + (n & 1), s_col = lane_base + C::kSCol + kTreeKeys * x;
                 ok = warp_wait(&s_full[x], (n >> 1) & 1);
@@ -558,20 +562,36 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
                         ok = warp_wait(&pv_done[x ^ 1], ((n - 1) >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        const float f = move ? ex2_approx((m - mx) * a.scale) : 1.f;  // 0 for m = -inf, whose l and O are 0
+                        const float f = move ? reference_factor(m, mx, a.scale) : 1.f;  // 0 for m = -inf, whose l and O are 0
                         l *= f;
                         rescale_row<D>(o_col, f);
                     }
-                    if (move) m = mx;
-                    const float less = m == -INFINITY ? 0.f : -m;
-                    const uint64_t less2 = pack2(less, less), scale2 = pack2(a.scale, a.scale), eight2 = pack2(8.f, 8.f);
+                    if (__any_sync(0xffffffffu, move)) {
+                        if (move) {
+                            m = mx;
+                            offset = __fsub_rn(8.f, __fmul_rn(m, a.scale));
+                        }
+                        huge = __any_sync(0xffffffffu, valid && is_huge(offset)) != 0;
+                    }
+                    uint64_t scale2 = pack2(a.scale, a.scale), offset2 = pack2(offset, offset);
+                    if (huge) {
+                        // (the scores less m, scaled: s - m here, the rest below)
+                        const float less = m == -INFINITY ? 0.f : -m;
+                        const uint64_t less2 = pack2(less, less);
+#pragma unroll
+                        for (int k = 0; k < kTreeKeys; k += 2) {
+                            const float2 y = unpack2(add2(pack2(v[k], v[k + 1]), less2));
+                            v[k] = y.x, v[k + 1] = y.y;
+                        }
+                        offset2 = pack2(8.f, 8.f);
+                    }
                     uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
                     for (int c = 0; c < kTreeKeys; c += 32) {
                         uint32_t p16[16];
 #pragma unroll
                         for (int k = 0; k < 32; k += 2) {
-                            const uint64_t p2 = exp2_pair(fma2(add2(pack2(v[c + k], v[c + k + 1]), less2), scale2, eight2));
+                            const uint64_t p2 = exp2_pair(fma2(pack2(v[c + k], v[c + k + 1]), scale2, offset2));
                             sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], p2);
                             const float2 p = unpack2(p2);
                             p16[k / 2] = Pair<T>::pack(p.x, p.y);
@@ -667,7 +687,7 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
             if (whole) {
                 if (valid && a.lse != nullptr)
                     a.lse[static_cast<long long>(first_row + node) * a.heads + w.h * a.group + head] =
-                        l == 0.f ? -INFINITY : (m * a.scale - 8.f) * 0.6931471805599453f + logf(l);
+                        l == 0.f ? -INFINITY : (__fmul_rn(m, a.scale) - 8.f) * 0.6931471805599453f + logf(l);
             } else {
                 if (valid) __stcg(reinterpret_cast<float2*>(part + D / 4 * kChunkRows) + row, make_float2(m, l));
                 if (threadIdx.x == 0 && begun)  // the item's first part: what the join needs to know
@@ -728,7 +748,7 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
         for (int u = 0; u < kJoinAhead; ++u) {
             if (ml[u].y == 0.f) continue;  // saw no key
             const float most = fmaxf(top, ml[u].x);
-            const float f = total == 0.f ? 0.f : ex2_approx((top - most) * a.scale), g = ex2_approx((ml[u].x - most) * a.scale);
+            const float f = total == 0.f ? 0.f : reference_factor(top, most, a.scale), g = reference_factor(ml[u].x, most, a.scale);
             top = most;
             total = total * f + ml[u].y * g;
 #pragma unroll
@@ -741,8 +761,8 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
     // the two sides
     const float top1 = __shfl_down_sync(0xffffffffu, top, 16), total1 = __shfl_down_sync(0xffffffffu, total, 16);
     const float most = fmaxf(top, top1);
-    const float f = total == 0.f ? 0.f : ex2_approx((top - most) * a.scale);
-    const float g = total1 == 0.f ? 0.f : ex2_approx((top1 - most) * a.scale);
+    const float f = total == 0.f ? 0.f : reference_factor(top, most, a.scale);
+    const float g = total1 == 0.f ? 0.f : reference_factor(top1, most, a.scale);
     total = total * f + total1 * g;
     const float scale = total != 0.f ? 1.0f / total : 0.f;
     uint32_t words[2 * kCols];
@@ -762,7 +782,7 @@ __global__ void __launch_bounds__(kTreeJoinThreads) tree_join_kernel(const Atten
         *reinterpret_cast<uint4*>(out + 2 * k) = make_uint4(words[k], words[k + 1], words[k + 2], words[k + 3]);
     if (a.lse != nullptr && c == 0)
         a.lse[out_row * a.heads + out_head] =
-            total == 0.f ? -INFINITY : (most * a.scale - 8.f) * 0.6931471805599453f + logf(total);
+            total == 0.f ? -INFINITY : (__fmul_rn(most, a.scale) - 8.f) * 0.6931471805599453f + logf(total);
 }
 
 template <typename T, int D, int ROWS, int TILES>

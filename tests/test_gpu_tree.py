@@ -117,6 +117,15 @@ def test_window_and_sinks(heads, kv_heads, dim, page, dtype, window, sinks):
           sinks=sinks, seed=2).check()
 
 
+@pytest.mark.parametrize("page", [16, 512, 1024])
+@pytest.mark.parametrize("n", [3, 20, 33])
+def test_page_sizes(n, page):
+    """Pages that end inside a tile, and tiles inside a page (one and two tiles of rows)."""
+    for dim in (64, 128):
+        Trees([draft(n, 4), draft(n, 2, seed=1)], [1500 + n, 1020 + n], heads=16, kv_heads=2, dim=dim, page=page,
+              dtype=torch.bfloat16, seed=7).check()
+
+
 @pytest.mark.parametrize("hint", [1, 2, 4, 20, 256, 100000])
 def test_the_expected_size_changes_no_answer(hint):
     parents = [draft(n, 4, seed=n) for n in (1, 9, 70, 0, 256)]

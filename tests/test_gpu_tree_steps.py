@@ -411,3 +411,80 @@ def test_a_layer_of_a_verify_step():
             assert torch.equal(k[where[0], :, where[1]], slow_k[where[0], :, where[1]])
             assert torch.equal(v[where[0], :, where[1]], slow_v[where[0], :, where[1]])
     assert int(lens[0]) > 42 and _lib.device_status() == 0
+
+
+def test_a_captured_step_follows_its_inputs():
+    """Norm, append, attention, acceptance and keep in one graph, replayed with other trees, logits and lengths, on another
+    stream than the tensors'."""
+    heads, kv_heads, dim, page, vocab = 8, 2, 128, 16, 700
+    width = (heads + 2 * kv_heads) * dim
+    g = torch.Generator("cuda").manual_seed(1)
+    weight = torch.rand(width, generator=g, device="cuda") + 0.5
+    angles = torch.rand(400, dim // 2, generator=g, device="cuda") * 6
+    rope = dict(rope_cos=angles.cos(), rope_sin=angles.sin())
+    table = torch.randperm(40, generator=g, device="cuda").to(torch.int32).view(2, 20)
+    offsets = ints([0, 40, 47])
+
+    def inputs(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        trees = [draft(40, 3, seed=seed), draft(7, 2, seed=seed + 1)]
+        targets, tokens = drafted(trees, vocab, seed)
+        logits = torch.randn(47, vocab, generator=g, device="cuda")
+        logits.scatter_(1, torch.tensor(targets, device="cuda")[:, None], 9.0)
+        pages = torch.randn(2, 40, kv_heads, page, dim, generator=g, device="cuda").half()
+        return dict(x=torch.randn(47, width, generator=g, device="cuda"), delta=torch.randn(47, width, generator=g, device="cuda"),
+                    parents=ints([p for t in trees for p in t]), tokens=ints(tokens), logits=logits,
+                    lens=ints([40 + 31 * seed, 7 + 90 * seed]), k=pages[0].clone(), v=pages[1].clone())
+
+    attend, accept = ops.paged_workspace(), ops.accept_workspace(47, 2)
+
+    def step(s):
+        x8, scales, sums = ops.rmsnorm_quantize_rows(s["x"], weight, 1e-6, delta=s["delta"])
+        q = ops.paged_append(s["x"], s["k"], s["v"], table, offsets, s["lens"], heads=heads, parents=s["parents"], **rope)
+        out = ops.paged_tree_attention(q, s["k"], s["v"], table, offsets, s["lens"], s["parents"], workspace=attend)
+        path, counts, following, targets = ops.accept_tree(s["tokens"], s["parents"], offsets, s["logits"], max_path=9,
+                                                           workspace=accept)
+        lengths = ops.keep_tokens(s["k"], s["v"], table, offsets, s["lens"], path, counts)
+        return [x8, scales, sums, s["x"], out, path, counts, following, targets, lengths, s["k"], s["v"]]
+
+    want = {seed: [t.clone() for t in step(inputs(seed))] for seed in (1, 2, 3)}
+    held = inputs(1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step(held)
+    for seed in (2, 3, 1, 3):
+        fresh = inputs(seed)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for name, t in held.items():
+                t.copy_(fresh[name])
+            graph.replay()
+        stream.synchronize()
+        for a, b in zip(got, want[seed]):
+            assert torch.equal(a, b)
+    assert _lib.device_status() == 0
+
+
+def test_accept_and_keep_run_on_the_current_stream():
+    trees = FORESTS["few"]
+    targets, tokens = drafted(trees, 50, 3)
+    logits = torch.zeros(13, 50, device="cuda")
+    want = torch.zeros_like(logits).scatter_(1, torch.tensor(targets, device="cuda")[:, None], 9.0)
+    k = torch.randn(1, 8, 1, 16, 64, device="cuda").half()
+    v, table = k.clone(), torch.arange(5, dtype=torch.int32, device="cuda").view(5, 1)
+    offsets, lens, parents = offsets_of(trees), ints([9, 1, 7, 0, 3]), ints([p for t in trees for p in t])
+    ids = ints(tokens)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        workspace = ops.accept_workspace(13, 5)
+        torch.cuda._sleep(20_000_000)
+        logits.copy_(want)
+        path, counts, following, _ = ops.accept_tree(ids, parents, offsets, logits, max_path=8, workspace=workspace)
+        lengths = ops.keep_tokens(k, v, table, offsets, lens, path, counts)
+    stream.synchronize()
+    paths, numbers, tokens_after = follow(trees, tokens, targets, 8)
+    assert (path.tolist(), counts.tolist(), following.tolist()) == (paths, numbers, tokens_after)
+    assert lengths.tolist() == [n - len(t) + c for n, t, c in zip(lens.tolist(), trees, numbers)]
