@@ -37,11 +37,53 @@ struct NormRowsArgs {
     long long x_stride, delta_stride, out_stride;
     const float* weight;
     float eps;
-    int width;
+    int rows, width;
     int8_t* x8;
     float* scales;
     int32_t* sums;
 };
+
+// Eight quantised values; their sum.
+__device__ __forceinline__ int quantize_eight(int8_t* x8, const float (&v)[8], float qs) {
+    uint32_t w[2] = {0u, 0u};
+    int sum = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int q = quantize_one(v[e], qs);
+        sum += q;
+        w[e >> 2] |= static_cast<uint32_t>(q & 0xFF) << (8 * (e & 3));
+    }
+    *reinterpret_cast<uint2*>(x8) = make_uint2(w[0], w[1]);
+    return sum;
+}
+__device__ __forceinline__ float inverse_rms(float ss, const NormRowsArgs& a) {
+    const float mean = __fdiv_rn(ss, static_cast<float>(a.width));
+    return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.eps)));
+}
+__device__ __forceinline__ void scale_eight(float (&v)[8], float inv, const float (&gm)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], inv), gm[e]);
+}
+__device__ __forceinline__ float largest_of(float most, const float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+    return most;
+}
+// The row's sum of codes over the CTA, and its two numbers out. `ired` may be
+// written again after the CTA's next two barriers.
+__device__ __forceinline__ void finish_row(const NormRowsArgs& a, long long row, float m, int sum, int* ired) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((tid & 31) == 0) ired[tid >> 5] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        int t = 0;
+        for (int w = 0; w < 8; ++w) t += ired[w];
+        a.sums[row] = t;
+        a.scales[row] = dequant_scale(m);
+    }
+}
 
 // One CTA a row. kG groups of 8 a thread stay in registers; kG = 0: rows too
 // wide for that are read in each of three passes (a thread its own values, so
@@ -68,20 +110,7 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormRowsArgs a) {
     auto normed = [&](int g, float inv, float (&v)[8]) {
         float gm[8];
         load8(a.weight + 8 * g, gm);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __fmul_rn(__fmul_rn(v[e], inv), gm[e]);
-    };
-    auto quantize = [&](int g, float qs, const float (&v)[8]) {
-        uint32_t w[2] = {0u, 0u};
-        int sum = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int q = quantize_one(v[e], qs);
-            sum += q;
-            w[e >> 2] |= static_cast<uint32_t>(q & 0xFF) << (8 * (e & 3));
-        }
-        *reinterpret_cast<uint2*>(x8 + 8 * g) = make_uint2(w[0], w[1]);
-        return sum;
+        scale_eight(v, inv, gm);
     };
     constexpr int kHeld = kG > 0 ? kG : 1;
     float v[kHeld][8];
@@ -102,9 +131,7 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormRowsArgs a) {
             for (int e = 0; e < 8; ++e) ss = __fmaf_rn(v[0][e], v[0][e], ss);
         }
     }
-    ss = group_sum(ss, red, 8, 1);
-    const float mean = __fdiv_rn(ss, static_cast<float>(a.width));
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.eps)));
+    const float inv = inverse_rms(group_sum(ss, red, 8, 1), a);
     float local = 0.f;
     if constexpr (kG > 0) {
 #pragma unroll
@@ -113,15 +140,13 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormRowsArgs a) {
             if (g >= groups) continue;
             if (out) store_eight(out + 8 * g, v[k]);
             normed(g, inv, v[k]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) local = fmaxf(local, fabsf(v[k][e]));
+            local = largest_of(local, v[k]);
         }
     } else {
         for (int g = tid; g < groups; g += 256) {
             load(g, v[0]);
             normed(g, inv, v[0]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) local = fmaxf(local, fabsf(v[0][e]));
+            local = largest_of(local, v[0]);
         }
     }
     const float m = group_max(local, red, 8, 1);
@@ -130,47 +155,222 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormRowsArgs a) {
     if constexpr (kG > 0) {
 #pragma unroll
         for (int k = 0; k < kG; ++k)
-            if (tid + 256 * k < groups) sum += quantize(tid + 256 * k, qs, v[k]);
+            if (tid + 256 * k < groups) sum += quantize_eight(x8 + 8 * (tid + 256 * k), v[k], qs);
     } else {
         for (int g = tid; g < groups; g += 256) {
             load(g, v[0]);
             if (out) store_eight(out + 8 * g, v[0]);
             normed(g, inv, v[0]);
-            sum += quantize(g, qs, v[0]);
+            sum += quantize_eight(x8 + 8 * g, v[0], qs);
         }
     }
+    finish_row(a, row, m, sum, ired);
+}
+
+// Rows of up to 128 groups: a warp a row, without a barrier. Its lane l stands for the
+// lanes l of the first kWarps warps above (the others' sums are zeros), whose sums it
+// forms one after the other in the same order (16384 rows of 512 in bf16 33 -> 13 us,
+// 10000 of 1000 in fp32 21 -> 13; 16384 of 2048 in bf16 49, a warp a row 68).
+template <typename X, typename DT, int kWarps>
+__global__ void __launch_bounds__(256) norm_rows_warp_kernel(const NormRowsArgs a) {
+    const long long row = blockIdx.x * 8ll + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, groups = a.width >> 3;
+    if (row >= a.rows) return;
+    const X* x = static_cast<const X*>(a.x) + row * a.x_stride;
+    const DT* delta = a.delta ? static_cast<const DT*>(a.delta) + row * a.delta_stride : nullptr;
+    X* out = a.out ? static_cast<X*>(a.out) + row * a.out_stride : nullptr;
+    int8_t* x8 = a.x8 + row * a.width;
+    float v[kWarps][8], ss[kWarps];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((tid & 31) == 0) ired[tid >> 5] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        int t = 0;
-        for (int w = 0; w < 8; ++w) t += ired[w];
-        a.sums[row] = t;
+    for (int w = 0; w < kWarps; ++w) {
+        const int g = 32 * w + lane;
+        ss[w] = 0.f;
+        if (g >= groups) continue;
+        load_eight(x + 8 * g, v[w]);
+        if (delta) {
+            float d[8];
+            load_eight(delta + 8 * g, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[w][e] = __fadd_rn(v[w][e], d[e]);
+        }
+    }
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (32 * w + lane < groups) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss[w] = __fmaf_rn(v[w][e], v[w][e], ss[w]);
+        }
+        total += warp_sum(ss[w]);
+    }
+    const float inv = inverse_rms(total, a);
+    float m = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const int g = 32 * w + lane;
+        if (g >= groups) continue;
+        if (out) store_eight(out + 8 * g, v[w]);
+        float gm[8];
+        load8(a.weight + 8 * g, gm);
+        scale_eight(v[w], inv, gm);
+        m = largest_of(m, v[w]);
+    }
+    m = warp_max(m);
+    const float qs = quant_multiplier(m);
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+        if (32 * w + lane < groups) sum += quantize_eight(x8 + 8 * (32 * w + lane), v[w], qs);
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) {
+        a.sums[row] = sum;
         a.scales[row] = dequant_scale(m);
     }
 }
 
+// Many wider rows: every CTA takes each gridDim.x-th one. Bulk copies bring the next
+// rows into shared memory (two of them, x and delta behind each other) while this one
+// is normed and stored, and the weights stay in registers: with a CTA a row a thread's
+// loads, the two reductions and the stores followed each other, and the weights came
+// from the caches once a row (8192 rows of 9728 in bf16 112 -> 89 us, 6.3 TB/s; of
+// 2560 in fp32 51 -> 50; three stages leave room for one CTA an SM: 132). A row's
+// values are in registers before its first reduction, so its room is free at once.
+constexpr int kNormStages = 2;
+
+template <typename X, typename DT, int kG>
+__global__ void __launch_bounds__(256) norm_rows_stream_kernel(const NormRowsArgs a) {
+    extern __shared__ __align__(128) uint8_t norm_smem[];
+    __shared__ float red[32];
+    __shared__ int ired[8];
+    __shared__ uint64_t full[kNormStages];
+    const int tid = threadIdx.x, groups = a.width >> 3, grid = gridDim.x;
+    const uint32_t x_bytes = a.width * sizeof(X), delta_bytes = a.delta ? a.width * sizeof(DT) : 0;
+    auto stage_of = [&](int s) { return norm_smem + s * (x_bytes + delta_bytes); };
+    auto fetch = [&](long long row, int s) {  // by one thread
+        mbar_arrive_expect_tx(&full[s], x_bytes + delta_bytes);
+        bulk_g2s(stage_of(s), static_cast<const X*>(a.x) + row * a.x_stride, x_bytes, &full[s]);
+        if (delta_bytes)
+            bulk_g2s(stage_of(s) + x_bytes, static_cast<const DT*>(a.delta) + row * a.delta_stride, delta_bytes, &full[s]);
+    };
+    if (tid == 0) {
+        for (int s = 0; s < kNormStages; ++s) mbar_init(&full[s], 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    if (tid == 0)
+        for (int s = 0; s < kNormStages; ++s)
+            if (blockIdx.x + static_cast<long long>(s) * grid < a.rows) fetch(blockIdx.x + static_cast<long long>(s) * grid, s);
+    float gm[kG][8];
+#pragma unroll
+    for (int k = 0; k < kG; ++k)
+        if (tid + 256 * k < groups) load8(a.weight + 8 * (tid + 256 * k), gm[k]);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    long long row = blockIdx.x;
+    for (; row < a.rows; row += grid) {
+        ok = __syncthreads_and(mbar_wait(&full[stage], phase)) != 0;
+        if (!ok) break;
+        const X* x = reinterpret_cast<const X*>(stage_of(stage));
+        const DT* delta = reinterpret_cast<const DT*>(stage_of(stage) + x_bytes);
+        float v[kG][8], ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < kG; ++k) {
+            const int g = tid + 256 * k;
+            if (g >= groups) continue;
+            load_eight(x + 8 * g, v[k]);
+            if (delta_bytes) {
+                float d[8];
+                load_eight(delta + 8 * g, d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] = __fadd_rn(v[k][e], d[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = __fmaf_rn(v[k][e], v[k][e], ss);
+        }
+        const float inv = inverse_rms(group_sum(ss, red, 8, 1), a);  // (all have read the row)
+        if (tid == 0 && row + static_cast<long long>(kNormStages) * grid < a.rows)
+            fetch(row + static_cast<long long>(kNormStages) * grid, stage);
+        X* out = a.out ? static_cast<X*>(a.out) + row * a.out_stride : nullptr;
+        float local = 0.f;
+#pragma unroll
+        for (int k = 0; k < kG; ++k) {
+            const int g = tid + 256 * k;
+            if (g >= groups) continue;
+            if (out) store_eight(out + 8 * g, v[k]);
+            scale_eight(v[k], inv, gm[k]);
+            local = largest_of(local, v[k]);
+        }
+        const float m = group_max(local, red, 8, 1);
+        const float qs = quant_multiplier(m);
+        int8_t* x8 = a.x8 + row * a.width;
+        int sum = 0;
+#pragma unroll
+        for (int k = 0; k < kG; ++k)
+            if (tid + 256 * k < groups) sum += quantize_eight(x8 + 8 * (tid + 256 * k), v[k], qs);
+        finish_row(a, row, m, sum, ired);
+        if (++stage == kNormStages) stage = 0, phase ^= 1u;
+    }
+    if (!ok && tid == 0)  // the copies issued must land before the CTA may exit
+        for (int s = 0; s < kNormStages; ++s, row += grid) {
+            if (row < a.rows) mbar_wait(&full[stage], phase);
+            if (++stage == kNormStages) stage = 0, phase ^= 1u;
+        }
+}
+
+template <typename X, typename DT, int kG>
+static int launch_norm_rows_held(const NormRowsArgs& a, cudaStream_t stream) {
+    // CTAs an SM by the registers (weights and values) and by the room of the rows. One
+    // alone is slower than a CTA a row (8192 fp32 rows of 9728: 189 and 178 us), and so is
+    // a start without a second row to hide (1024 rows of 2560: 7.7 and 8.5 us, 600: 4.9 and
+    // 4.4).
+    constexpr int kMost = kG == 1 ? 6 : kG == 2 ? 4 : 2;
+    const long long smem = static_cast<long long>(kNormStages) * a.width * (sizeof(X) + (a.delta ? sizeof(DT) : 0));
+    const int ctas = static_cast<int>(std::min<long long>(kMost, 232448 / (smem + 1280)));
+    int sms = 0;
+    if (const int rc = paged_sm_count(&sms)) return rc;
+    if (ctas < 2 || 2ll * a.rows < 3ll * ctas * sms) {
+        norm_rows_kernel<X, DT, kG><<<a.rows, 256, 0, stream>>>(a);
+    } else {
+        static std::atomic<bool> opted_in[kMaxDevices];
+        int dev = 0;
+        H4B_CUDA_TRY(cudaGetDevice(&dev));
+        if (!opted_in[dev].load(std::memory_order_acquire)) {
+            H4B_CUDA_TRY(cudaFuncSetAttribute(norm_rows_stream_kernel<X, DT, kG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                              232448 - 1024));
+            opted_in[dev].store(true, std::memory_order_release);
+        }
+        norm_rows_stream_kernel<X, DT, kG><<<ctas * sms, 256, static_cast<size_t>(smem), stream>>>(a);
+    }
+    H4B_CUDA_TRY(cudaGetLastError());
+    return 0;
+}
+
 template <typename X, typename DT>
-static int launch_norm_rows(const NormRowsArgs& a, int rows, cudaStream_t stream) {
-    const int per = (a.width / 8 + 255) / 256;
-    if (per <= 1)
-        norm_rows_kernel<X, DT, 1><<<rows, 256, 0, stream>>>(a);
-    else if (per <= 2)
-        norm_rows_kernel<X, DT, 2><<<rows, 256, 0, stream>>>(a);
-    else if (per <= 5)
-        norm_rows_kernel<X, DT, 5><<<rows, 256, 0, stream>>>(a);
-    else
-        norm_rows_kernel<X, DT, 0><<<rows, 256, 0, stream>>>(a);
+static int launch_norm_rows(const NormRowsArgs& a, cudaStream_t stream) {
+    const int groups = a.width / 8, per = (groups + 255) / 256;
+    if (groups <= 128) {
+        const unsigned grid = (static_cast<unsigned>(a.rows) + 7) / 8;
+        if (groups <= 64)
+            norm_rows_warp_kernel<X, DT, 2><<<grid, 256, 0, stream>>>(a);
+        else
+            norm_rows_warp_kernel<X, DT, 4><<<grid, 256, 0, stream>>>(a);
+        H4B_CUDA_TRY(cudaGetLastError());
+        return 0;
+    }
+    if (per <= 1) return launch_norm_rows_held<X, DT, 1>(a, stream);
+    if (per <= 2) return launch_norm_rows_held<X, DT, 2>(a, stream);
+    if (per <= 5) return launch_norm_rows_held<X, DT, 5>(a, stream);
+    norm_rows_kernel<X, DT, 0><<<a.rows, 256, 0, stream>>>(a);
     H4B_CUDA_TRY(cudaGetLastError());
     return 0;
 }
 
 template <typename X>
-static int launch_norm_rows_delta(const NormRowsArgs& a, int delta_dtype, int rows, cudaStream_t stream) {
-    if (a.delta == nullptr || delta_dtype == H4B_FP32) return launch_norm_rows<X, float>(a, rows, stream);
-    if (delta_dtype == H4B_FP16) return launch_norm_rows<X, __half>(a, rows, stream);
-    return launch_norm_rows<X, __nv_bfloat16>(a, rows, stream);
+static int launch_norm_rows_delta(const NormRowsArgs& a, int delta_dtype, cudaStream_t stream) {
+    if (a.delta == nullptr || delta_dtype == H4B_FP32) return launch_norm_rows<X, float>(a, stream);
+    if (delta_dtype == H4B_FP16) return launch_norm_rows<X, __half>(a, stream);
+    return launch_norm_rows<X, __nv_bfloat16>(a, stream);
 }
 
 }  // namespace h4b
@@ -191,9 +391,10 @@ extern "C" int h4b_rmsnorm_quantize_rows(const void* x, int x_dtype, long long x
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(delta) | reinterpret_cast<uintptr_t>(out) |
           reinterpret_cast<uintptr_t>(weight)) & 15) || (reinterpret_cast<uintptr_t>(x8) & 7))
         return H4B_EINVAL;
-    const NormRowsArgs a{x, delta, delta ? out : nullptr, x_stride, delta_stride, out_stride, weight, eps, width, x8, scales, sums};
+    const NormRowsArgs a{x,      delta, delta ? out : nullptr, x_stride, delta_stride, out_stride, weight, eps,
+                         rows,   width, x8,                    scales,   sums};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (x_dtype == H4B_FP32) return launch_norm_rows_delta<float>(a, delta_dtype, rows, s);
-    if (x_dtype == H4B_FP16) return launch_norm_rows_delta<__half>(a, delta_dtype, rows, s);
-    return launch_norm_rows_delta<__nv_bfloat16>(a, delta_dtype, rows, s);
+    if (x_dtype == H4B_FP32) return launch_norm_rows_delta<float>(a, delta_dtype, s);
+    if (x_dtype == H4B_FP16) return launch_norm_rows_delta<__half>(a, delta_dtype, s);
+    return launch_norm_rows_delta<__nv_bfloat16>(a, delta_dtype, s);
 }

@@ -101,7 +101,8 @@ __device__ __forceinline__ void find_sights(const int (&parent)[kTreeWords], int
         const uint32_t mine = descent(p, 32 * k, &above);
         uint32_t* bits = sights + i * kTreeWords;
 #pragma unroll
-        for (int w = 0; w < kTreeWords; ++w) bits[w] = w < k ? (above >= 0 ? sights[above * kTreeWords + w] : 0u) : w == k ? mine : 0u;
+        for (int w = 0; w < kTreeWords; ++w)
+            bits[w] = w < k ? (above >= 0 ? sights[above * kTreeWords + w] : 0u) : w == k ? mine : 0u;
         depths[i] = static_cast<int16_t>(__popc(mine) - 1 + (above >= 0 ? depths[above] + 1 : 0));
         __syncwarp();
     }
@@ -621,7 +622,8 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
             const float f = l == 0.f ? 0.f : whole ? 1.0f / l : 1.f;  // l = 0: saw no key
             constexpr int kPart = kChunkRows * (D + 2);
             // [D / 4][row] float4, then [row] (m, l): a warp's accesses are contiguous
-            float4* part = reinterpret_cast<float4*>(a.partials + static_cast<long long>((2 * blockIdx.x + (begun ? 1 : 0)) * TILES + t) * kPart);
+            const long long my_part = static_cast<long long>(2 * blockIdx.x + (begun ? 1 : 0)) * TILES + t;
+            float4* part = reinterpret_cast<float4*>(a.partials + my_part * kPart);
             if (live) {
                 T* out_tile = static_cast<T*>(a.out) + first_row * a.out_stride + w.h * a.group * D;
                 const long long my_place = valid ? node * a.out_stride + head * D : -1;

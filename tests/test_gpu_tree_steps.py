@@ -38,6 +38,31 @@ def test_rmsnorm_quantize_rows(rows, width, dtype, delta):
     assert torch.equal(sums, x8.sum(-1, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("rows,width,dtype,delta", [
+    (2000, 2560, "fp32", "bf16"), (1500, 9728, "bf16", "bf16"), (700, 9728, "fp16", None), (3001, 1032, "bf16", "fp32"),
+    (2500, 2048, "fp32", None), (1301, 520, "fp16", "fp16"), (900, 1024, "fp32", "fp32"), (5000, 4104, "bf16", None)])
+def test_norm_of_many_rows_is_that_of_each(rows, width, dtype, delta):
+    """However the rows are shared out, every one has the bits that it has alone."""
+    g = torch.Generator("cuda").manual_seed(width)
+    x = torch.empty(rows, width + 8, device="cuda").normal_(generator=g).to(VALUES[dtype])[:, 8:]
+    d = None if delta is None else torch.empty(rows, width, device="cuda").normal_(generator=g).to(VALUES[delta])
+    weight = torch.rand(width, generator=g, device="cuda")
+    out = torch.full((rows + 1, width), 5.0, dtype=VALUES[dtype], device="cuda")
+    got = ops.rmsnorm_quantize_rows(x, weight, 1e-6, delta=d, out=out[:rows])
+    total = x.float() if d is None else x.float() + d.float()
+    if d is not None:
+        assert torch.equal(out[:rows], total.to(x.dtype))
+    assert (out[rows] == 5).all()
+    for part in range(0, rows, 97):
+        few = total[part:part + 97].contiguous()  # fp32 rows of the same values, few at a time
+        want = ops.rmsnorm_quantize_rows(few, weight, 1e-6)
+        assert all(torch.equal(a[part:part + 97], b) for a, b in zip(got, want))
+    normed = torch.stack([ops.rmsnorm(total[r].contiguous(), weight, 1e-6) for r in (0, 1, rows // 2, rows - 1)])
+    want8, want_scales, want_sums = ops.quantize_rows(normed)
+    for k, r in enumerate((0, 1, rows // 2, rows - 1)):
+        assert torch.equal(got[0][r], want8[k]) and got[1][r] == want_scales[k] and got[2][r] == want_sums[k]
+
+
 def test_norm_strided_rows_and_outputs():
     x, d = torch.randn(2, 40, 2560, device="cuda"), torch.randn(40, 2, 2560, device="cuda")
     weight = torch.rand(2560, device="cuda")
