@@ -496,8 +496,14 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
             const int my_tokens = min(half_tokens, tile.tokens - t * half_tokens);
             const uint32_t* sight = sights + (first_node + node) * kTreeWords;  // this row's
             if (w.b != sight_b || w.t != sight_t) {  // (the same for every kv head)
-                __syncwarp();
-                if (tiles > 0 && lane == 0) mbar_arrive(sight_free);
+                if (tiles > 0) {
+                    // (each warp waits for every tile's sights, needed or not: none can count
+                    // twice towards their release, however far it is ahead of the others)
+                    if (!sighted) ok = warp_wait(sight_full, (tiles - 1) & 1);
+                    if (!ok) break;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(sight_free);
+                }
                 sight_b = w.b, sight_t = w.t;
                 ++tiles;
                 sighted = false;

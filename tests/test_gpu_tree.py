@@ -152,6 +152,21 @@ def test_many_sequences():
     Trees(parents, total, heads=4, kv_heads=1, dim=128, page=16, dtype=torch.float16, seed=4).check()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_trees_among_large_ones(dim):
+    """Most trees fill a part of one tile of rows, some two tiles, and their keys a block or two: what the warps of a
+    tile without rows pass by at once, the others still read."""
+    sizes = [1 + (7 * i) % 12 if i % 9 else 30 for i in range(260)]
+    parents = [draft(n, 1 + i % 5, seed=i) for i, n in enumerate(sizes)]
+    total = [n + (11 * i) % 70 for i, n in enumerate(sizes)]
+    trees = Trees(parents, total, heads=8, kv_heads=1, dim=dim, page=16, dtype=torch.float16, seed=8)
+    first = [t.clone() for t in trees.call()]
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(trees.call(), first))
+    trees.check()
+    Trees(parents, total, heads=8, kv_heads=1, dim=dim, page=16, dtype=torch.float16, seed=8, window=9, sinks=1).check()
+
+
 @pytest.mark.parametrize("n,total", [(1, 33000), (5, 20011), (64, 12345), (32, 16384 + 128)])
 def test_long_contexts_are_split(n, total):
     Trees([draft(n, 4)], [total], heads=8, kv_heads=2, dim=128, page=64, dtype=torch.bfloat16, seed=5).check()
