@@ -279,6 +279,19 @@ def test_accept_parents_out_of_range_and_large_trees():
         assert path.tolist() == [[0, 1, -1, -1, -1], [-1] * 5, [0, 1, -1, -1, -1]]
 
 
+def test_batches_without_nodes():
+    none, offsets = ints([]), ints([0, 0, 0])
+    for how in (dict(logits=torch.zeros(0, 9, device="cuda")), dict(targets=none)):
+        path, counts, following, _ = ops.accept_tree(none, none, offsets, max_path=4, **how)
+        assert path.tolist() == [[-1] * 4] * 2 and counts.tolist() == [0, 0] and following.tolist() == [-1, -1]
+    path, counts, following, _ = ops.accept_tree(none, none, ints([0]), targets=none)
+    assert path.shape[0] == counts.numel() == following.numel() == 0
+    k = torch.randn(2, 4, 2, 16, 64, device="cuda").half()
+    before, lens = k.clone(), ints([17, 0])
+    lengths = ops.keep_tokens(k, k.clone(), ints([0, 1, 2, 3]).view(2, 2), offsets, lens, ints([[0], [-1]]).view(2, 1), ints([0, 0]))
+    assert torch.equal(lengths, lens) and torch.equal(k, before) and _lib.device_status() == 0
+
+
 def test_accept_refusals():
     tokens, parents, offsets = ints([1, 2]), ints([-1, 0]), ints([0, 2])
     logits = torch.zeros(2, 10, device="cuda")

@@ -120,3 +120,8 @@ def test_norm_refuses(library, change):
 def test_norm_supports_no_such_type(library):
     assert norm(library, x_dtype=3) == EUNSUPPORTED and norm(library, delta_dtype=-1) == EUNSUPPORTED
     assert norm(library, rows=0) == 0
+
+
+def test_the_models_step_needs_parents(library):
+    assert library.h4b_forward_paged_tree(None, None, None, None) == EINVAL
+    assert library.h4b_forward_paged_tree(None, None, 64, None) == EINVAL
