@@ -372,6 +372,7 @@ struct AttendArgs {
     int4* entries;            // [CTAs] the item that begins last in each (chunk kernel)
     int half_tokens;          // new tokens of each of an item's two tiles (chunk kernel), or of its one (tree kernel)
     const int32_t* parents;   // of a tree's nodes (TREE)
+    bool whole;               // items are not cut: one is the CTA's whose range holds its first unit (TREE)
 };
 
 // A sequence as this kernel's share of the batch has it: without new tokens if
@@ -577,7 +578,14 @@ struct Walk {
             left += unit;
             unit = 0;
         }
-        return left > 0;
+        if (TREE && a.whole && unit > 0) {  // begun in an earlier range
+            left -= tile.units() - unit + a.extra;
+            if (left <= 0) return false;
+            next_item(a, tile_tokens);
+        }
+        const bool any = left > 0;
+        if (TREE && a.whole) left = max(left, tile.units());
+        return any;
     }
     // Past the item's last unit: to the next item that has any.
     __device__ __forceinline__ void next_item(const AttendArgs& a, int tile_tokens) {
@@ -603,10 +611,12 @@ struct Walk {
         const bool over = item_ends();
         left -= over ? 1 + a.extra : 1;
         if (left <= 0) return false;
-        if (over)
+        if (over) {
             next_item(a, tile_tokens);
-        else
+            if (TREE && a.whole) left = max(left, tile.units());
+        } else {
             ++unit;
+        }
         return true;
     }
 };

@@ -117,6 +117,23 @@ def test_window_and_sinks(heads, kv_heads, dim, page, dtype, window, sinks):
           sinks=sinks, seed=2).check()
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", SHAPES[:4])
+@pytest.mark.parametrize("longest,sequences", [(384, 1), (384, 9), (900, 9), (900, 160)])
+def test_short_tables_and_long_ones_give_the_same(heads, kv_heads, dim, page, dtype, longest, sequences):
+    """Tables that bound the lengths keep items whole, wider ones do not: the keys' sums differ in their order only."""
+    rng = random.Random(sequences)
+    parents = [draft(rng.randint(0, 40 if sequences < 100 else 6), 3, seed=i) for i in range(sequences)]
+    total = [max(len(p), rng.randint(0, longest - 64)) for p in parents]
+    trees = Trees(parents, total, heads=heads, kv_heads=kv_heads, dim=dim, page=page, dtype=dtype, seed=9)
+    width = -(-max(max(total), 1) // page)  # pages that the longest needs
+    wide = torch.full((sequences, trees.table.shape[1] + 4096 // page), -1, dtype=torch.int32, device="cuda")
+    wide[:, :trees.table.shape[1]] = trees.table
+    trees.table = wide[:, :width].contiguous()
+    trees.check()
+    trees.table = wide
+    trees.check()
+
+
 @pytest.mark.parametrize("page", [16, 512, 1024])
 @pytest.mark.parametrize("n", [3, 20, 33])
 def test_page_sizes(n, page):
