@@ -534,7 +534,7 @@ struct Walk {
     RawSpan following;        // of sequence b + 1, requested when b was entered
     Tile tile;
     int b, t, h, unit;        // unit within the item
-    int left;                 // places of the range from this unit on
+    int left;                 // places of the range from this unit on (of a whole item, its units at least)
 
     __device__ __forceinline__ void request(const AttendArgs& a) {
         if (b + 1 < a.p.sequences) following = raw_span(a.p, b + 1);

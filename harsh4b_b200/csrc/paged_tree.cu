@@ -640,9 +640,11 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
                 // Columns c .. c + 31 of the values that the cleaning warp took out of
                 // the blocks of this part, from the pages, where the row sees their key.
                 auto add_wild = [&](float (&v)[32], int c) {
+                    // the part's first unit, from the place of the item's unit 0 (a whole
+                    // item has all its units here, and `left` may reach past the range)
                     const Range& r = *shared_range;
-                    const long long first = r.end - w.left - w.unit;  // place of the item's unit 0
-                    for (int u = static_cast<int>(max(r.begin - first, 0ll)); u <= w.unit; ++u) {
+                    const int from = a.whole ? 0 : static_cast<int>(max(r.begin - (r.end - w.left - w.unit), 0ll));
+                    for (int u = from; u <= w.unit; ++u) {
                         const int block = tile.block(u) * kTreeKeys;
                         for (int j = block; j < block + kTreeKeys; ++j) {
                             if (!tile_sees(tile, a.window, a.sinks, j) || tree_all_see(tile, a.window, a.sinks, j, j)) continue;

@@ -220,6 +220,36 @@ def test_values_that_are_not_finite_reach_who_sees_them(n, what, value):
                 assert torch.isnan(out[touched]).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n", [20, 40, 150])
+@pytest.mark.parametrize("total", [300, 380, 700])
+def test_a_value_that_is_not_finite_in_any_block(n, dim, total):
+    """Each of a tree's blocks in turn, with tables that keep items whole and others that cut them: a key that
+    some rows see, at the windows' first places and among the nodes."""
+    for window in (0, 200):
+        trees = Trees([draft(n, 4, roots=3)], [total], heads=8, kv_heads=2, dim=dim, page=16, dtype=torch.float16,
+                      window=window)
+        clean, _ = trees.call()
+        context = total - n
+        places = list(range(context, total, 13)) + (list(range(max(0, context - window + 1), context - window + 30, 5)) if window else [])
+        wide = torch.full((1, trees.table.shape[1] + 256), -1, dtype=torch.int32, device="cuda")
+        wide[:, :trees.table.shape[1]] = trees.table
+        narrow, values = trees.table, trees.v_pages.clone()
+        for j in places:
+            rows = trees.seen(0)[:, j]
+            trees.set_key(0, j, v=float("inf"))
+            for table in (narrow, wide):
+                trees.table = table
+                out, _ = trees.call()
+                assert not torch.isfinite(out[rows]).any(), (window, j)
+                if table is narrow:
+                    assert torch.equal(out[~rows], clean[~rows])
+                else:
+                    assert torch.isfinite(out[~rows]).all()
+            trees.table = narrow
+            trees.v_pages.copy_(values)
+
+
 def test_scores_of_any_finite_size():
     """Rising and huge scores: the running maximum moves, the weights stay finite."""
     for factor in (8.0, 3000.0):
