@@ -140,11 +140,17 @@ class PagedCache:
         return with an earlier end: see check_visible."""
         if not 0 <= length <= self._lengths[sequence]:
             raise ValueError("length must be within the sequence")
-        table = self._tables[sequence]
-        for page in table[-(-length // self.page_size):]:
-            self._drop(page)
-        del table[-(-length // self.page_size):]
         self._lengths[sequence] = length
+        self.release(sequence)
+
+    def release(self, sequence: int, pages: int = 0) -> None:
+        """Give back the pages reserved behind the sequence's last token, but
+        for the first `pages` that it holds."""
+        table = self._tables[sequence]
+        held = max(pages, -(-self._lengths[sequence] // self.page_size))
+        for page in table[held:]:
+            self._drop(page)
+        del table[held:]
 
     def trim(self, sequence: int, window: int, sinks: int = 0) -> int:
         """Give back the pages that no later token sees under (window, sinks);
@@ -337,7 +343,7 @@ class PagedRunner:
         Returns the greedy tokens that follow node 0: the accepted branch's
         and the one after it, of which the last is not in the cache (node 0 of
         the next tree). The nodes' logits are `node_logits` until the next
-        call."""
+        call. Pages that only the other nodes needed are given back."""
         sequences = list(drafts)
         ids, new = self._checked([[int(t) for t in drafts[s][0]] for s in sequences])
         trees = [[int(p) for p in drafts[s][1]] for s in sequences]
@@ -351,6 +357,7 @@ class PagedRunner:
                 raise ValueError(f"a sequence would pass the model's {model.max_pos} positions")
             cache.check_visible(s, self.window, self.sinks)
         total = len(ids)
+        held = [len(cache.table(s)) for s in sequences]  # room of the caller's own stays
         with cache.ordered():
             cache.reserve(dict(zip(sequences, new)))
             if self.node_logits is None or self.node_logits.shape[0] < total:
@@ -369,6 +376,7 @@ class PagedRunner:
             result[s] = [targets[first + node] for node in path[b][:counts[b]]]
             first += n
             cache.advance(s, counts[b])
+            cache.release(s, held[b])
             if self.window:
                 cache.trim(s, self.window, self.sinks)
         return result
