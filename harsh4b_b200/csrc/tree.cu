@@ -297,7 +297,8 @@ extern "C" int h4b_tree_accept(const void* logits, int logits_dtype, long long l
     if (logits_dtype != H4B_FP32 && logits_dtype != H4B_FP16 && logits_dtype != H4B_BF16) return H4B_EUNSUPPORTED;
     const int size = logits_dtype == H4B_FP32 ? 4 : 2;
     if (vocab < 1 || logits_stride < vocab || (reinterpret_cast<uintptr_t>(logits) & (size - 1))) return H4B_EINVAL;
-    if (vocab > INT_MAX - 64) return H4B_EUNSUPPORTED;
+    // (the parts' ends, rounded up to 16 values each, and a thread's place behind them fit 32 bits)
+    if (vocab > INT_MAX - 16 * kAcceptCtas - kAcceptThreads) return H4B_EUNSUPPORTED;
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
         workspace_bytes < h4b_tree_accept_workspace_bytes(rows, sequences))
         return H4B_EINVAL;

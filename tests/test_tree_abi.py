@@ -125,3 +125,10 @@ def test_norm_supports_no_such_type(library):
 def test_the_models_step_needs_parents(library):
     assert library.h4b_forward_paged_tree(None, None, None, None) == EINVAL
     assert library.h4b_forward_paged_tree(None, None, 64, None) == EINVAL
+
+
+@pytest.mark.parametrize("below", [65, 100, 255, 300, 592, 600, 9000])
+@pytest.mark.parametrize("rows,dtype", [(1, 1), (4, 0), (1 << 20, 2)])
+def test_logits_whose_parts_pass_32_bits_are_refused(library, below, rows, dtype):
+    """The ends of a row's parts lie up to 16 values a part behind the row's."""
+    assert accept(library, vocab=BIG - 1 - below, stride=BIG, rows=rows, dtype=dtype, nbytes=1 << 30) == EUNSUPPORTED
