@@ -177,6 +177,8 @@ def rmsnorm_quantize_rows(x: torch.Tensor, weight: torch.Tensor, eps: float, *, 
     if x.dim() != 2 or weight.numel() != x.shape[1]:
         raise ValueError("x must be [rows][width], weight [width]")
     (rows, width), dtype, device = x.shape, x.dtype, x.get_device()
+    if rows > 0x7fffffff or width > 0x7fffffff:
+        raise ValueError("rows and width must fit 32 bits")
     code = _VALUE_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"x must be float32, float16 or bfloat16, got {dtype}")
@@ -503,6 +505,8 @@ def accept_workspace(rows: int, sequences: int, device=None) -> torch.Tensor:
     """A workspace for accept_tree calls of up to so many rows and sequences
     that follow each other (one stream): zeroed once, every call leaves it ready
     for the next."""
+    if max(rows, sequences) > 0x7fffffff:
+        raise ValueError("rows and sequences must fit 32 bits")
     nbytes = int(lib().h4b_tree_accept_workspace_bytes(rows, sequences))
     if nbytes < 0:
         check(nbytes, "h4b_tree_accept_workspace_bytes")
@@ -533,6 +537,8 @@ def accept_tree(tokens: torch.Tensor, parents: torch.Tensor, q_offsets: torch.Te
         max_path = max(1, min(rows, TREE_NODES))
     if not 1 <= max_path <= 0x7fffffff:
         raise ValueError("max_path must be positive and fit 32 bits")
+    if max(rows, sequences, *(() if logits is None else logits.shape)) > 0x7fffffff:
+        raise ValueError("rows, sequences and a row's logits must fit 32 bits")
     at = _on(tokens, torch.int32, "tokens", device), _parents(parents, rows, device), _on(q_offsets, torch.int32, "q_offsets",
                                                                                          device)
     vocab, code, data, stride = 0, 0, None, 0
@@ -572,7 +578,7 @@ def keep_tokens(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.
     device, sequences, shape = k_pages.get_device(), kv.sequences, path.shape
     if layers == 0:
         raise ValueError("k_pages and v_pages must hold a layer")
-    if len(shape) != 2 or shape[0] != sequences or shape[1] < 1 or counts.numel() != sequences:
+    if len(shape) != 2 or shape[0] != sequences or not 1 <= shape[1] <= 0x7fffffff or counts.numel() != sequences:
         raise ValueError("path must be [sequences][nodes], counts [sequences]")
     if lengths is None:
         lengths = torch.empty_like(kv_lens)

@@ -132,3 +132,33 @@ def test_the_models_step_needs_parents(library):
 def test_logits_whose_parts_pass_32_bits_are_refused(library, below, rows, dtype):
     """The ends of a row's parts lie up to 16 values a part behind the row's."""
     assert accept(library, vocab=BIG - 1 - below, stride=BIG, rows=rows, dtype=dtype, nbytes=1 << 30) == EUNSUPPORTED
+
+
+# ---- sizes that a C int cuts off ---------------------------------------------------------
+CUT = (1 << 32) + 8  # 8, cut off
+
+
+def meta(*shape, dtype=None):
+    import torch
+
+    return torch.empty(shape, dtype=dtype or torch.int32, device="meta")
+
+
+def test_sizes_past_32_bits_are_refused_not_cut_off(library):
+    import torch
+
+    from harsh4b_b200 import ops
+
+    half, full = torch.float16, torch.float32
+    for rows, width in ((CUT, 8), (1, CUT)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.rmsnorm_quantize_rows(meta(rows, width, dtype=half), meta(width, dtype=full), 1e-6)
+    for rows, sequences, vocab in ((CUT, 1, 8), (8, CUT, 8), (8, 1, CUT)):
+        batch = meta(rows), meta(rows), meta(sequences + 1)
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.accept_tree(*batch, meta(rows, vocab, dtype=half))
+        if vocab == 8:
+            with pytest.raises(ValueError, match="32 bits"):
+                ops.accept_tree(*batch, targets=meta(rows))
+            with pytest.raises(ValueError, match="32 bits"):
+                ops.accept_workspace(rows, sequences, "meta")
