@@ -205,8 +205,9 @@ static int accept_splits(int rows, long long row_bytes) {
 // (a later step j > i reads path[j] >= j). kKeepBatch loads are in flight at a time: the
 // stores of a batch lie below all later reads.
 // Bound by HBM: twice the bytes of the nodes that move (64 branches of up to 6 nodes in
-// 36 layers of 8 heads of 128: 10 us, 2.7 TB/s: few bytes a CTA behind the chain of
-// counts, path, page and row; one branch: 2.6).
+// 36 layers of 8 heads of 128: 8.6 us, 3.1 TB/s: few bytes a CTA behind the chain of
+// counts, path, page and row; one branch: 2.3). Path and pages are checked at once by as
+// many threads, before anything moves: 10 and 2.6 us with the pages checked at each token.
 constexpr int kKeepThreads = 128, kKeepBatch = 4;
 
 struct KeepArgs {
@@ -223,11 +224,19 @@ __global__ void __launch_bounds__(kKeepThreads) keep_tokens_kernel(const KeepArg
     const int b = blockIdx.x, count = a.counts[b];
     const SequenceSpan s = sequence_span(a.p, b);
     const int32_t* path = a.path + static_cast<long long>(b) * a.max_path;
-    // checked before anything moves
+    const int32_t* table = a.p.table + static_cast<long long>(b) * a.p.table_stride;
+    auto page_of = [&](int slot) { return table[slot >> a.p.page_shift]; };
+    // checked before anything moves: the path, and the pages of its nodes' places, old and new
     bool good = s.base >= 0 && count >= 0 && count <= min(s.count, a.max_path);
     if (good)
-        for (int i = threadIdx.x; i < count; i += kKeepThreads)
-            good = good && path[i] > (i > 0 ? path[i - 1] : -1) && path[i] < s.count;
+        for (int i = threadIdx.x; i < count; i += kKeepThreads) {
+            const int node = path[i];
+            good = node >= i && node < s.count && (i == 0 || node > path[i - 1]);
+            if (!good) break;
+            const int from = page_of(s.base + node), to = page_of(s.base + i);
+            good = min(from, to) >= 0 && max(from, to) < a.p.pages;
+            if (!good) break;
+        }
     good = __syncthreads_and(good) != 0;
     if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
         if (!good) report(kStatusBadPage);
@@ -235,14 +244,11 @@ __global__ void __launch_bounds__(kKeepThreads) keep_tokens_kernel(const KeepArg
     }
     if (!good) return;
     uint8_t* pages = (blockIdx.z ? a.v_pages : a.k_pages) + blockIdx.y * a.layer_bytes;
-    const int32_t* table = a.p.table + static_cast<long long>(b) * a.p.table_stride;
     const int chunks = a.head_bytes / 16, mask = (1 << a.p.page_shift) - 1;
     for (int unit = threadIdx.x; unit < a.p.kv_heads * chunks; unit += kKeepThreads) {
         const int h = unit / chunks, c = unit - h * chunks;
-        auto place = [&](int slot) -> uint4* {  // null: no such page
-            const int page = table[slot >> a.p.page_shift];
-            if (page < 0 || page >= a.p.pages) return nullptr;
-            const long long row = ((static_cast<long long>(page) * a.p.kv_heads + h) << a.p.page_shift) + (slot & mask);
+        auto place = [&](int slot) -> uint4* {
+            const long long row = ((static_cast<long long>(page_of(slot)) * a.p.kv_heads + h) << a.p.page_shift) + (slot & mask);
             return reinterpret_cast<uint4*>(pages + row * a.head_bytes) + c;
         };
         for (int i0 = 0; i0 < count; i0 += kKeepBatch) {
@@ -253,14 +259,8 @@ __global__ void __launch_bounds__(kKeepThreads) keep_tokens_kernel(const KeepArg
                 to[k] = nullptr;
                 const int i = i0 + k;
                 if (i >= count || path[i] == i) continue;
-                const uint4* from = place(s.base + path[i]);
+                v[k] = *place(s.base + path[i]);
                 to[k] = place(s.base + i);
-                if (from == nullptr || to[k] == nullptr) {
-                    report(kStatusBadPage);
-                    to[k] = nullptr;
-                } else {
-                    v[k] = *from;
-                }
             }
 #pragma unroll
             for (int k = 0; k < kKeepBatch; ++k)
