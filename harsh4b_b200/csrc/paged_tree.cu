@@ -25,10 +25,12 @@
 // sees need no mask. p = 2^(s scale - b + 8) with b the product m scale of a score m,
 // rounded on its own: what the rounding adds to b it adds to all weights of the row
 // alike, and the log-sum-exp takes it off again. m moves only where a score passes it
-// by 2^7. From |b| = 2^20 on, where the rounding would reach p's exponent, p = 2^((s - m)
+// by 2^7. From |b - 8| = 2^20 on, where the rounding would reach p's exponent, p = 2^((s - m)
 // scale + 8), in which equal scores cancel whatever their size: one more operation a
 // pair, which costs nothing in time but, under the power cap, clock (16 x 32 nodes
-// over 32768 tokens, sustained: 420 -> 411 us without it). p is rounded to the cache's
+// over 32768 tokens, sustained: 420 -> 411 us without it), so it is left out where no row
+// of the warp needs it. Which form a row's weights have goes by its own m, so l and O of
+// other blocks and parts are carried over with the right factor. p is rounded to the cache's
 // type for the product as in the other kernels (see paged.cu), l is its fp32 sum.
 //
 // V rows of keys that no row sees are zeroed and values that are not finite are
@@ -124,11 +126,15 @@ __device__ __forceinline__ void find_sights(const int (&parent)[kTreeWords], int
     __syncwarp();
 }
 
-// What weights relative to score m are worth relative to `top`, the way the weights
-// were formed (see above).
+// Whether weights relative to score m, b = m scale, have the form for huge scores.
+__device__ __forceinline__ bool is_huge_reference(float b) { return is_huge(__fsub_rn(8.f, b)); }
+// What weights relative to score m are worth relative to `top`, each in its form:
+// relative to the rounded product or, if it is huge, to the product itself.
 __device__ __forceinline__ float reference_factor(float m, float top, float scale) {
-    const float b = __fmul_rn(top, scale);
-    return is_huge(b) ? ex2_approx((m - top) * scale) : ex2_approx(__fsub_rn(__fmul_rn(m, scale), b));
+    const float a = __fmul_rn(m, scale), b = __fmul_rn(top, scale);
+    const bool huge = is_huge_reference(a);
+    if (is_huge_reference(b)) return ex2_approx(huge ? (m - top) * scale : __fmaf_rn(-top, scale, a));
+    return ex2_approx(huge ? __fmaf_rn(m, scale, -b) : __fsub_rn(a, b));
 }
 
 // Whether every row of the tile sees keys `key` .. `end`.
@@ -529,7 +535,7 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
                 const uint32_t low = sight[off >> 5], high = (off >> 5) + 1 < kTreeWords ? sight[(off >> 5) + 1] : 0u;
                 return earlier | __funnelshift_r(low, high, off & 31);
             };
-            float m = -INFINITY, l = 0.f, offset = 8.f;  // offset: 8 - b
+            float m = -INFINITY, l = 0.f, offset = 8.f;  // offset: 8 - b, or 8 where s - m is scaled
             bool done = false, huge = false;
             while (true) {
                 const uint32_t x = 2 * t + (n & 1), s_col = lane_base + C::kSCol + kTreeKeys * x;
@@ -578,20 +584,20 @@ __global__ void __launch_bounds__(TreeCfg<D, ROWS, TILES>::kThreads, TreeCfg<D, 
                         if (move) {
                             m = mx;
                             offset = __fsub_rn(8.f, __fmul_rn(m, a.scale));
+                            if (is_huge(offset)) offset = 8.f;
                         }
-                        huge = __any_sync(0xffffffffu, valid && is_huge(offset)) != 0;
+                        huge = __any_sync(0xffffffffu, m != -INFINITY && is_huge_reference(__fmul_rn(m, a.scale))) != 0;
                     }
-                    uint64_t scale2 = pack2(a.scale, a.scale), offset2 = pack2(offset, offset);
+                    const uint64_t scale2 = pack2(a.scale, a.scale), offset2 = pack2(offset, offset);
                     if (huge) {
-                        // (the scores less m, scaled: s - m here, the rest below)
-                        const float less = m == -INFINITY ? 0.f : -m;
+                        // (the scores less m, scaled: s - m here, the rest below; the other rows' as they are)
+                        const float less = m != -INFINITY && is_huge_reference(__fmul_rn(m, a.scale)) ? -m : 0.f;
                         const uint64_t less2 = pack2(less, less);
 #pragma unroll
                         for (int k = 0; k < kTreeKeys; k += 2) {
                             const float2 y = unpack2(add2(pack2(v[k], v[k + 1]), less2));
                             v[k] = y.x, v[k + 1] = y.y;
                         }
-                        offset2 = pack2(8.f, 8.f);
                     }
                     uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
