@@ -208,15 +208,16 @@ __device__ __forceinline__ void rescale_row(uint32_t o_col, float f) {
 
 // The softmax of a tile's row from a block on whose scores are huge for some row
 // of the warp, to the end of the part: scaled before the subtraction, 32 at a
-// time, the maximum first and then p. A call of its own, which leaves the usual
-// way its registers. The first block's scores have come and its turn is taken.
+// time, the maximum first and then p. Rows whose own m is not huge keep the usual
+// fused form, in which their earlier weights were formed. A call of its own, which leaves
+// the usual way its registers. The first block's scores have come and its turn is taken.
 struct HugeRow {
     Walk<kChunkKeys> w;
     float m, l;
     uint32_t s_count, turns;
     int pos;                  // -1: no row
     uint32_t s_col, o_col;
-    bool ok;
+    bool ok, huge;            // huge: of this row's m
 };
 template <typename T, int D>
 __device__ __noinline__ void huge_scores(const AttendArgs& a, HugeRow& row, int half_tokens, uint64_t* s_full,
@@ -227,37 +228,44 @@ __device__ __noinline__ void huge_scores(const AttendArgs& a, HugeRow& row, int 
     const bool second = threadIdx.x >= 128;  // tile B, whose turns start one later
     while (true) {
         const int key = r.w.tile.block(r.w.unit) * kChunkKeys;
-        auto scaled = [&](float (&v)[32], int c) {
+        auto scores = [&](float (&v)[32], int c) {
             tmem_ld16_nowait(r.s_col + c, v, 0);
             tmem_ld16_nowait(r.s_col + c + 16, v, 16);
             tmem_wait_regs(v);
             uint32_t seen = bits_below(r.pos - key - c + 1);
             if (a.window > 0) seen &= ~bits_below(r.pos - a.window - key - c + 1) | bits_below(a.sinks - key - c);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = (seen >> k) & 1u ? __fmul_rn(v[k], a.scale) : -INFINITY;
+            for (int k = 0; k < 32; ++k) v[k] = (seen >> k) & 1u ? v[k] : -INFINITY;
         };
         float v[32], mx = -INFINITY;
 #pragma unroll 1
         for (int c = 0; c < kChunkKeys; c += 32) {
-            scaled(v, c);
+            scores(v, c);
 #pragma unroll
             for (int k = 0; k < 32; ++k) mx = fmaxf(mx, v[k]);
         }
+        mx = __fmul_rn(mx, a.scale);
         const bool move = mx - r.m > kMostExponent;
         if (__any_sync(0xffffffffu, move && r.m != -INFINITY)) {
             const float f = move ? ex2_approx(r.m - softmax_reference(mx)) : 1.f;
             r.l *= f;
             rescale_row<D>(r.o_col, f);
         }
-        if (move) r.m = softmax_reference(mx);
+        if (move) {
+            r.m = softmax_reference(mx);
+            r.huge = is_huge(mx);
+        }
         const float base = r.m == -INFINITY ? 0.f : r.m;
+        auto weight = [&](float s) {
+            return ex2_approx(r.huge ? __fsub_rn(__fmul_rn(s, a.scale), base) : __fmaf_rn(s, a.scale, -base));
+        };
 #pragma unroll 1
         for (int c = 0; c < kChunkKeys; c += 32) {
-            scaled(v, c);
+            scores(v, c);
             uint32_t p16[16];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-                const float p0 = ex2_approx(__fsub_rn(v[k], base)), p1 = ex2_approx(__fsub_rn(v[k + 1], base));
+                const float p0 = weight(v[k]), p1 = weight(v[k + 1]);
                 r.l += p0 + p1;
                 p16[k / 2] = Pair<T>::pack(p0, p1);
             }
@@ -718,7 +726,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
                         for (int c = 0; c < kHalf; c += 16) tmem_st16(s_col + c, s1, c);
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        HugeRow row{w, m, l, s_count, turns, pos, s_col, o_col, true};
+                        HugeRow row{w, m, l, s_count, turns, pos, s_col, o_col, true, false};
                         huge_scores<T, D>(a, row, half_tokens, s_full + x, p_half + x, p_full + x, turn + 4 * x + (warp & 3),
                                           turn + 4 * (x ^ 1) + (warp & 3));
                         w = row.w, m = row.m, l = row.l, s_count = row.s_count, turns = row.turns, ok = row.ok;
