@@ -1232,7 +1232,8 @@ static int paged_sm_count(int* sms) {
 // The few-row kernel's CTAs an SM and largest tile; as many q heads may share a
 // kv head (a token's group stays in one tile of either kernel).
 constexpr int kFewCtasPerSm = 2, kFewMaxRows = 32;
-constexpr long long kCounterBytes = 4096, kEntryBytes = 8192;
+constexpr long long kCounterBytes = 4096, kEntryBytes = 4096;
+constexpr long long kTreeEntryBytes = 8192;  // (the tree kernel may have two CTAs an SM)
 
 template <typename S, typename T, int D, bool TREE>
 static int launch_append(AppendArgs a, cudaStream_t stream) {
@@ -1403,8 +1404,10 @@ extern "C" int h4b_pages_copy(void* k_pages, void* v_pages, int layers, int page
     return 0;
 }
 
-extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
-    using namespace h4b;
+namespace h4b {
+
+// Workspace bytes of either attention, of trees or not; negative: an error.
+static long long attention_workspace_bytes(int head_dim, bool tree) {
     int sms = 0;
     if (head_dim != 64 && head_dim != 128) return H4B_EUNSUPPORTED;
     if (const int rc = paged_sm_count(&sms)) return rc > 0 ? -1000 - rc : rc;
@@ -1412,11 +1415,10 @@ extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
     // the 256 of the chunk kernel's CTA
     static_assert(kFewCtasPerSm * kFewMaxRows <= 2 * kChunkRows, "the chunk kernel's parts are the larger");
     // (the tree kernel's are as many rows an SM: two CTAs of 128 or one of 256)
-    if (kFewCtasPerSm * sms * 4 > kCounterBytes || 2 * sms * 16 > kEntryBytes) return H4B_EUNSUPPORTED;
-    return kCounterBytes + kEntryBytes + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
+    if (kFewCtasPerSm * sms * 4 > kCounterBytes || sms * 16 > kEntryBytes || 2 * sms * 16 > kTreeEntryBytes)
+        return H4B_EUNSUPPORTED;
+    return kCounterBytes + (tree ? kTreeEntryBytes : kEntryBytes) + 2ll * sms * 2 * kChunkRows * (head_dim + 2) * 4;
 }
-
-namespace h4b {
 
 // `parents`: the new tokens are a tree's nodes (null: one after the other).
 static int paged_attention(const h4b_paged_kv* kv, const int32_t* parents, const void* q, long long q_stride, int heads,
@@ -1439,7 +1441,7 @@ static int paged_attention(const h4b_paged_kv* kv, const int32_t* parents, const
         ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) &
          15))
         return H4B_EINVAL;
-    const long long need = h4b_paged_attention_workspace_bytes(kv->head_dim);
+    const long long need = attention_workspace_bytes(kv->head_dim, parents != nullptr);
     if (need < 0 || workspace_bytes < need) return H4B_EINVAL;
     int sms = 0;
     if (const int rc = paged_sm_count(&sms)) return rc;
@@ -1448,7 +1450,8 @@ static int paged_attention(const h4b_paged_kv* kv, const int32_t* parents, const
     a.window = window < kMaxLength ? window : kMaxLength, a.sinks = sinks, a.scale = base2_scale;
     a.counters = static_cast<unsigned int*>(workspace);
     a.entries = reinterpret_cast<int4*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
-    a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes + kEntryBytes);
+    a.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes +
+                                          (parents != nullptr ? kTreeEntryBytes : kEntryBytes));
     a.parents = parents;
     const int longest = max_query < kv->tokens ? max_query : kv->tokens;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1465,6 +1468,10 @@ static int paged_attention(const h4b_paged_kv* kv, const int32_t* parents, const
 }
 
 }  // namespace h4b
+
+extern "C" long long h4b_paged_attention_workspace_bytes(int head_dim) {
+    return h4b::attention_workspace_bytes(head_dim, true);  // for both: the larger
+}
 
 extern "C" int h4b_paged_attention(const h4b_paged_kv* kv, const void* q, long long q_stride, int heads, float scale,
                                    int window, int sinks, int max_query, void* out, long long out_stride, float* lse,

@@ -508,8 +508,8 @@ int h4b_paged_append(const h4b_paged_kv *kv, const void *qkv, int qkv_dtype, lon
 int h4b_paged_attention(const h4b_paged_kv *kv, const void *q, long long q_stride, int heads, float scale, int window,
                         int sinks, int max_query, void *out, long long out_stride, float *lse, void *workspace,
                         long long workspace_bytes, void *stream);
-/* Workspace bytes of h4b_paged_attention on the current device, for any batch
- * of that head_dim. */
+/* Workspace bytes of h4b_paged_attention and h4b_paged_tree_attention on the
+ * current device, for any batch of that head_dim (4096 fewer do for the former). */
 long long h4b_paged_attention_workspace_bytes(int head_dim);
 
 /* Copies page src[i] to page dst[i], i < count, in every layer's K and V
