@@ -329,11 +329,16 @@ extern "C" int h4b_tree_keep(const h4b_paged_kv* kv, int layers, long long layer
     if (layers > 1 && (layer_bytes < need || (layer_bytes & 15))) return H4B_EINVAL;
     if (kv->sequences == 0) return 0;
     if (path == nullptr || counts == nullptr || lengths == nullptr) return H4B_EINVAL;
-    // (kv_lens and counts are read by all CTAs of a sequence, lengths is written by one)
-    const uintptr_t bytes = 4ull * kv->sequences, to = reinterpret_cast<uintptr_t>(lengths);
-    for (const int32_t* p : {kv->kv_lens, counts}) {
-        const uintptr_t from = reinterpret_cast<uintptr_t>(p);
-        if (to < from + bytes && from < to + bytes) return H4B_EINVAL;
+    // (what all CTAs of a sequence read, while one of them writes lengths)
+    const long long n = kv->sequences;
+    const struct {
+        const int32_t* at;
+        long long count;
+    } read[] = {{kv->kv_lens, n}, {counts, n}, {kv->q_offsets, n + 1}, {path, n * max_path}, {kv->page_table, n * kv->table_stride}};
+    const uintptr_t to = reinterpret_cast<uintptr_t>(lengths);
+    for (const auto& r : read) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(r.at);
+        if (to < from + 4ull * r.count && from < to + 4ull * n) return H4B_EINVAL;
     }
     a.k_pages = static_cast<uint8_t*>(kv->k_pages), a.v_pages = static_cast<uint8_t*>(kv->v_pages);
     a.layer_bytes = layer_bytes, a.head_bytes = kv->head_dim * 2;

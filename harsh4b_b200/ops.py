@@ -571,8 +571,9 @@ def keep_tokens(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.
     """h4b_tree_keep: the K and V of the accepted nodes path[b][:counts[b]]
     (accept_tree), moved behind the tokens before the tree, in every layer of
     [layers][pages][kv_heads][page_size][head_dim] (or one layer's [pages]...)
-    caches. Returns the new lengths (int32 [sequences]; `lengths`, if given,
-    overlaps neither kv_lens nor counts)."""
+    caches. A sequence whose path does not ascend within its nodes, or meets a
+    missing page, stays as it was. Returns the new lengths (int32 [sequences];
+    `lengths`, if given, overlaps none of the other tables)."""
     layers, layered = (k_pages.shape[0], True) if k_pages.dim() == 5 else (1, False)
     kv = _paged(k_pages, v_pages, page_table, q_offsets, kv_lens, 0x7fffffff, layered)
     device, sequences, shape = k_pages.get_device(), kv.sequences, path.shape

@@ -571,7 +571,7 @@ long long h4b_tree_accept_workspace_bytes(int rows, int sequences);
 /* Moves the accepted nodes' K and V behind the tokens before the tree: node
  * path[b][i] to place i, i < counts[b], in every layer (kv.k_pages / v_pages are
  * layer 0's, layer l's lie l * layer_bytes further). lengths[b] = the tokens
- * before the tree + counts[b]; it may overlap neither kv_lens nor counts. A path
+ * before the tree + counts[b]; it may overlap none of the arrays read. A path
  * that does not ascend within the tree's nodes, or has a place (old or new)
  * whose page is out of range, leaves its sequence as it was (lengths[b] =
  * kv_lens[b]) and sets status bit 8. The places written must not be shared with

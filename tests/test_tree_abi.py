@@ -162,3 +162,9 @@ def test_sizes_past_32_bits_are_refused_not_cut_off(library):
                 ops.accept_tree(*batch, targets=meta(rows))
             with pytest.raises(ValueError, match="32 bits"):
                 ops.accept_workspace(rows, sequences, "meta")
+
+
+@pytest.mark.parametrize("at", [1 << 22, 1 << 23, (1 << 23) + 4, 1 << 24, 1 << 12, (1 << 12) + 8, 1 << 14])
+def test_keep_refuses_lengths_over_what_it_reads(library, at):
+    """The table, the offsets, the lengths, path and counts of one sequence: other CTAs read them while one writes."""
+    assert keep(library, path=1 << 12, counts=1 << 14, lengths=at) == EINVAL
