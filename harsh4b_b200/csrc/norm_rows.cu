@@ -87,7 +87,8 @@ __device__ __forceinline__ void finish_row(const NormRowsArgs& a, long long row,
 
 // One CTA a row. kG groups of 8 a thread stay in registers; kG = 0: rows too
 // wide for that are read in each of three passes (a thread its own values, so
-// `out` may be x).
+// `out` may be x), the second and third from L2 (4096 rows of 16384 in bf16 with delta
+// 99 us, 4.7 TB/s of the bytes of one pass).
 template <typename X, typename DT, int kG>
 __global__ void __launch_bounds__(256) norm_rows_kernel(const NormRowsArgs a) {
     __shared__ float red[32];
@@ -169,8 +170,9 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormRowsArgs a) {
 
 // Rows of up to 128 groups: a warp a row, without a barrier. Its lane l stands for the
 // lanes l of the first kWarps warps above (the others' sums are zeros), whose sums it
-// forms one after the other in the same order (16384 rows of 512 in bf16 33 -> 13 us,
-// 10000 of 1000 in fp32 21 -> 13; 16384 of 2048 in bf16 49, a warp a row 68).
+// forms one after the other in the same order (16384 rows of 512 in bf16 with delta 33 ->
+// 13.6 us, 4.3 TB/s, without 11.2; 10000 of 1000 in fp32 without delta 21 -> 14.0, 3.6
+// TB/s, with it 29, 4.5; 16384 of 2048 in bf16 49, a warp a row 68).
 template <typename X, typename DT, int kWarps>
 __global__ void __launch_bounds__(256) norm_rows_warp_kernel(const NormRowsArgs a) {
     const long long row = blockIdx.x * 8ll + (threadIdx.x >> 5);

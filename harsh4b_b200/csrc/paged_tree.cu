@@ -9,8 +9,8 @@
 // 64 keys, and an item's start and end. So two CTAs share an SM, each with half of
 // its tensor memory and shared memory: what one waits for the other fills. (One
 // CTA with two warpgroups that took an item's blocks of 128 keys in turn: 64 trees
-// of 16 nodes over ragged 2100 tokens 100 us, now 71; 16 x 32 nodes over 32768
-// 386, now 375; over 16-token pages 570, now 402.)
+// of 16 nodes over ragged 2100 tokens 100 us, two CTAs 71 and, with the steps below,
+// 69; 16 x 32 nodes over 32768 386, 375 and 365 to 371; over 16-token pages 570 and 402.)
 //
 // Warps: 0-3 are the softmax (thread = query row = TMEM lane), 4 issues the loads,
 // 5 the MMAs, 6 cleans V tiles. For block n, x = n % 2:
@@ -30,8 +30,17 @@
 // pair, which costs nothing in time but, under the power cap, clock (16 x 32 nodes
 // over 32768 tokens, sustained: 420 -> 411 us without it), so it is left out where no row
 // of the warp needs it. Which form a row's weights have goes by its own m, so l and O of
-// other blocks and parts are carried over with the right factor. p is rounded to the cache's
-// type for the product as in the other kernels (see paged.cu), l is its fp32 sum.
+// other blocks and parts are carried over with the right factor.
+//
+// l is summed from the fp32 p, which is rounded to the cache's type for the product
+// with V only, where both operands have one type. The rest of p as a second operand of
+// that product (it fits into the columns of the scores) costs most where the tensor pipe
+// and the softmax are the bound, and something everywhere: one tree of 8 nodes 12.8 ->
+// 13.6 us, 64 ragged trees of 16 69 -> 76, 16 x 32 nodes over 32768 tokens 368 -> 424 (under
+// the power cap 444 -> 528), of 64 nodes 620 -> 783, windowed trees at head_dim 64 58 -> 68
+// to 72. The rounding is to 2^-12 of a weight (bf16 2^-9), independent from key to key,
+// and its part of a sum stays below the result's own rounding: against 64 bits 2.6e-4 in
+// fp16 and 2.1 to 2.3e-3 in bf16 of the result's rms, 2.1e-4 and 1.7e-3 without it.
 //
 // V rows of keys that no row sees are zeroed and values that are not finite are
 // taken out of rows that only some see, and added at the item's end, as in
@@ -808,8 +817,10 @@ static int launch_tree_rows(AttendArgs a, const h4b_paged_kv* kv, int tile_token
     a.extra = kTreeExtra;
     a.least = kTreeLeast;
     a.half_tokens = tile_tokens;
-    // Where no item can have many blocks (the tables' width bounds the lengths) they stay
-    // whole: no parts, and no launch of the join, which the host needs 3 us for. Cut and
+    // Where no item can have many blocks (the tables' width bounds the lengths, which only
+    // the device knows: wide tables leave items cut) they stay whole: no parts, and no
+    // launch of the join, which the host needs 3 us for. A sequence counts as one item a kv
+    // head here, though a large tree has several tiles. Cut and
     // whole, in us on the device: 8 items of 6 blocks 11.6 and 13.5, of 4 11.0 and 11.2;
     // 64 items of 6 14.9 and 14.3 (two tiles of rows 21.0 and 15.8), of 8 14.9 and 16.4;
     // 512 of 6 33.9 and 28.9, of 16 58.1 and 54.9 (95.6 and 95.0).
