@@ -358,25 +358,29 @@ class PagedRunner:
             cache.check_visible(s, self.window, self.sinks)
         total = len(ids)
         held = [len(cache.table(s)) for s in sequences]  # room of the caller's own stays
-        with cache.ordered():
-            cache.reserve(dict(zip(sequences, new)))
-            if self.node_logits is None or self.node_logits.shape[0] < total:
-                self.node_logits = None  # (given back first)
-                self.node_logits = torch.empty(total, model.vocab, dtype=torch.float32, device=cache.device)
-            if self.accept_workspace is None:
-                self.accept_workspace = ops.accept_workspace(self.max_tokens, self.max_sequences, cache.device)
-            parents = torch.tensor([p for tree in trees for p in tree], dtype=torch.int32).to(cache.device)
-            table, offsets, lengths = self._launch(sequences, new, ids, parents)
-            path, counts, _, targets = ops.accept_tree(self.tokens[:total], parents, offsets, self.node_logits[:total],
-                                                       max_path=max(new), workspace=self.accept_workspace)
-            ops.keep_tokens(cache.k_pages, cache.v_pages, table, offsets, lengths, path, counts)
-            path, counts, targets = path.tolist(), counts.tolist(), targets.tolist()
+        try:
+            with cache.ordered():
+                cache.reserve(dict(zip(sequences, new)))
+                if self.node_logits is None or self.node_logits.shape[0] < total:
+                    self.node_logits = None  # (given back first)
+                    self.node_logits = torch.empty(total, model.vocab, dtype=torch.float32, device=cache.device)
+                if self.accept_workspace is None:
+                    self.accept_workspace = ops.accept_workspace(self.max_tokens, self.max_sequences, cache.device)
+                parents = torch.tensor([p for tree in trees for p in tree], dtype=torch.int32).to(cache.device)
+                table, offsets, lengths = self._launch(sequences, new, ids, parents)
+                path, counts, _, targets = ops.accept_tree(self.tokens[:total], parents, offsets, self.node_logits[:total],
+                                                           max_path=max(new), workspace=self.accept_workspace)
+                ops.keep_tokens(cache.k_pages, cache.v_pages, table, offsets, lengths, path, counts)
+                path, counts, targets = path.tolist(), counts.tolist(), targets.tolist()
+            for s, count in zip(sequences, counts):
+                cache.advance(s, count)
+        finally:  # (a step that fails keeps none of its room)
+            for s, pages in zip(sequences, held):
+                cache.release(s, pages)
         result, first = {}, 0
-        for b, (s, n) in enumerate(zip(sequences, new)):
-            result[s] = [targets[first + node] for node in path[b][:counts[b]]]
+        for s, n, nodes, count in zip(sequences, new, path, counts):
+            result[s] = [targets[first + node] for node in nodes[:count]]
             first += n
-            cache.advance(s, counts[b])
-            cache.release(s, held[b])
             if self.window:
                 cache.trim(s, self.window, self.sinks)
         return result

@@ -71,3 +71,21 @@ def test_under_a_window_and_from_a_shared_page(cache, monkeypatch):  # noqa: F81
     assert cache.length(a) == 41 and cache.length(b) == 43
     assert len(cache.table(a)) == 3 and len(cache.table(b)) == 3
     consistent(cache)
+
+
+def test_a_step_that_fails_keeps_no_pages(cache, monkeypatch):  # noqa: F811
+    runner = verifying(monkeypatch, cache, [1, 1])
+    a, b = cache.new_sequence(), cache.new_sequence()
+    grow(cache, a, 20)
+    grow(cache, b, 3)
+    tables, free = [cache.table(a), cache.table(b)], cache.free_pages
+
+    def fails(*args, **kwargs):
+        raise RuntimeError("no memory")
+
+    monkeypatch.setattr(paged.ops, "accept_tree", fails)
+    with pytest.raises(RuntimeError, match="no memory"):
+        runner.verify({a: wide(40), b: wide(20)})
+    assert [cache.table(a), cache.table(b)] == tables and cache.free_pages == free
+    assert (cache.length(a), cache.length(b)) == (20, 3)
+    consistent(cache)
